@@ -80,6 +80,11 @@ _SIGS = {
                                    _VP], ctypes.c_int),
     "gfd_moe_route_gather": ([_VP, _VP, ctypes.c_int64, ctypes.c_int, ctypes.c_int, _VP, ctypes.c_size_t,
                               _VP, ctypes.c_size_t, _VP, _VP, _VP, _VP, ctypes.c_uint32], ctypes.c_int),
+    "gfd_kv_append": ([_VP, _VP, _VP, _VP, _VP], ctypes.c_int),
+    "gfd_kv_attend": ([_VP, _VP, _VP, _VP, _VP], ctypes.c_int),
+    "gfd_kv_attend_shared": ([_VP, _VP, _VP, _VP, ctypes.c_int64, _VP, _VP], ctypes.c_int),
+    "gfd_kv_attend_workspace": ([_VP, _VP, _VP, _VP, ctypes.c_int64, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
+    "gfd_kv_merge": ([_VP, _VP, _VP], ctypes.c_int),
     "gfd_ring_create": ([_VP, _VP, _VP, _VP, ctypes.POINTER(_VP)], ctypes.c_int),
     "gfd_ring_destroy": ([_VP], ctypes.c_int),
     "gfd_ring_start": ([_VP], ctypes.c_int),

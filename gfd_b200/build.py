@@ -37,6 +37,8 @@ SOURCES = [
     "context.cpp",
     "noalloc.cu",
     "moe.cu",
+    "kv.cu",
+    "kv_api.cpp",
     "ring.cu",
     "agent.cu",
     "copy_engine.cpp",

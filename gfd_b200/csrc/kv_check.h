@@ -1,0 +1,183 @@
+#pragma once
+// Argument checks of the paged KV-cache entry points and the sequence arithmetic that
+// their kernels share with the host.  Nothing here touches CUDA state, so the CPU tests
+// compile it with a plain C++ compiler.
+
+#include <cmath>
+#include <cstdint>
+#include <initializer_list>
+
+#include "gfd_b200.h"
+
+#if defined(__CUDACC__)
+#define GFD_HD __host__ __device__ __forceinline__
+#else
+#define GFD_HD inline
+#endif
+
+namespace gfdb {
+
+constexpr int kKvPage = 16;           // tokens one load takes: block_tokens is a multiple
+constexpr int kKvMaxHeads = 1024;
+constexpr int kKvMaxBlockTokens = 1024;
+constexpr int kKvMaxParts = 1024;
+constexpr int64_t kKvMaxTokens = 1ll << 30;  // positions of a sequence, so that they fit 32 bits with room
+
+// ---------------------------------------------------------------------------
+// Sequences
+// ---------------------------------------------------------------------------
+// Rows [row0, row0 + rows) of sequence s and its keys; ok == false: skipped (BAD_LENGTH).
+struct KvSeq {
+    int32_t row0;
+    int32_t rows;
+    int32_t keys;  // kv_len
+    bool ok;
+};
+
+GFD_HD KvSeq kv_seq(int32_t start, int32_t end, int32_t kv_len, int64_t capacity, int32_t max_q_len) {
+    KvSeq q{start, end - start, kv_len, true};
+    if (q.rows > 0 && (kv_len < q.rows || kv_len > capacity || (max_q_len > 0 && q.rows > max_q_len))) q.ok = false;
+    if (q.rows <= 0) q.rows = q.keys = 0;  // nothing to do, whatever kv_len says
+    return q;
+}
+
+// What the row at position p sees of n keys: [0, pre) and [lo, hi).  lo >= pre and
+// hi >= lo, so the two never overlap.
+struct KvSpan {
+    int32_t pre, lo, hi;
+};
+
+GFD_HD KvSpan kv_span(int32_t p, int32_t n, int32_t prefix, int32_t window, bool causal) {
+    KvSpan s;
+    s.pre = prefix < 0 ? 0 : (prefix > n ? n : prefix);
+    s.hi = causal ? (p + 1 < n ? p + 1 : n) : n;
+    s.lo = window > 0 && p + 1 > window ? p + 1 - window : 0;
+    if (s.lo < s.pre) s.lo = s.pre;
+    if (s.hi < s.lo) s.hi = s.lo;
+    return s;
+}
+
+// ---------------------------------------------------------------------------
+// Checks: each returns nullptr, or what is wrong
+// ---------------------------------------------------------------------------
+inline int kv_elt(int32_t dtype) { return dtype == GFD_FP32 ? 4 : 2; }
+
+inline bool kv_aligned(const void* p, uint64_t n) { return (reinterpret_cast<uint64_t>(p) & (n - 1)) == 0; }
+
+// Bytes from the first to behind the last element of [n0][n1][...][inner], or 0 when that
+// does not fit 2^62.
+inline uint64_t kv_extent(const int64_t* n, const int64_t* stride, int dims, int64_t inner, int elt) {
+    unsigned __int128 e = static_cast<unsigned __int128>(inner);
+    for (int i = 0; i < dims; ++i) {
+        if (n[i] <= 0 || stride[i] < 0) return 0;
+        e += static_cast<unsigned __int128>(n[i] - 1) * static_cast<unsigned __int128>(stride[i]);
+    }
+    e *= static_cast<unsigned>(elt);
+    return (e >> 62) != 0 ? 0 : static_cast<uint64_t>(e);
+}
+
+// True when no two index tuples of [n0][n1].. share an element (strides nest in some order).
+inline bool kv_distinct(const int64_t* n, const int64_t* stride, int dims, int64_t inner) {
+    bool used[4] = {};
+    unsigned __int128 span = static_cast<unsigned __int128>(inner);
+    for (int k = 0; k < dims; ++k) {
+        int best = -1;
+        for (int i = 0; i < dims; ++i)
+            if (!used[i] && n[i] > 1 && (best < 0 || stride[i] < stride[best])) best = i;
+        if (best < 0) break;
+        used[best] = true;
+        if (stride[best] < 0 || static_cast<unsigned __int128>(stride[best]) < span) return false;
+        span += static_cast<unsigned __int128>(n[best] - 1) * static_cast<unsigned __int128>(stride[best]);
+    }
+    return true;
+}
+
+// A row array; `out`: written, so its elements must be distinct.  *bytes: its extent.
+inline const char* kv_check_rows(const gfd_kv_rows& r, int64_t rows, int64_t heads, int64_t dim, int32_t dtype, bool out,
+                                 uint64_t* bytes) {
+    const int64_t n[2] = {rows, heads};
+    const int64_t st[2] = {rows > 1 ? r.row_stride : 0, heads > 1 ? r.head_stride : 0};
+    if (r.data == nullptr) return "a row array is NULL";
+    if (!kv_aligned(r.data, 16)) return "a row array is not 16-byte aligned";
+    if (st[0] < 0 || st[1] < 0 || st[0] % 8 != 0 || st[1] % 8 != 0) return "row and head strides must be multiples of 8, not negative";
+    *bytes = kv_extent(n, st, 2, dim, kv_elt(dtype));
+    if (*bytes == 0) return "a row array is too large";
+    if (out && !kv_distinct(n, st, 2, dim)) return "elements of an output row array overlap";
+    return nullptr;
+}
+
+inline const char* kv_check_cache(const gfd_kv_cache& c, bool write, uint64_t* bytes) {
+    if (c.dtype != GFD_BF16 && c.dtype != GFD_FP16) return "the cache is neither bf16 nor fp16";
+    if (c.head_dim != 64 && c.head_dim != 128) return "head_dim must be 64 or 128";
+    if (c.heads < 1 || c.heads > kKvMaxHeads) return "bad number of KV heads";
+    if (c.block_tokens < kKvPage || c.block_tokens > kKvMaxBlockTokens || c.block_tokens % kKvPage != 0)
+        return "block_tokens must be a multiple of 16, at most 1024";
+    if (c.blocks < 1 || c.blocks > 0x7fffffffll) return "bad number of blocks";
+    if (c.k == nullptr || c.v == nullptr) return "K or V of the cache is NULL";
+    if (!kv_aligned(c.k, 16) || !kv_aligned(c.v, 16)) return "the cache is not 16-byte aligned";
+    const int64_t n[3] = {c.blocks, c.block_tokens, c.heads};
+    const int64_t st[3] = {c.blocks > 1 ? c.block_stride : 0, c.token_stride, c.heads > 1 ? c.head_stride : 0};
+    for (int64_t s : st)
+        if (s < 0 || s % 8 != 0 || s >= (1ll << 38)) return "cache strides must be multiples of 8, not negative and below 2^38";
+    if (!kv_distinct(n, st, 3, c.head_dim)) return "elements of the cache overlap";
+    *bytes = kv_extent(n, st, 3, c.head_dim, 2);
+    if (*bytes == 0) return "the cache is too large";
+    if (write && c.k == c.v) return "K and V are the same array";
+    return nullptr;
+}
+
+inline const char* kv_check_batch(const gfd_kv_batch& b, const gfd_kv_cache& c, int64_t shared_len) {
+    if (b.rows < 0 || b.rows > 0x3fffffffll) return "bad number of rows";
+    if (b.seqs < 0 || b.seqs > GFD_KV_MAX_SEQS) return "bad number of sequences";
+    if (b.rows == 0 || b.seqs == 0) return nullptr;
+    if (b.table_width < 0 || b.table_stride < 0 || (b.seqs > 1 && b.table_stride < b.table_width)) return "bad block table shape";
+    if (shared_len < 0 || shared_len + static_cast<int64_t>(b.table_width) * c.block_tokens > kKvMaxTokens)
+        return "more than 2^30 tokens in a sequence's table";
+    if (b.row_start == nullptr || b.kv_len == nullptr || (b.table == nullptr && b.table_width > 0))
+        return "row_start, kv_len or table is NULL";
+    if (!kv_aligned(b.row_start, 4) || !kv_aligned(b.kv_len, 4) || !kv_aligned(b.table, 4))
+        return "row_start, kv_len or table is not 4-byte aligned";
+    return nullptr;
+}
+
+inline const char* kv_check_append(const gfd_kv_append_args& a, const gfd_kv_cache& c) {
+    if (a.q_heads < 0 || a.q_heads > 8 * kKvMaxHeads) return "bad number of query heads";
+    if (a.rot_dim < 0 || a.rot_dim > c.head_dim || a.rot_dim % 16 != 0) return "rot_dim must be a multiple of 16, at most head_dim";
+    if (a.rot_dim > 0 && (a.inv_freq == nullptr || !kv_aligned(a.inv_freq, 4))) return "inv_freq is NULL or not 4-byte aligned";
+    if (!kv_aligned(a.positions, 4) || !kv_aligned(a.status, 4)) return "positions or status is not 4-byte aligned";
+    if (a.q_heads > 0 && a.q.data == a.q_out.data && (a.q.row_stride != a.q_out.row_stride || a.q.head_stride != a.q_out.head_stride))
+        return "q_out is q with other strides";
+    return nullptr;
+}
+
+inline const char* kv_check_attend(const gfd_kv_attend_args& a, const gfd_kv_cache& c) {
+    if (a.q_heads < 1 || a.q_heads > 8 * kKvMaxHeads || a.q_heads % c.heads != 0)
+        return "query heads must be a multiple of the cache's heads";
+    if (a.out_dtype != c.dtype && a.out_dtype != GFD_FP32) return "out must be of the cache's type or fp32";
+    if (a.max_q_len < 0) return "max_q_len is negative";
+    if (a.window < 0 || a.window > kKvMaxTokens) return "bad window";
+    if (!std::isfinite(a.scale)) return "scale is not finite";
+    if (!std::isfinite(a.softcap) || a.softcap < 0.0f) return "softcap must be finite and not negative";
+    if (a.q.data == a.out.data) return "out must not be q";
+    if (!kv_aligned(a.lse, 4) || !kv_aligned(a.alibi, 4) || !kv_aligned(a.prefix_len, 4) || !kv_aligned(a.status, 4))
+        return "lse, alibi, prefix_len or status is not 4-byte aligned";
+    return nullptr;
+}
+
+inline const char* kv_check_merge(const gfd_kv_merge_args& a) {
+    if (a.rows < 0 || a.rows > 0x3fffffffll) return "bad number of rows";
+    if (a.part_count < 1 || a.part_count > kKvMaxParts) return "bad number of parts";
+    if (a.heads < 1 || a.heads > 8 * kKvMaxHeads) return "bad number of heads";
+    if (a.head_dim != 64 && a.head_dim != 128) return "head_dim must be 64 or 128";
+    for (int32_t t : {a.part_dtype, a.out_dtype})
+        if (t != GFD_BF16 && t != GFD_FP16 && t != GFD_FP32) return "unknown type";
+    if (a.part_stride < 0 || a.part_stride % 8 != 0) return "part_stride must be a multiple of 8, not negative";
+    if ((a.rows > 0 && a.part_lse == nullptr) || !kv_aligned(a.part_lse, 4) || !kv_aligned(a.lse, 4)) return "part_lse is NULL, or part_lse or lse not 4-byte aligned";
+    if (a.rows > 0)
+        for (int i = 0; i < a.part_count; ++i)
+            if (static_cast<const char*>(a.parts.data) + static_cast<int64_t>(i) * a.part_stride * kv_elt(a.part_dtype) == a.out.data)
+                return "out must not be a part";
+    return nullptr;
+}
+
+}  // namespace gfdb

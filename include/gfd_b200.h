@@ -217,6 +217,154 @@ int gfd_moe_route_gather(gfd_ctx* ctx, const float* d_logits, int64_t tokens, in
                          size_t dst_bytes, uint32_t* d_counts, uint32_t* d_offsets,
                          gfd_sg_entry* d_entries, void* stream, uint32_t flags);
 
+/* ---- paged KV cache ------------------------------------------------------------
+ * No counterpart in the reference: what a serving program does with the KV blocks that
+ * the gathers fetch.  A cache is a set of equal blocks in device memory, each holding
+ * block_tokens tokens of K and V for every KV head; a block table gives each sequence its
+ * blocks in order, so token j of sequence s lies in block table[s][j / block_tokens] at
+ * place j % block_tokens.  Every call is asynchronous on `stream` (NULL: the context's
+ * stream), allocates nothing and can be captured into a CUDA graph; lengths, tables and
+ * row starts are read on the device when the call runs.
+ *
+ * What is checked before anything is launched (GFD_ERR_INVALID): shapes, types, strides,
+ * alignment, and that every array lies in device memory of the context's GPU.  What only
+ * the device knows is checked there: offending parts are skipped and reported by OR-ing
+ * GFD_KV_* bits into *status (a device word, or NULL).                              */
+enum { GFD_BF16 = 0, GFD_FP16 = 1, GFD_FP32 = 2 };
+
+#define GFD_KV_BAD_PAGE 1u   /* a block id outside [0, blocks): its keys count as masked, a row
+                                that would be stored there is not stored                  */
+#define GFD_KV_BAD_LENGTH 2u /* kv_len[s] below 0, below the sequence's rows or beyond its
+                                table, or more rows than max_q_len: sequence s is skipped, its
+                                output rows stay as they were.  row_start not rising from
+                                >= 0 to <= rows: the whole call is skipped                 */
+#define GFD_KV_GAVE_UP 4u    /* a bounded wait inside a kernel ran out: outputs undefined  */
+
+#define GFD_KV_MAX_SEQS 4096
+
+/* Strides count elements, are multiples of 8, and (as the first element's address) keep
+ * every head's head_dim elements contiguous and 16-byte aligned. */
+typedef struct gfd_kv_cache {
+    void* k;               /* block 0, token 0, head 0 of K */
+    void* v;               /* the same of V; strides as K's */
+    int64_t blocks;
+    int64_t block_stride;
+    int64_t token_stride;
+    int64_t head_stride;
+    int32_t block_tokens;  /* a multiple of 16, at most 1024 */
+    int32_t heads;         /* KV heads, at most 1024         */
+    int32_t head_dim;      /* 64 or 128                      */
+    int32_t dtype;         /* GFD_BF16 or GFD_FP16           */
+} gfd_kv_cache;
+
+/* The sequences of one call.  Sequence s owns rows row_start[s] .. row_start[s + 1] - 1 of
+ * the call's row arrays (possibly none), and they are the last rows of its kv_len[s]
+ * tokens: row i of it stands at position kv_len[s] - (its rows) + i.  Rows before
+ * row_start[0] and from row_start[seqs] on belong to no sequence and are left alone. */
+typedef struct gfd_kv_batch {
+    const int32_t* row_start;  /* device, seqs + 1                          */
+    const int32_t* kv_len;     /* device, seqs                              */
+    const int32_t* table;      /* device, seqs rows of table_width block ids */
+    int64_t table_stride;      /* elements from one table row to the next    */
+    int64_t rows;              /* rows of the call's row arrays              */
+    int32_t seqs;              /* at most GFD_KV_MAX_SEQS                    */
+    int32_t table_width;
+} gfd_kv_batch;
+
+/* A row array [rows][heads][head_dim]. */
+typedef struct gfd_kv_rows {
+    void* data;
+    int64_t row_stride;
+    int64_t head_stride;
+} gfd_kv_rows;
+
+/* Appends the batch's rows of K and V to the cache, rotating K (and Q, when given) by
+ * position on the way.  The first rot_dim elements of a head are rotated in pairs by the
+ * angle position * inv_freq[i], i < rot_dim / 2: elements (i, i + rot_dim / 2), or
+ * (2 i, 2 i + 1) with interleaved; angles are formed in 64 bits, the rotation in 32, and
+ * each value rounds once.  rot_dim 0: copies.  q_out may be q (same strides).  Two rows of
+ * a call must not fall on the same place of the cache (sequences may share blocks that the
+ * call does not write). */
+typedef struct gfd_kv_append_args {
+    gfd_kv_rows k;             /* cache.heads heads, the cache's type                       */
+    gfd_kv_rows v;
+    gfd_kv_rows q;             /* q_heads heads, the cache's type; q_heads 0: no Q          */
+    gfd_kv_rows q_out;
+    const float* inv_freq;     /* device, rot_dim / 2                                      */
+    const int32_t* positions;  /* device, rows: angles' positions; NULL: the cache position */
+    uint32_t* status;
+    int32_t q_heads;
+    int32_t rot_dim;           /* a multiple of 16, at most head_dim                       */
+    int32_t interleaved;
+    int32_t _pad;
+} gfd_kv_append_args;
+int gfd_kv_append(gfd_ctx* ctx, const gfd_kv_cache* cache, const gfd_kv_batch* batch,
+                  const gfd_kv_append_args* args, void* stream);
+
+/* Attention of the batch's rows over the cache (each KV head serves q_heads / heads query
+ * heads in a row).  The row at position p sees key j < kv_len[s] when
+ *     j < prefix_len[s]  or  ((!causal or j <= p) and (window == 0 or j > p - window))
+ * with score  z = softcap * tanh(scale * q.k / softcap) + alibi[head] * (j - p)  (cap and
+ * bias only where given); out = sum exp(z) v / sum exp(z), lse = log sum exp(z) in 32 bits.
+ * A row that sees no key, or only scores of -inf, gets zeros and lse = -inf.  What lies in
+ * masked places of the cache (unwritten tokens, NaN, infinities) never reaches a result.
+ * out is of the cache's type or GFD_FP32 and must not be q.                          */
+typedef struct gfd_kv_attend_args {
+    gfd_kv_rows q;              /* q_heads heads, the cache's type                          */
+    gfd_kv_rows out;            /* q_heads heads, out_dtype                                 */
+    float* lse;                 /* device, rows x q_heads contiguous, or NULL               */
+    const float* alibi;         /* device, q_heads slopes, or NULL                          */
+    const int32_t* prefix_len;  /* device, seqs, or NULL                                    */
+    void* workspace;            /* device, 256-byte aligned; calls that may overlap (other
+                                   streams, graphs replayed side by side) need one each     */
+    size_t workspace_bytes;     /* at least gfd_kv_attend_workspace                         */
+    uint32_t* status;
+    int32_t q_heads;            /* a multiple of cache.heads                                */
+    int32_t out_dtype;
+    int32_t max_q_len;           /* the most rows any sequence has; 0: not known             */
+    int32_t causal;
+    int32_t window;             /* 0: no window                                             */
+    float scale;
+    float softcap;              /* 0: no cap                                                */
+    int32_t _pad;
+} gfd_kv_attend_args;
+int gfd_kv_attend(gfd_ctx* ctx, const gfd_kv_cache* cache, const gfd_kv_batch* batch,
+                  const gfd_kv_attend_args* args, void* stream);
+
+/* The same behind a prefix that all sequences share: shared_len tokens whose blocks
+ * shared_table (device) lists.  Position j < shared_len is the shared prefix's token j; the
+ * batch's lengths and tables describe what follows it, so position shared_len + j is token
+ * j of the sequence's own table, and rows stand at shared_len + kv_len[s] - (its rows) + i.
+ * The prefix is read once for all rows of the batch, not once per sequence.           */
+int gfd_kv_attend_shared(gfd_ctx* ctx, const gfd_kv_cache* cache, const gfd_kv_batch* batch,
+                         const int32_t* shared_table, int64_t shared_len,
+                         const gfd_kv_attend_args* args, void* stream);
+
+/* Bytes of workspace for a call of these shapes (only q_heads, max_q_len of args, rows and
+ * seqs of batch, and the cache's shape are read; no array is touched). */
+int gfd_kv_attend_workspace(gfd_ctx* ctx, const gfd_kv_cache* cache, const gfd_kv_batch* batch,
+                            const gfd_kv_attend_args* args, int64_t shared_len, size_t* bytes);
+
+/* Joins partial results over disjoint sets of keys (a resident and a fetched part of a
+ * context, say): lse = log sum_i exp(lse_i), out = sum_i exp(lse_i - lse) out_i.  A part
+ * with lse_i = -inf is not read into the sum; where every part has it, out is zero and lse
+ * -inf.  part i is the row array parts.data + i * part_stride.  out may not be a part. */
+typedef struct gfd_kv_merge_args {
+    gfd_kv_rows parts;        /* part 0                                                   */
+    int64_t part_stride;      /* elements                                                 */
+    const float* part_lse;    /* device, parts x rows x heads contiguous                  */
+    gfd_kv_rows out;
+    float* lse;               /* device, rows x heads contiguous, or NULL                 */
+    int64_t rows;
+    int32_t part_count;       /* 1 .. 1024                                                */
+    int32_t heads;
+    int32_t head_dim;         /* 64 or 128                                                */
+    int32_t part_dtype;       /* GFD_BF16, GFD_FP16 or GFD_FP32                           */
+    int32_t out_dtype;
+    int32_t _pad;
+} gfd_kv_merge_args;
+int gfd_kv_merge(gfd_ctx* ctx, const gfd_kv_merge_args* args, void* stream);
+
 /* ---- GPU-queued submit: descriptor ring consumer ------------------------------
  * Attaches to a gfd::DescriptorQueue written by GPU producers (device.cuh /
  * device_primitives.cuh / sg protocol).  Between gfd_ring_start and gfd_ring_stop a

@@ -1,0 +1,38 @@
+// C exports of the paged KV-cache checks and sequence arithmetic (gfd_b200/csrc/kv_check.h)
+// for the CPU tests.
+#include <cstddef>
+
+#include "kv_check.h"
+
+using namespace gfdb;
+
+extern "C" {
+
+const char* gfdt_kv_cache(const gfd_kv_cache* c, int write, uint64_t* bytes) { return kv_check_cache(*c, write != 0, bytes); }
+const char* gfdt_kv_batch(const gfd_kv_batch* b, const gfd_kv_cache* c, int64_t shared) { return kv_check_batch(*b, *c, shared); }
+const char* gfdt_kv_append(const gfd_kv_append_args* a, const gfd_kv_cache* c) { return kv_check_append(*a, *c); }
+const char* gfdt_kv_attend(const gfd_kv_attend_args* a, const gfd_kv_cache* c) { return kv_check_attend(*a, *c); }
+const char* gfdt_kv_merge(const gfd_kv_merge_args* a) { return kv_check_merge(*a); }
+const char* gfdt_kv_rows(const gfd_kv_rows* r, int64_t rows, int64_t heads, int64_t dim, int32_t dtype, int out, uint64_t* bytes) {
+    return kv_check_rows(*r, rows, heads, dim, dtype, out != 0, bytes);
+}
+void gfdt_kv_span(int32_t p, int32_t n, int32_t prefix, int32_t window, int causal, int32_t* out) {
+    const KvSpan s = kv_span(p, n, prefix, window, causal != 0);
+    out[0] = s.pre, out[1] = s.lo, out[2] = s.hi;
+}
+int gfdt_kv_seq(int32_t start, int32_t end, int32_t len, int64_t capacity, int32_t max_q, int32_t* out) {
+    const KvSeq q = kv_seq(start, end, len, capacity, max_q);
+    out[0] = q.row0, out[1] = q.rows, out[2] = q.keys;
+    return q.ok;
+}
+// sizes and last offsets of the argument structures
+void gfdt_kv_layout(uint64_t* out) {
+    const uint64_t v[] = {sizeof(gfd_kv_cache),       offsetof(gfd_kv_cache, dtype),
+                          sizeof(gfd_kv_batch),       offsetof(gfd_kv_batch, table_width),
+                          sizeof(gfd_kv_rows),        offsetof(gfd_kv_rows, head_stride),
+                          sizeof(gfd_kv_append_args), offsetof(gfd_kv_append_args, interleaved),
+                          sizeof(gfd_kv_attend_args), offsetof(gfd_kv_attend_args, softcap),
+                          sizeof(gfd_kv_merge_args),  offsetof(gfd_kv_merge_args, out_dtype)};
+    for (unsigned i = 0; i < sizeof(v) / sizeof(v[0]); ++i) out[i] = v[i];
+}
+}
