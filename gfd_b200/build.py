@@ -38,6 +38,7 @@ SOURCES = [
     "noalloc.cu",
     "moe.cu",
     "kv.cu",
+    "kv_decode.cu",
     "kv_api.cpp",
     "ring.cu",
     "agent.cu",

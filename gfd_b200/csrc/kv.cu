@@ -155,6 +155,7 @@ __global__ void __launch_bounds__(kPlainThreads) kv_attend_plain_kernel(const Kv
             if (t == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
             continue;
         }
+        if (p.skip_few && q.rows * p.group <= kKvFewRows) continue;
         const int32_t n = p.shared_len + q.keys;
         const int kvh = h / p.group;
         const float slope = p.alibi != nullptr ? p.alibi[h] : 0.0f;

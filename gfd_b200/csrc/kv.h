@@ -54,7 +54,14 @@ struct KvAttendParams {
     int32_t q_heads, group;
     int32_t max_q_len, causal, window;
     float scale, softcap;
+    float scale2;    // scale in base 2
+    float cap_rate;  // 2 log2(e) / softcap
+    int32_t out_f32;
+    int32_t skip_few;  // the plain kernel leaves sequences of at most kKvFewRows packed rows out
+    float* partial;    // kv_decode's partial results
 };
+
+constexpr int kKvFewRows = 16;  // packed rows (rows x group) up to which kv_decode takes a sequence
 
 struct KvMergeParams {
     KvRowsView parts;
@@ -68,6 +75,8 @@ struct KvMergeParams {
 // dtype: GFD_* of the cache; out: of the output rows
 cudaError_t launch_kv_append(const KvAppendParams& p, int head_dim, int dtype, int num_sms, cudaStream_t st);
 cudaError_t launch_kv_attend(const KvAttendParams& p, int head_dim, int dtype, int out_dtype, int num_sms, cudaStream_t st);
+cudaError_t launch_kv_decode(const KvAttendParams& p, int head_dim, int dtype, int num_sms, cudaStream_t st);
+size_t kv_decode_workspace(int num_sms, int head_dim);
 cudaError_t launch_kv_merge(const KvMergeParams& p, int head_dim, int part_dtype, int out_dtype, int num_sms,
                             cudaStream_t st);
 

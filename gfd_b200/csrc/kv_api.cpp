@@ -60,6 +60,11 @@ uint64_t table_bytes(const gfd_kv_batch& b) {
     return b.table_width == 0 ? 0 : (static_cast<uint64_t>(b.seqs - 1) * b.table_stride + b.table_width) * sizeof(int32_t);
 }
 
+// Bytes of workspace of an attention call.
+size_t attend_workspace(const gfd_ctx* ctx, const gfd_kv_cache& c, int64_t shared_len) {
+    return shared_len > 0 ? 0 : kv_decode_workspace(ctx->num_sms, c.head_dim);
+}
+
 int append(gfd_ctx* ctx, const gfd_kv_cache* c, const gfd_kv_batch* b, const gfd_kv_append_args* a, void* stream) {
     if (c == nullptr || b == nullptr || a == nullptr) return set_error(ctx, GFD_ERR_INVALID, "kv_append: NULL argument");
     uint64_t cache_bytes = 0, kb = 0, vb = 0, qb = 0, qob = 0;
@@ -121,6 +126,11 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
     const bool empty = b->rows == 0 || b->seqs == 0;
     if (!why && !empty) why = kv_check_rows(a->q, b->rows, a->q_heads, c->head_dim, c->dtype, false, &qb);
     if (!why && !empty) why = kv_check_rows(a->out, b->rows, a->q_heads, c->head_dim, a->out_dtype, true, &ob);
+    const size_t need = attend_workspace(ctx, *c, shared_len);
+    if (!why && !empty && need > 0) {
+        if (a->workspace == nullptr || !kv_aligned(a->workspace, 256)) why = "workspace is NULL or not 256-byte aligned";
+        else if (a->workspace_bytes < need) why = "workspace is smaller than gfd_kv_attend_workspace says";
+    }
     if (why) return set_error(ctx, GFD_ERR_INVALID, "%s: %s", call, why);
     if (empty) return GFD_OK;
     const uint64_t shared_blocks = (static_cast<uint64_t>(shared_len) + c->block_tokens - 1) / c->block_tokens;
@@ -135,6 +145,7 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
                               {a->lse, static_cast<uint64_t>(b->rows) * a->q_heads * 4, "lse"},
                               {a->alibi, static_cast<uint64_t>(a->q_heads) * 4, "alibi"},
                               {a->prefix_len, static_cast<uint64_t>(b->seqs) * 4, "prefix_len"},
+                              {a->workspace, need, "workspace"},
                               {a->status, 4, "status"}};
     const int rc = check_regions(ctx, call, regions, static_cast<int>(sizeof(regions) / sizeof(regions[0])));
     if (rc != GFD_OK) return rc;
@@ -157,8 +168,18 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
     p.window = a->window;
     p.scale = a->scale;
     p.softcap = a->softcap;
+    p.scale2 = a->scale * 1.4426950408889634f;
+    p.cap_rate = a->softcap > 0.0f ? 2.0f * 1.4426950408889634f / a->softcap : 0.0f;
+    p.out_f32 = a->out_dtype == GFD_FP32;
+    p.partial = static_cast<float*>(a->workspace);
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
-    const cudaError_t e = launch_kv_attend(p, c->head_dim, c->dtype, a->out_dtype, ctx->num_sms, st);
+    cudaError_t e = cudaSuccess;
+    if (shared_len == 0) {
+        p.skip_few = 1;
+        e = launch_kv_decode(p, c->head_dim, c->dtype, ctx->num_sms, st);
+    }
+    const bool all_few = shared_len == 0 && a->max_q_len > 0 && static_cast<int64_t>(a->max_q_len) * p.group <= kKvFewRows;
+    if (e == cudaSuccess && !all_few) e = launch_kv_attend(p, c->head_dim, c->dtype, a->out_dtype, ctx->num_sms, st);
     return e == cudaSuccess ? GFD_OK : cuda_error(ctx, e, "kv_attend: kernel launch");
 }
 
@@ -233,7 +254,10 @@ int gfd_kv_attend_workspace(gfd_ctx* ctx, const gfd_kv_cache* cache, const gfd_k
     return guarded(ctx, [&] {
         if (bytes == nullptr || cache == nullptr || batch == nullptr || args == nullptr || shared_len < 0)
             return set_error(ctx, GFD_ERR_INVALID, "kv_attend_workspace: NULL argument");
-        *bytes = 0;
+        uint64_t unused = 0;
+        const char* why = kv_check_cache(*cache, false, &unused);
+        if (why) return set_error(ctx, GFD_ERR_INVALID, "kv_attend_workspace: %s", why);
+        *bytes = attend_workspace(ctx, *cache, shared_len);
         return static_cast<int>(GFD_OK);
     });
 }

@@ -57,6 +57,35 @@ GFD_HD KvSpan kv_span(int32_t p, int32_t n, int32_t prefix, int32_t window, bool
     return s;
 }
 
+// The span within the keys [base, base + len), in their own count.
+GFD_HD KvSpan kv_clip(KvSpan s, int32_t base, int32_t len) {
+    auto c = [&](int32_t x) { return x < base ? 0 : (x - base > len ? len : x - base); };
+    return KvSpan{c(s.pre), c(s.lo), c(s.hi)};
+}
+
+// Tiles of `size` keys that hold a visible key of some row: tiles [0, npre), then
+// [first, first + count - npre).  The span's lo and hi are the least and the greatest of the rows'.
+struct KvTiles {
+    int32_t npre, first, count;
+    GFD_HD int32_t at(int32_t i) const { return i < npre ? i : i - npre + first; }
+};
+
+GFD_HD KvTiles kv_tiles(KvSpan s, int32_t size) {
+    KvTiles t;
+    t.npre = (s.pre + size - 1) / size;
+    t.first = s.lo / size;
+    if (t.first < t.npre) t.first = t.npre;
+    const int32_t end = s.hi > s.lo ? (s.hi + size - 1) / size : 0;
+    t.count = t.npre + (end > t.first ? end - t.first : 0);
+    return t;
+}
+
+// All tiles of a launch form one line, unit after unit; CTA c of n takes [kv_cut(c), kv_cut(c + 1)).
+// A unit that lies in one CTA is finished there.  One that is cut leaves partial results, one
+// in each CTA it touches, in slot 1 of the CTA where it begins and slot 0 of the others; the
+// first cut inside a unit names the one who joins them.
+GFD_HD int64_t kv_cut(int64_t total, int c, int n) { return total / n * c + (total % n) * c / n; }
+
 // ---------------------------------------------------------------------------
 // Checks: each returns nullptr, or what is wrong
 // ---------------------------------------------------------------------------

@@ -1,0 +1,642 @@
+// Attention for sequences with few rows (decode steps, short drafts): at most 16 packed rows
+// per KV head, where a packed row is one (row, query head) pair of the head's group.
+//
+// The work is reading the cache once: 4 D bytes per key and KV head against 4 D * 16 operations,
+// so memory bounds it.  All (sequence, KV head) units are laid out as one line of 64-key tiles
+// and every CTA takes an equal stretch (kv_cut): a batch of mixed lengths, one long context and
+// a hundred short ones keep every SM equally busy, with nothing known on the host.  A unit
+// that a cut divides leaves partial sums in the workspace, joined by kv_decode_join_kernel.
+//
+// Inside a CTA each of the 4 warps owns the 16 keys (one page or part of it) w of a tile and runs
+// alone: its own ring of stages filled with 16-byte cp.async (a page id per stage, ids fetched
+// 32 stages at a time), its own running maximum and sum, scores and sums by mma.m16n8k16 from
+// ldmatrix fragments.  No barrier between tiles; the warps join once per unit.
+
+#include "kv_device.cuh"
+
+namespace gfdb {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kTile = kKvPage * kWarps;  // keys a CTA takes per step
+constexpr int kRows = 16;
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// 16 bytes into shared memory, zeros where !take
+__device__ __forceinline__ void copy16(uint32_t dst, const char* src, bool take) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// One sequence as this kernel sees it: its rows and, in the count of its own keys (behind the
+// shared prefix), what its rows see together.
+struct Seq {
+    KvSeq q;
+    KvSpan all;  // pre, least lo, greatest hi
+    KvTiles tiles;
+    bool bad;
+};
+
+__device__ __forceinline__ Seq few_seq(const KvAttendParams& p, int s) {
+    const KvBatchView& b = p.batch;
+    Seq r;
+    r.q = kv_seq(b.row_start[s], b.row_start[s + 1], b.kv_len[s], b.capacity, p.max_q_len);
+    r.bad = !r.q.ok;
+    if (r.bad || r.q.rows * p.group > kRows) r.q.rows = r.q.keys = 0;
+    r.all = KvSpan{0, 0, 0};
+    r.tiles = KvTiles{0, 0, 0};
+    if (r.q.rows > 0) {
+        const int32_t n = p.shared_len + r.q.keys;
+        const int32_t prefix = p.prefix_len != nullptr ? p.prefix_len[s] : 0;
+        const KvSpan first = kv_clip(kv_span(n - r.q.rows, n, prefix, p.window, p.causal != 0), p.shared_len, r.q.keys);
+        const KvSpan last = kv_clip(kv_span(n - 1, n, prefix, p.window, p.causal != 0), p.shared_len, r.q.keys);
+        r.all = KvSpan{first.pre, first.lo, last.hi};
+        r.tiles = kv_tiles(r.all, kTile);
+        // a sequence that sees none of its own keys still has rows to write
+        if (r.tiles.count == 0) r.tiles = KvTiles{1, 0, 1};
+    }
+    return r;
+}
+
+// Where a stretch of the line begins: sequence, head and tile of position `at`, found by the
+// CTA together; *total: tiles of the line.  Returns false when the line ends before `at`.
+struct Place {
+    int32_t s, h, t;
+    int64_t begin;  // the unit's first tile on the line
+};
+
+template <typename F>
+__device__ __forceinline__ int64_t line_total(const KvAttendParams& p, int64_t* mine, F count) {
+    __shared__ int64_t s_warp[kWarps];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int per = (p.batch.seqs + kThreads - 1) / kThreads;
+    int64_t sum = 0;
+    for (int s = t * per; s < min((t + 1) * per, p.batch.seqs); ++s) sum += count(s);
+    int64_t incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    __syncthreads();
+    if (lane == 31) s_warp[warp] = incl;
+    __syncthreads();
+    int64_t before = 0, total = 0;
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += s_warp[w];
+        total += s_warp[w];
+    }
+    *mine = before + incl - sum;
+    return total;
+}
+
+__device__ __forceinline__ void find_place(const KvAttendParams& p, int64_t mine, int64_t at, Place* out) {
+    const int per = (p.batch.seqs + kThreads - 1) / kThreads;
+    const int t = threadIdx.x;
+    int64_t run = mine;
+    for (int s = t * per; s < min((t + 1) * per, p.batch.seqs); ++s) {
+        const int32_t n = few_seq(p, s).tiles.count;
+        const int64_t here = static_cast<int64_t>(n) * p.cache.heads;
+        if (n > 0 && at >= run && at < run + here) {
+            out->s = s;
+            out->h = static_cast<int32_t>((at - run) / n);
+            out->t = static_cast<int32_t>((at - run) % n);
+            out->begin = run + static_cast<int64_t>(out->h) * n;
+        }
+        run += here;
+    }
+}
+
+// Walks the units of a stretch.
+struct Cursor {
+    Seq q;
+    int32_t s, h, t, end;  // tiles [t, end) of the unit lie in the stretch
+    int64_t left;          // tiles of the stretch behind `end`
+    bool done;
+
+    __device__ __forceinline__ void enter(const KvAttendParams& p, int32_t s_, int32_t h_, int32_t t_, int64_t left_) {
+        s = s_;
+        h = h_;
+        t = t_;
+        q = few_seq(p, s);
+        clamp(left_);
+    }
+    __device__ __forceinline__ void clamp(int64_t l) {
+        done = l <= 0;
+        end = static_cast<int32_t>(min(static_cast<int64_t>(q.tiles.count), t + l));
+        left = l - (end - t);
+    }
+    __device__ __forceinline__ void next_unit(const KvAttendParams& p) {
+        if (left <= 0) {
+            done = true;
+            return;
+        }
+        t = 0;
+        if (++h == p.cache.heads) {
+            h = 0;
+            do {
+                q = few_seq(p, ++s);
+            } while (q.tiles.count == 0);
+        }
+        clamp(left);
+    }
+};
+
+__device__ __forceinline__ constexpr int few_slot_floats(int d) { return kRows * d + 2 * kRows; }
+
+template <typename T>
+__device__ __forceinline__ void store_out(const KvAttendParams& p, int64_t row, int head, int d0, const float* v, int n) {
+    char* at = p.out.data + row * p.out.row_stride + head * p.out.head_stride;
+    if (p.out_f32) {
+        float* o = reinterpret_cast<float*>(at) + d0;
+        for (int i = 0; i < n; i += 4) *reinterpret_cast<float4*>(o + i) = *reinterpret_cast<const float4*>(v + i);
+    } else {
+        uint32_t* o = reinterpret_cast<uint32_t*>(at + 2 * d0);
+        for (int i = 0; i < n; i += 4)
+            *reinterpret_cast<uint2*>(o + i / 2) = make_uint2(Pack<T>::pair(v[i], v[i + 1]), Pack<T>::pair(v[i + 2], v[i + 3]));
+    }
+}
+
+// Score in base 2: scale and cap of the product, bias by distance.
+template <bool kPlain>
+__device__ __forceinline__ float score2(const KvAttendParams& p, float dot, float slope, int32_t dist) {
+    if (kPlain) return dot * p.scale2;
+    float z = dot * p.scale;
+    if (p.softcap > 0.0f) {
+        // tanh x = 1 - 2 / (1 + e^2x), to about 2^-21 of the cap
+        const float e = fast_exp2(z * p.cap_rate);
+        z = p.softcap - p.softcap * __fdividef(2.0f, 1.0f + e);
+        if (e == INFINITY) z = p.softcap;
+    }
+    return (z + slope * static_cast<float>(dist)) * kLog2e;
+}
+
+// The sum of one packed row over the keys of tiles [t0, t1) of a unit, key by key and only where
+// the row sees them; for rows whose sum by matrix products met a NaN or an infinity, which a
+// key that other rows see may have put there (0 * inf).  m: the row's maximum in base 2.
+template <typename T, int D, bool kPlain>
+__device__ __noinline__ void exact_row(const KvAttendParams& p, const Seq& q, int s, int h, int t0, int t1, int r, float m,
+                                       float* acc_out, float* room) {
+    float* s_w = room;
+    const char** s_v = reinterpret_cast<const char**>(room + kThreads);
+    const int t = threadIdx.x;
+    const int i = r / p.group, g = r % p.group;
+    const int32_t n = p.shared_len + q.q.keys, pos = n - q.q.rows + i;
+    const int prefix = p.prefix_len != nullptr ? p.prefix_len[s] : 0;
+    const KvSpan sp = kv_clip(kv_span(pos, n, prefix, p.window, p.causal != 0), p.shared_len, q.q.keys);
+    const int head = h * p.group + g;
+    const char* qrow = p.q.data + (q.q.row0 + i) * p.q.row_stride + head * p.q.head_stride;
+    const float slope = !kPlain && p.alibi != nullptr ? p.alibi[head] : 0.0f;
+    float acc = 0.0f;
+    for (int c = t0 * kTile; c < t1 * kTile; c += kThreads) {
+        const int ti = (c + t) / kTile;
+        const int32_t j = ti < t1 ? q.tiles.at(ti) * kTile + (c + t) % kTile : 0x7fffffff;
+        const char* v = nullptr;
+        float w = 0.0f;
+        if (j < sp.pre || (j >= sp.lo && j < sp.hi)) {
+            const int32_t id = p.batch.table[s * p.batch.table_stride + j / p.cache.block_tokens];
+            if (id >= 0 && id < p.cache.blocks) {
+                const int64_t at = id * p.cache.block_stride + j % p.cache.block_tokens * p.cache.token_stride + h * p.cache.head_stride;
+                float dot = 0.0f;
+                for (int e = 0; e < D; e += 8) {
+                    float a[8], b[8];
+                    Pack<T>::load(p.cache.k + at + 2 * e, a);
+                    Pack<T>::load(qrow + 2 * e, b);
+                    for (int x = 0; x < 8; ++x) dot = fmaf(a[x], b[x], dot);
+                }
+                const float z = score2<kPlain>(p, dot, slope, p.shared_len + j - pos);
+                w = z == -INFINITY ? 0.0f : fast_exp2(z - m);
+                v = p.cache.v + at;
+            }
+        }
+        __syncthreads();
+        s_w[t] = w;
+        s_v[t] = v;
+        __syncthreads();
+        if (t < D)
+            for (int x = 0; x < kThreads; ++x)
+                if (s_v[x] != nullptr && s_w[x] != 0.0f) acc = fmaf(s_w[x], static_cast<float>(reinterpret_cast<const T*>(s_v[x])[t]), acc);
+    }
+    __syncthreads();
+    if (t < D) acc_out[t] = acc;
+    __syncthreads();
+}
+
+template <int D>
+struct Shape {
+    static constexpr int kStages = D == 128 ? 3 : 6;
+    static constexpr int kRow = 2 * D;               // bytes of a key
+    static constexpr int kStage = 2 * kKvPage * kRow;  // K and V of 16 keys
+    static constexpr int kRing = kStages * kStage;
+    static constexpr int kJoin = kWarps * 8 * D * 4;  // 8 rows of every warp
+    static constexpr int kSmem = kWarps * kRing + kJoin;
+};
+
+template <typename T, int D, bool kPlain>
+__global__ void __launch_bounds__(kThreads) kv_decode_kernel(const KvAttendParams p) {
+    using S = Shape<D>;
+    constexpr int kSteps = D / 16;   // k-steps of the scores, pairs of n-tiles of the sums
+    constexpr int kChunks = D / 8;   // 16-byte pieces of a key
+    extern __shared__ __align__(128) char smem[];
+    __shared__ Place s_place;
+    __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
+    __shared__ uint32_t s_odd;
+    float* s_join = reinterpret_cast<float*>(smem + kWarps * S::kRing);
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const KvBatchView& b = p.batch;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (!kv_starts_ok(b)) {
+        if (blockIdx.x == 0 && t == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
+        return;
+    }
+    int64_t mine;
+    const int64_t total = line_total(p, &mine, [&](int s) {
+        const Seq q = few_seq(p, s);
+        if (q.bad && blockIdx.x == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
+        return static_cast<int64_t>(q.tiles.count) * p.cache.heads;
+    });
+    const int64_t at = kv_cut(total, blockIdx.x, gridDim.x), to = kv_cut(total, blockIdx.x + 1, gridDim.x);
+    if (at >= to) return;
+    find_place(p, mine, at, &s_place);
+    __syncthreads();
+
+    Cursor load, use;
+    load.enter(p, s_place.s, s_place.h, s_place.t, to - at);
+    use = load;
+
+    // ---- stages ----
+    const uint32_t ring = smem_addr(smem) + warp * S::kRing;
+    const int pages = p.cache.block_tokens / kKvPage;
+    int32_t ids = -1;       // lane i: block id of tile ids_from + i
+    int32_t ids_from = 0;
+    bool ids_ok = false;
+    uint32_t live = 0;      // bit i: the stage issued i stages ago holds keys
+    int put = 0;
+    auto issue = [&]() {
+        live <<= 1;
+        if (!load.done) {
+            const KvSpan& a = load.q.all;
+            if (!ids_ok || load.t >= ids_from + 32) {
+                ids_from = load.t;
+                ids_ok = true;
+                const int32_t i = ids_from + lane;
+                ids = -1;
+                if (i < load.end) {
+                    const int32_t j = load.q.tiles.at(i) * kTile + warp * kKvPage;
+                    if (j < a.pre || (j + kKvPage > a.lo && j < a.hi)) {
+                        ids = b.table[load.s * b.table_stride + j / kKvPage / pages];
+                        if (ids < 0 || ids >= p.cache.blocks) {
+                            kv_report(p.status, GFD_KV_BAD_PAGE);
+                            ids = -1;
+                        }
+                    }
+                }
+            }
+            const int32_t id = __shfl_sync(0xffffffffu, ids, load.t - ids_from);
+            if (id >= 0) {
+                live |= 1u;
+                const int32_t j = load.q.tiles.at(load.t) * kTile + warp * kKvPage;
+                const int32_t place = (j / kKvPage % pages) * kKvPage;
+                const int64_t base = id * p.cache.block_stride + place * p.cache.token_stride + load.h * p.cache.head_stride;
+                const uint32_t dst = ring + put * S::kStage;
+#pragma unroll
+                for (int i = 0; i < kKvPage * kChunks / 32; ++i) {
+                    const int r = (i * 32 + lane) / kChunks, c = lane % kChunks;
+                    const int64_t off = base + r * p.cache.token_stride + 16 * c;
+                    // keys no row sees stay zero, so that what lies there cannot reach a sum
+                    const bool take = j + r < a.pre || (j + r >= a.lo && j + r < a.hi);
+                    const uint32_t o = r * S::kRow + ((c ^ (r & 7)) << 4);
+                    copy16(dst + o, p.cache.k + off, take);
+                    copy16(dst + kKvPage * S::kRow + o, p.cache.v + off, take);
+                }
+            }
+            if (++load.t == load.end) {
+                load.next_unit(p);
+                ids_ok = false;
+            }
+        }
+        copy_commit();
+        put = put + 1 == S::kStages ? 0 : put + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < S::kStages - 1; ++i) issue();
+
+    // ---- units ----
+    int get = 0;
+    const int row_a = lane >> 2;  // this thread's rows: row_a and row_a + 8
+    while (!use.done) {
+        const int32_t rows = use.q.q.rows * p.group;
+        const int32_t n = p.shared_len + use.q.q.keys;
+        uint32_t qf[kSteps][4];
+        KvSpan sp[2];
+        int32_t pos[2];
+        float slope[2] = {0.0f, 0.0f};
+        const int prefix = p.prefix_len != nullptr ? p.prefix_len[use.s] : 0;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int r = row_a + 8 * x;
+            const int i = r / p.group, head = use.h * p.group + r % p.group;
+            pos[x] = n - use.q.q.rows + i;
+            sp[x] = KvSpan{0, 0, 0};
+            if (r < rows) {
+                sp[x] = kv_clip(kv_span(pos[x], n, prefix, p.window, p.causal != 0), p.shared_len, use.q.q.keys);
+                if (!kPlain && p.alibi != nullptr) slope[x] = p.alibi[head];
+            }
+            const char* src = p.q.data + (use.q.q.row0 + i) * p.q.row_stride + head * p.q.head_stride + 4 * (lane & 3);
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                qf[k][x] = r < rows ? *reinterpret_cast<const uint32_t*>(src + 32 * k) : 0u;
+                qf[k][2 + x] = r < rows ? *reinterpret_cast<const uint32_t*>(src + 32 * k + 16) : 0u;
+            }
+        }
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        float acc[2 * kSteps][4];
+#pragma unroll
+        for (int i = 0; i < 2 * kSteps; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][e] = 0.0f;
+        const int32_t t0 = use.t;
+
+        for (; use.t < use.end; ++use.t) {
+            issue();
+            copy_wait<S::kStages - 1>();
+            __syncwarp();
+            if ((live >> (S::kStages - 1)) & 1u) {
+                const uint32_t kb = ring + get * S::kStage, vb = kb + kKvPage * S::kRow;
+                float z[2][4] = {};
+                const int row = (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    uint32_t f[4];
+                    const int c = 2 * k + ((lane >> 3) & 1);
+                    ldsm4(f, kb + row * S::kRow + ((c ^ (row & 7)) << 4));
+                    mma<T>(z[0], qf[k], f[0], f[1]);
+                    mma<T>(z[1], qf[k], f[2], f[3]);
+                }
+                const int32_t j0 = use.q.tiles.at(use.t) * kTile + warp * kKvPage + 2 * (lane & 3);
+                float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int x = e >> 1;
+                        const int32_t j = j0 + 8 * nt + (e & 1);
+                        const bool seen = j < sp[x].pre || (j >= sp[x].lo && j < sp[x].hi);
+                        const float v = score2<kPlain>(p, z[nt][e], slope[x], p.shared_len + j - pos[x]);
+                        z[nt][e] = seen ? v : -INFINITY;
+                        mx[x] = fmaxf(mx[x], z[nt][e]);
+                    }
+                float base[2];
+                bool grew = false;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
+                    mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
+                    grew |= mx[x] > m[x];
+                    mx[x] = fmaxf(mx[x], m[x]);
+                    base[x] = mx[x] == -INFINITY ? 0.0f : mx[x];
+                }
+                if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float keep = fast_exp2(m[x] - base[x]);
+                        m[x] = mx[x];
+                        l[x] *= keep;
+#pragma unroll
+                        for (int i = 0; i < 2 * kSteps; ++i) {
+                            acc[i][2 * x] *= keep;
+                            acc[i][2 * x + 1] *= keep;
+                        }
+                    }
+                }
+                // weights: summed in 32 bits, rounded to the cache's type for the product with V
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        z[nt][e] = fast_exp2(z[nt][e] - base[e >> 1]);
+                        l[e >> 1] += z[nt][e];
+                    }
+                const uint32_t pf[4] = {Pack<T>::pair(z[0][0], z[0][1]), Pack<T>::pair(z[0][2], z[0][3]),
+                                        Pack<T>::pair(z[1][0], z[1][1]), Pack<T>::pair(z[1][2], z[1][3])};
+                const int vrow = (lane & 7) + (((lane >> 3) & 1) << 3);
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    uint32_t f[4];
+                    const int c = 2 * i + (lane >> 4);
+                    ldsm4t(f, vb + vrow * S::kRow + ((c ^ (vrow & 7)) << 4));
+                    mma<T>(acc[2 * i], pf, f[0], f[1]);
+                    mma<T>(acc[2 * i + 1], pf, f[2], f[3]);
+                }
+            }
+            __syncwarp();
+            get = get + 1 == S::kStages ? 0 : get + 1;
+        }
+
+        // ---- the warps join ----
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+            l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+            if ((lane & 3) == 0) {
+                s_m[warp][row_a + 8 * x] = m[x];
+                s_l[warp][row_a + 8 * x] = l[x];
+            }
+        }
+        const bool whole = t0 == 0 && use.end == use.q.tiles.count;
+        float* slot = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0)) * few_slot_floats(D);
+        for (int half = 0; half < 2 && 8 * half < rows; ++half) {
+            if (t == 0) s_odd = 0;
+            __syncthreads();
+            const int r = row_a + 8 * half;
+            const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+            const float keep = m[half] == -INFINITY ? 0.0f : fast_exp2(m[half] - top);
+            float* w = s_join + (warp * 8 + row_a) * D + 2 * (lane & 3);
+#pragma unroll
+            for (int i = 0; i < 2 * kSteps; ++i)
+                *reinterpret_cast<float2*>(w + 8 * i) = make_float2(acc[i][2 * half] * keep, acc[i][2 * half + 1] * keep);
+            __syncthreads();
+            // 16 threads a row, D / 16 elements each
+            constexpr int kEach = D / 16;
+            const int jr = t >> 4, d0 = (t & 15) * kEach, rr = jr + 8 * half;
+            float sum[kEach] = {}, ml = 0.0f, mt = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < kWarps; ++x) mt = fmaxf(mt, s_m[x][rr]);
+#pragma unroll
+            for (int x = 0; x < kWarps; ++x) {
+                if (s_m[x][rr] != -INFINITY) ml += s_l[x][rr] * fast_exp2(s_m[x][rr] - mt);
+                else ml += s_l[x][rr];  // 0, or NaN from scores that are NaN
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) sum[e] += s_join[(x * 8 + jr) * D + d0 + e];
+            }
+            bool odd = false;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) odd |= !(fabsf(sum[e]) < INFINITY);
+            if (odd && rr < rows) atomicOr(&s_odd, 1u << jr);
+            __syncthreads();
+            const uint32_t redo = s_odd;
+            for (int x = 0; x < 8; ++x)
+                if ((redo >> x) & 1u) {
+                    float mm = -INFINITY;
+                    for (int y = 0; y < kWarps; ++y) mm = fmaxf(mm, s_m[y][x + 8 * half]);
+                    exact_row<T, D, kPlain>(p, use.q, use.s, use.h, t0, use.end, x + 8 * half, mm, s_join + x * D,
+                                             s_join + 8 * D);
+                }
+            if ((redo >> jr) & 1u)
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) sum[e] = s_join[jr * D + d0 + e];
+            if (rr < rows) {
+                if (whole) {
+                    const int64_t row = use.q.q.row0 + rr / p.group;
+                    const int head = use.h * p.group + rr % p.group;
+                    const float inv = ml == 0.0f ? 0.0f : 1.0f / ml;
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e) sum[e] = ml == 0.0f ? 0.0f : sum[e] * inv;
+                    store_out<T>(p, row, head, d0, sum, kEach);
+                    if (p.lse != nullptr && d0 == 0)
+                        p.lse[row * p.q_heads + head] = ml == 0.0f ? -INFINITY : mt * kLn2 + logf(ml);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kEach; e += 4)
+                        *reinterpret_cast<float4*>(slot + rr * D + d0 + e) = *reinterpret_cast<float4*>(sum + e);
+                    if (d0 == 0) {
+                        slot[kRows * D + rr] = mt;
+                        slot[kRows * D + kRows + rr] = ml;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        use.next_unit(p);
+    }
+    copy_wait<0>();
+}
+
+// One CTA per cut of the line: the unit whose first cut it is.  Each thread sums 4 elements of
+// a packed row over the unit's parts, in their order.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) kv_decode_join_kernel(const KvAttendParams p) {
+    __shared__ Place s_place;
+    const int t = threadIdx.x;
+    const int c = blockIdx.x + 1, n = gridDim.x + 1;  // cuts 1 .. n - 1 of n CTAs
+    int64_t mine = 0, total = 0, cut = 0;
+    const bool ok = kv_starts_ok(p.batch);
+    if (ok) {
+        total = line_total(p, &mine, [&](int s) { return static_cast<int64_t>(few_seq(p, s).tiles.count) * p.cache.heads; });
+        cut = kv_cut(total, c, n);
+        if (cut < total) find_place(p, mine, cut, &s_place);
+        __syncthreads();
+    }
+    // every CTA waits for the attention kernel, so that this grid never ends before it
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!ok || cut >= total) return;
+    const Place u = s_place;
+    // a cut between two units joins nothing; of several inside a unit the first does
+    if (u.t == 0 || kv_cut(total, c - 1, n) > u.begin) return;
+    const Seq q = few_seq(p, u.s);
+    const int64_t end = u.begin + q.tiles.count;
+    int last = c;  // parts: CTA c - 1 (slot 1), c .. last (slot 0)
+    while (last + 1 < n && kv_cut(total, last + 1, n) < end) ++last;
+    for (int i = t; i < q.q.rows * p.group * (D / 4); i += kThreads) {
+        const int r = i / (D / 4), d0 = i % (D / 4) * 4;
+        float m = -INFINITY;
+        for (int x = c - 1; x <= last; ++x) {
+            if (x >= c && kv_cut(total, x, n) == kv_cut(total, x + 1, n)) continue;
+            m = fmaxf(m, p.partial[(2 * static_cast<int64_t>(x) + (x < c ? 1 : 0)) * few_slot_floats(D) + kRows * D + r]);
+        }
+        float sum[4] = {}, l = 0.0f;
+        for (int x = c - 1; x <= last; ++x) {
+            if (x >= c && kv_cut(total, x, n) == kv_cut(total, x + 1, n)) continue;
+            const float* slot = p.partial + (2 * static_cast<int64_t>(x) + (x < c ? 1 : 0)) * few_slot_floats(D);
+            const float pm = slot[kRows * D + r], pl = slot[kRows * D + kRows + r];
+            const float w = pm == -INFINITY ? 0.0f : fast_exp2(pm - m);
+            l += pm == -INFINITY ? pl : pl * w;  // -inf: 0, or NaN from scores that are NaN
+            const float4 v = *reinterpret_cast<const float4*>(slot + r * D + d0);
+            if (w != 0.0f) {
+                sum[0] = fmaf(v.x, w, sum[0]);
+                sum[1] = fmaf(v.y, w, sum[1]);
+                sum[2] = fmaf(v.z, w, sum[2]);
+                sum[3] = fmaf(v.w, w, sum[3]);
+            }
+        }
+        const int64_t row = q.q.row0 + r / p.group;
+        const int head = u.h * p.group + r % p.group;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = l == 0.0f ? 0.0f : sum[e] * inv;
+        store_out<T>(p, row, head, d0, sum, 4);
+        if (p.lse != nullptr && d0 == 0) p.lse[row * p.q_heads + head] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
+    }
+}
+
+template <typename T, int D>
+cudaError_t launch(const KvAttendParams& p, int ctas, cudaStream_t st) {
+    const bool plain = p.softcap == 0.0f && p.alibi == nullptr;
+    auto* k = plain ? kv_decode_kernel<T, D, true> : kv_decode_kernel<T, D, false>;
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
+    if (e != cudaSuccess) return e;
+    k<<<ctas, kThreads, Shape<D>::kSmem, st>>>(p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas - 1);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kv_decode_join_kernel<T, D>, p);
+}
+
+}  // namespace
+
+int kv_decode_ctas(int num_sms) { return 2 * num_sms; }
+
+size_t kv_decode_workspace(int num_sms, int head_dim) {
+    return static_cast<size_t>(kv_decode_ctas(num_sms)) * 2 * (kRows * head_dim + 2 * kRows) * sizeof(float);
+}
+
+cudaError_t launch_kv_decode(const KvAttendParams& p, int head_dim, int dtype, int num_sms, cudaStream_t st) {
+    const int ctas = kv_decode_ctas(num_sms);
+    if (dtype == GFD_BF16) return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, ctas, st) : launch<__nv_bfloat16, 128>(p, ctas, st);
+    return head_dim == 64 ? launch<__half, 64>(p, ctas, st) : launch<__half, 128>(p, ctas, st);
+}
+
+}  // namespace gfdb

@@ -14,6 +14,13 @@ namespace gfdb {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// 2^x by the hardware instruction: within 2^-22 of the value, results below 2^-126 are 0
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 template <typename T>
 struct Pack;  // 8 elements of T <-> 8 floats, and rounding to nearest even
 template <>

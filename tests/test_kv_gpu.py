@@ -427,7 +427,7 @@ def test_shared_equals_tables_that_name_it(gpu_ctx):
     t = torch.cat([s.shared_table[None].expand(3, n), s.table], 1).contiguous()
     whole = kv.Batch(s.starts, (s.lens + 160).int(), t)
     b, lb = torch.empty_like(a), torch.empty_like(la)
-    ws = s.workspace(2)
+    ws = torch.empty(max(16, s.cache.workspace_bytes(s.rows, s.hq, 3, 2)), dtype=torch.uint8, device="cuda")
     s.cache.attend(whole, s.q, b, lse=lb, max_q_len=2, workspace=ws, stream=torch.cuda.current_stream())
     torch.cuda.synchronize()
     want = s.want()
