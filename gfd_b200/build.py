@@ -39,6 +39,7 @@ SOURCES = [
     "moe.cu",
     "kv.cu",
     "kv_decode.cu",
+    "kv_prompt.cu",
     "kv_api.cpp",
     "ring.cu",
     "agent.cu",

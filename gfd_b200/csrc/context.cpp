@@ -120,6 +120,7 @@ const Driver& driver() {
         resolve("cuDevicePrimaryCtxRelease", &d.primary_release);
         resolve("cuPointerGetAttributes", &d.ptr_attrs);
         resolve("cuCtxGetId", &d.ctx_get_id);  // optional (CUDA 12.0+)
+        resolve("cuTensorMapEncodeTiled", &d.tensor_map);
         d.ok = d.ctx_get_current && d.ctx_set_current && d.ctx_push && d.ctx_pop && d.device_get &&
                d.primary_retain && d.primary_release && d.ptr_attrs;
     });

@@ -277,6 +277,9 @@ struct Driver {
     CUresult (*primary_release)(CUdevice) = nullptr;
     CUresult (*ptr_attrs)(unsigned int, CUpointer_attribute*, void**, CUdeviceptr) = nullptr;
     CUresult (*ctx_get_id)(CUcontext, unsigned long long*) = nullptr;  // may be null (older drivers)
+    CUresult (*tensor_map)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                           const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                           CUtensorMapFloatOOBfill) = nullptr;  // kv_prompt's loads
     bool ok = false;
 };
 const Driver& driver();

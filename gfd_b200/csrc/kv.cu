@@ -1,5 +1,5 @@
-// Paged KV-cache operators: append with rotation, merge of partial results, and the
-// plain attention kernel (one CTA per row and head).
+// Paged KV-cache operators: append with rotation, merge of partial results, and the join of an
+// attention launch's own partial results.
 
 #include "kv_device.cuh"
 
@@ -131,106 +131,6 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvAppen
 }
 
 // ---------------------------------------------------------------------------
-// Attention, plain: one CTA per (row, query head), one thread per key for the scores and
-// one per element for the sums; running maximum and sum in 32 bits.
-// ---------------------------------------------------------------------------
-constexpr int kPlainThreads = 128;
-
-template <typename T, typename O, int D>
-__global__ void __launch_bounds__(kPlainThreads) kv_attend_plain_kernel(const KvAttendParams p) {
-    __shared__ float s_q[D];
-    __shared__ float s_p[kPlainThreads];
-    __shared__ const char* s_v[kPlainThreads];
-    __shared__ float s_red[4];
-    const KvBatchView& b = p.batch;
-    const int t = threadIdx.x;
-    if (!kv_starts_ok(b)) {
-        if (blockIdx.x == 0 && blockIdx.y == 0 && t == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
-        return;
-    }
-    for (int64_t u = blockIdx.x; u < static_cast<int64_t>(b.seqs) * p.q_heads; u += gridDim.x) {
-        const int s = static_cast<int>(u / p.q_heads), h = static_cast<int>(u % p.q_heads);
-        const KvSeq q = kv_seq(b.row_start[s], b.row_start[s + 1], b.kv_len[s], b.capacity, p.max_q_len);
-        if (!q.ok) {
-            if (t == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
-            continue;
-        }
-        if (p.skip_few && q.rows * p.group <= kKvFewRows) continue;
-        const int32_t n = p.shared_len + q.keys;
-        const int kvh = h / p.group;
-        const float slope = p.alibi != nullptr ? p.alibi[h] : 0.0f;
-        for (int i = blockIdx.y; i < q.rows; i += gridDim.y) {
-            const int64_t row = q.row0 + i;
-            const int32_t pos = n - q.rows + i;
-            const KvSpan sp = kv_span(pos, n, p.prefix_len != nullptr ? p.prefix_len[s] : 0, p.window, p.causal != 0);
-            __syncthreads();
-            if (t < D / 8) {
-                float f[8];
-                Pack<T>::load(p.q.data + row * p.q.row_stride + h * p.q.head_stride + 16 * t, f);
-                for (int e = 0; e < 8; ++e) s_q[8 * t + e] = f[e];
-            }
-            __syncthreads();
-            float m = -INFINITY, l = 0.0f, acc = 0.0f;
-            const int32_t seen = sp.pre + (sp.hi - sp.lo);
-            for (int32_t j0 = 0; j0 < seen; j0 += kPlainThreads) {
-                const int32_t c = j0 + t;
-                float z = -INFINITY;
-                const char* v = nullptr;
-                if (c < seen) {
-                    const int32_t j = c < sp.pre ? c : c - sp.pre + sp.lo;
-                    int32_t place;
-                    const int32_t block = kv_block(b, s, j, p.cache.block_tokens, p.shared_table, p.shared_len, &place);
-                    if (block >= 0 && block < p.cache.blocks) {
-                        const int64_t at = block * p.cache.block_stride + place * p.cache.token_stride + kvh * p.cache.head_stride;
-                        v = p.cache.v + at;
-                        float dot = 0.0f;
-                        for (int e = 0; e < D; e += 8) {
-                            float f[8];
-                            Pack<T>::load(p.cache.k + at + 2 * e, f);
-                            for (int x = 0; x < 8; ++x) dot = fmaf(f[x], s_q[e + x], dot);
-                        }
-                        z = dot * p.scale;
-                        if (p.softcap > 0.0f) z = p.softcap * tanhf(z / p.softcap);
-                        z += slope * static_cast<float>(j - pos);
-                    } else {
-                        kv_report(p.status, GFD_KV_BAD_PAGE);
-                    }
-                }
-                float mx = z;
-                for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                if ((t & 31) == 0) s_red[t >> 5] = mx;
-                __syncthreads();
-                mx = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-                const float mn = fmaxf(m, mx);
-                const float keep = mn == -INFINITY ? 1.0f : __expf(m - mn);
-                const float e = v == nullptr || z == -INFINITY ? 0.0f : expf(z - mn);
-                s_p[t] = e;
-                s_v[t] = v;
-                float sum = e;
-                for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                __syncthreads();
-                if ((t & 31) == 0) s_red[t >> 5] = sum;
-                __syncthreads();
-                l = l * keep + ((s_red[0] + s_red[1]) + (s_red[2] + s_red[3]));
-                m = mn;
-                if (t < D) {
-                    acc *= keep;
-                    for (int x = 0; x < kPlainThreads; ++x)
-                        if (s_v[x] != nullptr && s_p[x] != 0.0f)
-                            acc = fmaf(s_p[x], static_cast<float>(reinterpret_cast<const T*>(s_v[x])[t]), acc);
-                }
-                __syncthreads();
-            }
-            const bool none = m == -INFINITY && l == 0.0f;
-            if (t < D)
-                reinterpret_cast<O*>(p.out.data + row * p.out.row_stride + h * p.out.head_stride)[t] =
-                    static_cast<O>(none ? 0.0f : acc / l);
-            if (t == 0 && p.lse != nullptr) p.lse[row * p.q_heads + h] = none ? -INFINITY : m + logf(l);
-        }
-    }
-}
-
-// ---------------------------------------------------------------------------
 // Merge: one group of D / 8 threads per (row, head), 8 elements a thread
 // ---------------------------------------------------------------------------
 constexpr int kMergeThreads = 256;
@@ -243,6 +143,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const KvMergePa
     const int64_t step = static_cast<int64_t>(gridDim.x) * (kMergeThreads / kLanes);
     for (int64_t u = blockIdx.x * static_cast<int64_t>(kMergeThreads / kLanes) + threadIdx.x / kLanes; u < n; u += step) {
         const int64_t row = u / p.heads, h = u % p.heads;
+        if (p.last_marks && __float_as_uint(p.part_lse[(p.part_count - 1) * n + u]) == kKvUnwritten) continue;
         float m = -INFINITY;
         for (int i = 0; i < p.part_count; ++i) m = fmaxf(m, p.part_lse[i * n + u]);
         const float base = m == -INFINITY ? 0.0f : m;
@@ -263,6 +164,58 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const KvMergePa
         for (int e = 0; e < 8; ++e) acc[e] = total == 0.0f ? 0.0f : acc[e] * inv;
         Pack<O>::store(p.out.data + row * p.out.row_stride + h * p.out.head_stride + lane * 8 * sizeof(O), acc);
         if (lane == 0 && p.lse != nullptr) p.lse[u] = total == 0.0f ? -INFINITY : base + logf(total);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Join of an attention launch's partial results: CTAs (c - 1, *) for cut c of the line.  Each
+// thread sums 4 elements of a packed row over the unit's parts, in their order.
+// ---------------------------------------------------------------------------
+constexpr int kJoinThreads = 128;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendParams p, int slot_rows) {
+    const int c = blockIdx.x + 1, n = gridDim.x + 1;  // cuts 1 .. n - 1 of n CTAs
+    // every CTA waits for the attention kernel, so that this grid never ends before it
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const KvPlace u = p.line.places[c];
+    const int64_t total = u.total, cut = kv_cut(total, c, n);
+    // a cut between two units joins nothing; of several inside a unit the first does
+    if (cut >= total || u.t == 0 || kv_cut(total, c - 1, n) > u.begin) return;
+    const int64_t end = u.begin + u.count;
+    int last = c;  // parts: CTA c - 1 (slot 1), c .. last (slot 0)
+    while (last + 1 < n && kv_cut(total, last + 1, n) < end) ++last;
+    const int64_t size = static_cast<int64_t>(slot_rows) * (D + 2);
+    for (int i = blockIdx.y * kJoinThreads + threadIdx.x; i < u.packed * (D / 4); i += kJoinThreads * gridDim.y) {
+        const int r = i / (D / 4), d0 = i % (D / 4) * 4;
+        float m = -INFINITY;
+        for (int x = c - 1; x <= last; ++x) {
+            if (x >= c && kv_cut(total, x, n) == kv_cut(total, x + 1, n)) continue;  // no stretch
+            m = fmaxf(m, p.line.slots[(2 * static_cast<int64_t>(x) + (x < c ? 1 : 0)) * size + slot_rows * D + r]);
+        }
+        float sum[4] = {}, l = 0.0f;
+        for (int x = c - 1; x <= last; ++x) {
+            if (x >= c && kv_cut(total, x, n) == kv_cut(total, x + 1, n)) continue;
+            const float* slot = p.line.slots + (2 * static_cast<int64_t>(x) + (x < c ? 1 : 0)) * size;
+            const float pm = slot[slot_rows * D + r], pl = slot[slot_rows * D + slot_rows + r];
+            const float w = pm == -INFINITY ? 0.0f : fast_exp2(pm - m);
+            l += pm == -INFINITY ? pl : pl * w;  // -inf: 0, or NaN from scores that are NaN
+            const float4 v = *reinterpret_cast<const float4*>(slot + r * D + d0);
+            if (w != 0.0f) {
+                sum[0] = fmaf(v.x, w, sum[0]);
+                sum[1] = fmaf(v.y, w, sum[1]);
+                sum[2] = fmaf(v.z, w, sum[2]);
+                sum[3] = fmaf(v.w, w, sum[3]);
+            }
+        }
+        const int packed = u.packed0 + r;
+        const int64_t row = u.row0 + packed / p.group;
+        const int head = u.h * p.group + packed % p.group;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = l == 0.0f ? 0.0f : sum[e] * inv;
+        kv_store_out<T>(p, row, head, d0, sum, 4);
+        if (p.lse != nullptr && d0 == 0) p.lse[row * p.q_heads + head] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
     }
 }
 
@@ -288,22 +241,21 @@ cudaError_t launch_kv_append(const KvAppendParams& p, int head_dim, int dtype, i
     return cudaGetLastError();
 }
 
-template <typename T, typename O>
-static cudaError_t attend_plain(const KvAttendParams& p, int head_dim, dim3 grid, cudaStream_t st) {
-    if (head_dim == 64) kv_attend_plain_kernel<T, O, 64><<<grid, kPlainThreads, 0, st>>>(p);
-    else kv_attend_plain_kernel<T, O, 128><<<grid, kPlainThreads, 0, st>>>(p);
-    return cudaGetLastError();
-}
-
-cudaError_t launch_kv_attend(const KvAttendParams& p, int head_dim, int dtype, int out_dtype, int num_sms, cudaStream_t st) {
-    const int64_t units = static_cast<int64_t>(p.batch.seqs) * p.q_heads;
-    const dim3 grid(static_cast<unsigned>(units < 65535 ? units : 65535), p.batch.rows < 64 ? p.batch.rows : 64);
-    (void)num_sms;
+cudaError_t launch_kv_join(const KvAttendParams& p, int head_dim, int dtype, int ctas, int slot_rows, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas - 1, slot_rows / 16);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     if (dtype == GFD_BF16)
-        return out_dtype == GFD_FP32 ? attend_plain<__nv_bfloat16, float>(p, head_dim, grid, st)
-                                     : attend_plain<__nv_bfloat16, __nv_bfloat16>(p, head_dim, grid, st);
-    return out_dtype == GFD_FP32 ? attend_plain<__half, float>(p, head_dim, grid, st)
-                                 : attend_plain<__half, __half>(p, head_dim, grid, st);
+        return head_dim == 64 ? cudaLaunchKernelEx(&cfg, kv_join_kernel<__nv_bfloat16, 64>, p, slot_rows)
+                              : cudaLaunchKernelEx(&cfg, kv_join_kernel<__nv_bfloat16, 128>, p, slot_rows);
+    return head_dim == 64 ? cudaLaunchKernelEx(&cfg, kv_join_kernel<__half, 64>, p, slot_rows)
+                          : cudaLaunchKernelEx(&cfg, kv_join_kernel<__half, 128>, p, slot_rows);
 }
 
 cudaError_t launch_kv_merge(const KvMergeParams& p, int head_dim, int part_dtype, int out_dtype, int num_sms,

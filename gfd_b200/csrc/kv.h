@@ -1,6 +1,7 @@
 #pragma once
 // Kernel parameters and launchers of the paged KV-cache operators (kv*.cu, kv_api.cpp).
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -41,6 +42,24 @@ struct KvAppendParams {
     int32_t q_heads, rot_dim, interleaved;
 };
 
+// Where a CTA's stretch of the line of tiles begins (kv_cut), left for the joining kernel.
+struct KvPlace {
+    int64_t total;    // tiles of the line
+    int64_t begin;    // the unit's first tile on the line
+    int32_t t, count; // tile t of the unit's `count`
+    int32_t row0;     // first row of its sequence
+    int32_t packed0, packed;  // packed rows [packed0, packed0 + packed) of the sequence
+    int32_t h;        // KV head
+    int32_t s, _pad;
+};
+
+// A launch's places (one per CTA) and partial results (two slots per CTA: [rows][D] sums, then
+// the rows' base and weight sum).
+struct KvLine {
+    KvPlace* places;
+    float* slots;
+};
+
 struct KvAttendParams {
     KvCacheView cache;
     KvBatchView batch;
@@ -57,10 +76,11 @@ struct KvAttendParams {
     float scale2;    // scale in base 2
     float cap_rate;  // 2 log2(e) / softcap
     int32_t out_f32;
-    int32_t skip_few;  // the plain kernel leaves sequences of at most kKvFewRows packed rows out
-    float* partial;    // kv_decode's partial results
+    int32_t shared_pass;  // kv_prompt: all rows against the shared prefix
+    KvLine line;
 };
 
+constexpr int kKvManyRows = 256;  // packed rows of a unit of kv_prompt
 constexpr int kKvFewRows = 16;  // packed rows (rows x group) up to which kv_decode takes a sequence
 
 struct KvMergeParams {
@@ -70,13 +90,29 @@ struct KvMergeParams {
     KvRowsView out;
     float* lse;
     int32_t rows, heads, part_count;
+    int32_t last_marks;  // rows whose last part's lse still holds kKvUnwritten are left alone
 };
+constexpr uint32_t kKvUnwritten = 0xffffffffu;
 
 // dtype: GFD_* of the cache; out: of the output rows
 cudaError_t launch_kv_append(const KvAppendParams& p, int head_dim, int dtype, int num_sms, cudaStream_t st);
-cudaError_t launch_kv_attend(const KvAttendParams& p, int head_dim, int dtype, int out_dtype, int num_sms, cudaStream_t st);
+cudaError_t launch_kv_join(const KvAttendParams& p, int head_dim, int dtype, int ctas, int slot_rows, cudaStream_t st);
+int kv_decode_ctas(int num_sms);
+int kv_prompt_ctas(int num_sms);
+// cuTensorMapEncodeTiled, resolved through the runtime (libcuda is not linked)
+using KvEncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+cudaError_t launch_kv_prompt(const KvAttendParams& p, int head_dim, int dtype, int num_sms, KvEncodeFn encode, cudaStream_t st);
 cudaError_t launch_kv_decode(const KvAttendParams& p, int head_dim, int dtype, int num_sms, cudaStream_t st);
-size_t kv_decode_workspace(int num_sms, int head_dim);
+
+// Bytes of a line's places and slots, and the line laid out in them.
+inline size_t kv_line_bytes(int ctas, int slot_rows, int head_dim) {
+    return (sizeof(KvPlace) * ctas + 255) / 256 * 256 +
+           (static_cast<size_t>(ctas) * 2 * (static_cast<size_t>(slot_rows) * head_dim + 2 * slot_rows) * sizeof(float) + 255) / 256 * 256;
+}
+inline KvLine kv_line_at(void* p, int ctas) {
+    return KvLine{static_cast<KvPlace*>(p), reinterpret_cast<float*>(static_cast<char*>(p) + (sizeof(KvPlace) * ctas + 255) / 256 * 256)};
+}
 cudaError_t launch_kv_merge(const KvMergeParams& p, int head_dim, int part_dtype, int out_dtype, int num_sms,
                             cudaStream_t st);
 

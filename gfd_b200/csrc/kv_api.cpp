@@ -60,9 +60,38 @@ uint64_t table_bytes(const gfd_kv_batch& b) {
     return b.table_width == 0 ? 0 : (static_cast<uint64_t>(b.seqs - 1) * b.table_stride + b.table_width) * sizeof(int32_t);
 }
 
-// Bytes of workspace of an attention call.
-size_t attend_workspace(const gfd_ctx* ctx, const gfd_kv_cache& c, int64_t shared_len) {
-    return shared_len > 0 ? 0 : kv_decode_workspace(ctx->num_sms, c.head_dim);
+// An attention call's kernels and where each keeps its intermediate results in the workspace.
+struct AttendPlan {
+    bool few, many;       // sequences of few / many rows may be among the batch's
+    size_t few_line, many_line, prefix_line;  // offsets of the kernels' lines
+    size_t parts, part_lse;                   // behind a shared prefix: results over it and over the own keys
+    size_t part_elems, bytes;
+};
+
+AttendPlan plan_attend(const gfd_ctx* ctx, const gfd_kv_cache& c, const gfd_kv_batch& b, const gfd_kv_attend_args& a, int64_t shared_len) {
+    AttendPlan r{};
+    if (b.rows <= 0 || b.seqs <= 0 || a.q_heads <= 0) return r;
+    const int64_t group = a.q_heads / c.heads > 0 ? a.q_heads / c.heads : 1;
+    const int64_t most = a.max_q_len > 0 && a.max_q_len < b.rows ? a.max_q_len : b.rows;  // rows of a sequence
+    r.few = group <= kKvFewRows;
+    r.many = most * group > kKvFewRows;
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        const size_t here = at;
+        at += (n + 255) / 256 * 256;
+        return here;
+    };
+    const size_t many_bytes = kv_line_bytes(kv_prompt_ctas(ctx->num_sms), kKvManyRows, c.head_dim);
+    if (r.few) r.few_line = take(kv_line_bytes(kv_decode_ctas(ctx->num_sms), kKvFewRows, c.head_dim));
+    if (r.many) r.many_line = take(many_bytes);
+    if (shared_len > 0) {
+        r.prefix_line = take(many_bytes);
+        r.part_elems = static_cast<size_t>(b.rows) * a.q_heads * c.head_dim;
+        r.parts = take(2 * r.part_elems * sizeof(float));
+        r.part_lse = take(2 * static_cast<size_t>(b.rows) * a.q_heads * sizeof(float));
+    }
+    r.bytes = at;
+    return r;
 }
 
 int append(gfd_ctx* ctx, const gfd_kv_cache* c, const gfd_kv_batch* b, const gfd_kv_append_args* a, void* stream) {
@@ -126,7 +155,8 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
     const bool empty = b->rows == 0 || b->seqs == 0;
     if (!why && !empty) why = kv_check_rows(a->q, b->rows, a->q_heads, c->head_dim, c->dtype, false, &qb);
     if (!why && !empty) why = kv_check_rows(a->out, b->rows, a->q_heads, c->head_dim, a->out_dtype, true, &ob);
-    const size_t need = attend_workspace(ctx, *c, shared_len);
+    const AttendPlan plan = plan_attend(ctx, *c, *b, *a, shared_len);
+    const size_t need = plan.bytes;
     if (!why && !empty && need > 0) {
         if (a->workspace == nullptr || !kv_aligned(a->workspace, 256)) why = "workspace is NULL or not 256-byte aligned";
         else if (a->workspace_bytes < need) why = "workspace is smaller than gfd_kv_attend_workspace says";
@@ -171,15 +201,52 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
     p.scale2 = a->scale * 1.4426950408889634f;
     p.cap_rate = a->softcap > 0.0f ? 2.0f * 1.4426950408889634f / a->softcap : 0.0f;
     p.out_f32 = a->out_dtype == GFD_FP32;
-    p.partial = static_cast<float*>(a->workspace);
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
-    cudaError_t e = cudaSuccess;
-    if (shared_len == 0) {
-        p.skip_few = 1;
-        e = launch_kv_decode(p, c->head_dim, c->dtype, ctx->num_sms, st);
+    char* ws = static_cast<char*>(a->workspace);
+    const KvEncodeFn encode = driver().tensor_map;
+    if ((plan.many || shared_len > 0) && encode == nullptr)
+        return set_error(ctx, GFD_ERR_UNSUPPORTED, "%s: the driver has no cuTensorMapEncodeTiled", call);
+    KvAttendParams own = p;
+    if (shared_len > 0) {
+        // the results over the prefix and over the own keys go to the workspace in 32 bits
+        own.out = KvRowsView{ws + plan.parts + plan.part_elems * sizeof(float), static_cast<int64_t>(a->q_heads) * c->head_dim * 4,
+                             static_cast<int64_t>(c->head_dim) * 4};
+        own.lse = reinterpret_cast<float*>(ws + plan.part_lse) + b->rows * a->q_heads;
+        own.out_f32 = 1;
     }
-    const bool all_few = shared_len == 0 && a->max_q_len > 0 && static_cast<int64_t>(a->max_q_len) * p.group <= kKvFewRows;
-    if (e == cudaSuccess && !all_few) e = launch_kv_attend(p, c->head_dim, c->dtype, a->out_dtype, ctx->num_sms, st);
+    cudaError_t e = cudaSuccess;
+    if (shared_len > 0) {
+        e = cudaMemsetAsync(own.lse, 0xff, static_cast<size_t>(b->rows) * a->q_heads * sizeof(float), st);
+        KvAttendParams pre = own;
+        pre.out.data = ws + plan.parts;
+        pre.lse = reinterpret_cast<float*>(ws + plan.part_lse);
+        pre.shared_pass = 1;
+        pre.line = kv_line_at(ws + plan.prefix_line, kv_prompt_ctas(ctx->num_sms));
+        if (e == cudaSuccess) e = launch_kv_prompt(pre, c->head_dim, c->dtype, ctx->num_sms, encode, st);
+    }
+    if (e == cudaSuccess && plan.many) {
+        own.line = kv_line_at(ws + plan.many_line, kv_prompt_ctas(ctx->num_sms));
+        e = launch_kv_prompt(own, c->head_dim, c->dtype, ctx->num_sms, encode, st);
+    }
+    if (e == cudaSuccess && plan.few) {
+        own.line = kv_line_at(ws + plan.few_line, kv_decode_ctas(ctx->num_sms));
+        e = launch_kv_decode(own, c->head_dim, c->dtype, ctx->num_sms, st);
+    }
+    if (e == cudaSuccess && shared_len > 0) {
+        KvMergeParams m;
+        std::memset(&m, 0, sizeof(m));
+        m.parts = own.out;
+        m.parts.data = ws + plan.parts;
+        m.part_stride = static_cast<int64_t>(plan.part_elems * sizeof(float));
+        m.part_lse = reinterpret_cast<float*>(ws + plan.part_lse);
+        m.out = p.out;
+        m.lse = p.lse;
+        m.rows = p.batch.rows;
+        m.heads = a->q_heads;
+        m.part_count = 2;
+        m.last_marks = 1;
+        e = launch_kv_merge(m, c->head_dim, GFD_FP32, a->out_dtype, ctx->num_sms, st);
+    }
     return e == cudaSuccess ? GFD_OK : cuda_error(ctx, e, "kv_attend: kernel launch");
 }
 
@@ -257,7 +324,7 @@ int gfd_kv_attend_workspace(gfd_ctx* ctx, const gfd_kv_cache* cache, const gfd_k
         uint64_t unused = 0;
         const char* why = kv_check_cache(*cache, false, &unused);
         if (why) return set_error(ctx, GFD_ERR_INVALID, "kv_attend_workspace: %s", why);
-        *bytes = attend_workspace(ctx, *cache, shared_len);
+        *bytes = plan_attend(ctx, *cache, *batch, *args, shared_len).bytes;
         return static_cast<int>(GFD_OK);
     });
 }

@@ -5,12 +5,14 @@
 // so memory bounds it.  All (sequence, KV head) units are laid out as one line of 64-key tiles
 // and every CTA takes an equal stretch (kv_cut): a batch of mixed lengths, one long context and
 // a hundred short ones keep every SM equally busy, with nothing known on the host.  A unit
-// that a cut divides leaves partial sums in the workspace, joined by kv_decode_join_kernel.
+// that a cut divides leaves partial sums in the workspace, joined by kv_join_kernel.
 //
 // Inside a CTA each of the 4 warps owns the 16 keys (one page or part of it) w of a tile and runs
 // alone: its own ring of stages filled with 16-byte cp.async (a page id per stage, ids fetched
 // 32 stages at a time), its own running maximum and sum, scores and sums by mma.m16n8k16 from
 // ldmatrix fragments.  No barrier between tiles; the warps join once per unit.
+
+#include <type_traits>
 
 #include "kv_device.cuh"
 
@@ -20,7 +22,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = kKvPage * kWarps;  // keys a CTA takes per step
-constexpr int kRows = 16;
+constexpr int kRows = kKvFewRows;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
@@ -92,13 +94,6 @@ __device__ __forceinline__ Seq few_seq(const KvAttendParams& p, int s) {
     return r;
 }
 
-// Where a stretch of the line begins: sequence, head and tile of position `at`, found by the
-// CTA together; *total: tiles of the line.  Returns false when the line ends before `at`.
-struct Place {
-    int32_t s, h, t;
-    int64_t begin;  // the unit's first tile on the line
-};
-
 template <typename F>
 __device__ __forceinline__ int64_t line_total(const KvAttendParams& p, int64_t* mine, F count) {
     __shared__ int64_t s_warp[kWarps];
@@ -124,18 +119,24 @@ __device__ __forceinline__ int64_t line_total(const KvAttendParams& p, int64_t* 
     return total;
 }
 
-__device__ __forceinline__ void find_place(const KvAttendParams& p, int64_t mine, int64_t at, Place* out) {
+// Position `at` of the line, found by the CTA together.
+__device__ __forceinline__ void find_place(const KvAttendParams& p, int64_t mine, int64_t at, KvPlace* out) {
     const int per = (p.batch.seqs + kThreads - 1) / kThreads;
     const int t = threadIdx.x;
     int64_t run = mine;
     for (int s = t * per; s < min((t + 1) * per, p.batch.seqs); ++s) {
-        const int32_t n = few_seq(p, s).tiles.count;
+        const Seq q = few_seq(p, s);
+        const int32_t n = q.tiles.count;
         const int64_t here = static_cast<int64_t>(n) * p.cache.heads;
         if (n > 0 && at >= run && at < run + here) {
             out->s = s;
             out->h = static_cast<int32_t>((at - run) / n);
             out->t = static_cast<int32_t>((at - run) % n);
+            out->count = n;
             out->begin = run + static_cast<int64_t>(out->h) * n;
+            out->row0 = q.q.row0;
+            out->packed0 = 0;
+            out->packed = q.q.rows * p.group;
         }
         run += here;
     }
@@ -176,86 +177,6 @@ struct Cursor {
     }
 };
 
-__device__ __forceinline__ constexpr int few_slot_floats(int d) { return kRows * d + 2 * kRows; }
-
-template <typename T>
-__device__ __forceinline__ void store_out(const KvAttendParams& p, int64_t row, int head, int d0, const float* v, int n) {
-    char* at = p.out.data + row * p.out.row_stride + head * p.out.head_stride;
-    if (p.out_f32) {
-        float* o = reinterpret_cast<float*>(at) + d0;
-        for (int i = 0; i < n; i += 4) *reinterpret_cast<float4*>(o + i) = *reinterpret_cast<const float4*>(v + i);
-    } else {
-        uint32_t* o = reinterpret_cast<uint32_t*>(at + 2 * d0);
-        for (int i = 0; i < n; i += 4)
-            *reinterpret_cast<uint2*>(o + i / 2) = make_uint2(Pack<T>::pair(v[i], v[i + 1]), Pack<T>::pair(v[i + 2], v[i + 3]));
-    }
-}
-
-// Score in base 2: scale and cap of the product, bias by distance.
-template <bool kPlain>
-__device__ __forceinline__ float score2(const KvAttendParams& p, float dot, float slope, int32_t dist) {
-    if (kPlain) return dot * p.scale2;
-    float z = dot * p.scale;
-    if (p.softcap > 0.0f) {
-        // tanh x = 1 - 2 / (1 + e^2x), to about 2^-21 of the cap
-        const float e = fast_exp2(z * p.cap_rate);
-        z = p.softcap - p.softcap * __fdividef(2.0f, 1.0f + e);
-        if (e == INFINITY) z = p.softcap;
-    }
-    return (z + slope * static_cast<float>(dist)) * kLog2e;
-}
-
-// The sum of one packed row over the keys of tiles [t0, t1) of a unit, key by key and only where
-// the row sees them; for rows whose sum by matrix products met a NaN or an infinity, which a
-// key that other rows see may have put there (0 * inf).  m: the row's maximum in base 2.
-template <typename T, int D, bool kPlain>
-__device__ __noinline__ void exact_row(const KvAttendParams& p, const Seq& q, int s, int h, int t0, int t1, int r, float m,
-                                       float* acc_out, float* room) {
-    float* s_w = room;
-    const char** s_v = reinterpret_cast<const char**>(room + kThreads);
-    const int t = threadIdx.x;
-    const int i = r / p.group, g = r % p.group;
-    const int32_t n = p.shared_len + q.q.keys, pos = n - q.q.rows + i;
-    const int prefix = p.prefix_len != nullptr ? p.prefix_len[s] : 0;
-    const KvSpan sp = kv_clip(kv_span(pos, n, prefix, p.window, p.causal != 0), p.shared_len, q.q.keys);
-    const int head = h * p.group + g;
-    const char* qrow = p.q.data + (q.q.row0 + i) * p.q.row_stride + head * p.q.head_stride;
-    const float slope = !kPlain && p.alibi != nullptr ? p.alibi[head] : 0.0f;
-    float acc = 0.0f;
-    for (int c = t0 * kTile; c < t1 * kTile; c += kThreads) {
-        const int ti = (c + t) / kTile;
-        const int32_t j = ti < t1 ? q.tiles.at(ti) * kTile + (c + t) % kTile : 0x7fffffff;
-        const char* v = nullptr;
-        float w = 0.0f;
-        if (j < sp.pre || (j >= sp.lo && j < sp.hi)) {
-            const int32_t id = p.batch.table[s * p.batch.table_stride + j / p.cache.block_tokens];
-            if (id >= 0 && id < p.cache.blocks) {
-                const int64_t at = id * p.cache.block_stride + j % p.cache.block_tokens * p.cache.token_stride + h * p.cache.head_stride;
-                float dot = 0.0f;
-                for (int e = 0; e < D; e += 8) {
-                    float a[8], b[8];
-                    Pack<T>::load(p.cache.k + at + 2 * e, a);
-                    Pack<T>::load(qrow + 2 * e, b);
-                    for (int x = 0; x < 8; ++x) dot = fmaf(a[x], b[x], dot);
-                }
-                const float z = score2<kPlain>(p, dot, slope, p.shared_len + j - pos);
-                w = z == -INFINITY ? 0.0f : fast_exp2(z - m);
-                v = p.cache.v + at;
-            }
-        }
-        __syncthreads();
-        s_w[t] = w;
-        s_v[t] = v;
-        __syncthreads();
-        if (t < D)
-            for (int x = 0; x < kThreads; ++x)
-                if (s_v[x] != nullptr && s_w[x] != 0.0f) acc = fmaf(s_w[x], static_cast<float>(reinterpret_cast<const T*>(s_v[x])[t]), acc);
-    }
-    __syncthreads();
-    if (t < D) acc_out[t] = acc;
-    __syncthreads();
-}
-
 template <int D>
 struct Shape {
     static constexpr int kStages = D == 128 ? 3 : 6;
@@ -272,7 +193,7 @@ __global__ void __launch_bounds__(kThreads) kv_decode_kernel(const KvAttendParam
     constexpr int kSteps = D / 16;   // k-steps of the scores, pairs of n-tiles of the sums
     constexpr int kChunks = D / 8;   // 16-byte pieces of a key
     extern __shared__ __align__(128) char smem[];
-    __shared__ Place s_place;
+    __shared__ KvPlace s_place;
     __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
     __shared__ uint32_t s_odd;
     float* s_join = reinterpret_cast<float*>(smem + kWarps * S::kRing);
@@ -280,8 +201,10 @@ __global__ void __launch_bounds__(kThreads) kv_decode_kernel(const KvAttendParam
     const KvBatchView& b = p.batch;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (t == 0) s_place = KvPlace{};
     if (!kv_starts_ok(b)) {
         if (blockIdx.x == 0 && t == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
+        if (t == 0) p.line.places[blockIdx.x] = s_place;
         return;
     }
     int64_t mine;
@@ -291,9 +214,13 @@ __global__ void __launch_bounds__(kThreads) kv_decode_kernel(const KvAttendParam
         return static_cast<int64_t>(q.tiles.count) * p.cache.heads;
     });
     const int64_t at = kv_cut(total, blockIdx.x, gridDim.x), to = kv_cut(total, blockIdx.x + 1, gridDim.x);
-    if (at >= to) return;
-    find_place(p, mine, at, &s_place);
+    if (at < total) find_place(p, mine, at, &s_place);
     __syncthreads();
+    if (t == 0) {
+        s_place.total = total;
+        p.line.places[blockIdx.x] = s_place;
+    }
+    if (at >= to) return;
 
     Cursor load, use;
     load.enter(p, s_place.s, s_place.h, s_place.t, to - at);
@@ -417,7 +344,7 @@ __global__ void __launch_bounds__(kThreads) kv_decode_kernel(const KvAttendParam
                         const int x = e >> 1;
                         const int32_t j = j0 + 8 * nt + (e & 1);
                         const bool seen = j < sp[x].pre || (j >= sp[x].lo && j < sp[x].hi);
-                        const float v = score2<kPlain>(p, z[nt][e], slope[x], p.shared_len + j - pos[x]);
+                        const float v = kv_score2<kPlain>(p, z[nt][e], slope[x], p.shared_len + j - pos[x]);
                         z[nt][e] = seen ? v : -INFINITY;
                         mx[x] = fmaxf(mx[x], z[nt][e]);
                     }
@@ -479,7 +406,7 @@ __global__ void __launch_bounds__(kThreads) kv_decode_kernel(const KvAttendParam
             }
         }
         const bool whole = t0 == 0 && use.end == use.q.tiles.count;
-        float* slot = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0)) * few_slot_floats(D);
+        float* slot = p.line.slots + (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0)) * (kRows * D + 2 * kRows);
         for (int half = 0; half < 2 && 8 * half < rows; ++half) {
             if (t == 0) s_odd = 0;
             __syncthreads();
@@ -510,13 +437,27 @@ __global__ void __launch_bounds__(kThreads) kv_decode_kernel(const KvAttendParam
             if (odd && rr < rows) atomicOr(&s_odd, 1u << jr);
             __syncthreads();
             const uint32_t redo = s_odd;
-            for (int x = 0; x < 8; ++x)
+            for (int x = warp; x < 8; x += kWarps)
                 if ((redo >> x) & 1u) {
-                    float mm = -INFINITY;
-                    for (int y = 0; y < kWarps; ++y) mm = fmaxf(mm, s_m[y][x + 8 * half]);
-                    exact_row<T, D, kPlain>(p, use.q, use.s, use.h, t0, use.end, x + 8 * half, mm, s_join + x * D,
-                                             s_join + 8 * D);
+                    const int r = x + 8 * half, i = r / p.group;
+                    const float mm = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+                    KvExact y;
+                    y.table = b.table + use.s * b.table_stride;
+                    y.tiles = use.q.tiles;
+                    y.pos = n - use.q.q.rows + i;
+                    y.seen = kv_clip(kv_span(y.pos, n, prefix, p.window, p.causal != 0), p.shared_len, use.q.q.keys);
+                    y.base = p.shared_len;
+                    y.t0 = t0;
+                    y.t1 = use.end;
+                    y.size = kTile;
+                    y.row = use.q.q.row0 + i;
+                    y.head = use.h * p.group + r % p.group;
+                    y.kvh = use.h;
+                    float part[D / 32];
+                    kv_exact_row<T, D, kPlain>(p, y, mm, part);
+                    for (int e = 0; e < D / 32; ++e) s_join[x * D + lane * (D / 32) + e] = part[e];
                 }
+            if (redo != 0) __syncthreads();
             if ((redo >> jr) & 1u)
 #pragma unroll
                 for (int e = 0; e < kEach; ++e) sum[e] = s_join[jr * D + d0 + e];
@@ -527,7 +468,7 @@ __global__ void __launch_bounds__(kThreads) kv_decode_kernel(const KvAttendParam
                     const float inv = ml == 0.0f ? 0.0f : 1.0f / ml;
 #pragma unroll
                     for (int e = 0; e < kEach; ++e) sum[e] = ml == 0.0f ? 0.0f : sum[e] * inv;
-                    store_out<T>(p, row, head, d0, sum, kEach);
+                    kv_store_out<T>(p, row, head, d0, sum, kEach);
                     if (p.lse != nullptr && d0 == 0)
                         p.lse[row * p.q_heads + head] = ml == 0.0f ? -INFINITY : mt * kLn2 + logf(ml);
                 } else {
@@ -547,63 +488,6 @@ __global__ void __launch_bounds__(kThreads) kv_decode_kernel(const KvAttendParam
     copy_wait<0>();
 }
 
-// One CTA per cut of the line: the unit whose first cut it is.  Each thread sums 4 elements of
-// a packed row over the unit's parts, in their order.
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) kv_decode_join_kernel(const KvAttendParams p) {
-    __shared__ Place s_place;
-    const int t = threadIdx.x;
-    const int c = blockIdx.x + 1, n = gridDim.x + 1;  // cuts 1 .. n - 1 of n CTAs
-    int64_t mine = 0, total = 0, cut = 0;
-    const bool ok = kv_starts_ok(p.batch);
-    if (ok) {
-        total = line_total(p, &mine, [&](int s) { return static_cast<int64_t>(few_seq(p, s).tiles.count) * p.cache.heads; });
-        cut = kv_cut(total, c, n);
-        if (cut < total) find_place(p, mine, cut, &s_place);
-        __syncthreads();
-    }
-    // every CTA waits for the attention kernel, so that this grid never ends before it
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (!ok || cut >= total) return;
-    const Place u = s_place;
-    // a cut between two units joins nothing; of several inside a unit the first does
-    if (u.t == 0 || kv_cut(total, c - 1, n) > u.begin) return;
-    const Seq q = few_seq(p, u.s);
-    const int64_t end = u.begin + q.tiles.count;
-    int last = c;  // parts: CTA c - 1 (slot 1), c .. last (slot 0)
-    while (last + 1 < n && kv_cut(total, last + 1, n) < end) ++last;
-    for (int i = t; i < q.q.rows * p.group * (D / 4); i += kThreads) {
-        const int r = i / (D / 4), d0 = i % (D / 4) * 4;
-        float m = -INFINITY;
-        for (int x = c - 1; x <= last; ++x) {
-            if (x >= c && kv_cut(total, x, n) == kv_cut(total, x + 1, n)) continue;
-            m = fmaxf(m, p.partial[(2 * static_cast<int64_t>(x) + (x < c ? 1 : 0)) * few_slot_floats(D) + kRows * D + r]);
-        }
-        float sum[4] = {}, l = 0.0f;
-        for (int x = c - 1; x <= last; ++x) {
-            if (x >= c && kv_cut(total, x, n) == kv_cut(total, x + 1, n)) continue;
-            const float* slot = p.partial + (2 * static_cast<int64_t>(x) + (x < c ? 1 : 0)) * few_slot_floats(D);
-            const float pm = slot[kRows * D + r], pl = slot[kRows * D + kRows + r];
-            const float w = pm == -INFINITY ? 0.0f : fast_exp2(pm - m);
-            l += pm == -INFINITY ? pl : pl * w;  // -inf: 0, or NaN from scores that are NaN
-            const float4 v = *reinterpret_cast<const float4*>(slot + r * D + d0);
-            if (w != 0.0f) {
-                sum[0] = fmaf(v.x, w, sum[0]);
-                sum[1] = fmaf(v.y, w, sum[1]);
-                sum[2] = fmaf(v.z, w, sum[2]);
-                sum[3] = fmaf(v.w, w, sum[3]);
-            }
-        }
-        const int64_t row = q.q.row0 + r / p.group;
-        const int head = u.h * p.group + r % p.group;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] = l == 0.0f ? 0.0f : sum[e] * inv;
-        store_out<T>(p, row, head, d0, sum, 4);
-        if (p.lse != nullptr && d0 == 0) p.lse[row * p.q_heads + head] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
-    }
-}
-
 template <typename T, int D>
 cudaError_t launch(const KvAttendParams& p, int ctas, cudaStream_t st) {
     const bool plain = p.softcap == 0.0f && p.alibi == nullptr;
@@ -613,25 +497,12 @@ cudaError_t launch(const KvAttendParams& p, int ctas, cudaStream_t st) {
     k<<<ctas, kThreads, Shape<D>::kSmem, st>>>(p);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas - 1);
-    cfg.blockDim = dim3(kThreads);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv_decode_join_kernel<T, D>, p);
+    return launch_kv_join(p, D, std::is_same<T, __half>::value ? GFD_FP16 : GFD_BF16, ctas, kRows, st);
 }
 
 }  // namespace
 
 int kv_decode_ctas(int num_sms) { return 2 * num_sms; }
-
-size_t kv_decode_workspace(int num_sms, int head_dim) {
-    return static_cast<size_t>(kv_decode_ctas(num_sms)) * 2 * (kRows * head_dim + 2 * kRows) * sizeof(float);
-}
 
 cudaError_t launch_kv_decode(const KvAttendParams& p, int head_dim, int dtype, int num_sms, cudaStream_t st) {
     const int ctas = kv_decode_ctas(num_sms);

@@ -88,8 +88,7 @@ __device__ __forceinline__ void kv_report(uint32_t* status, uint32_t bits) {
     if (status != nullptr && bits != 0) atomicOr(status, bits);
 }
 
-// Address of token j of a sequence (its own table and the shared prefix in front of it);
-// null: the block id is outside the cache.
+// Block id and place of token j of a sequence (its own table behind the shared prefix).
 __device__ __forceinline__ int32_t kv_block(const KvBatchView& b, int s, int32_t j, int32_t bt, const int32_t* shared_table,
                                             int32_t shared_len, int32_t* place) {
     const int32_t* t = shared_table;
@@ -99,6 +98,86 @@ __device__ __forceinline__ int32_t kv_block(const KvBatchView& b, int s, int32_t
     }
     *place = j % bt;
     return t[j / bt];
+}
+
+template <typename T>
+__device__ __forceinline__ void kv_store_out(const KvAttendParams& p, int64_t row, int head, int d0, const float* v, int n) {
+    char* at = p.out.data + row * p.out.row_stride + head * p.out.head_stride;
+    if (p.out_f32) {
+        float* o = reinterpret_cast<float*>(at) + d0;
+        for (int i = 0; i < n; i += 4) *reinterpret_cast<float4*>(o + i) = *reinterpret_cast<const float4*>(v + i);
+    } else {
+        uint32_t* o = reinterpret_cast<uint32_t*>(at + 2 * d0);
+        for (int i = 0; i < n; i += 4)
+            *reinterpret_cast<uint2*>(o + i / 2) = make_uint2(Pack<T>::pair(v[i], v[i + 1]), Pack<T>::pair(v[i + 2], v[i + 3]));
+    }
+}
+
+// Score in base 2: scale and cap of the product, bias by distance.
+template <bool kPlain>
+__device__ __forceinline__ float kv_score2(const KvAttendParams& p, float dot, float slope, int32_t dist) {
+    if (kPlain) return dot * p.scale2;
+    float z = dot * p.scale;
+    if (p.softcap > 0.0f) {
+        // tanh x = 1 - 2 / (1 + e^2x), to about 2^-21 of the cap
+        const float e = fast_exp2(z * p.cap_rate);
+        z = p.softcap - p.softcap * __fdividef(2.0f, 1.0f + e);
+        if (e == INFINITY) z = p.softcap;
+    }
+    return (z + slope * static_cast<float>(dist)) * kLog2e;
+}
+
+// A stretch of one sequence's keys that one packed row (row `row` of the batch at position
+// pos, query head `head`, KV head kvh) is summed over: keys [0, n) named by `table`, of which
+// key j stands at position base + j, in tiles [t0, t1) of `size` keys.
+struct KvExact {
+    const int32_t* table;
+    KvTiles tiles;
+    KvSpan seen;  // of this row
+    int32_t base, pos, t0, t1, size;
+    int64_t row;
+    int32_t head, kvh;
+};
+
+// The sum of the row's weights times values, key by key and only over keys that it sees, by one
+// warp; lane i gets elements [i D / 32, (i + 1) D / 32).  For rows whose sum by matrix products
+// met a NaN or an infinity, which a key that only other rows see may have put there (0 * inf).
+// m: what the weights are relative to, in base 2.
+template <typename T, int D, bool kPlain>
+__device__ __noinline__ void kv_exact_row(const KvAttendParams& p, const KvExact& x, float m, float* acc) {
+    constexpr int kEach = D / 32;
+    const int lane = threadIdx.x & 31;
+    const char* qrow = p.q.data + x.row * p.q.row_stride + x.head * p.q.head_stride;
+    const float slope = !kPlain && p.alibi != nullptr ? p.alibi[x.head] : 0.0f;
+    for (int e = 0; e < kEach; ++e) acc[e] = 0.0f;
+    for (int t = x.t0; t < x.t1; ++t)
+        for (int c = 0; c < x.size; c += 32) {
+            const int32_t j = x.tiles.at(t) * x.size + c + lane;
+            int64_t at = -1;
+            float w = 0.0f;
+            if (j < x.seen.pre || (j >= x.seen.lo && j < x.seen.hi)) {
+                const int32_t id = x.table[j / p.cache.block_tokens];
+                if (id >= 0 && id < p.cache.blocks) {
+                    at = id * p.cache.block_stride + j % p.cache.block_tokens * p.cache.token_stride + x.kvh * p.cache.head_stride;
+                    float dot = 0.0f;
+                    for (int e = 0; e < D; e += 8) {
+                        float a[8], b[8];
+                        Pack<T>::load(p.cache.k + at + 2 * e, a);
+                        Pack<T>::load(qrow + 2 * e, b);
+                        for (int y = 0; y < 8; ++y) dot = fmaf(a[y], b[y], dot);
+                    }
+                    const float z = kv_score2<kPlain>(p, dot, slope, x.base + j - x.pos);
+                    w = z == -INFINITY ? 0.0f : fast_exp2(z - m);
+                }
+            }
+            for (int y = 0; y < 32; ++y) {
+                const float wy = __shfl_sync(0xffffffffu, w, y);
+                const int64_t ay = __shfl_sync(0xffffffffu, at, y);
+                if (ay < 0 || wy == 0.0f) continue;
+                for (int e = 0; e < kEach; ++e)
+                    acc[e] = fmaf(wy, static_cast<float>(reinterpret_cast<const T*>(p.cache.v + ay)[lane * kEach + e]), acc[e]);
+            }
+        }
 }
 
 }  // namespace gfdb

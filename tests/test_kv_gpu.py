@@ -560,7 +560,7 @@ def test_graph_reads_lengths_at_replay(gpu_ctx, shape):
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, stream=st):
             s.cache.attend(s.batch, s.q, out, **kw)
-        runs.append((g, out, lse))
+        runs.append((g, out, lse, ws))  # a graph holds addresses: its workspace lives as long
     for s in (a, b):  # other inputs in the same arrays
         s.q.copy_(s.normal(*s.q.shape))
         s.kv_lens = [n - 3 if n > 60 and m < n - 3 else n for n, m in zip(s.kv_lens, s.q_lens)]
@@ -568,11 +568,11 @@ def test_graph_reads_lengths_at_replay(gpu_ctx, shape):
         s.table.copy_(torch.flip(s.table, [0]) if len(set(-(-n // s.k.shape[1]) for n in s.kv_lens)) == 1 else s.table)
     torch.cuda.synchronize()
     for _ in range(3):
-        for (g, _, _), st in zip(runs, streams):
+        for (g, _, _, _), st in zip(runs, streams):
             with torch.cuda.stream(st):
                 g.replay()
     torch.cuda.synchronize()
-    for s, (g, out, lse) in zip((a, b), runs):
+    for s, (g, out, lse, _) in zip((a, b), runs):
         oracle.check_attend(out, lse, s.want())
 
 
