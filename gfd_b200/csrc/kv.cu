@@ -168,39 +168,41 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const KvMergePa
 }
 
 // ---------------------------------------------------------------------------
-// Join of an attention launch's partial results: CTAs (c - 1, *) for cut c of the line.  Each
+// Join of an attention launch's partial results: one CTA (times gridDim.y) per
+// cut of the line.  Each
 // thread sums 4 elements of a packed row over the unit's parts, in their order.
 // ---------------------------------------------------------------------------
 constexpr int kJoinThreads = 128;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendParams p, int slot_rows) {
-    const int c = blockIdx.x + 1, n = gridDim.x + 1;  // cuts 1 .. n - 1 of n CTAs
+    const uint32_t c = blockIdx.x + 1;  // cuts 1 .. CTAs - 1
     // every CTA waits for the attention kernel, so that this grid never ends before it
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const KvPlace u = p.line.places[c];
-    const int64_t total = u.total, cut = kv_cut(total, c, n);
+    const KvCuts cuts(u.total, gridDim.x + 1);
     // a cut between two units joins nothing; of several inside a unit the first does
-    if (cut >= total || u.t == 0 || kv_cut(total, c - 1, n) > u.begin) return;
+    if (c >= cuts.ctas || u.t == 0 || cuts.at(c - 1) > u.begin) return;
     const int64_t end = u.begin + u.count;
-    int last = c;  // parts: CTA c - 1 (slot 1), c .. last (slot 0)
-    while (last + 1 < n && kv_cut(total, last + 1, n) < end) ++last;
+    uint32_t last = c;  // parts: CTA c - 1 (slot 1), c .. last (slot 0)
+    while (last + 1 < cuts.ctas && cuts.at(last + 1) < end) ++last;
     const int64_t size = static_cast<int64_t>(slot_rows) * (D + 2);
+    const float* slot1 = p.line.slots + (2 * static_cast<int64_t>(c - 1) + 1) * size;
+    const float* slot0 = p.line.slots + 2 * static_cast<int64_t>(c) * size;
+    const int parts = static_cast<int>(last - c) + 2;
     for (int i = blockIdx.y * kJoinThreads + threadIdx.x; i < u.packed * (D / 4); i += kJoinThreads * gridDim.y) {
         const int r = i / (D / 4), d0 = i % (D / 4) * 4;
-        float m = -INFINITY;
-        for (int x = c - 1; x <= last; ++x) {
-            if (x >= c && kv_cut(total, x, n) == kv_cut(total, x + 1, n)) continue;  // no stretch
-            m = fmaxf(m, p.line.slots[(2 * static_cast<int64_t>(x) + (x < c ? 1 : 0)) * size + slot_rows * D + r]);
-        }
+        float m = slot1[slot_rows * D + r];
+#pragma unroll 4
+        for (int x = 1; x < parts; ++x) m = fmaxf(m, slot0[2 * (x - 1) * size + slot_rows * D + r]);
         float sum[4] = {}, l = 0.0f;
-        for (int x = c - 1; x <= last; ++x) {
-            if (x >= c && kv_cut(total, x, n) == kv_cut(total, x + 1, n)) continue;
-            const float* slot = p.line.slots + (2 * static_cast<int64_t>(x) + (x < c ? 1 : 0)) * size;
+#pragma unroll 4
+        for (int x = 0; x < parts; ++x) {
+            const float* slot = x == 0 ? slot1 : slot0 + 2 * (x - 1) * size;
             const float pm = slot[slot_rows * D + r], pl = slot[slot_rows * D + slot_rows + r];
+            const float4 v = *reinterpret_cast<const float4*>(slot + r * D + d0);
             const float w = pm == -INFINITY ? 0.0f : fast_exp2(pm - m);
             l += pm == -INFINITY ? pl : pl * w;  // -inf: 0, or NaN from scores that are NaN
-            const float4 v = *reinterpret_cast<const float4*>(slot + r * D + d0);
             if (w != 0.0f) {
                 sum[0] = fmaf(v.x, w, sum[0]);
                 sum[1] = fmaf(v.y, w, sum[1]);

@@ -42,7 +42,7 @@ struct KvAppendParams {
     int32_t q_heads, rot_dim, interleaved;
 };
 
-// Where a CTA's stretch of the line of tiles begins (kv_cut), left for the joining kernel.
+// Where a CTA's stretch of the line of tiles begins (KvCuts), left for the joining kernel.
 struct KvPlace {
     int64_t total;    // tiles of the line
     int64_t begin;    // the unit's first tile on the line

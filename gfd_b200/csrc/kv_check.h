@@ -80,11 +80,21 @@ GFD_HD KvTiles kv_tiles(KvSpan s, int32_t size) {
     return t;
 }
 
-// All tiles of a launch form one line, unit after unit; CTA c of n takes [kv_cut(c), kv_cut(c + 1)).
-// A unit that lies in one CTA is finished there.  One that is cut leaves partial results, one
-// in each CTA it touches, in slot 1 of the CTA where it begins and slot 0 of the others; the
-// first cut inside a unit names the one who joins them.
-GFD_HD int64_t kv_cut(int64_t total, int c, int n) { return total / n * c + (total % n) * c / n; }
+// All tiles of a launch form one line, unit after unit; CTA c takes [at(c), at(c + 1)), at least
+// one tile each: CTAs beyond n() have none.  A unit that lies in one CTA is finished there.  One
+// that is cut leaves partial results, one in each CTA it touches, in slot 1 of the CTA where it
+// begins and slot 0 of the others; the first cut inside a unit names the one who joins them.
+struct KvCuts {
+    int64_t each;
+    uint32_t more, ctas;
+    GFD_HD KvCuts(int64_t total, uint32_t most) {
+        ctas = total < static_cast<int64_t>(most) ? static_cast<uint32_t>(total) : most;
+        each = ctas > 0 ? total / ctas : 0;
+        more = ctas > 0 ? static_cast<uint32_t>(total - each * ctas) : 0;
+    }
+    GFD_HD int n() const { return static_cast<int>(ctas); }
+    GFD_HD int64_t at(uint32_t c) const { return each * c + more * c / ctas; }  // more * c < 2^32: ctas < 2^16
+};
 
 // ---------------------------------------------------------------------------
 // Checks: each returns nullptr, or what is wrong

@@ -3,7 +3,7 @@
 //
 // The work is reading the cache once: 4 D bytes per key and KV head against 4 D * 16 operations,
 // so memory bounds it.  All (sequence, KV head) units are laid out as one line of 64-key tiles
-// and every CTA takes an equal stretch (kv_cut): a batch of mixed lengths, one long context and
+// and every CTA takes an equal stretch (KvCuts): a batch of mixed lengths, one long context and
 // a hundred short ones keep every SM equally busy, with nothing known on the host.  A unit
 // that a cut divides leaves partial sums in the workspace, joined by kv_join_kernel.
 //
@@ -188,7 +188,7 @@ struct Shape {
 };
 
 template <typename T, int D, bool kPlain>
-__global__ void __launch_bounds__(kThreads) kv_decode_kernel(const KvAttendParams p) {
+__global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendParams p) {
     using S = Shape<D>;
     constexpr int kSteps = D / 16;   // k-steps of the scores, pairs of n-tiles of the sums
     constexpr int kChunks = D / 8;   // 16-byte pieces of a key
@@ -213,14 +213,18 @@ __global__ void __launch_bounds__(kThreads) kv_decode_kernel(const KvAttendParam
         if (q.bad && blockIdx.x == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
         return static_cast<int64_t>(q.tiles.count) * p.cache.heads;
     });
-    const int64_t at = kv_cut(total, blockIdx.x, gridDim.x), to = kv_cut(total, blockIdx.x + 1, gridDim.x);
-    if (at < total) find_place(p, mine, at, &s_place);
+    const KvCuts cuts(total, gridDim.x);
+    if (static_cast<int>(blockIdx.x) >= cuts.n()) {
+        if (t == 0) p.line.places[blockIdx.x].total = total;
+        return;
+    }
+    const int64_t at = cuts.at(blockIdx.x), to = cuts.at(blockIdx.x + 1);
+    find_place(p, mine, at, &s_place);
     __syncthreads();
     if (t == 0) {
         s_place.total = total;
         p.line.places[blockIdx.x] = s_place;
     }
-    if (at >= to) return;
 
     Cursor load, use;
     load.enter(p, s_place.s, s_place.h, s_place.t, to - at);

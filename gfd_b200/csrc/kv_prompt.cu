@@ -367,6 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             s0 = lo;
         }
         int64_t per_head = 0, total = 0, at = 0;
+        bool none = false;
         for (int pass = 0; pass < 2; ++pass) {
             int s = s0;
             Many m{};
@@ -376,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 while (u - first[s] >= m.tiles) m = many_seq(p, ++s);
                 const int rt = static_cast<int>(u - first[s]);
                 const Unit x = many_unit(p, s, m.q, rt);
-                if (pass == 1 && at < total) {
+                if (pass == 1 && !none) {
                     const int64_t want = at % per_head, here = mine + sum;
                     if (want >= here && want < here + x.tiles.count) {
                         s_place.s = s;
@@ -394,8 +395,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (pass == 0) {
                 mine = cta_scan(sum, s_warps, &per_head) - sum;
                 total = per_head * p.cache.heads;
-                at = kv_cut(total, blockIdx.x, gridDim.x);
-                len = kv_cut(total, blockIdx.x + 1, gridDim.x) - at;
+                const KvCuts cuts(total, gridDim.x);
+                none = static_cast<int>(blockIdx.x) >= cuts.n();
+                if (!none) {
+                    at = cuts.at(blockIdx.x);
+                    len = cuts.at(blockIdx.x + 1) - at;
+                }
             }
         }
         __syncthreads();
