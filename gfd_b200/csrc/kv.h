@@ -71,6 +71,7 @@ struct KvAttendParams {
     uint32_t* status;
     int32_t shared_len;
     int32_t q_heads, group;
+    uint64_t group_magic;  // ceil(2^44 / group), see kv_div_group
     int32_t max_q_len, causal, window;
     float scale, softcap;
     float scale2;    // scale in base 2

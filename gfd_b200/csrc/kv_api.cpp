@@ -193,6 +193,7 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
     p.shared_len = static_cast<int32_t>(shared_len);
     p.q_heads = a->q_heads;
     p.group = a->q_heads / c->heads;
+    p.group_magic = ((1ull << 44) + p.group - 1) / p.group;
     p.max_q_len = a->max_q_len;
     p.causal = a->causal != 0;
     p.window = a->window;

@@ -74,6 +74,12 @@ struct Pack<float> {
     }
 };
 
+// n / group for 0 <= n < 2^31: the rounded-up reciprocal errs by less than group <= 2^13 in 2^44, so
+// n times it stays below the next whole quotient.
+__device__ __forceinline__ int32_t kv_div_group(const KvAttendParams& p, int32_t n) {
+    return static_cast<int32_t>(__umul64hi(static_cast<uint64_t>(n) << 20, p.group_magic));
+}
+
 // row_start rises from >= 0 to <= rows (every thread of the CTA calls; same answer for all).
 __device__ __forceinline__ bool kv_starts_ok(const KvBatchView& b) {
     bool bad = false;
@@ -144,7 +150,7 @@ struct KvExact {
 // met a NaN or an infinity, which a key that only other rows see may have put there (0 * inf).
 // m: what the weights are relative to, in base 2.
 template <typename T, int D, bool kPlain>
-__device__ __noinline__ void kv_exact_row(const KvAttendParams& p, const KvExact& x, float m, float* acc) {
+__device__ __forceinline__ void kv_exact_row(const KvAttendParams& p, const KvExact& x, float m, float* acc) {
     constexpr int kEach = D / 32;
     const int lane = threadIdx.x & 31;
     const char* qrow = p.q.data + x.row * p.q.row_stride + x.head * p.q.head_stride;

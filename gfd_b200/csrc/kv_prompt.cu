@@ -13,10 +13,14 @@
 // of O is rare.  Sums and maxima are 32-bit; the weights' rounding to the 16-bit type for the
 // second product is the only one before the result's.
 //
-// Roles: warps 0-3 softmax of half A, 4-7 of half B, warp 8 issues the products, warp 9 loads K
-// and V (TMA boxes of 16 tokens x 64 elements, so that every page is found by its id).
-// Units lie on one line of tiles that the CTAs (one per SM) share evenly; a cut unit leaves
-// partial sums for kv_join_kernel, as in kv_decode.cu.
+// The exponentials bound the softmax (16 a cycle and SM against 4096 products): a part of them
+// runs as a polynomial on the FMA units instead (exp2_pair).
+//
+// Roles: warps 0-3 softmax of half A, 4-7 of half B; 8-11 write finished rows while the softmax
+// is in the next unit; 12 issues the products, 13 loads K and V (TMA boxes of 16 tokens x 64
+// elements, so that every page is found by its id), 14 loads Q, 15 walks the units.  Units lie
+// on one line of tiles that the CTAs (one per SM) share evenly; a cut unit leaves partial sums
+// for kv_join_kernel, as in kv_decode.cu.
 
 #include <cuda.h>
 
@@ -31,7 +35,9 @@ constexpr int kRows = kKvManyRows;  // packed rows of a unit
 constexpr int kHalf = 128;          // rows of a half: one tensor-core tile
 constexpr int kTile = 128;          // keys of a step
 constexpr int kPages = kTile / kKvPage;
-constexpr int kThreads = 320;
+constexpr int kThreads = 512;
+constexpr int kAux = 88, kMain = 168;  // registers of the helpers' and the softmax warps: 256 x (88 + 168) = 64 K
+constexpr int kStageBytes = 32 * 64; // a softmax warp's room for results on their way out
 constexpr int kBadRing = 8;         // tiles whose bad pages are remembered
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -62,22 +68,19 @@ __device__ __forceinline__ uint64_t clock_ns() {
     return t;
 }
 // false: the wait ran out, or another warp's did
-__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-    const uint64_t t0 = clock_ns();
-    for (;;) {
-        for (int i = 0; i < 64; ++i)
-            if (bar_try(bar, parity)) return true;
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+    uint64_t t0 = 0;
+    for (uint32_t i = 1; !bar_try(bar, parity); ++i) {
+        if ((i & 255u) != 0) continue;
         if (*gave_up != 0) return false;
-        if (clock_ns() - t0 > kWaitLimitNs) {
+        const uint64_t now = clock_ns();
+        if (t0 == 0) t0 = now;
+        if (now - t0 > kWaitLimitNs) {
             *gave_up = 1;
             return false;
         }
     }
-}
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-    for (int i = 0; i < 16; ++i)
-        if (bar_try(bar, parity)) return true;
-    return bar_wait_slow(bar, parity, gave_up);
+    return true;
 }
 
 // ---- tensor memory and products ----
@@ -254,6 +257,22 @@ struct Cursor {
     }
 };
 
+// A unit as the walking warp hands it to the others.
+struct Desc {
+    int32_t s, h;
+    int32_t t0, nt;              // its tiles in this CTA
+    int32_t count;               // all its tiles
+    int32_t npre, first;         // KvTiles
+    int32_t pre, lo, hi;         // what its rows see together
+    int32_t packed0, packed;
+    int32_t row0, rows, keys;    // of its sequence
+    int32_t prefix;
+    __device__ __forceinline__ int32_t key(int i) const {  // first key of tile t0 + i
+        const int32_t t = t0 + i;
+        return (t < npre ? t : t - npre + first) * kTile;
+    }
+};
+
 // Inclusive sum over the CTA's threads.
 __device__ __forceinline__ int64_t cta_scan(int64_t v, int64_t* warps, int64_t* total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -283,14 +302,19 @@ struct Shape {
     static constexpr int kOperand = kHalf * D * 2;        // bytes of Q of a half, K or V of a tile
     static constexpr int kBlock = kHalf * 128;            // bytes of a 64-element block of one
     static constexpr int kSlots = 4;                      // K and V tiles in flight
-    static constexpr int kSmem = 2 * kOperand + kSlots * kOperand + 1024;
+    static constexpr int kSmem = 2 * kOperand + kSlots * kOperand + 4 * kStageBytes + 1024;
     static constexpr uint32_t kColumns = 512;             // S, S, O, O
     static constexpr uint32_t kO = 256;                   // O of half A
 };
 
+constexpr int kUnitRing = 4;
+constexpr int kUnitReaders = 4 + 4 + 4 + 3;  // warps
+
 struct Bars {
-    uint64_t full[8], empty[8];
-    uint64_t q[2], s[2], p[2], o[2];
+    uint64_t full[4], empty[4];                       // K and V slots
+    uint64_t unit[kUnitRing], unit_read[kUnitRing];
+    uint64_t q[2], q_read[2], s[2], p[2];             // Q there / products with it done, scores, weights
+    uint64_t o[2], o_read[2], ml[2], ml_read[2];      // sums done / taken, their base and weight sum
 };
 
 template <typename T>
@@ -298,6 +322,80 @@ struct Shift {  // weights reach 2^(shift + 8): fp16 keeps them clear of its sma
     static constexpr float value = std::is_same<T, __half>::value ? 6.0f : 0.0f;
 };
 constexpr float kGrow = 8.0f;
+constexpr int kByFma = 4;  // of 16 pairs of exponentials, how many run on the FMA units
+
+// Position of row r of the unit and what it sees of this pass's keys; rows that do not exist see
+// everything.  `exact`: the position itself is needed, not only the span.
+__device__ __forceinline__ KvSpan row_span(const KvAttendParams& p, const Desc& u, int r, int32_t* pos, bool exact) {
+    *pos = 0;
+    if (r >= u.packed) return KvSpan{0x7fffffff, 0, 0};
+    const int32_t of = kv_div_group(p, u.packed0 + r);
+    int32_t n = p.shared_len + u.keys, prefix = u.prefix;
+    *pos = n - u.rows + of;
+    if (p.shared_pass) {
+        // all rows of the batch: the position is that of the row's own sequence, and without a
+        // window, a prefix mask or a bias it does not matter
+        const KvBatchView& b = p.batch;
+        n = p.shared_len;
+        *pos = 0x3fffffff;
+        if (exact || p.window > 0 || p.prefix_len != nullptr) {
+            const int32_t row = u.row0 + of;
+            int lo = 0, hi = b.seqs - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (b.row_start[mid] <= row) lo = mid;
+                else hi = mid - 1;
+            }
+            n = p.shared_len + min(max(b.kv_len[lo], 0), static_cast<int32_t>(b.capacity));
+            *pos = n - (b.row_start[lo + 1] - row);
+            prefix = p.prefix_len != nullptr ? p.prefix_len[lo] : 0;
+        }
+    }
+    return kv_clip(kv_span(*pos, n, prefix, p.window, p.causal != 0), p.shared_pass ? 0 : p.shared_len, u.keys);
+}
+
+// 2^x for two arguments of at most 2^7, on the FMA units: x = n + r with |r| <= 1/2 (n by adding 1.5 * 2^23),
+// a polynomial of degree 5 for 2^r (least largest relative error with a constant of 1: 2^-23.3,
+// 2^-22.3 with the roundings), n added to the exponent.  Below -127 the result is 0 (n = -127
+// takes 1 to 0).  Not for NaN: the caller sees those in the maximum.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+    float a, b;
+    unpack2(x, a, b);
+    x = pack2(fmaxf(a, -127.0f), fmaxf(b, -127.0f));
+    const uint64_t n = add2(x, pack2(12582912.0f, 12582912.0f));
+    const uint64_t r = add2(x, fma2(n, pack2(-1.0f, -1.0f), pack2(12582912.0f, 12582912.0f)));
+    uint64_t y = fma2(r, pack2(0.001326472731307149f, 0.001326472731307149f), pack2(0.009671512991189957f, 0.009671512991189957f));
+    y = fma2(y, r, pack2(0.05550733581185341f, 0.05550733581185341f));
+    y = fma2(y, r, pack2(0.24022242426872253f, 0.24022242426872253f));
+    y = fma2(y, r, pack2(0.6931470036506653f, 0.6931470036506653f));
+    y = fma2(y, r, pack2(1.0f, 1.0f));
+    float ya, yb, na, nb;
+    unpack2(y, ya, yb);
+    unpack2(n, na, nb);
+    return pack2(__uint_as_float(__float_as_uint(ya) + (__float_as_uint(na) << 23)), __uint_as_float(__float_as_uint(yb) + (__float_as_uint(nb) << 23)));
+}
+// largest of three; NaN if one is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 
 template <typename T, int D, bool kPlain>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -310,6 +408,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     __shared__ uint32_t s_bad[kBadRing];
+    __shared__ Desc s_unit[kUnitRing];
+    __shared__ float s_base[2][kHalf], s_sum[2][kHalf];
     char* smem = reinterpret_cast<char*>((reinterpret_cast<uint64_t>(smem_raw) + 1023) & ~1023ull);
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const KvBatchView& b = p.batch;
@@ -322,11 +422,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             bar_init(smem_addr(&bars.full[i]), 1);
             bar_init(smem_addr(&bars.empty[i]), 1);
         }
+        for (int i = 0; i < kUnitRing; ++i) {
+            bar_init(smem_addr(&bars.unit[i]), 1);
+            bar_init(smem_addr(&bars.unit_read[i]), kUnitReaders);
+        }
         for (int i = 0; i < 2; ++i) {
-            bar_init(smem_addr(&bars.q[i]), kHalf);
+            bar_init(smem_addr(&bars.q[i]), 1);
+            bar_init(smem_addr(&bars.q_read[i]), 1);
             bar_init(smem_addr(&bars.s[i]), 1);
-            bar_init(smem_addr(&bars.p[i]), kHalf);
+            bar_init(smem_addr(&bars.p[i]), 4);
             bar_init(smem_addr(&bars.o[i]), 1);
+            bar_init(smem_addr(&bars.o_read[i]), 4);
+            bar_init(smem_addr(&bars.ml[i]), 4);
+            bar_init(smem_addr(&bars.ml_read[i]), 4);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -411,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (len <= 0) return;
 
-    if (warp == 8) {
+    if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(S::kColumns)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -422,90 +530,280 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = s_tmem;
     const uint32_t sq = smem_addr(smem), ring = sq + 2 * S::kOperand;
     volatile int* gave_up = &s_gave_up;
-    const KvPlace place = s_place;
+    // The next unit, read by a whole warp (every role takes every unit, in order).
+    int unit = 0;
+    auto take = [&](Desc* d) -> bool {
+        const int i = unit % kUnitRing;
+        if (!bar_wait(smem_addr(&bars.unit[i]), (unit / kUnitRing) & 1, gave_up)) return false;
+        *d = s_unit[i];
+        __syncwarp();
+        if (lane == 0) bar_arrive(smem_addr(&bars.unit_read[i]));
+        ++unit;
+        return d->nt > 0;
+    };
 
-    if (warp == 9) {
-        // ---- K and V ----
-        Cursor c;
-        c.enter(p, place, len);
-        int slot = 0, seen = 0;  // seen: tiles so far
-        uint32_t phase = 0;      // bit i: parity that slot i's `empty` has to reach
-        bool good = true;
-        const int pages = p.cache.block_tokens / kKvPage;
-        while (good && !c.done) {
-            const int32_t* table = p.shared_pass ? p.shared_table : b.table + c.s * b.table_stride;
-            const int32_t n = c.m.q.keys;
-            for (; good && c.t < c.end; ++c.t, ++seen) {
-                const int32_t j0 = c.u.tiles.at(c.t) * kTile;
-                // lane i: page i % 8 of the tile
-                const int32_t j = j0 + (lane % kPages) * kKvPage;
-                int32_t id = p.cache.blocks;  // a block outside the map: loads as zeros
-                bool bad = false;
-                if ((j < c.u.all.pre || (j + kKvPage > c.u.all.lo && j < c.u.all.hi)) && j < n) {
-                    id = table[j / kKvPage / pages];
-                    if (id < 0 || id >= p.cache.blocks) {
-                        bad = true;
-                        id = p.cache.blocks;
-                        kv_report(p.status, GFD_KV_BAD_PAGE);
-                    }
-                }
-                const int32_t in_block = (j / kKvPage % pages) * kKvPage;
-                const uint32_t bad_pages = __ballot_sync(0xffffffffu, bad) & 0xffu;
-                // a page that the sequence ends in: V's tokens behind the end are kept out by hand,
-                // whatever lies there would meet weights of zero
-                const int32_t rest = n - j0;
-                const int cut_page = rest > 0 && rest < kTile && rest % kKvPage != 0 ? rest / kKvPage : -1;
-                for (int which = 0; good && which < 2; ++which) {  // K, V
-                    const uint32_t full = smem_addr(&bars.full[slot]);
-                    good = bar_wait(smem_addr(&bars.empty[slot]), ((phase >> slot) & 1u) ^ 1u, gave_up);
-                    if (!good) break;
-                    const uint32_t dst = ring + slot * S::kOperand;
-                    const bool by_hand = which == 1 && cut_page >= 0;
-                    if (which == 0 && lane == 0) s_bad[seen % kBadRing] = bad_pages;
-                    if (by_hand) {
-                        const int32_t hid = __shfl_sync(0xffffffffu, id, cut_page), hpl = __shfl_sync(0xffffffffu, in_block, cut_page);
-                        const char* src = p.cache.v + (hid < p.cache.blocks ? hid : 0) * p.cache.block_stride + hpl * p.cache.token_stride +
-                                          c.h * p.cache.head_stride;
-                        for (int i = lane; i < kKvPage * D / 8; i += 32) {
-                            const int r = i / (D / 8), ch = i % (D / 8);
-                            uint4 v = make_uint4(0, 0, 0, 0);
-                            if (hid < p.cache.blocks && r < rest % kKvPage)
-                                v = *reinterpret_cast<const uint4*>(src + r * p.cache.token_stride + 16 * ch);
-                            const uint32_t o = dst + (ch / 8) * S::kBlock + (cut_page * kKvPage + r) * 128 + (((ch % 8) ^ (r & 7)) << 4);
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(o), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    }
-                    __syncwarp();
-                    if (lane == 0) bar_expect(full, S::kOperand - (by_hand ? kKvPage * D * 2 : 0));
-                    __syncwarp();
-                    const int page = lane % kPages, block = lane / kPages;
-                    if (block < S::kBlocks && !(by_hand && page == cut_page))
-                        tma_page(dst + block * S::kBlock + page * kKvPage * 128, which == 0 ? &map_k : &map_v, block * 64, c.h, in_block, id,
-                                 full);
-                    phase ^= 1u << slot;
-                    slot = slot + 1 == S::kSlots ? 0 : slot + 1;
-                }
+    if (warp < 8) {
+        // ---- softmax: one thread per packed row ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMain));
+        const int x = warp >> 2;
+        const int rr = t & (kHalf - 1);                                        // row of the half
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;  // this warp's lanes of tensor memory
+        const uint32_t ts = tmem + lanes + x * kTile, to = tmem + lanes + S::kO + x * D;
+        const int32_t base_key = p.shared_pass ? 0 : p.shared_len;
+        uint32_t s_phase = 0, ml_phase = 0;
+        int seen = 0;
+        Desc u;
+        while (take(&u)) {
+            if (x * kHalf >= u.packed) {  // this half has no rows
+                seen += u.nt;
+                continue;
             }
-            if (good) c.next(p);
-        }
-        if (!good) {
-            // the copies in flight land before the block ends: `full` flips once more for each slot
-            // that was filled and not yet waited for
-            for (int i = 0; i < S::kSlots; ++i) {
-                const uint64_t t0 = clock_ns();
-                while (!bar_try(smem_addr(&bars.full[i]), ((phase >> i) & 1u) ^ 1u) && clock_ns() - t0 < kWaitLimitNs) {
-                }
-            }
-        }
-    } else if (warp == 8) {
-        // ---- products ----
-        if (lane == 0) {
-            Cursor c;
-            c.enter(p, place, len);
-            int slot = 0;
-            uint32_t full_phase = 0, q_phase = 0, p_phase = 0;
+            int32_t pos;
+            const KvSpan sp = row_span(p, u, x * kHalf + rr, &pos, !kPlain);
+            float slope = 0.0f;
+            if (!kPlain && p.alibi != nullptr) slope = p.alibi[u.h * p.group + (u.packed0 + x * kHalf + rr) % p.group];
+            const float scale = kPlain ? p.scale2 : 1.0f;
+            float base = -INFINITY, l = 0.0f;  // the weights' base (2^base), -inf before the first key; their sum
             bool good = true;
+            for (int i = 0; i < u.nt; ++i, ++seen) {
+                good = bar_wait(smem_addr(&bars.s[x]), s_phase, gave_up);
+                s_phase ^= 1u;
+                if (!good) break;
+                tm_after();
+                const int32_t j0 = u.key(i);
+                const uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&s_bad[seen % kBadRing]);
+                const bool inside = (j0 >= sp.lo && j0 + kTile <= sp.hi) || sp.pre >= j0 + kTile;
+                const bool masked = __any_sync(0xffffffffu, !inside) || bad != 0;
+                uint32_t buf[2][32];
+                float m0 = -INFINITY, m1 = -INFINITY;
+                if (kPlain && !masked) {
+                    tm_ld32(ts, buf[0]);
+#pragma unroll
+                    for (int k = 0; k < kTile / 32; ++k) {
+                        uint32_t* z = buf[k & 1];
+                        tm_wait32(z);
+                        if (k + 1 < kTile / 32) tm_ld32(ts + 32 * (k + 1), buf[(k + 1) & 1]);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            m0 = max3(m0, __uint_as_float(z[e]), __uint_as_float(z[e + 1]));
+                            m1 = max3(m1, __uint_as_float(z[e + 2]), __uint_as_float(z[e + 3]));
+                        }
+                    }
+                } else {
+                    // what cap, bias and masks make of the scores goes back in place
+#pragma unroll 1
+                    for (int k = 0; k < kTile; k += 32) {
+                        uint32_t* z = buf[0];
+                        tm_ld32(ts + k, z);
+                        tm_wait32(z);
+                        if (!kPlain)
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                z[e] = __float_as_uint(kv_score2<false>(p, __uint_as_float(z[e]), slope, base_key + j0 + k + e - pos));
+                        if (masked) {
+                            const int32_t j = j0 + k;
+                            const uint32_t out0 = (bad >> (k / kKvPage)) & 1u, out1 = (bad >> (k / kKvPage + 1)) & 1u;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                const bool sees = (j + e < sp.pre || (j + e >= sp.lo && j + e < sp.hi)) && (e < kKvPage ? out0 : out1) == 0;
+                                z[e] = sees ? z[e] : 0xff800000u;
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) m0 = max3(m0, __uint_as_float(z[e]), __uint_as_float(z[e + 1]));
+                        tm_st32(ts + k, z);
+                    }
+                    tm_wait_st();
+                }
+                const float most = max3(m0, m1, m1);
+                if (!(most < INFINITY)) l = __int_as_float(0x7fffffff);  // a NaN or an infinity among the scores
+                const float top = most * scale - Shift<T>::value;
+                const bool grew = top > base + kGrow || (base == -INFINITY && top > -INFINITY);
+                if (__any_sync(0xffffffffu, grew)) {
+                    const float to_base = fmaxf(base, top);
+                    const float keep = to_base == -INFINITY ? 1.0f : fast_exp2(base - to_base);
+                    base = to_base;
+                    l *= keep;
+                    if (i > 0) {
+#pragma unroll 1
+                        for (int k = 0; k < D; k += 32) {
+                            uint32_t* o = buf[1];
+                            tm_ld32(to + k, o);
+                            tm_wait32(o);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tm_st32(to + k, o);
+                        }
+                    }
+                }
+                tm_ld32(ts, buf[0]);
+                const float less = base == -INFINITY ? 0.0f : -base;
+                const uint64_t scale_2 = pack2(scale, scale), less_2 = pack2(less, less);
+                uint64_t sum0 = 0, sum1 = 0;  // pairs of 0.0f
+#pragma unroll
+                for (int k = 0; k < kTile / 32; ++k) {
+                    const uint32_t* z = buf[k & 1];
+                    tm_wait32(buf[k & 1]);
+                    // the weights of columns 32 k .. 32 k + 31 take columns 16 k .. 16 k + 15, read before
+                    if (k + 1 < kTile / 32) tm_ld32(ts + 32 * (k + 1), buf[(k + 1) & 1]);
+                    uint32_t w[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        uint64_t y = fma2(pack2(__uint_as_float(z[2 * e]), __uint_as_float(z[2 * e + 1])), scale_2, less_2);
+                        float a, c;
+                        if (e % 16 < kByFma) {
+                            y = exp2_pair(y);
+                            unpack2(y, a, c);
+                        } else {
+                            unpack2(y, a, c);
+                            a = fast_exp2(a);
+                            c = fast_exp2(c);
+                            y = pack2(a, c);
+                        }
+                        if (e & 1) sum1 = add2(sum1, y);
+                        else sum0 = add2(sum0, y);
+                        w[e] = Pack<T>::pair(a, c);
+                    }
+                    tm_st16(ts + 16 * k, w);
+                }
+                {
+                    float a, c;
+                    unpack2(add2(sum0, sum1), a, c);
+                    l += a + c;
+                }
+                tm_wait_st();
+                tm_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(smem_addr(&bars.p[x]));
+            }
+            if (!good) break;
+            // base and sum go to the warps that write the rows
+            if (!bar_wait(smem_addr(&bars.ml_read[x]), ml_phase ^ 1u, gave_up)) break;
+            ml_phase ^= 1u;
+            s_base[x][rr] = base;
+            s_sum[x][rr] = l;
+            __syncwarp();
+            if (lane == 0) bar_arrive(smem_addr(&bars.ml[x]));
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAux));
+        if (warp < 12) {
+            // ---- finished rows ----
+            const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+            const uint32_t stage = sq + (2 + S::kSlots) * S::kOperand + (warp & 3) * kStageBytes;
+            uint32_t o_phase = 0;  // bit x
+            Desc u;
+            bool good = true;
+            while (good && take(&u)) {
+                const bool whole = u.nt == u.count;
+                float* slot = p.line.slots + (2 * static_cast<int64_t>(blockIdx.x) + (u.t0 == 0 ? 1 : 0)) * (static_cast<int64_t>(kRows) * (D + 2));
+                const bool wide = !whole || p.out_f32;  // 32-bit results
+                for (int x = 0; x * kHalf < u.packed; ++x) {
+                    const int rr = (warp & 3) * 32 + lane, r = x * kHalf + rr;
+                    const bool valid = r < u.packed;
+                    const int32_t packed = u.packed0 + (valid ? r : 0);
+                    const int32_t of = kv_div_group(p, packed);
+                    const int64_t row = u.row0 + of;
+                    const int32_t head = u.h * p.group + packed - of * p.group;
+                    uint64_t dst = 0;
+                    if (valid)
+                        dst = whole ? reinterpret_cast<uint64_t>(p.out.data + row * p.out.row_stride + head * p.out.head_stride)
+                                    : reinterpret_cast<uint64_t>(slot + static_cast<int64_t>(r) * D);
+                    uint64_t to_row[4];  // this lane writes rows lane / 4 + 8 i
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) to_row[i] = __shfl_sync(0xffffffffu, dst, lane / 4 + 8 * i);
+                    const uint32_t phase = (o_phase >> x) & 1u;
+                    o_phase ^= 1u << x;
+                    good = bar_wait(smem_addr(&bars.ml[x]), phase, gave_up) && bar_wait(smem_addr(&bars.o[x]), phase, gave_up);
+                    if (!good) break;
+                    tm_after();
+                    const float base = s_base[x][rr], l = s_sum[x][rr];
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(smem_addr(&bars.ml_read[x]));
+                    const float inv = !whole ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+                    float odd = 0.0f;  // NaN once a sum is not finite
+#pragma unroll 1
+                    for (int k = 0; k < D; k += 32) {
+                        uint32_t o[32];
+                        tm_ld32(tmem + lanes + S::kO + x * D + k, o);
+                        tm_wait32(o);
+                        if (k + 32 == D) {
+                            tm_before();
+                            __syncwarp();
+                            if (lane == 0) bar_arrive(smem_addr(&bars.o_read[x]));
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const float f = __uint_as_float(o[e]);
+                            odd = fmaf(f, 0.0f, odd);
+                            o[e] = __float_as_uint(f * inv);
+                        }
+                        // 64 bytes of every row at a time through shared memory, so that 4 lanes write
+                        // them side by side
+                        const int steps = wide ? 2 : 1;
+                        if (!wide)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = Pack<T>::pair(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
+                        for (int st = 0; st < steps; ++st) {
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) {
+                                const uint32_t* w = o + 4 * y;
+                                const bool up = st == 1;
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((y ^ ((lane >> 1) & 3)) << 4)),
+                                             "r"(up ? w[16] : w[0]), "r"(up ? w[17] : w[1]), "r"(up ? w[18] : w[2]), "r"(up ? w[19] : w[3])
+                                             : "memory");
+                            }
+                            __syncwarp();
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int rw = lane / 4 + 8 * i;
+                                uint4 v;
+                                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                             : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                             : "r"(stage + rw * 64 + (((lane & 3) ^ ((rw >> 1) & 3)) << 4))
+                                             : "memory");
+                                if (to_row[i] != 0) *reinterpret_cast<uint4*>(to_row[i] + (wide ? 4 : 2) * k + 64 * st + 16 * (lane & 3)) = v;
+                            }
+                            __syncwarp();
+                        }
+                    }
+                    if (valid) {
+                        if (whole) {
+                            if (p.lse != nullptr) p.lse[row * p.q_heads + head] = l == 0.0f ? -INFINITY : base * kLn2 + logf(l);
+                        } else {
+                            slot[static_cast<int64_t>(kRows) * D + r] = base;
+                            slot[static_cast<int64_t>(kRows) * D + kRows + r] = l;
+                        }
+                    }
+                    for (uint32_t redo = __ballot_sync(0xffffffffu, valid && odd != 0.0f); redo != 0; redo &= redo - 1) {
+                        const int src = __ffs(redo) - 1;
+                        KvExact y;
+                        y.table = p.shared_pass ? p.shared_table : b.table + u.s * b.table_stride;
+                        y.tiles = KvTiles{u.npre, u.first, u.count};
+                        y.seen = row_span(p, u, x * kHalf + (warp & 3) * 32 + src, &y.pos, true);
+                        y.base = p.shared_pass ? 0 : p.shared_len;
+                        y.t0 = u.t0;
+                        y.t1 = u.t0 + u.nt;
+                        y.size = kTile;
+                        y.row = __shfl_sync(0xffffffffu, row, src);
+                        y.head = __shfl_sync(0xffffffffu, head, src);
+                        y.kvh = u.h;
+                        const float rb = __shfl_sync(0xffffffffu, base, src), ri = __shfl_sync(0xffffffffu, inv, src);
+                        const uint64_t rd = __shfl_sync(0xffffffffu, dst, src);
+                        constexpr int kEach = D / 32;
+                        float part[kEach];
+                        kv_exact_row<T, D, kPlain>(p, y, rb, part);
+                        for (int e = 0; e < kEach; ++e) {
+                            if (wide) reinterpret_cast<float*>(rd)[lane * kEach + e] = part[e] * ri;
+                            else reinterpret_cast<T*>(rd)[lane * kEach + e] = static_cast<T>(part[e] * ri);
+                        }
+                    }
+                }
+            }
+        } else if (warp == 12) {
+            // ---- products ----
+            int slot = 0;
+            uint32_t full_phase = 0, q_phase = 0, p_phase = 0, or_phase = 0;
             constexpr uint32_t kQk = product<T>(kHalf, kTile, false);
             constexpr uint32_t kPv = product<T>(kHalf, D, true);
             auto scores = [&](int x, int k) {
@@ -516,271 +814,209 @@ __global__ void __launch_bounds__(kThreads, 1)
                            i > 0);
                 }
             };
-            while (good && !c.done) {
-                const int halves = c.u.packed > kHalf ? 2 : 1;
-                const int nt = c.end - c.t;
-                for (int x = 0; good && x < halves; ++x) {
-                    good = bar_wait(smem_addr(&bars.q[x]), (q_phase >> x) & 1u, gave_up);
-                    q_phase ^= 1u << x;
-                }
-                if (good) good = bar_wait(smem_addr(&bars.full[slot]), (full_phase >> slot) & 1u, gave_up);
-                if (!good) break;
-                tm_after();
-                for (int x = 0; x < halves; ++x) {
-                    scores(x, slot);
-                    tm_commit(smem_addr(&bars.s[x]));
-                }
-                tm_commit(smem_addr(&bars.empty[slot]));
-                full_phase ^= 1u << slot;
-                slot = slot + 1 == S::kSlots ? 0 : slot + 1;
-                for (int i = 0; good && i < nt; ++i) {
-                    const int v = slot, k = slot + 1 == S::kSlots ? 0 : slot + 1;
-                    good = bar_wait(smem_addr(&bars.full[v]), (full_phase >> v) & 1u, gave_up);
-                    full_phase ^= 1u << v;
+            Desc u;
+            bool good = true;
+            while (good && take(&u)) {
+                if (lane == 0) {
+                    const int halves = u.packed > kHalf ? 2 : 1;
+                    good = bar_wait(smem_addr(&bars.full[slot]), (full_phase >> slot) & 1u, gave_up);
                     for (int x = 0; good && x < halves; ++x) {
-                        good = bar_wait(smem_addr(&bars.p[x]), (p_phase >> x) & 1u, gave_up);
-                        p_phase ^= 1u << x;
+                        good = bar_wait(smem_addr(&bars.q[x]), (q_phase >> x) & 1u, gave_up);
+                        q_phase ^= 1u << x;
                         if (!good) break;
                         tm_after();
-#pragma unroll
-                        for (int j = 0; j < kTile / 16; ++j)
-                            mma_ts(tmem + S::kO + x * D, tmem + x * kTile + j * 8, operand(ring + v * S::kOperand + j * 2048, S::kBlock, 1024),
-                                   kPv, i > 0 || j > 0);
-                        if (x == halves - 1) tm_commit(smem_addr(&bars.empty[v]));
-                        if (i + 1 < nt) {
-                            if (x == 0) {
-                                good = bar_wait(smem_addr(&bars.full[k]), (full_phase >> k) & 1u, gave_up);
-                                full_phase ^= 1u << k;
+                        scores(x, slot);
+                        tm_commit(smem_addr(&bars.s[x]));
+                        if (u.nt == 1) tm_commit(smem_addr(&bars.q_read[x]));
+                    }
+                    if (good) tm_commit(smem_addr(&bars.empty[slot]));
+                    full_phase ^= 1u << slot;
+                    slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+                    for (int i = 0; good && i < u.nt; ++i) {
+                        const int v = slot, k = slot + 1 == S::kSlots ? 0 : slot + 1;
+                        good = bar_wait(smem_addr(&bars.full[v]), (full_phase >> v) & 1u, gave_up);
+                        full_phase ^= 1u << v;
+                        for (int x = 0; good && x < halves; ++x) {
+                            if (i == 0) {  // the last unit's sums have been taken
+                                good = bar_wait(smem_addr(&bars.o_read[x]), ((or_phase >> x) & 1u) ^ 1u, gave_up);
+                                or_phase ^= 1u << x;
                                 if (!good) break;
-                                tm_after();
                             }
-                            scores(x, k);
-                            tm_commit(smem_addr(&bars.s[x]));
-                            if (x == halves - 1) tm_commit(smem_addr(&bars.empty[k]));
-                        } else {
-                            tm_commit(smem_addr(&bars.o[x]));
+                            good = bar_wait(smem_addr(&bars.p[x]), (p_phase >> x) & 1u, gave_up);
+                            p_phase ^= 1u << x;
+                            if (!good) break;
+                            tm_after();
+#pragma unroll
+                            for (int j = 0; j < kTile / 16; ++j)
+                                mma_ts(tmem + S::kO + x * D, tmem + x * kTile + j * 8,
+                                       operand(ring + v * S::kOperand + j * 2048, S::kBlock, 1024), kPv, i > 0 || j > 0);
+                            if (x == halves - 1) tm_commit(smem_addr(&bars.empty[v]));
+                            if (i + 1 < u.nt) {
+                                if (x == 0) {
+                                    good = bar_wait(smem_addr(&bars.full[k]), (full_phase >> k) & 1u, gave_up);
+                                    full_phase ^= 1u << k;
+                                    if (!good) break;
+                                    tm_after();
+                                }
+                                scores(x, k);
+                                tm_commit(smem_addr(&bars.s[x]));
+                                if (i + 2 == u.nt) tm_commit(smem_addr(&bars.q_read[x]));
+                                if (x == halves - 1) tm_commit(smem_addr(&bars.empty[k]));
+                            } else {
+                                tm_commit(smem_addr(&bars.o[x]));
+                            }
+                        }
+                        slot = k;
+                        if (i + 1 < u.nt) slot = k + 1 == S::kSlots ? 0 : k + 1;
+                    }
+                }
+                good = __shfl_sync(0xffffffffu, good, 0);
+            }
+        } else if (warp == 13) {
+            // ---- K and V ----
+            int slot = 0, seen = 0;  // seen: tiles so far
+            uint32_t phase = 0;      // bit i: parity that slot i's `empty` has to reach
+            const int pages = p.cache.block_tokens / kKvPage;
+            Desc u;
+            bool good = true;
+            while (good && take(&u)) {
+                const int32_t* table = p.shared_pass ? p.shared_table : b.table + u.s * b.table_stride;
+                const int32_t n = u.keys;
+                for (int i = 0; good && i < u.nt; ++i, ++seen) {
+                    const int32_t j0 = u.key(i);
+                    // lane i: page i % 8 of the tile
+                    const int32_t j = j0 + (lane % kPages) * kKvPage;
+                    int32_t id = p.cache.blocks;  // a block outside the map: loads as zeros
+                    bool bad = false;
+                    if ((j < u.pre || (j + kKvPage > u.lo && j < u.hi)) && j < n) {
+                        id = table[j / kKvPage / pages];
+                        if (id < 0 || id >= p.cache.blocks) {
+                            bad = true;
+                            id = p.cache.blocks;
+                            kv_report(p.status, GFD_KV_BAD_PAGE);
                         }
                     }
-                    slot = k;
-                    if (i + 1 < nt) slot = k + 1 == S::kSlots ? 0 : k + 1;
+                    const int32_t in_block = (j / kKvPage % pages) * kKvPage;
+                    const uint32_t bad_pages = __ballot_sync(0xffffffffu, bad) & 0xffu;
+                    // a page that the sequence ends in: V's tokens behind the end are kept out by hand,
+                    // whatever lies there would meet weights of zero
+                    const int32_t rest = n - j0;
+                    const int cut_page = rest > 0 && rest < kTile && rest % kKvPage != 0 ? rest / kKvPage : -1;
+                    for (int which = 0; good && which < 2; ++which) {  // K, V
+                        const uint32_t full = smem_addr(&bars.full[slot]);
+                        good = bar_wait(smem_addr(&bars.empty[slot]), ((phase >> slot) & 1u) ^ 1u, gave_up);
+                        if (!good) break;
+                        const uint32_t dst = ring + slot * S::kOperand;
+                        const bool by_hand = which == 1 && cut_page >= 0;
+                        if (which == 0 && lane == 0) s_bad[seen % kBadRing] = bad_pages;
+                        if (by_hand) {
+                            const int32_t hid = __shfl_sync(0xffffffffu, id, cut_page), hpl = __shfl_sync(0xffffffffu, in_block, cut_page);
+                            const char* src = p.cache.v + (hid < p.cache.blocks ? hid : 0) * p.cache.block_stride +
+                                              hpl * p.cache.token_stride + u.h * p.cache.head_stride;
+                            for (int y = lane; y < kKvPage * D / 8; y += 32) {
+                                const int r = y / (D / 8), ch = y % (D / 8);
+                                uint4 v = make_uint4(0, 0, 0, 0);
+                                if (hid < p.cache.blocks && r < rest % kKvPage)
+                                    v = *reinterpret_cast<const uint4*>(src + r * p.cache.token_stride + 16 * ch);
+                                const uint32_t o = dst + (ch / 8) * S::kBlock + (cut_page * kKvPage + r) * 128 + (((ch % 8) ^ (r & 7)) << 4);
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(o), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                                             : "memory");
+                            }
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        }
+                        __syncwarp();
+                        if (lane == 0) bar_expect(full, S::kOperand - (by_hand ? kKvPage * D * 2 : 0));
+                        __syncwarp();
+                        const int page = lane % kPages, block = lane / kPages;
+                        if (block < S::kBlocks && !(by_hand && page == cut_page))
+                            tma_page(dst + block * S::kBlock + page * kKvPage * 128, which == 0 ? &map_k : &map_v, block * 64, u.h, in_block,
+                                     id, full);
+                        phase ^= 1u << slot;
+                        slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+                    }
                 }
-                if (good) c.next(p);
             }
-        }
-        __syncwarp();
-    } else {
-        // ---- softmax: one thread per packed row ----
-        const int x = warp >> 2;
-        const int rr = t & (kHalf - 1);                                        // row of the half
-        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;  // this warp's lanes of tensor memory
-        const uint32_t ts = tmem + lanes + x * kTile, to = tmem + lanes + S::kO + x * D;
-        Cursor c;
-        c.enter(p, place, len);
-        uint32_t s_phase = 0, o_phase = 0;
-        int seen = 0;
-        bool good = true;
-        while (good && !c.done) {
-            const int32_t t0 = c.t, nt = c.end - c.t;
-            if (x * kHalf >= c.u.packed) {  // this half has no rows
-                seen += nt;
+            if (*gave_up != 0) {
+                // the copies in flight land before the block ends: `full` flips once more for each slot
+                // that was filled and not yet waited for
+                for (int i = 0; i < S::kSlots; ++i) {
+                    const uint64_t t0 = clock_ns();
+                    while (!bar_try(smem_addr(&bars.full[i]), ((phase >> i) & 1u) ^ 1u) && clock_ns() - t0 < kWaitLimitNs) {
+                    }
+                }
+            }
+        } else if (warp == 14) {
+            // ---- Q: every row by neighbouring lanes, zeros for rows that do not exist ----
+            constexpr int kLanes = D / 8, kPer = 32 / kLanes;  // lanes of a row, rows a step
+            uint32_t phase = 0;                                // bit x
+            Desc u;
+            bool good = true;
+            while (good && take(&u)) {
+                for (int x = 0; x * kHalf < u.packed; ++x) {
+                    uint64_t src[4];  // rows lane + 32 i of the half
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = x * kHalf + 32 * i + lane;
+                        const int32_t packed = u.packed0 + r, of = kv_div_group(p, packed);
+                        src[i] = r < u.packed ? reinterpret_cast<uint64_t>(p.q.data + static_cast<int64_t>(u.row0 + of) * p.q.row_stride +
+                                                                           (u.h * p.group + packed - of * p.group) * p.q.head_stride)
+                                              : 0;
+                    }
+                    good = bar_wait(smem_addr(&bars.q_read[x]), ((phase >> x) & 1u) ^ 1u, gave_up);
+                    phase ^= 1u << x;
+                    if (!good) break;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int y = 0; y < 32 / kPer; ++y) {
+                            const int row = 32 * i + y * kPer + lane / kLanes, ch = lane % kLanes;
+                            const uint64_t at = __shfl_sync(0xffffffffu, src[i], y * kPer + lane / kLanes);
+                            const char* from = at != 0 ? reinterpret_cast<const char*>(at) + 16 * ch : p.q.data;
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                             sq + x * S::kOperand + (ch / 8) * S::kBlock + row * 128 + (((ch % 8) ^ (row & 7)) << 4)),
+                                         "l"(from), "r"(at != 0 ? 16 : 0)
+                                         : "memory");
+                        }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(smem_addr(&bars.q[x]));
+                }
+            }
+        } else {
+            // ---- the units of the stretch ----
+            Cursor c;
+            c.enter(p, s_place, len);
+            for (int i = 0;; ++i) {
+                const int k = i % kUnitRing;
+                if (!bar_wait(smem_addr(&bars.unit_read[k]), ((i / kUnitRing) & 1) ^ 1, gave_up)) break;
+                if (lane == 0) {
+                    Desc d{};
+                    if (!c.done) {
+                        d.s = c.s;
+                        d.h = c.h;
+                        d.t0 = c.t;
+                        d.nt = c.end - c.t;
+                        d.count = c.u.tiles.count;
+                        d.npre = c.u.tiles.npre;
+                        d.first = c.u.tiles.first;
+                        d.pre = c.u.all.pre;
+                        d.lo = c.u.all.lo;
+                        d.hi = c.u.all.hi;
+                        d.packed0 = c.u.packed0;
+                        d.packed = c.u.packed;
+                        d.row0 = c.m.q.row0;
+                        d.rows = c.m.q.rows;
+                        d.keys = c.m.q.keys;
+                        d.prefix = !p.shared_pass && p.prefix_len != nullptr ? p.prefix_len[c.s] : 0;
+                    }
+                    s_unit[k] = d;
+                    bar_arrive(smem_addr(&bars.unit[k]));
+                }
+                __syncwarp();
+                if (c.done) break;
                 c.next(p);
-                continue;
             }
-            const int r = x * kHalf + rr;  // row of the unit
-            const bool valid = r < c.u.packed;
-            const int32_t packed = c.u.packed0 + (valid ? r : 0);
-            const int64_t row = c.m.q.row0 + packed / p.group;
-            const int32_t head = c.h * p.group + packed % p.group;
-            // position and span; rows that do not exist see everything, of a zero query
-            int32_t pos = p.shared_len + c.m.q.keys - c.m.q.rows + packed / p.group;
-            const int32_t base_key = p.shared_pass ? 0 : p.shared_len;
-            KvSpan sp{0x7fffffff, 0, 0};
-            if (valid) {
-                int s = c.s;
-                int32_t n = p.shared_len + c.m.q.keys;
-                if (p.shared_pass) {
-                    pos = 0x3fffffff;
-                    n = p.shared_len;
-                    if (p.window > 0 || p.prefix_len != nullptr || !kPlain) {
-                        int lo = 0, hi = b.seqs - 1;
-                        while (lo < hi) {
-                            const int mid = (lo + hi + 1) / 2;
-                            if (b.row_start[mid] <= row) lo = mid;
-                            else hi = mid - 1;
-                        }
-                        s = lo;
-                        n = p.shared_len + b.kv_len[s];
-                        pos = n - (b.row_start[s + 1] - static_cast<int32_t>(row));
-                    }
-                }
-                sp = kv_clip(kv_span(pos, n, p.prefix_len != nullptr ? p.prefix_len[s] : 0, p.window, p.causal != 0), base_key, c.m.q.keys);
-            }
-            const float slope = !kPlain && p.alibi != nullptr ? p.alibi[head] : 0.0f;
-            // this row of Q; the sign of the scale goes into it
-            {
-                const char* src = p.q.data + row * p.q.row_stride + head * p.q.head_stride;
-                const uint32_t flip = kPlain && p.scale2 < 0.0f ? 0x80008000u : 0u;
-                const uint32_t dst = sq + x * S::kOperand + rr * 128;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (valid) v = *reinterpret_cast<const uint4*>(src + 16 * i);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (i / 8) * S::kBlock + (((i % 8) ^ (rr & 7)) << 4)),
-                                 "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip)
-                                 : "memory");
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                bar_arrive(smem_addr(&bars.q[x]));
-            }
-            const float scale = kPlain ? fabsf(p.scale2) : 1.0f;
-            float base = -INFINITY, l = 0.0f;  // the weights' base (2^base), -inf before the first key; their sum
-            for (int i = 0; i < nt; ++i, ++seen) {
-                good = bar_wait(smem_addr(&bars.s[x]), s_phase & 1u, gave_up);
-                s_phase ^= 1u;
-                if (!good) break;
-                tm_after();
-                const int32_t j0 = c.u.tiles.at(t0 + i) * kTile;
-                const uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&s_bad[seen % kBadRing]);
-                const bool inside = (j0 >= sp.lo && j0 + kTile <= sp.hi) || sp.pre >= j0 + kTile;
-                const bool masked = __any_sync(0xffffffffu, !inside) || bad != 0;
-                uint32_t buf[2][32];
-                // the scores' maximum; what cap, bias and masks make of them goes back in place
-                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                tm_ld32(ts, buf[0]);
-#pragma unroll
-                for (int k = 0; k < kTile / 32; ++k) {
-                    uint32_t* z = buf[k & 1];
-                    tm_wait32(z);
-                    if (k + 1 < kTile / 32) tm_ld32(ts + 32 * (k + 1), buf[(k + 1) & 1]);
-                    if (!kPlain)
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            z[e] = __float_as_uint(kv_score2<false>(p, __uint_as_float(z[e]), slope, base_key + j0 + 32 * k + e - pos));
-                    if (masked)
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const int32_t j = j0 + 32 * k + e;
-                            const bool sees = (j < sp.pre || (j >= sp.lo && j < sp.hi)) && !((bad >> ((32 * k + e) / kKvPage)) & 1u);
-                            z[e] = sees ? z[e] : 0xff800000u;
-                        }
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(z[e]));
-                    if (!kPlain || masked) tm_st32(ts + 32 * k, z);
-                }
-                if (!kPlain || masked) tm_wait_st();
-                const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale - Shift<T>::value;
-                const bool grew = top > base + kGrow || (base == -INFINITY && top > -INFINITY);
-                if (__any_sync(0xffffffffu, grew)) {
-                    const float to_base = fmaxf(base, top);
-                    const float keep = to_base == -INFINITY ? 1.0f : fast_exp2(base - to_base);
-                    base = to_base;
-                    l *= keep;
-                    if (i > 0) {
-                        for (int k = 0; k < D / 32; ++k) {
-                            uint32_t* o = buf[1];
-                            tm_ld32(to + 32 * k, o);
-                            tm_wait32(o);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                            tm_st32(to + 32 * k, o);
-                        }
-                    }
-                }
-                tm_ld32(ts, buf[0]);
-                const float less = base == -INFINITY ? 0.0f : base;
-                float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int k = 0; k < kTile / 32; ++k) {
-                    const uint32_t* z = buf[k & 1];
-                    tm_wait32(buf[k & 1]);
-                    // the weights of columns 32 k .. 32 k + 31 take columns 16 k .. 16 k + 15, read before
-                    if (k + 1 < kTile / 32) tm_ld32(ts + 32 * (k + 1), buf[(k + 1) & 1]);
-                    uint32_t w[16];
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const float a = fast_exp2(fmaf(__uint_as_float(z[e]), scale, -less));
-                        const float d = fast_exp2(fmaf(__uint_as_float(z[e + 1]), scale, -less));
-                        l4[(e / 2) & 3] += a + d;
-                        w[e / 2] = Pack<T>::pair(a, d);
-                    }
-                    tm_st16(ts + 16 * k, w);
-                }
-                l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-                tm_wait_st();
-                tm_before();
-                bar_arrive(smem_addr(&bars.p[x]));
-            }
-            if (!good) break;
-            good = bar_wait(smem_addr(&bars.o[x]), o_phase & 1u, gave_up);
-            o_phase ^= 1u;
-            if (!good) break;
-            tm_after();
-
-            // ---- the unit's rows ----
-            const bool whole = t0 == 0 && c.end == c.u.tiles.count;
-            float* slot = p.line.slots + (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0)) * (static_cast<int64_t>(kRows) * (D + 2));
-            const float inv = !whole ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
-            bool odd = false;
-            for (int k = 0; k < D / 32; ++k) {
-                uint32_t o[32];
-                tm_ld32(to + 32 * k, o);
-                tm_wait32(o);
-                float f[32];
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    f[e] = __uint_as_float(o[e]);
-                    odd |= !(fabsf(f[e]) < INFINITY);
-                    f[e] = l == 0.0f ? 0.0f : f[e] * inv;
-                }
-                if (valid) {
-                    if (whole) {
-                        kv_store_out<T>(p, row, head, 32 * k, f, 32);
-                    } else {
-                        for (int e = 0; e < 32; e += 4)
-                            *reinterpret_cast<float4*>(slot + static_cast<int64_t>(r) * D + 32 * k + e) = *reinterpret_cast<const float4*>(f + e);
-                    }
-                }
-            }
-            if (valid) {
-                if (whole) {
-                    if (p.lse != nullptr) p.lse[row * p.q_heads + head] = l == 0.0f ? -INFINITY : base * kLn2 + logf(l);
-                } else {
-                    slot[static_cast<int64_t>(kRows) * D + r] = base;
-                    slot[static_cast<int64_t>(kRows) * D + kRows + r] = l;
-                }
-            }
-            for (uint32_t redo = __ballot_sync(0xffffffffu, odd && valid && l != 0.0f); redo != 0; redo &= redo - 1) {
-                const int src = __ffs(redo) - 1;
-                KvExact y;
-                y.table = p.shared_pass ? p.shared_table : b.table + c.s * b.table_stride;
-                y.tiles = c.u.tiles;
-                y.seen = KvSpan{__shfl_sync(0xffffffffu, sp.pre, src), __shfl_sync(0xffffffffu, sp.lo, src), __shfl_sync(0xffffffffu, sp.hi, src)};
-                y.base = base_key;
-                y.pos = __shfl_sync(0xffffffffu, pos, src);
-                y.t0 = t0;
-                y.t1 = c.end;
-                y.size = kTile;
-                y.row = __shfl_sync(0xffffffffu, row, src);
-                y.head = __shfl_sync(0xffffffffu, head, src);
-                y.kvh = c.h;
-                const float rb = __shfl_sync(0xffffffffu, base, src), ri = __shfl_sync(0xffffffffu, inv, src);
-                const int rrow = __shfl_sync(0xffffffffu, r, src);
-                constexpr int kEach = D / 32;
-                float part[4];
-                kv_exact_row<T, D, kPlain>(p, y, rb, part);
-                for (int e = 0; e < kEach; ++e) {
-                    part[e] *= ri;
-                    if (!whole) {
-                        slot[static_cast<int64_t>(rrow) * D + lane * kEach + e] = part[e];
-                    } else {
-                        char* at = p.out.data + y.row * p.out.row_stride + y.head * p.out.head_stride;
-                        if (p.out_f32) reinterpret_cast<float*>(at)[lane * kEach + e] = part[e];
-                        else reinterpret_cast<T*>(at)[lane * kEach + e] = static_cast<T>(part[e]);
-                    }
-                }
-            }
-            tm_before();
-            c.next(p);
         }
     }
 
@@ -789,7 +1025,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tm_after();
     if (t == 0 && s_gave_up != 0) kv_report(p.status, GFD_KV_GAVE_UP);
-    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns) : "memory");
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns) : "memory");
 }
 
 // The cache's K or V as [blocks][tokens][heads][D], read in boxes of 16 tokens x 64 elements.
@@ -809,7 +1045,7 @@ bool make_map(CUtensorMap* map, const KvAttendParams& p, const char* base, int h
 
 template <typename T, int D>
 cudaError_t launch(const KvAttendParams& p, const CUtensorMap& k, const CUtensorMap& v, int ctas, cudaStream_t st) {
-    const bool plain = p.softcap == 0.0f && p.alibi == nullptr && p.scale2 != 0.0f;
+    const bool plain = p.softcap == 0.0f && p.alibi == nullptr && p.scale2 > 0.0f;
     auto* f = plain ? kv_prompt_kernel<T, D, true> : kv_prompt_kernel<T, D, false>;
     cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
     if (e != cudaSuccess) return e;
