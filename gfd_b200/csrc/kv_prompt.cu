@@ -124,17 +124,20 @@ __device__ __forceinline__ void tm_wait32(uint32_t* r) {
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tm_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok));
+    return ok != 0;
+}
 __device__ __forceinline__ void tm_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// Shared-memory operand in 128-byte swizzle: rows of 128 bytes in groups of 8 (1024 bytes).
-// group: bytes from one group of 8 rows to the next; block: bytes between 64-element blocks of a
-// row-major second operand's columns (not used by the K-major ones).
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t block, uint32_t group) {
-    return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | static_cast<uint64_t>(block >> 4) << 16 |
-           static_cast<uint64_t>(group >> 4) << 32 | 1ull << 46 | 2ull << 61;
-}
+// Shared-memory operand in 128-byte swizzle: rows of 128 bytes in groups of 8 (1024 bytes, the
+// stride in bits 32-45), descriptor version 1.  The low word holds the address, and for a row-major
+// second operand the bytes from one 64-element block of its columns to the next.
+constexpr uint32_t kOperandHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t operand(uint32_t addr, uint32_t block) { return (addr >> 4) | (block >> 4) << 16; }
 // 32-bit sums of 16-bit products; second operand's columns contiguous (trans) or not
 template <typename T>
 __device__ __forceinline__ constexpr uint32_t product(int m, int n, bool trans) {
@@ -142,15 +145,19 @@ __device__ __forceinline__ constexpr uint32_t product(int m, int n, bool trans) 
     return 1u << 4 | fmt << 7 | fmt << 10 | (trans ? 1u << 16 : 0u) | static_cast<uint32_t>(n >> 3) << 17 |
            static_cast<uint32_t>(m >> 4) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
-                 "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
-                 : "memory");
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .b64 x, y;\nmov.b64 x, {%1, %5};\nmov.b64 y, {%2, %5};\nsetp.ne.u32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(add ? 1u : 0u), "n"(kOperandHigh)
+        : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a),
-                 "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
-                 : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .b64 y;\nmov.b64 y, {%2, %5};\nsetp.ne.u32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(add ? 1u : 0u), "n"(kOperandHigh)
+        : "memory");
 }
 __device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, int x, int head, int place, int block, uint32_t bar) {
     asm volatile(
@@ -313,7 +320,7 @@ constexpr int kUnitReaders = 4 + 4 + 4 + 3;  // warps
 struct Bars {
     uint64_t full[4], empty[4];                       // K and V slots
     uint64_t unit[kUnitRing], unit_read[kUnitRing];
-    uint64_t q[2], q_read[2], s[2], p[2];             // Q there / products with it done, scores, weights
+    uint64_t q[2], q_read[2], s[2], p[2], p2[2];      // Q there / products with it done, scores, weights (two parts)
     uint64_t o[2], o_read[2], ml[2], ml_read[2];      // sums done / taken, their base and weight sum
 };
 
@@ -322,7 +329,7 @@ struct Shift {  // weights reach 2^(shift + 8): fp16 keeps them clear of its sma
     static constexpr float value = std::is_same<T, __half>::value ? 6.0f : 0.0f;
 };
 constexpr float kGrow = 8.0f;
-constexpr int kByFma = 4;  // of 16 pairs of exponentials, how many run on the FMA units
+constexpr int kByFma = 6;  // of 16 pairs of exponentials, how many run on the FMA units
 
 // Position of row r of the unit and what it sees of this pass's keys; rows that do not exist see
 // everything.  `exact`: the position itself is needed, not only the span.
@@ -431,6 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bar_init(smem_addr(&bars.q_read[i]), 1);
             bar_init(smem_addr(&bars.s[i]), 1);
             bar_init(smem_addr(&bars.p[i]), 4);
+            bar_init(smem_addr(&bars.p2[i]), 4);
             bar_init(smem_addr(&bars.o[i]), 1);
             bar_init(smem_addr(&bars.o_read[i]), 4);
             bar_init(smem_addr(&bars.ml[i]), 4);
@@ -665,16 +673,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                         w[e] = Pack<T>::pair(a, c);
                     }
                     tm_st16(ts + 16 * k, w);
+                    if (k & 1) {
+                        tm_wait_st();
+                        tm_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(smem_addr(k == 1 ? &bars.p[x] : &bars.p2[x]));
+                    }
                 }
                 {
                     float a, c;
                     unpack2(add2(sum0, sum1), a, c);
                     l += a + c;
                 }
-                tm_wait_st();
-                tm_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive(smem_addr(&bars.p[x]));
             }
             if (!good) break;
             // base and sum go to the warps that write the rows
@@ -801,76 +811,88 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         } else if (warp == 12) {
-            // ---- products ----
+            // ---- products: the whole warp walks, one thread issues ----
             int slot = 0;
             uint32_t full_phase = 0, q_phase = 0, p_phase = 0, or_phase = 0;
             constexpr uint32_t kQk = product<T>(kHalf, kTile, false);
             constexpr uint32_t kPv = product<T>(kHalf, D, true);
+            const uint32_t q_low = operand(sq, 16), k_low = operand(ring, 16), v_low = operand(ring, S::kBlock);
             auto scores = [&](int x, int k) {
+                const uint32_t a = q_low + x * (S::kOperand >> 4), c = k_low + k * (S::kOperand >> 4);
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {
-                    const uint32_t o = (i / 4) * S::kBlock + (i % 4) * 32;
-                    mma_ss(tmem + x * kTile, operand(sq + x * S::kOperand + o, 16, 1024), operand(ring + k * S::kOperand + o, 16, 1024), kQk,
-                           i > 0);
+                    constexpr int kStep = S::kBlock >> 4;
+                    mma_ss(tmem + x * kTile, a + (i / 4) * kStep + (i % 4) * 2, c + (i / 4) * kStep + (i % 4) * 2, kQk, i > 0);
                 }
+            };
+            auto sums = [&](int x, int v, int j0, int j1, bool add) {
+                const uint32_t c = v_low + v * (S::kOperand >> 4);
+#pragma unroll
+                for (int j = j0; j < j1; ++j) mma_ts(tmem + S::kO + x * D, tmem + x * kTile + j * 8, c + j * (2048 >> 4), kPv, add || j > 0);
             };
             Desc u;
             bool good = true;
             while (good && take(&u)) {
-                if (lane == 0) {
-                    const int halves = u.packed > kHalf ? 2 : 1;
-                    good = bar_wait(smem_addr(&bars.full[slot]), (full_phase >> slot) & 1u, gave_up);
-                    for (int x = 0; good && x < halves; ++x) {
-                        good = bar_wait(smem_addr(&bars.q[x]), (q_phase >> x) & 1u, gave_up);
-                        q_phase ^= 1u << x;
-                        if (!good) break;
-                        tm_after();
+                const int halves = u.packed > kHalf ? 2 : 1, nt = u.nt;
+                good = bar_wait(smem_addr(&bars.full[slot]), (full_phase >> slot) & 1u, gave_up);
+                for (int x = 0; good && x < halves; ++x) {
+                    good = bar_wait(smem_addr(&bars.q[x]), (q_phase >> x) & 1u, gave_up);
+                    q_phase ^= 1u << x;
+                    if (!good) break;
+                    tm_after();
+                    if (elect_one()) {
                         scores(x, slot);
                         tm_commit(smem_addr(&bars.s[x]));
-                        if (u.nt == 1) tm_commit(smem_addr(&bars.q_read[x]));
+                        if (nt == 1) tm_commit(smem_addr(&bars.q_read[x]));
+                        if (x == halves - 1) tm_commit(smem_addr(&bars.empty[slot]));
                     }
-                    if (good) tm_commit(smem_addr(&bars.empty[slot]));
-                    full_phase ^= 1u << slot;
-                    slot = slot + 1 == S::kSlots ? 0 : slot + 1;
-                    for (int i = 0; good && i < u.nt; ++i) {
-                        const int v = slot, k = slot + 1 == S::kSlots ? 0 : slot + 1;
-                        good = bar_wait(smem_addr(&bars.full[v]), (full_phase >> v) & 1u, gave_up);
-                        full_phase ^= 1u << v;
-                        for (int x = 0; good && x < halves; ++x) {
-                            if (i == 0) {  // the last unit's sums have been taken
-                                good = bar_wait(smem_addr(&bars.o_read[x]), ((or_phase >> x) & 1u) ^ 1u, gave_up);
-                                or_phase ^= 1u << x;
-                                if (!good) break;
-                            }
-                            good = bar_wait(smem_addr(&bars.p[x]), (p_phase >> x) & 1u, gave_up);
-                            p_phase ^= 1u << x;
+                    __syncwarp();
+                }
+                full_phase ^= 1u << slot;
+                slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+                for (int i = 0; good && i < nt; ++i) {
+                    const int v = slot, k = slot + 1 == S::kSlots ? 0 : slot + 1;
+                    const bool more = i + 1 < nt;
+                    good = bar_wait(smem_addr(&bars.full[v]), (full_phase >> v) & 1u, gave_up);
+                    full_phase ^= 1u << v;
+                    for (int x = 0; good && x < halves; ++x) {
+                        if (i == 0) {  // the last unit's sums have been taken
+                            good = bar_wait(smem_addr(&bars.o_read[x]), ((or_phase >> x) & 1u) ^ 1u, gave_up);
+                            or_phase ^= 1u << x;
                             if (!good) break;
-                            tm_after();
-#pragma unroll
-                            for (int j = 0; j < kTile / 16; ++j)
-                                mma_ts(tmem + S::kO + x * D, tmem + x * kTile + j * 8,
-                                       operand(ring + v * S::kOperand + j * 2048, S::kBlock, 1024), kPv, i > 0 || j > 0);
+                        }
+                        // the weights come in two parts of 64 keys
+                        good = bar_wait(smem_addr(&bars.p[x]), (p_phase >> x) & 1u, gave_up);
+                        if (!good) break;
+                        tm_after();
+                        if (elect_one()) sums(x, v, 0, kTile / 32, i > 0);
+                        __syncwarp();
+                        good = bar_wait(smem_addr(&bars.p2[x]), (p_phase >> x) & 1u, gave_up);
+                        p_phase ^= 1u << x;
+                        if (!good) break;
+                        if (more && x == 0) {
+                            good = bar_wait(smem_addr(&bars.full[k]), (full_phase >> k) & 1u, gave_up);
+                            full_phase ^= 1u << k;
+                            if (!good) break;
+                        }
+                        tm_after();
+                        if (elect_one()) {
+                            sums(x, v, kTile / 32, kTile / 16, true);
                             if (x == halves - 1) tm_commit(smem_addr(&bars.empty[v]));
-                            if (i + 1 < u.nt) {
-                                if (x == 0) {
-                                    good = bar_wait(smem_addr(&bars.full[k]), (full_phase >> k) & 1u, gave_up);
-                                    full_phase ^= 1u << k;
-                                    if (!good) break;
-                                    tm_after();
-                                }
+                            if (more) {
                                 scores(x, k);
                                 tm_commit(smem_addr(&bars.s[x]));
-                                if (i + 2 == u.nt) tm_commit(smem_addr(&bars.q_read[x]));
+                                if (i + 2 == nt) tm_commit(smem_addr(&bars.q_read[x]));
                                 if (x == halves - 1) tm_commit(smem_addr(&bars.empty[k]));
                             } else {
                                 tm_commit(smem_addr(&bars.o[x]));
                             }
                         }
-                        slot = k;
-                        if (i + 1 < u.nt) slot = k + 1 == S::kSlots ? 0 : k + 1;
+                        __syncwarp();
                     }
+                    slot = k;
+                    if (more) slot = k + 1 == S::kSlots ? 0 : k + 1;
                 }
-                good = __shfl_sync(0xffffffffu, good, 0);
             }
         } else if (warp == 13) {
             // ---- K and V ----
