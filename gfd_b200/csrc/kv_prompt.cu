@@ -13,9 +13,6 @@
 // of O is rare.  Sums and maxima are 32-bit; the weights' rounding to the 16-bit type for the
 // second product is the only one before the result's.
 //
-// The exponentials bound the softmax (16 a cycle and SM against 4096 products): a part of them
-// runs as a polynomial on the FMA units instead (exp2_pair).
-//
 // Roles: warps 0-3 softmax of half A, 4-7 of half B; 8-11 write finished rows while the softmax
 // is in the next unit; 12 issues the products, 13 loads K and V (TMA boxes of 16 tokens x 64
 // elements, so that every page is found by its id), 14 loads Q, 15 walks the units.  Units lie
@@ -36,8 +33,10 @@ constexpr int kHalf = 128;          // rows of a half: one tensor-core tile
 constexpr int kTile = 128;          // keys of a step
 constexpr int kPages = kTile / kKvPage;
 constexpr int kThreads = 512;
-constexpr int kAux = 88, kMain = 168;  // registers of the helpers' and the softmax warps: 256 x (88 + 168) = 64 K
+constexpr int kAux = 80, kMain = 176;  // registers of the helpers' and the softmax warps: 256 x (80 + 176) = 64 K
 constexpr int kStageBytes = 32 * 64; // a softmax warp's room for results on their way out
+// On the line every unit is as much longer than its tiles: what beginning and finishing one costs.
+constexpr int kUnitCost = 3;
 constexpr int kBadRing = 8;         // tiles whose bad pages are remembered
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -94,22 +93,19 @@ __device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t* r) {
           "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
-__device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
-        "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
-        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
-        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
-        "r"(addr)
-        : "memory");
-}
 __device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
         "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
         "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
         : "memory");
+}
+__device__ __forceinline__ void tm_ld16(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
 }
 // waits for the loads issued so far; r, loaded by one of them, is not read before
 __device__ __forceinline__ void tm_wait32(uint32_t* r) {
@@ -118,6 +114,13 @@ __device__ __forceinline__ void tm_wait32(uint32_t* r) {
                    "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
                    "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
                    "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tm_wait16(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), 
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                  :
                  : "memory");
 }
@@ -224,27 +227,29 @@ __device__ __forceinline__ Unit many_unit(const KvAttendParams& p, int s, const 
 struct Cursor {
     Many m;
     Unit u;
-    int32_t s, h, rt, t, end;
-    int64_t left;
+    int32_t s, h, rt, t, end;  // tiles [t, end) of the unit lie in the stretch
+    int64_t begin, to;         // of the unit's first tile, and of the stretch's end, on the line
     bool done;
 
-    __device__ __forceinline__ void enter(const KvAttendParams& p, const KvPlace& at, int64_t len) {
+    __device__ __forceinline__ void enter(const KvAttendParams& p, const KvPlace& at, int64_t to_) {
         s = at.s;
         h = at.h;
         rt = at.packed0 / kRows;
         t = at.t;
+        begin = at.begin;
+        to = to_;
         m = many_seq(p, s);
         u = many_unit(p, s, m.q, rt);
-        clamp(len);
+        clamp();
     }
-    __device__ __forceinline__ void clamp(int64_t l) {
-        done = l <= 0;
-        end = static_cast<int32_t>(min(static_cast<int64_t>(u.tiles.count), t + l));
-        left = l - (end - t);
+    __device__ __forceinline__ void clamp() {
+        end = static_cast<int32_t>(min(static_cast<int64_t>(u.tiles.count), max(to - begin, static_cast<int64_t>(0))));
+        done = t >= end;
     }
     // The line runs over KV heads, within a head over sequences, within a sequence over row tiles.
     __device__ __forceinline__ void next(const KvAttendParams& p) {
-        if (left <= 0) {
+        begin += u.tiles.count + kUnitCost;
+        if (begin >= to) {
             done = true;
             return;
         }
@@ -260,7 +265,7 @@ struct Cursor {
             } while (m.tiles == 0);
         }
         u = many_unit(p, s, m.q, rt);
-        clamp(left);
+        clamp();
     }
 };
 
@@ -320,7 +325,7 @@ constexpr int kUnitReaders = 4 + 4 + 4 + 3;  // warps
 struct Bars {
     uint64_t full[4], empty[4];                       // K and V slots
     uint64_t unit[kUnitRing], unit_read[kUnitRing];
-    uint64_t q[2], q_read[2], s[2], p[2], p2[2];      // Q there / products with it done, scores, weights (two parts)
+    uint64_t q[2], q_read[2], s[2], p[2], p2[2];      // Q there / products with it done, scores, weights in two parts
     uint64_t o[2], o_read[2], ml[2], ml_read[2];      // sums done / taken, their base and weight sum
 };
 
@@ -329,7 +334,7 @@ struct Shift {  // weights reach 2^(shift + 8): fp16 keeps them clear of its sma
     static constexpr float value = std::is_same<T, __half>::value ? 6.0f : 0.0f;
 };
 constexpr float kGrow = 8.0f;
-constexpr int kByFma = 6;  // of 16 pairs of exponentials, how many run on the FMA units
+
 
 // Position of row r of the unit and what it sees of this pass's keys; rows that do not exist see
 // everything.  `exact`: the position itself is needed, not only the span.
@@ -361,10 +366,7 @@ __device__ __forceinline__ KvSpan row_span(const KvAttendParams& p, const Desc& 
     return kv_clip(kv_span(*pos, n, prefix, p.window, p.causal != 0), p.shared_pass ? 0 : p.shared_len, u.keys);
 }
 
-// 2^x for two arguments of at most 2^7, on the FMA units: x = n + r with |r| <= 1/2 (n by adding 1.5 * 2^23),
-// a polynomial of degree 5 for 2^r (least largest relative error with a constant of 1: 2^-23.3,
-// 2^-22.3 with the roundings), n added to the exponent.  Below -127 the result is 0 (n = -127
-// takes 1 to 0).  Not for NaN: the caller sees those in the maximum.
+// Pairs of 32-bit numbers, one instruction for both.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -381,22 +383,8 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
-    float a, b;
-    unpack2(x, a, b);
-    x = pack2(fmaxf(a, -127.0f), fmaxf(b, -127.0f));
-    const uint64_t n = add2(x, pack2(12582912.0f, 12582912.0f));
-    const uint64_t r = add2(x, fma2(n, pack2(-1.0f, -1.0f), pack2(12582912.0f, 12582912.0f)));
-    uint64_t y = fma2(r, pack2(0.001326472731307149f, 0.001326472731307149f), pack2(0.009671512991189957f, 0.009671512991189957f));
-    y = fma2(y, r, pack2(0.05550733581185341f, 0.05550733581185341f));
-    y = fma2(y, r, pack2(0.24022242426872253f, 0.24022242426872253f));
-    y = fma2(y, r, pack2(0.6931470036506653f, 0.6931470036506653f));
-    y = fma2(y, r, pack2(1.0f, 1.0f));
-    float ya, yb, na, nb;
-    unpack2(y, ya, yb);
-    unpack2(n, na, nb);
-    return pack2(__uint_as_float(__float_as_uint(ya) + (__float_as_uint(na) << 23)), __uint_as_float(__float_as_uint(yb) + (__float_as_uint(nb) << 23)));
-}
+// the n lowest bits, n clamped to 0 .. 32
+__device__ __forceinline__ uint32_t below(int32_t n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 // largest of three; NaN if one is
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
@@ -417,6 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ uint32_t s_bad[kBadRing];
     __shared__ Desc s_unit[kUnitRing];
     __shared__ float s_base[2][kHalf], s_sum[2][kHalf];
+    __shared__ const char* s_rows[kRows];
     char* smem = reinterpret_cast<char*>((reinterpret_cast<uint64_t>(smem_raw) + 1023) & ~1023ull);
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const KvBatchView& b = p.batch;
@@ -449,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 
     // ---- this CTA's stretch of the line ----
-    int64_t len = 0;
+    int64_t stretch_end = 0;
     {
         const bool ok = kv_starts_ok(b);  // syncs
         if (!ok && blockIdx.x == 0 && t == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
@@ -495,18 +484,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const Unit x = many_unit(p, s, m.q, rt);
                 if (pass == 1 && !none) {
                     const int64_t want = at % per_head, here = mine + sum;
-                    if (want >= here && want < here + x.tiles.count) {
+                    if (want >= here && want < here + x.tiles.count + kUnitCost) {
                         s_place.s = s;
                         s_place.h = static_cast<int32_t>(at / per_head);
-                        s_place.t = static_cast<int32_t>(want - here);
+                        s_place.t = static_cast<int32_t>(max(want - here - kUnitCost, static_cast<int64_t>(0)));
                         s_place.count = x.tiles.count;
-                        s_place.begin = at - (want - here);
+                        s_place.begin = at - (want - here) + kUnitCost;
                         s_place.row0 = m.q.row0;
                         s_place.packed0 = x.packed0;
                         s_place.packed = x.packed;
                     }
                 }
-                sum += x.tiles.count;
+                sum += x.tiles.count + kUnitCost;
             }
             if (pass == 0) {
                 mine = cta_scan(sum, s_warps, &per_head) - sum;
@@ -515,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 none = static_cast<int>(blockIdx.x) >= cuts.n();
                 if (!none) {
                     at = cuts.at(blockIdx.x);
-                    len = cuts.at(blockIdx.x + 1) - at;
+                    stretch_end = cuts.at(blockIdx.x + 1);
                 }
             }
         }
@@ -525,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             p.line.places[blockIdx.x] = s_place;
         }
     }
-    if (len <= 0) return;
+    if (stretch_end == 0) return;
 
     if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(S::kColumns)
@@ -582,48 +571,34 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t bad = *reinterpret_cast<volatile uint32_t*>(&s_bad[seen % kBadRing]);
                 const bool inside = (j0 >= sp.lo && j0 + kTile <= sp.hi) || sp.pre >= j0 + kTile;
                 const bool masked = __any_sync(0xffffffffu, !inside) || bad != 0;
-                uint32_t buf[2][32];
-                float m0 = -INFINITY, m1 = -INFINITY;
-                if (kPlain && !masked) {
-                    tm_ld32(ts, buf[0]);
+                uint32_t z[kTile];
 #pragma unroll
-                    for (int k = 0; k < kTile / 32; ++k) {
-                        uint32_t* z = buf[k & 1];
-                        tm_wait32(z);
-                        if (k + 1 < kTile / 32) tm_ld32(ts + 32 * (k + 1), buf[(k + 1) & 1]);
+                for (int k = 0; k < kTile; k += 32) tm_ld32(ts + k, z + k);
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            m0 = max3(m0, __uint_as_float(z[e]), __uint_as_float(z[e + 1]));
-                            m1 = max3(m1, __uint_as_float(z[e + 2]), __uint_as_float(z[e + 3]));
-                        }
-                    }
-                } else {
-                    // what cap, bias and masks make of the scores goes back in place
-#pragma unroll 1
+                for (int k = 0; k < kTile; k += 32) tm_wait32(z + k);
+                if (!kPlain)
+#pragma unroll
+                    for (int e = 0; e < kTile; ++e)
+                        z[e] = __float_as_uint(kv_score2<false>(p, __uint_as_float(z[e]), slope, base_key + j0 + e - pos));
+                if (masked)
+#pragma unroll
                     for (int k = 0; k < kTile; k += 32) {
-                        uint32_t* z = buf[0];
-                        tm_ld32(ts + k, z);
-                        tm_wait32(z);
-                        if (!kPlain)
+                        const int32_t j = j0 + k;
+                        const uint32_t out = (((bad >> (k / kKvPage)) & 1u) ? 0x0000ffffu : 0u) | (((bad >> (k / kKvPage)) & 2u) ? 0xffff0000u : 0u);
+                        const uint32_t sees = (below(sp.pre - j) | (below(sp.hi - j) & ~below(sp.lo - j))) & ~out;
 #pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                z[e] = __float_as_uint(kv_score2<false>(p, __uint_as_float(z[e]), slope, base_key + j0 + k + e - pos));
-                        if (masked) {
-                            const int32_t j = j0 + k;
-                            const uint32_t out0 = (bad >> (k / kKvPage)) & 1u, out1 = (bad >> (k / kKvPage + 1)) & 1u;
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const bool sees = (j + e < sp.pre || (j + e >= sp.lo && j + e < sp.hi)) && (e < kKvPage ? out0 : out1) == 0;
-                                z[e] = sees ? z[e] : 0xff800000u;
-                            }
-                        }
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) m0 = max3(m0, __uint_as_float(z[e]), __uint_as_float(z[e + 1]));
-                        tm_st32(ts + k, z);
+                        for (int e = 0; e < 32; ++e) z[k + e] = (sees & (1u << e)) != 0 ? z[k + e] : 0xff800000u;
                     }
-                    tm_wait_st();
-                }
-                const float most = max3(m0, m1, m1);
+                float m8[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m8[e] = __uint_as_float(z[e]);
+#pragma unroll
+                for (int e = 8; e < 120; e += 16)
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) m8[y] = max3(m8[y], __uint_as_float(z[e + 2 * y]), __uint_as_float(z[e + 2 * y + 1]));
+#pragma unroll
+                for (int y = 0; y < 4; ++y) m8[y] = max3(m8[y], __uint_as_float(z[120 + 2 * y]), __uint_as_float(z[121 + 2 * y]));
+                const float most = max3(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], m8[5]), max3(m8[6], m8[7], m8[7]));
                 if (!(most < INFINITY)) l = __int_as_float(0x7fffffff);  // a NaN or an infinity among the scores
                 const float top = most * scale - Shift<T>::value;
                 const bool grew = top > base + kGrow || (base == -INFINITY && top > -INFINITY);
@@ -634,50 +609,38 @@ __global__ void __launch_bounds__(kThreads, 1)
                     l *= keep;
                     if (i > 0) {
 #pragma unroll 1
-                        for (int k = 0; k < D; k += 32) {
-                            uint32_t* o = buf[1];
-                            tm_ld32(to + k, o);
-                            tm_wait32(o);
+                        for (int k = 0; k < D; k += 16) {
+                            uint32_t o[16];
+                            tm_ld16(to + k, o);
+                            tm_wait16(o);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                            tm_st32(to + k, o);
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tm_st16(to + k, o);
                         }
                     }
                 }
-                tm_ld32(ts, buf[0]);
                 const float less = base == -INFINITY ? 0.0f : -base;
                 const uint64_t scale_2 = pack2(scale, scale), less_2 = pack2(less, less);
                 uint64_t sum0 = 0, sum1 = 0;  // pairs of 0.0f
 #pragma unroll
-                for (int k = 0; k < kTile / 32; ++k) {
-                    const uint32_t* z = buf[k & 1];
-                    tm_wait32(buf[k & 1]);
-                    // the weights of columns 32 k .. 32 k + 31 take columns 16 k .. 16 k + 15, read before
-                    if (k + 1 < kTile / 32) tm_ld32(ts + 32 * (k + 1), buf[(k + 1) & 1]);
+                for (int k = 0; k < kTile; k += 32) {
                     uint32_t w[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        uint64_t y = fma2(pack2(__uint_as_float(z[2 * e]), __uint_as_float(z[2 * e + 1])), scale_2, less_2);
                         float a, c;
-                        if (e % 16 < kByFma) {
-                            y = exp2_pair(y);
-                            unpack2(y, a, c);
-                        } else {
-                            unpack2(y, a, c);
-                            a = fast_exp2(a);
-                            c = fast_exp2(c);
-                            y = pack2(a, c);
-                        }
-                        if (e & 1) sum1 = add2(sum1, y);
-                        else sum0 = add2(sum0, y);
+                        unpack2(fma2(pack2(__uint_as_float(z[k + 2 * e]), __uint_as_float(z[k + 2 * e + 1])), scale_2, less_2), a, c);
+                        a = fast_exp2(a);
+                        c = fast_exp2(c);
+                        if (e & 1) sum1 = add2(sum1, pack2(a, c));
+                        else sum0 = add2(sum0, pack2(a, c));
                         w[e] = Pack<T>::pair(a, c);
                     }
-                    tm_st16(ts + 16 * k, w);
-                    if (k & 1) {
+                    tm_st16(ts + k / 2, w);
+                    if (k == 32 || k == 96) {
                         tm_wait_st();
                         tm_before();
                         __syncwarp();
-                        if (lane == 0) bar_arrive(smem_addr(k == 1 ? &bars.p[x] : &bars.p2[x]));
+                        if (lane == 0) bar_arrive(smem_addr(k == 32 ? &bars.p[x] : &bars.p2[x]));
                     }
                 }
                 {
@@ -970,35 +933,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else if (warp == 14) {
             // ---- Q: every row by neighbouring lanes, zeros for rows that do not exist ----
             constexpr int kLanes = D / 8, kPer = 32 / kLanes;  // lanes of a row, rows a step
+            const int ch = lane % kLanes, sub = lane / kLanes;
+            const uint32_t to = sq + (ch / 8) * S::kBlock + sub * 128;
             uint32_t phase = 0;                                // bit x
             Desc u;
             bool good = true;
             while (good && take(&u)) {
-                for (int x = 0; x * kHalf < u.packed; ++x) {
-                    uint64_t src[4];  // rows lane + 32 i of the half
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = x * kHalf + 32 * i + lane;
-                        const int32_t packed = u.packed0 + r, of = kv_div_group(p, packed);
-                        src[i] = r < u.packed ? reinterpret_cast<uint64_t>(p.q.data + static_cast<int64_t>(u.row0 + of) * p.q.row_stride +
-                                                                           (u.h * p.group + packed - of * p.group) * p.q.head_stride)
-                                              : 0;
-                    }
+                // where the unit's rows lie, and a start on bringing them into L2
+                __syncwarp();
+                for (int r = lane; r < u.packed; r += 32) {
+                    const int32_t packed = u.packed0 + r, of = kv_div_group(p, packed);
+                    const char* at = p.q.data + static_cast<int64_t>(u.row0 + of) * p.q.row_stride +
+                                     (u.h * p.group + packed - of * p.group) * p.q.head_stride;
+                    s_rows[r] = at;
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+                    if (D == 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + 128));
+                }
+                __syncwarp();
+                for (int x = 0; good && x * kHalf < u.packed; ++x) {
                     good = bar_wait(smem_addr(&bars.q_read[x]), ((phase >> x) & 1u) ^ 1u, gave_up);
                     phase ^= 1u << x;
                     if (!good) break;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int y = 0; y < 32 / kPer; ++y) {
-                            const int row = 32 * i + y * kPer + lane / kLanes, ch = lane % kLanes;
-                            const uint64_t at = __shfl_sync(0xffffffffu, src[i], y * kPer + lane / kLanes);
-                            const char* from = at != 0 ? reinterpret_cast<const char*>(at) + 16 * ch : p.q.data;
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                             sq + x * S::kOperand + (ch / 8) * S::kBlock + row * 128 + (((ch % 8) ^ (row & 7)) << 4)),
-                                         "l"(from), "r"(at != 0 ? 16 : 0)
-                                         : "memory");
-                        }
+                    const int n = min(kHalf, u.packed - x * kHalf);
+#pragma unroll 8
+                    for (int y = 0; y < kHalf; y += kPer) {
+                        const char* at = p.q.data;
+                        const bool live = y + sub < n;
+                        if (live) at = s_rows[x * kHalf + y + sub] + 16 * ch;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + x * S::kOperand + y * 128 +
+                                                                                           (((ch % 8) ^ ((y + sub) & 7)) << 4)),
+                                     "l"(at), "r"(live ? 16 : 0)
+                                     : "memory");
+                    }
                     asm volatile("cp.async.wait_all;" ::: "memory");
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
@@ -1008,7 +974,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
             // ---- the units of the stretch ----
             Cursor c;
-            c.enter(p, s_place, len);
+            c.enter(p, s_place, stretch_end);
             for (int i = 0;; ++i) {
                 const int k = i % kUnitRing;
                 if (!bar_wait(smem_addr(&bars.unit_read[k]), ((i / kUnitRing) & 1) ^ 1, gave_up)) break;
