@@ -75,7 +75,8 @@ struct KvAttendParams {
     int32_t max_q_len, causal, window;
     float scale, softcap;
     float scale2;    // scale in base 2
-    float cap_rate;  // 2 log2(e) / softcap
+    float cap_x;     // scale / softcap
+    float cap2;      // softcap in base 2
     int32_t out_f32;
     int32_t shared_pass;  // kv_prompt: all rows against the shared prefix
     KvLine line;

@@ -200,7 +200,8 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
     p.scale = a->scale;
     p.softcap = a->softcap;
     p.scale2 = a->scale * 1.4426950408889634f;
-    p.cap_rate = a->softcap > 0.0f ? 2.0f * 1.4426950408889634f / a->softcap : 0.0f;
+    p.cap_x = a->softcap > 0.0f ? a->scale / a->softcap : 0.0f;
+    p.cap2 = a->softcap * 1.4426950408889634f;
     p.out_f32 = a->out_dtype == GFD_FP32;
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
     char* ws = static_cast<char*>(a->workspace);

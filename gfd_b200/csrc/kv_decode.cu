@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
             sp[x] = KvSpan{0, 0, 0};
             if (r < rows) {
                 sp[x] = kv_clip(kv_span(pos[x], n, prefix, p.window, p.causal != 0), p.shared_len, use.q.q.keys);
-                if (!kPlain && p.alibi != nullptr) slope[x] = p.alibi[head];
+                if (!kPlain && p.alibi != nullptr) slope[x] = p.alibi[head] * kLog2e;
             }
             const char* src = p.q.data + (use.q.q.row0 + i) * p.q.row_stride + head * p.q.head_stride + 4 * (lane & 3);
 #pragma unroll
@@ -341,6 +341,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
                 }
                 const int32_t j0 = use.q.tiles.at(use.t) * kTile + warp * kKvPage + 2 * (lane & 3);
                 float mx[2] = {-INFINITY, -INFINITY};
+                if (!kPlain) kv_cap<8>(p, reinterpret_cast<uint32_t*>(&z[0][0]));
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
                         const int x = e >> 1;
                         const int32_t j = j0 + 8 * nt + (e & 1);
                         const bool seen = j < sp[x].pre || (j >= sp[x].lo && j < sp[x].hi);
-                        const float v = kv_score2<kPlain>(p, z[nt][e], slope[x], p.shared_len + j - pos[x]);
+                        const float v = kPlain ? z[nt][e] * p.scale2 : fmaf(slope[x], static_cast<float>(p.shared_len + j - pos[x]), z[nt][e]);
                         z[nt][e] = seen ? v : -INFINITY;
                         mx[x] = fmaxf(mx[x], z[nt][e]);
                     }

@@ -119,18 +119,77 @@ __device__ __forceinline__ void kv_store_out(const KvAttendParams& p, int64_t ro
     }
 }
 
-// Score in base 2: scale and cap of the product, bias by distance.
+// Pairs of 32-bit numbers, one instruction for both.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// cap * tanh(x) in base 2 for any x: tanh x = 1 - 2 / (1 + e^2x), to about 2^-21
+__device__ __forceinline__ float kv_tanh2(const KvAttendParams& p, float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + fast_exp2(x * (2.0f * kLog2e))));
+    return fmaf(-2.0f * p.cap2, r, p.cap2);
+}
+
+// N products of queries and keys to scores in base 2: scaled, capped where the call has a cap.
+// Where the warp's products all lie within the cap (|x| <= 1, the usual case) tanh x is x P(x^2)
+// on the FMA units, P of degree 5 by least largest error (2^-22; 2^-21.6 with the roundings):
+// the special-function unit, which the exponentials need, is left out.
+template <int N>
+__device__ __forceinline__ void kv_cap(const KvAttendParams& p, uint32_t* z) {
+    if (p.softcap > 0.0f) {
+        float m = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) m = fmaxf(m, fabsf(__uint_as_float(z[e])));
+        if (__all_sync(0xffffffffu, m * fabsf(p.cap_x) <= 1.0f)) {
+            const uint64_t sx = pack2(p.cap_x, p.cap_x), amp = pack2(p.cap2, p.cap2);
+#pragma unroll
+            for (int e = 0; e < N; e += 2) {
+                const uint64_t x = mul2(pack2(__uint_as_float(z[e]), __uint_as_float(z[e + 1])), sx), y = mul2(x, x);
+                uint64_t q = fma2(y, pack2(-0.0028394656255841255f, -0.0028394656255841255f), pack2(0.01611418090760708f, 0.01611418090760708f));
+                q = fma2(q, y, pack2(-0.05097286403179169f, -0.05097286403179169f));
+                q = fma2(q, y, pack2(0.13253524899482727f, 0.13253524899482727f));
+                q = fma2(q, y, pack2(-0.3332400321960449f, -0.3332400321960449f));
+                q = fma2(q, y, pack2(0.9999968409538269f, 0.9999968409538269f));
+                float a, b;
+                unpack2(mul2(mul2(q, x), amp), a, b);
+                z[e] = __float_as_uint(a);
+                z[e + 1] = __float_as_uint(b);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) z[e] = __float_as_uint(kv_tanh2(p, __uint_as_float(z[e]) * p.cap_x));
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) z[e] = __float_as_uint(__uint_as_float(z[e]) * p.scale2);
+    }
+}
+
+// One score in base 2: scale and cap of the product, bias by distance.
 template <bool kPlain>
 __device__ __forceinline__ float kv_score2(const KvAttendParams& p, float dot, float slope, int32_t dist) {
     if (kPlain) return dot * p.scale2;
-    float z = dot * p.scale;
-    if (p.softcap > 0.0f) {
-        // tanh x = 1 - 2 / (1 + e^2x), to about 2^-21 of the cap
-        const float e = fast_exp2(z * p.cap_rate);
-        z = p.softcap - p.softcap * __fdividef(2.0f, 1.0f + e);
-        if (e == INFINITY) z = p.softcap;
-    }
-    return (z + slope * static_cast<float>(dist)) * kLog2e;
+    const float z = p.softcap > 0.0f ? kv_tanh2(p, dot * p.cap_x) : dot * p.scale2;
+    return fmaf(slope * kLog2e, static_cast<float>(dist), z);
 }
 
 // A stretch of one sequence's keys that one packed row (row `row` of the batch at position

@@ -366,23 +366,6 @@ __device__ __forceinline__ KvSpan row_span(const KvAttendParams& p, const Desc& 
     return kv_clip(kv_span(*pos, n, prefix, p.window, p.causal != 0), p.shared_pass ? 0 : p.shared_len, u.keys);
 }
 
-// Pairs of 32-bit numbers, one instruction for both.
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
 // the n lowest bits, n clamped to 0 .. 32
 __device__ __forceinline__ uint32_t below(int32_t n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 // largest of three; NaN if one is
@@ -558,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             int32_t pos;
             const KvSpan sp = row_span(p, u, x * kHalf + rr, &pos, !kPlain);
             float slope = 0.0f;
-            if (!kPlain && p.alibi != nullptr) slope = p.alibi[u.h * p.group + (u.packed0 + x * kHalf + rr) % p.group];
+            if (!kPlain && p.alibi != nullptr) slope = p.alibi[u.h * p.group + (u.packed0 + x * kHalf + rr) % p.group] * kLog2e;
             const float scale = kPlain ? p.scale2 : 1.0f;
             float base = -INFINITY, l = 0.0f;  // the weights' base (2^base), -inf before the first key; their sum
             bool good = true;
@@ -576,10 +559,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int k = 0; k < kTile; k += 32) tm_ld32(ts + k, z + k);
 #pragma unroll
                 for (int k = 0; k < kTile; k += 32) tm_wait32(z + k);
-                if (!kPlain)
+                if (!kPlain) {
+                    kv_cap<kTile>(p, z);
+                    if (p.alibi != nullptr) {
+                        const float d0 = static_cast<float>(base_key + j0 - pos);
+                        const uint64_t from = pack2(d0, d0), by = pack2(slope, slope);
 #pragma unroll
-                    for (int e = 0; e < kTile; ++e)
-                        z[e] = __float_as_uint(kv_score2<false>(p, __uint_as_float(z[e]), slope, base_key + j0 + e - pos));
+                        for (int e = 0; e < kTile; e += 2) {
+                            float a, c;
+                            unpack2(fma2(add2(from, pack2(static_cast<float>(e), static_cast<float>(e + 1))), by,
+                                         pack2(__uint_as_float(z[e]), __uint_as_float(z[e + 1]))), a, c);
+                            z[e] = __float_as_uint(a);
+                            z[e + 1] = __float_as_uint(c);
+                        }
+                    }
+                }
                 if (masked)
 #pragma unroll
                     for (int k = 0; k < kTile; k += 32) {
