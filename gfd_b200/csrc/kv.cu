@@ -138,6 +138,7 @@ constexpr int kMergeThreads = 256;
 template <typename T, typename O, int D>
 __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const KvMergeParams p) {
     constexpr int kLanes = D / 8;
+    kv_wait_last();
     const int64_t n = static_cast<int64_t>(p.rows) * p.heads;
     const int lane = threadIdx.x % kLanes;
     const int64_t step = static_cast<int64_t>(gridDim.x) * (kMergeThreads / kLanes);
@@ -168,110 +169,175 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const KvMergePa
 }
 
 // ---------------------------------------------------------------------------
-// Join of an attention launch's partial results: one CTA (times gridDim.y) per
-// cut of the line.  Each
-// thread sums 4 elements of a packed row over the unit's parts, in their order.
+// Join of an attention launch's partial results.
+//
+// Every CTA reads the launch's places, lists the units that a cut divides and takes its share of
+// their rows, a warp per row: lane i first weighs part i (32 at a time), then every lane sums D / 32
+// elements over the parts, in their order.  Three rounds of loads, each of them wide.
 // ---------------------------------------------------------------------------
-constexpr int kJoinThreads = 128;
+constexpr int kJoinThreads = 256;
+constexpr int kJoinCtas = 512;  // most CTAs of the launch to join
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendParams p, int slot_rows) {
-    const uint32_t c = blockIdx.x + 1;  // cuts 1 .. CTAs - 1
-    // every CTA waits for the attention kernel, so that this grid never ends before it
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const KvPlace u = p.line.places[c];
-    const KvCuts cuts(u.total, gridDim.x + 1);
-    // a cut between two units joins nothing; of several inside a unit the first does
-    if (c >= cuts.ctas || u.t == 0 || cuts.at(c - 1) > u.begin) return;
-    const int64_t end = u.begin + u.count;
-    uint32_t last = c;  // parts: CTA c - 1 (slot 1), c .. last (slot 0)
-    while (last + 1 < cuts.ctas && cuts.at(last + 1) < end) ++last;
-    const int64_t size = static_cast<int64_t>(slot_rows) * (D + 2);
-    const float* slot1 = p.line.slots + (2 * static_cast<int64_t>(c - 1) + 1) * size;
-    const float* slot0 = p.line.slots + 2 * static_cast<int64_t>(c) * size;
-    const int parts = static_cast<int>(last - c) + 2;
-    for (int i = blockIdx.y * kJoinThreads + threadIdx.x; i < u.packed * (D / 4); i += kJoinThreads * gridDim.y) {
-        const int r = i / (D / 4), d0 = i % (D / 4) * 4;
-        float m = slot1[slot_rows * D + r];
-#pragma unroll 4
-        for (int x = 1; x < parts; ++x) m = fmaxf(m, slot0[2 * (x - 1) * size + slot_rows * D + r]);
-        float sum[4] = {}, l = 0.0f;
-#pragma unroll 4
-        for (int x = 0; x < parts; ++x) {
-            const float* slot = x == 0 ? slot1 : slot0 + 2 * (x - 1) * size;
-            const float pm = slot[slot_rows * D + r], pl = slot[slot_rows * D + slot_rows + r];
-            const float4 v = *reinterpret_cast<const float4*>(slot + r * D + d0);
-            const float w = pm == -INFINITY ? 0.0f : fast_exp2(pm - m);
-            l += pm == -INFINITY ? pl : pl * w;  // -inf: 0, or NaN from scores that are NaN
-            if (w != 0.0f) {
-                sum[0] = fmaf(v.x, w, sum[0]);
-                sum[1] = fmaf(v.y, w, sum[1]);
-                sum[2] = fmaf(v.z, w, sum[2]);
-                sum[3] = fmaf(v.w, w, sum[3]);
-            }
+__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendParams p, int ctas, int slot_rows) {
+    __shared__ int32_t s_cut[kJoinCtas], s_row[kJoinCtas + 1];
+    __shared__ int32_t s_count[kJoinThreads / 32][2];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    constexpr int kEach = D / 32;
+    kv_let_next();
+    kv_wait_last();
+    const KvCuts cuts(p.line.places[0].total, ctas);
+    // cuts that are the first inside their unit: the list of units, and where their rows begin
+    int units = 0, rows = 0;
+    for (int c0 = 1; c0 < cuts.n(); c0 += kJoinThreads) {
+        const int c = c0 + t;
+        int mine = 0;
+        if (c < cuts.n()) {
+            const KvPlace& u = p.line.places[c];
+            if (u.t > 0 && cuts.at(c - 1) <= u.begin) mine = u.packed;
         }
-        const int packed = u.packed0 + r;
-        const int64_t row = u.row0 + packed / p.group;
-        const int head = u.h * p.group + packed % p.group;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const unsigned ball = __ballot_sync(0xffffffffu, mine > 0);
+        int incl = mine;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] = l == 0.0f ? 0.0f : sum[e] * inv;
-        kv_store_out<T>(p, row, head, d0, sum, 4);
-        if (p.lse != nullptr && d0 == 0) p.lse[row * p.q_heads + head] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) {
+            s_count[warp][0] = __popc(ball);
+            s_count[warp][1] = incl;
+        }
+        __syncthreads();
+        int k = units + __popc(ball & ((1u << lane) - 1u)), r = rows + incl - mine;
+        for (int w = 0; w < kJoinThreads / 32; ++w) {
+            if (w < warp) {
+                k += s_count[w][0];
+                r += s_count[w][1];
+            }
+            units += s_count[w][0];
+            rows += s_count[w][1];
+        }
+        if (mine > 0) {
+            s_cut[k] = c;
+            s_row[k] = r;
+        }
+        __syncthreads();
+    }
+    const int64_t size = static_cast<int64_t>(slot_rows) * (D + 2);
+    for (int i = blockIdx.x * (kJoinThreads / 32) + warp; i < rows; i += gridDim.x * (kJoinThreads / 32)) {
+        int lo = 0, hi = units - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (s_row[mid] <= i) lo = mid;
+            else hi = mid - 1;
+        }
+        const int c = s_cut[lo], r = i - s_row[lo];
+        const KvPlace& u = p.line.places[c];
+        const int64_t end = u.begin + u.count;
+        const int32_t packed = u.packed0 + r, h = u.h, row0 = u.row0;
+        // part 0 is CTA c - 1 (slot 1), part x >= 1 CTA c - 1 + x (slot 0), to the last cut inside the unit
+        const float* base = p.line.slots + (2 * static_cast<int64_t>(c - 1)) * size;
+        float m = -INFINITY, l = 0.0f, sum[kEach] = {};
+        for (int x0 = 0;; x0 += 32) {
+            const int x = x0 + lane;
+            const bool live = x == 0 || (c - 1 + x < cuts.n() && cuts.at(c - 1 + x) < end);
+            const float* slot = base + (x == 0 ? size : 2 * x * size);
+            float pm = -INFINITY, pl = 0.0f;
+            if (live) {
+                pm = slot[slot_rows * D + r];
+                pl = slot[slot_rows * D + slot_rows + r];
+            }
+            float top = pm;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top = fmaxf(top, m);
+            const float keep = m == -INFINITY ? 0.0f : fast_exp2(m - top);
+            const float w = pm == -INFINITY ? 0.0f : fast_exp2(pm - top);
+            float part = pm == -INFINITY ? pl : pl * w;  // -inf: 0, or NaN from scores that are NaN
+#pragma unroll
+            for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+            l = (m == -INFINITY ? l : l * keep) + part;
+            m = top;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) sum[e] *= keep;
+            const int n = __popc(__ballot_sync(0xffffffffu, live));
+#pragma unroll 8
+            for (int y = 0; y < n; ++y) {
+                const float wy = __shfl_sync(0xffffffffu, w, y);
+                const float* v = base + (x0 + y == 0 ? size : 2 * (x0 + y) * size) + r * D + lane * kEach;
+                float f[kEach];
+                if constexpr (kEach == 4) *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(v);
+                else *reinterpret_cast<float2*>(f) = *reinterpret_cast<const float2*>(v);
+                if (wy != 0.0f)
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e) sum[e] = fmaf(f[e], wy, sum[e]);
+            }
+            if (n < 32) break;
+        }
+        const int32_t of = kv_div_group(p, packed);
+        const int64_t row = row0 + of;
+        const int head = h * p.group + packed - of * p.group;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        char* at = p.out.data + row * p.out.row_stride + head * p.out.head_stride;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) sum[e] = l == 0.0f ? 0.0f : sum[e] * inv;
+        if (p.out_f32) {
+            if constexpr (kEach == 4) reinterpret_cast<float4*>(at)[lane] = *reinterpret_cast<const float4*>(sum);
+            else reinterpret_cast<float2*>(at)[lane] = *reinterpret_cast<const float2*>(sum);
+        } else {
+            if constexpr (kEach == 4) reinterpret_cast<uint2*>(at)[lane] = make_uint2(Pack<T>::pair(sum[0], sum[1]), Pack<T>::pair(sum[2], sum[3]));
+            else reinterpret_cast<uint32_t*>(at)[lane] = Pack<T>::pair(sum[0], sum[1]);
+        }
+        if (p.lse != nullptr && lane == 0) p.lse[row * p.q_heads + head] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
     }
 }
 
 template <typename F>
-cudaError_t by_type(int dtype, F f) {
-    if (dtype == GFD_BF16) return f(__nv_bfloat16());
-    if (dtype == GFD_FP16) return f(__half());
-    return f(0.0f);
+cudaError_t by_type(int dtype, F f) {  // the types of a cache
+    return dtype == GFD_BF16 ? f(__nv_bfloat16()) : f(__half());
+}
+template <typename F>
+cudaError_t by_any_type(int dtype, F f) {
+    return dtype == GFD_FP32 ? f(0.0f) : by_type(dtype, f);
 }
 
 }  // namespace
 
 cudaError_t launch_kv_append(const KvAppendParams& p, int head_dim, int dtype, int num_sms, cudaStream_t st) {
     const int rows_per_cta = p.batch.rows > 8 * num_sms ? 4 : 1;
-    const int grid = (p.batch.rows + rows_per_cta - 1) / rows_per_cta;
-    if (dtype == GFD_BF16) {
-        if (head_dim == 64) kv_append_kernel<__nv_bfloat16, 64><<<grid, kAppendThreads, 0, st>>>(p, rows_per_cta);
-        else kv_append_kernel<__nv_bfloat16, 128><<<grid, kAppendThreads, 0, st>>>(p, rows_per_cta);
-    } else {
-        if (head_dim == 64) kv_append_kernel<__half, 64><<<grid, kAppendThreads, 0, st>>>(p, rows_per_cta);
-        else kv_append_kernel<__half, 128><<<grid, kAppendThreads, 0, st>>>(p, rows_per_cta);
-    }
-    return cudaGetLastError();
+    const dim3 grid((p.batch.rows + rows_per_cta - 1) / rows_per_cta);
+    return by_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        return head_dim == 64 ? kv_launch(kv_append_kernel<T, 64>, grid, kAppendThreads, 0, st, false, p, rows_per_cta)
+                              : kv_launch(kv_append_kernel<T, 128>, grid, kAppendThreads, 0, st, false, p, rows_per_cta);
+    });
 }
 
 cudaError_t launch_kv_join(const KvAttendParams& p, int head_dim, int dtype, int ctas, int slot_rows, cudaStream_t st) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas - 1, slot_rows / 16);
-    cfg.blockDim = dim3(kJoinThreads);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (dtype == GFD_BF16)
-        return head_dim == 64 ? cudaLaunchKernelEx(&cfg, kv_join_kernel<__nv_bfloat16, 64>, p, slot_rows)
-                              : cudaLaunchKernelEx(&cfg, kv_join_kernel<__nv_bfloat16, 128>, p, slot_rows);
-    return head_dim == 64 ? cudaLaunchKernelEx(&cfg, kv_join_kernel<__half, 64>, p, slot_rows)
-                          : cudaLaunchKernelEx(&cfg, kv_join_kernel<__half, 128>, p, slot_rows);
+    if (ctas > kJoinCtas) return cudaErrorInvalidValue;
+    // at most ctas - 1 units are cut; a warp per row
+    const int64_t rows = static_cast<int64_t>(ctas - 1) * slot_rows, warps = kJoinThreads / 32;
+    const int64_t all = static_cast<int64_t>(p.batch.rows) * p.q_heads;
+    const int64_t want = ((rows < all ? rows : all) + warps - 1) / warps;
+    const dim3 grid(static_cast<unsigned>(want < 1 ? 1 : (want > 4 * ctas ? 4 * ctas : want)));
+    return by_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        return head_dim == 64 ? kv_launch(kv_join_kernel<T, 64>, grid, kJoinThreads, 0, st, true, p, ctas, slot_rows)
+                              : kv_launch(kv_join_kernel<T, 128>, grid, kJoinThreads, 0, st, true, p, ctas, slot_rows);
+    });
 }
 
-cudaError_t launch_kv_merge(const KvMergeParams& p, int head_dim, int part_dtype, int out_dtype, int num_sms,
+cudaError_t launch_kv_merge(const KvMergeParams& p, int head_dim, int part_dtype, int out_dtype, int num_sms, bool chained,
                             cudaStream_t st) {
     const int64_t per_cta = kMergeThreads / (head_dim / 8);
-    int64_t grid = (static_cast<int64_t>(p.rows) * p.heads + per_cta - 1) / per_cta;
-    if (grid > 16ll * num_sms) grid = 16ll * num_sms;
-    return by_type(part_dtype, [&](auto t) {
-        return by_type(out_dtype, [&](auto o) {
+    const int64_t want = (static_cast<int64_t>(p.rows) * p.heads + per_cta - 1) / per_cta;
+    const dim3 grid(static_cast<unsigned>(want > 16ll * num_sms ? 16ll * num_sms : want));
+    return by_any_type(part_dtype, [&](auto t) {
+        return by_any_type(out_dtype, [&](auto o) {
             using T = decltype(t);
             using O = decltype(o);
-            if (head_dim == 64) kv_merge_kernel<T, O, 64><<<static_cast<unsigned>(grid), kMergeThreads, 0, st>>>(p);
-            else kv_merge_kernel<T, O, 128><<<static_cast<unsigned>(grid), kMergeThreads, 0, st>>>(p);
-            return cudaGetLastError();
+            return head_dim == 64 ? kv_launch(kv_merge_kernel<T, O, 64>, grid, kMergeThreads, 0, st, chained, p)
+                                  : kv_launch(kv_merge_kernel<T, O, 128>, grid, kMergeThreads, 0, st, chained, p);
         });
     });
 }

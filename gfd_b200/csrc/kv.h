@@ -96,7 +96,8 @@ struct KvMergeParams {
 };
 constexpr uint32_t kKvUnwritten = 0xffffffffu;
 
-// dtype: GFD_* of the cache; out: of the output rows
+// dtype: GFD_* of the cache.  chained: the launch may start before the one before it on the stream has
+// ended (it was made by the same call and touches nothing of this one's, or waits for it).
 cudaError_t launch_kv_append(const KvAppendParams& p, int head_dim, int dtype, int num_sms, cudaStream_t st);
 cudaError_t launch_kv_join(const KvAttendParams& p, int head_dim, int dtype, int ctas, int slot_rows, cudaStream_t st);
 int kv_decode_ctas(int num_sms);
@@ -104,8 +105,8 @@ int kv_prompt_ctas(int num_sms);
 // cuTensorMapEncodeTiled, resolved through the runtime (libcuda is not linked)
 using KvEncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-cudaError_t launch_kv_prompt(const KvAttendParams& p, int head_dim, int dtype, int num_sms, KvEncodeFn encode, cudaStream_t st);
-cudaError_t launch_kv_decode(const KvAttendParams& p, int head_dim, int dtype, int num_sms, cudaStream_t st);
+cudaError_t launch_kv_prompt(const KvAttendParams& p, int head_dim, int dtype, int num_sms, KvEncodeFn encode, bool chained, cudaStream_t st);
+cudaError_t launch_kv_decode(const KvAttendParams& p, int head_dim, int dtype, int num_sms, bool chained, cudaStream_t st);
 
 // Bytes of a line's places and slots, and the line laid out in them.
 inline size_t kv_line_bytes(int ctas, int slot_rows, int head_dim) {
@@ -115,7 +116,7 @@ inline size_t kv_line_bytes(int ctas, int slot_rows, int head_dim) {
 inline KvLine kv_line_at(void* p, int ctas) {
     return KvLine{static_cast<KvPlace*>(p), reinterpret_cast<float*>(static_cast<char*>(p) + (sizeof(KvPlace) * ctas + 255) / 256 * 256)};
 }
-cudaError_t launch_kv_merge(const KvMergeParams& p, int head_dim, int part_dtype, int out_dtype, int num_sms,
+cudaError_t launch_kv_merge(const KvMergeParams& p, int head_dim, int part_dtype, int out_dtype, int num_sms, bool chained,
                             cudaStream_t st);
 
 }  // namespace gfdb

@@ -17,12 +17,25 @@ struct Region {
     const char* what;
 };
 
-// Every region lies in device memory of the context's GPU (regions of no bytes pass).
+// Every region lies in device memory of the context's GPU (regions of no bytes pass).  The driver
+// is asked once per allocation and call: arrays of one allocation follow one another often.
 int check_regions(gfd_ctx* ctx, const char* call, const Region* r, int n) {
-    for (int i = 0; i < n; ++i)
-        if (r[i].p != nullptr && r[i].bytes > 0 && !check_dev(ctx, reinterpret_cast<uint64_t>(r[i].p), r[i].bytes))
-            return set_error(ctx, GFD_ERR_INVALID, "%s: %s is not inside one device allocation of GPU %d", call, r[i].what,
-                             ctx->device);
+    uint64_t lo[16], hi[16];
+    int known = 0;
+    for (int i = 0; i < n; ++i) {
+        const uint64_t a = reinterpret_cast<uint64_t>(r[i].p), b = a + r[i].bytes;
+        if (r[i].p == nullptr || r[i].bytes == 0) continue;
+        bool in = false;
+        for (int k = 0; k < known && !in; ++k) in = a >= lo[k] && b <= hi[k] && b > a;
+        if (in) continue;
+        if (!check_dev(ctx, a, r[i].bytes))
+            return set_error(ctx, GFD_ERR_INVALID, "%s: %s is not inside one device allocation of GPU %d", call, r[i].what, ctx->device);
+        const Range* range = ctx->dev_ranges.find(a, r[i].bytes);
+        if (range != nullptr && known < 16) {
+            lo[known] = range->lo;
+            hi[known++] = range->hi;
+        }
+    }
     return GFD_OK;
 }
 
@@ -217,22 +230,25 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
         own.out_f32 = 1;
     }
     cudaError_t e = cudaSuccess;
-    if (shared_len > 0) {
-        e = cudaMemsetAsync(own.lse, 0xff, static_cast<size_t>(b->rows) * a->q_heads * sizeof(float), st);
+    bool chained = false;  // kernels of this call behind one another: they share nothing until the last
+    if (shared_len > 0) e = cudaMemsetAsync(own.lse, 0xff, static_cast<size_t>(b->rows) * a->q_heads * sizeof(float), st);
+    if (e == cudaSuccess && plan.few) {
+        own.line = kv_line_at(ws + plan.few_line, kv_decode_ctas(ctx->num_sms));
+        e = launch_kv_decode(own, c->head_dim, c->dtype, ctx->num_sms, chained, st);
+        chained = true;
+    }
+    if (e == cudaSuccess && plan.many) {
+        own.line = kv_line_at(ws + plan.many_line, kv_prompt_ctas(ctx->num_sms));
+        e = launch_kv_prompt(own, c->head_dim, c->dtype, ctx->num_sms, encode, chained, st);
+        chained = true;
+    }
+    if (e == cudaSuccess && shared_len > 0) {
         KvAttendParams pre = own;
         pre.out.data = ws + plan.parts;
         pre.lse = reinterpret_cast<float*>(ws + plan.part_lse);
         pre.shared_pass = 1;
         pre.line = kv_line_at(ws + plan.prefix_line, kv_prompt_ctas(ctx->num_sms));
-        if (e == cudaSuccess) e = launch_kv_prompt(pre, c->head_dim, c->dtype, ctx->num_sms, encode, st);
-    }
-    if (e == cudaSuccess && plan.many) {
-        own.line = kv_line_at(ws + plan.many_line, kv_prompt_ctas(ctx->num_sms));
-        e = launch_kv_prompt(own, c->head_dim, c->dtype, ctx->num_sms, encode, st);
-    }
-    if (e == cudaSuccess && plan.few) {
-        own.line = kv_line_at(ws + plan.few_line, kv_decode_ctas(ctx->num_sms));
-        e = launch_kv_decode(own, c->head_dim, c->dtype, ctx->num_sms, st);
+        e = launch_kv_prompt(pre, c->head_dim, c->dtype, ctx->num_sms, encode, chained, st);
     }
     if (e == cudaSuccess && shared_len > 0) {
         KvMergeParams m;
@@ -247,7 +263,7 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
         m.heads = a->q_heads;
         m.part_count = 2;
         m.last_marks = 1;
-        e = launch_kv_merge(m, c->head_dim, GFD_FP32, a->out_dtype, ctx->num_sms, st);
+        e = launch_kv_merge(m, c->head_dim, GFD_FP32, a->out_dtype, ctx->num_sms, true, st);
     }
     return e == cudaSuccess ? GFD_OK : cuda_error(ctx, e, "kv_attend: kernel launch");
 }
@@ -280,7 +296,7 @@ int merge(gfd_ctx* ctx, const gfd_kv_merge_args* a, void* stream) {
     p.heads = a->heads;
     p.part_count = a->part_count;
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
-    const cudaError_t e = launch_kv_merge(p, a->head_dim, a->part_dtype, a->out_dtype, ctx->num_sms, st);
+    const cudaError_t e = launch_kv_merge(p, a->head_dim, a->part_dtype, a->out_dtype, ctx->num_sms, false, st);
     return e == cudaSuccess ? GFD_OK : cuda_error(ctx, e, "kv_merge: kernel launch");
 }
 

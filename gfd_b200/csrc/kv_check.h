@@ -197,6 +197,7 @@ inline const char* kv_check_attend(const gfd_kv_attend_args& a, const gfd_kv_cac
     if (a.window < 0 || a.window > kKvMaxTokens) return "bad window";
     if (!std::isfinite(a.scale)) return "scale is not finite";
     if (!std::isfinite(a.softcap) || a.softcap < 0.0f) return "softcap must be finite and not negative";
+    if (a.softcap > 0.0f && (!std::isfinite(a.scale / a.softcap) || a.softcap > 1e30f)) return "softcap is out of range";
     if (a.q.data == a.out.data) return "out must not be q";
     if (!kv_aligned(a.lse, 4) || !kv_aligned(a.alibi, 4) || !kv_aligned(a.prefix_len, 4) || !kv_aligned(a.status, 4))
         return "lse, alibi, prefix_len or status is not 4-byte aligned";

@@ -200,11 +200,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const KvBatchView& b = p.batch;
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    kv_let_next();
     if (t == 0) s_place = KvPlace{};
     if (!kv_starts_ok(b)) {
         if (blockIdx.x == 0 && t == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
         if (t == 0) p.line.places[blockIdx.x] = s_place;
+        kv_wait_last();
         return;
     }
     int64_t mine;
@@ -216,6 +217,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
     const KvCuts cuts(total, gridDim.x);
     if (static_cast<int>(blockIdx.x) >= cuts.n()) {
         if (t == 0) p.line.places[blockIdx.x].total = total;
+        kv_wait_last();
         return;
     }
     const int64_t at = cuts.at(blockIdx.x), to = cuts.at(blockIdx.x + 1);
@@ -491,16 +493,14 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
         use.next_unit(p);
     }
     copy_wait<0>();
+    kv_wait_last();
 }
 
 template <typename T, int D>
-cudaError_t launch(const KvAttendParams& p, int ctas, cudaStream_t st) {
+cudaError_t launch(const KvAttendParams& p, int ctas, bool chained, cudaStream_t st) {
     const bool plain = p.softcap == 0.0f && p.alibi == nullptr;
-    auto* k = plain ? kv_decode_kernel<T, D, true> : kv_decode_kernel<T, D, false>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
-    if (e != cudaSuccess) return e;
-    k<<<ctas, kThreads, Shape<D>::kSmem, st>>>(p);
-    e = cudaGetLastError();
+    const cudaError_t e = kv_launch(plain ? kv_decode_kernel<T, D, true> : kv_decode_kernel<T, D, false>, dim3(ctas), kThreads,
+                                    Shape<D>::kSmem, st, chained, p);
     if (e != cudaSuccess) return e;
     return launch_kv_join(p, D, std::is_same<T, __half>::value ? GFD_FP16 : GFD_BF16, ctas, kRows, st);
 }
@@ -509,10 +509,11 @@ cudaError_t launch(const KvAttendParams& p, int ctas, cudaStream_t st) {
 
 int kv_decode_ctas(int num_sms) { return 2 * num_sms; }
 
-cudaError_t launch_kv_decode(const KvAttendParams& p, int head_dim, int dtype, int num_sms, cudaStream_t st) {
+cudaError_t launch_kv_decode(const KvAttendParams& p, int head_dim, int dtype, int num_sms, bool chained, cudaStream_t st) {
     const int ctas = kv_decode_ctas(num_sms);
-    if (dtype == GFD_BF16) return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, ctas, st) : launch<__nv_bfloat16, 128>(p, ctas, st);
-    return head_dim == 64 ? launch<__half, 64>(p, ctas, st) : launch<__half, 128>(p, ctas, st);
+    if (dtype == GFD_BF16)
+        return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, ctas, chained, st) : launch<__nv_bfloat16, 128>(p, ctas, chained, st);
+    return head_dim == 64 ? launch<__half, 64>(p, ctas, chained, st) : launch<__half, 128>(p, ctas, chained, st);
 }
 
 }  // namespace gfdb

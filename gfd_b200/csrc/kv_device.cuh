@@ -74,6 +74,12 @@ struct Pack<float> {
     }
 };
 
+// Launches of one call overlap (programmatic dependent launch): each lets the next one start at
+// once and, before it reads what an earlier one wrote or ends, waits for that one to complete.  As
+// every CTA waits before it ends, the completion of a launch implies that of all before it.
+__device__ __forceinline__ void kv_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void kv_wait_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // n / group for 0 <= n < 2^31: the rounded-up reciprocal errs by less than group <= 2^13 in 2^44, so
 // n times it stays below the next whole quotient.
 __device__ __forceinline__ int32_t kv_div_group(const KvAttendParams& p, int32_t n) {
@@ -243,6 +249,25 @@ __device__ __forceinline__ void kv_exact_row(const KvAttendParams& p, const KvEx
                     acc[e] = fmaf(wy, static_cast<float>(reinterpret_cast<const T*>(p.cache.v + ay)[lane * kEach + e]), acc[e]);
             }
         }
+}
+
+template <typename... P, typename... A>
+cudaError_t kv_launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, bool chained, A... args) {
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = chained ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 }  // namespace gfdb

@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const KvBatchView& b = p.batch;
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    kv_let_next();
     if (t == 0) {
         s_place = KvPlace{};
         s_gave_up = 0;
@@ -497,7 +497,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             p.line.places[blockIdx.x] = s_place;
         }
     }
-    if (stretch_end == 0) return;
+    if (stretch_end == 0) {
+        kv_wait_last();
+        return;
+    }
 
     if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(S::kColumns)
@@ -1008,6 +1011,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tm_after();
     if (t == 0 && s_gave_up != 0) kv_report(p.status, GFD_KV_GAVE_UP);
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns) : "memory");
+    kv_wait_last();
 }
 
 // The cache's K or V as [blocks][tokens][heads][D], read in boxes of 16 tokens x 64 elements.
@@ -1026,13 +1030,10 @@ bool make_map(CUtensorMap* map, const KvAttendParams& p, const char* base, int h
 }
 
 template <typename T, int D>
-cudaError_t launch(const KvAttendParams& p, const CUtensorMap& k, const CUtensorMap& v, int ctas, cudaStream_t st) {
+cudaError_t launch(const KvAttendParams& p, const CUtensorMap& k, const CUtensorMap& v, int ctas, bool chained, cudaStream_t st) {
     const bool plain = p.softcap == 0.0f && p.alibi == nullptr && p.scale2 > 0.0f;
-    auto* f = plain ? kv_prompt_kernel<T, D, true> : kv_prompt_kernel<T, D, false>;
-    cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
-    if (e != cudaSuccess) return e;
-    f<<<ctas, kThreads, Shape<D>::kSmem, st>>>(p, k, v);
-    e = cudaGetLastError();
+    const cudaError_t e = kv_launch(plain ? kv_prompt_kernel<T, D, true> : kv_prompt_kernel<T, D, false>, dim3(ctas), kThreads,
+                                    Shape<D>::kSmem, st, chained, p, k, v);
     if (e != cudaSuccess) return e;
     return launch_kv_join(p, D, std::is_same<T, __half>::value ? GFD_FP16 : GFD_BF16, ctas, kRows, st);
 }
@@ -1041,13 +1042,15 @@ cudaError_t launch(const KvAttendParams& p, const CUtensorMap& k, const CUtensor
 
 int kv_prompt_ctas(int num_sms) { return num_sms; }
 
-cudaError_t launch_kv_prompt(const KvAttendParams& p, int head_dim, int dtype, int num_sms, KvEncodeFn encode, cudaStream_t st) {
+cudaError_t launch_kv_prompt(const KvAttendParams& p, int head_dim, int dtype, int num_sms, KvEncodeFn encode, bool chained,
+                             cudaStream_t st) {
     CUtensorMap k, v;
     if (!make_map(&k, p, p.cache.k, head_dim, dtype, encode) || !make_map(&v, p, p.cache.v, head_dim, dtype, encode))
         return cudaErrorInvalidValue;
     const int ctas = kv_prompt_ctas(num_sms);
-    if (dtype == GFD_BF16) return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, k, v, ctas, st) : launch<__nv_bfloat16, 128>(p, k, v, ctas, st);
-    return head_dim == 64 ? launch<__half, 64>(p, k, v, ctas, st) : launch<__half, 128>(p, k, v, ctas, st);
+    if (dtype == GFD_BF16)
+        return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, k, v, ctas, chained, st) : launch<__nv_bfloat16, 128>(p, k, v, ctas, chained, st);
+    return head_dim == 64 ? launch<__half, 64>(p, k, v, ctas, chained, st) : launch<__half, 128>(p, k, v, ctas, chained, st);
 }
 
 }  // namespace gfdb

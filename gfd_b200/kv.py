@@ -68,17 +68,26 @@ def _stream(s) -> _VP:
     return _VP(s.cuda_stream or 1)  # 1: the legacy default stream, which torch calls 0
 
 
+_codes = {}  # dtype object -> code or None: naming a type costs as much as a whole call
+
+
+def _code(dtype):
+    if dtype not in _codes:
+        _codes[dtype] = _TYPES.get(str(dtype), str(dtype))
+    return _codes[dtype]
+
+
 def _dtype(x, what: str) -> int:
-    d = _TYPES.get(str(x.dtype))
-    if d is None:
+    d = _code(x.dtype)
+    if not isinstance(d, int):
         raise ValueError(f"{what}: unsupported type {x.dtype}")
     return d
 
 
 def _rows(x, what: str, rows: int, heads: int, dim: int, dtype: int) -> _Rows:
-    if tuple(x.shape) != (rows, heads, dim):
+    if x.shape != (rows, heads, dim):
         raise ValueError(f"{what}: shape {tuple(x.shape)}, expected {(rows, heads, dim)}")
-    if _dtype(x, what) != dtype:
+    if _code(x.dtype) != dtype:
         raise ValueError(f"{what}: type {x.dtype} does not match")
     st = x.stride()
     if st[2] != 1:
@@ -90,8 +99,9 @@ def _vector(x, what: str, shape, dtype: str) -> int:
     """Address of a contiguous vector or matrix (None: NULL)."""
     if x is None:
         return None
-    if tuple(x.shape) != tuple(shape) or str(x.dtype) != dtype or not x.is_contiguous():
-        raise ValueError(f"{what}: expected contiguous {dtype} of shape {tuple(shape)}, got {x.dtype} {tuple(x.shape)}")
+    if x.shape != tuple(shape) or _code(x.dtype) != dtype or not x.is_contiguous():
+        raise ValueError(f"{what}: expected contiguous {'torch.float32' if dtype == FP32 else dtype} of shape {tuple(shape)}, "
+                         f"got {x.dtype} {tuple(x.shape)}")
     return x.data_ptr()
 
 
@@ -101,7 +111,7 @@ class Batch:
 
     def __init__(self, row_start, kv_len, table):
         seqs = kv_len.shape[0]
-        if table.dim() != 2 or table.shape[0] != seqs or str(table.dtype) != "torch.int32":
+        if table.dim() != 2 or table.shape[0] != seqs or _code(table.dtype) != "torch.int32":
             raise ValueError(f"table: expected int32 of shape ({seqs}, width), got {table.dtype} {tuple(table.shape)}")
         if table.shape[1] > 1 and table.stride(1) != 1:
             raise ValueError("table: the entries of a row must be contiguous")
@@ -181,7 +191,7 @@ class PagedCache:
             a.q_out = _rows(q_out, "q_out", rows, a.q_heads, self.head_dim, self.dtype)
         if inv_freq is not None:
             a.rot_dim = 2 * inv_freq.shape[0]
-            a.inv_freq = _vector(inv_freq, "inv_freq", (inv_freq.shape[0],), "torch.float32")
+            a.inv_freq = _vector(inv_freq, "inv_freq", (inv_freq.shape[0],), FP32)
         a.interleaved = bool(interleaved)
         a.positions = _vector(positions, "positions", (rows,), "torch.int32")
         a.status = _vector(status, "status", (1,), "torch.int32")
@@ -203,8 +213,8 @@ class PagedCache:
         a.q = _rows(q, "q", rows, heads, self.head_dim, self.dtype)
         a.out_dtype = _dtype(out, "out")
         a.out = _rows(out, "out", rows, heads, self.head_dim, a.out_dtype)
-        a.lse = _vector(lse, "lse", (rows, heads), "torch.float32")
-        a.alibi = _vector(alibi, "alibi", (heads,), "torch.float32")
+        a.lse = _vector(lse, "lse", (rows, heads), FP32)
+        a.alibi = _vector(alibi, "alibi", (heads,), FP32)
         a.prefix_len = _vector(prefix_len, "prefix_len", (batch.seqs,), "torch.int32")
         if workspace is not None:
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
@@ -243,9 +253,9 @@ def merge(ctx: Context, parts, part_lse, out, lse=None, stream=0):
     a, st = _Merge(), parts.stride()
     a.parts = _Rows(parts.data_ptr(), st[1] if rows > 1 else 0, st[2] if heads > 1 else 0)
     a.part_stride = st[0] if n > 1 else 0
-    a.part_lse = _vector(part_lse, "part_lse", (n, rows, heads), "torch.float32")
+    a.part_lse = _vector(part_lse, "part_lse", (n, rows, heads), FP32)
     a.part_dtype, a.out_dtype = _dtype(parts, "parts"), _dtype(out, "out")
     a.out = _rows(out, "out", rows, heads, dim, a.out_dtype)
-    a.lse = _vector(lse, "lse", (rows, heads), "torch.float32")
+    a.lse = _vector(lse, "lse", (rows, heads), FP32)
     a.rows, a.part_count, a.heads, a.head_dim = rows, n, heads, dim
     ctx._check(ctx.lib.gfd_kv_merge(ctx.handle, ctypes.byref(a), _stream(stream)))
