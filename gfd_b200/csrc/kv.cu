@@ -138,13 +138,11 @@ constexpr int kMergeThreads = 256;
 template <typename T, typename O, int D>
 __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const KvMergeParams p) {
     constexpr int kLanes = D / 8;
-    kv_wait_last();
     const int64_t n = static_cast<int64_t>(p.rows) * p.heads;
     const int lane = threadIdx.x % kLanes;
     const int64_t step = static_cast<int64_t>(gridDim.x) * (kMergeThreads / kLanes);
     for (int64_t u = blockIdx.x * static_cast<int64_t>(kMergeThreads / kLanes) + threadIdx.x / kLanes; u < n; u += step) {
         const int64_t row = u / p.heads, h = u % p.heads;
-        if (p.last_marks && __float_as_uint(p.part_lse[(p.part_count - 1) * n + u]) == kKvUnwritten) continue;
         float m = -INFINITY;
         for (int i = 0; i < p.part_count; ++i) m = fmaxf(m, p.part_lse[i * n + u]);
         const float base = m == -INFINITY ? 0.0f : m;
@@ -169,102 +167,55 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const KvMergePa
 }
 
 // ---------------------------------------------------------------------------
-// Join of an attention launch's partial results.
-//
-// Every CTA reads the launch's places, lists the units that a cut divides and takes its share of
-// their rows, a warp per row: lane i first weighs part i (32 at a time), then every lane sums D / 32
-// elements over the parts, in their order.  Three rounds of loads, each of them wide.
+// Join of an attention launch's partial results: CTA x (times gridDim.y) sees to cut x + 1.
 // ---------------------------------------------------------------------------
-constexpr int kJoinThreads = 256;
-constexpr int kJoinCtas = 512;  // most CTAs of the launch to join
+// Weight of a part whose sums are relative to 2^base, and its share of the weight sum: a part without
+// keys (-inf) adds nothing but a NaN that its scores left.
+__device__ __forceinline__ void part_weight(float base, float top, float* w, float* l) {
+    *w = base == -INFINITY ? 0.0f : fast_exp2(base - top);
+    if (base != -INFINITY) *l *= *w;
+}
+
+// Of kv_decode, with up to hundreds of parts of a few rows: a warp per row, whose lanes weigh 32 parts
+// at a time and then sum D / 32 elements each over the parts, in their order.
+constexpr int kJoinFewThreads = 128;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendParams p, int ctas, int slot_rows) {
-    __shared__ int32_t s_cut[kJoinCtas], s_row[kJoinCtas + 1];
-    __shared__ int32_t s_count[kJoinThreads / 32][2];
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    constexpr int kEach = D / 32;
+__global__ void __launch_bounds__(kJoinFewThreads) kv_join_few_kernel(const KvAttendParams p) {
+    constexpr int kEach = D / 32, kSlot = kKvFewRows * (D + 2);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x + 1;
     kv_let_next();
     kv_wait_last();
-    const KvCuts cuts(p.line.places[0].total, ctas);
-    // cuts that are the first inside their unit: the list of units, and where their rows begin
-    int units = 0, rows = 0;
-    for (int c0 = 1; c0 < cuts.n(); c0 += kJoinThreads) {
-        const int c = c0 + t;
-        int mine = 0;
-        if (c < cuts.n()) {
-            const KvPlace& u = p.line.places[c];
-            if (u.t > 0 && cuts.at(c - 1) <= u.begin) mine = u.packed;
-        }
-        const unsigned ball = __ballot_sync(0xffffffffu, mine > 0);
-        int incl = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += y;
-        }
-        if (lane == 31) {
-            s_count[warp][0] = __popc(ball);
-            s_count[warp][1] = incl;
-        }
-        __syncthreads();
-        int k = units + __popc(ball & ((1u << lane) - 1u)), r = rows + incl - mine;
-        for (int w = 0; w < kJoinThreads / 32; ++w) {
-            if (w < warp) {
-                k += s_count[w][0];
-                r += s_count[w][1];
-            }
-            units += s_count[w][0];
-            rows += s_count[w][1];
-        }
-        if (mine > 0) {
-            s_cut[k] = c;
-            s_row[k] = r;
-        }
-        __syncthreads();
-    }
-    const int64_t size = static_cast<int64_t>(slot_rows) * (D + 2);
-    for (int i = blockIdx.x * (kJoinThreads / 32) + warp; i < rows; i += gridDim.x * (kJoinThreads / 32)) {
-        int lo = 0, hi = units - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (s_row[mid] <= i) lo = mid;
-            else hi = mid - 1;
-        }
-        const int c = s_cut[lo], r = i - s_row[lo];
-        const KvPlace& u = p.line.places[c];
-        const int64_t end = u.begin + u.count;
-        const int32_t packed = u.packed0 + r, h = u.h, row0 = u.row0;
-        // part 0 is CTA c - 1 (slot 1), part x >= 1 CTA c - 1 + x (slot 0), to the last cut inside the unit
-        const float* base = p.line.slots + (2 * static_cast<int64_t>(c - 1)) * size;
+    const KvCut u = p.line.cuts[c];
+    if (u.parts == 0) return;
+    const float* slots = p.line.slots + 2 * static_cast<int64_t>(c - 1) * kSlot;  // part x: slot 1 for 0, else 2 x
+    for (int r = warp; r < u.packed; r += kJoinFewThreads / 32) {
         float m = -INFINITY, l = 0.0f, sum[kEach] = {};
-        for (int x0 = 0;; x0 += 32) {
-            const int x = x0 + lane;
-            const bool live = x == 0 || (c - 1 + x < cuts.n() && cuts.at(c - 1 + x) < end);
-            const float* slot = base + (x == 0 ? size : 2 * x * size);
+        for (int x0 = 0; x0 < u.parts; x0 += 32) {
+            const int x = x0 + lane, n = min(32, u.parts - x0);
+            const float* slot = slots + static_cast<int64_t>(x == 0 ? 1 : 2 * x) * kSlot + kKvFewRows * D + r;
             float pm = -INFINITY, pl = 0.0f;
-            if (live) {
-                pm = slot[slot_rows * D + r];
-                pl = slot[slot_rows * D + slot_rows + r];
+            if (lane < n) {
+                pm = slot[0];
+                pl = slot[kKvFewRows];
             }
             float top = pm;
 #pragma unroll
             for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             top = fmaxf(top, m);
-            const float keep = m == -INFINITY ? 0.0f : fast_exp2(m - top);
-            const float w = pm == -INFINITY ? 0.0f : fast_exp2(pm - top);
-            float part = pm == -INFINITY ? pl : pl * w;  // -inf: 0, or NaN from scores that are NaN
+            float keep, w;
+            part_weight(m, top, &keep, &l);
+            part_weight(pm, top, &w, &pl);
 #pragma unroll
-            for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-            l = (m == -INFINITY ? l : l * keep) + part;
+            for (int o = 16; o; o >>= 1) pl += __shfl_xor_sync(0xffffffffu, pl, o);
+            l += pl;
             m = top;
 #pragma unroll
             for (int e = 0; e < kEach; ++e) sum[e] *= keep;
-            const int n = __popc(__ballot_sync(0xffffffffu, live));
 #pragma unroll 8
             for (int y = 0; y < n; ++y) {
                 const float wy = __shfl_sync(0xffffffffu, w, y);
-                const float* v = base + (x0 + y == 0 ? size : 2 * (x0 + y) * size) + r * D + lane * kEach;
+                const float* v = slots + static_cast<int64_t>(x0 + y == 0 ? 1 : 2 * (x0 + y)) * kSlot + r * D + lane * kEach;
                 float f[kEach];
                 if constexpr (kEach == 4) *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(v);
                 else *reinterpret_cast<float2*>(f) = *reinterpret_cast<const float2*>(v);
@@ -272,15 +223,14 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendPar
 #pragma unroll
                     for (int e = 0; e < kEach; ++e) sum[e] = fmaf(f[e], wy, sum[e]);
             }
-            if (n < 32) break;
         }
-        const int32_t of = kv_div_group(p, packed);
-        const int64_t row = row0 + of;
-        const int head = h * p.group + packed - of * p.group;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        char* at = p.out.data + row * p.out.row_stride + head * p.out.head_stride;
+        const int32_t of = kv_div_group(p, r);
+        const int64_t row = u.row0 + of;
+        const int head = u.h * p.group + r - of * p.group;
+        const KvFinish f = kv_finish<false>(p, m, l, 0);
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) sum[e] = l == 0.0f ? 0.0f : sum[e] * inv;
+        for (int e = 0; e < kEach; ++e) sum[e] *= f.scale;
+        char* at = p.out.data + row * p.out.row_stride + head * p.out.head_stride;
         if (p.out_f32) {
             if constexpr (kEach == 4) reinterpret_cast<float4*>(at)[lane] = *reinterpret_cast<const float4*>(sum);
             else reinterpret_cast<float2*>(at)[lane] = *reinterpret_cast<const float2*>(sum);
@@ -288,7 +238,85 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendPar
             if constexpr (kEach == 4) reinterpret_cast<uint2*>(at)[lane] = make_uint2(Pack<T>::pair(sum[0], sum[1]), Pack<T>::pair(sum[2], sum[3]));
             else reinterpret_cast<uint32_t*>(at)[lane] = Pack<T>::pair(sum[0], sum[1]);
         }
-        if (p.lse != nullptr && lane == 0) p.lse[row * p.q_heads + head] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
+        if (p.lse != nullptr && lane == 0) p.lse[row * p.q_heads + head] = f.sum == 0.0f ? -INFINITY : f.base * kLn2 + logf(f.sum);
+    }
+}
+
+// Of kv_prompt, with many rows of mostly two parts: a CTA takes 32 rows, a lane per row and D / 8
+// elements a warp, so that the parts are read as they were written; the results go through shared
+// memory to be written row by row.
+constexpr int kJoinManyThreads = 256;
+
+template <typename T, int D, bool kShared>
+__global__ void __launch_bounds__(kJoinManyThreads) kv_join_many_kernel(const KvAttendParams p) {
+    constexpr int kEach = D / 8;  // elements of a thread
+    constexpr int64_t kSlot = static_cast<int64_t>(kKvManyRows) * (D + 2);
+    __shared__ float s_out[32][D + 4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x + 1;
+    kv_let_next();
+    kv_wait_last();
+    const KvCut u = p.line.cuts[c];
+    const int r0 = blockIdx.y * 32;
+    if (u.parts == 0 || r0 >= u.packed) return;
+    const float* slots = p.line.slots + 2 * (c - 1) * kSlot;
+    const int r = r0 + lane;
+    const bool live = r < u.packed;
+    float m = -INFINITY, l = 0.0f, sum[kEach] = {};
+    if (live)
+#pragma unroll 2
+        for (int x = 0; x < u.parts; ++x) {
+            const float* slot = slots + (x == 0 ? 1 : 2 * x) * kSlot;
+            const float pm = slot[kKvManyRows * D + r];
+            float pl = slot[kKvManyRows * D + kKvManyRows + r];
+            float f[kEach];
+#pragma unroll
+            for (int e = 0; e < kEach; e += 4)
+                *reinterpret_cast<float4*>(f + e) = *reinterpret_cast<const float4*>(slot + (static_cast<int64_t>(warp * kEach + e) / 4 * kKvManyRows + r) * 4);
+            const float top = fmaxf(m, pm);
+            float keep, w;
+            part_weight(m, top, &keep, &l);
+            part_weight(pm, top, &w, &pl);
+            l += pl;
+            m = top;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) sum[e] = w != 0.0f ? fmaf(f[e], w, sum[e] * keep) : sum[e] * keep;
+        }
+    const int32_t packed = u.packed0 + (live ? r : r0), of = kv_div_group(p, packed);
+    const int64_t row = u.row0 + of;
+    const int head = u.h * p.group + packed - of * p.group;
+    const bool valid = live && (!kShared || kv_row_ok(p, static_cast<int32_t>(row)));
+    if (valid) {
+        const KvFinish f = kv_finish<kShared>(p, m, l, row * p.q_heads + head);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) sum[e] *= f.scale;
+        if (kShared && f.own != 0.0f) {
+            const float* own = p.own_out + (row * p.q_heads + head) * D + warp * kEach;
+#pragma unroll
+            for (int e = 0; e < kEach; e += 4) {
+                const float4 y = *reinterpret_cast<const float4*>(own + e);
+                sum[e] = fmaf(y.x, f.own, sum[e]);
+                sum[e + 1] = fmaf(y.y, f.own, sum[e + 1]);
+                sum[e + 2] = fmaf(y.z, f.own, sum[e + 2]);
+                sum[e + 3] = fmaf(y.w, f.own, sum[e + 3]);
+            }
+        }
+        if (p.lse != nullptr && warp == 0) p.lse[row * p.q_heads + head] = f.sum == 0.0f ? -INFINITY : f.base * kLn2 + logf(f.sum);
+#pragma unroll
+        for (int e = 0; e < kEach; e += 4) *reinterpret_cast<float4*>(&s_out[lane][warp * kEach + e]) = *reinterpret_cast<const float4*>(sum + e);
+    }
+    const unsigned ok = __ballot_sync(0xffffffffu, valid);  // the same rows in every warp
+    __syncthreads();
+    constexpr int kLanes = D / 8;
+    for (int i = threadIdx.x / kLanes; i < 32; i += kJoinManyThreads / kLanes) {
+        if (!((ok >> i) & 1u)) continue;
+        const int32_t pk = u.packed0 + r0 + i, o = kv_div_group(p, pk);
+        char* at = p.out.data + static_cast<int64_t>(u.row0 + o) * p.out.row_stride + (u.h * p.group + pk - o * p.group) * p.out.head_stride;
+        const int d = threadIdx.x % kLanes * 8;
+        float f[8];
+        *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(&s_out[i][d]);
+        *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(&s_out[i][d + 4]);
+        if (p.out_f32) Pack<float>::store(at + 4 * d, f);
+        else Pack<T>::store(at + 2 * d, f);
     }
 }
 
@@ -313,22 +341,23 @@ cudaError_t launch_kv_append(const KvAppendParams& p, int head_dim, int dtype, i
     });
 }
 
-cudaError_t launch_kv_join(const KvAttendParams& p, int head_dim, int dtype, int ctas, int slot_rows, cudaStream_t st) {
-    if (ctas > kJoinCtas) return cudaErrorInvalidValue;
-    // at most ctas - 1 units are cut; a warp per row
-    const int64_t rows = static_cast<int64_t>(ctas - 1) * slot_rows, warps = kJoinThreads / 32;
-    const int64_t all = static_cast<int64_t>(p.batch.rows) * p.q_heads;
-    const int64_t want = ((rows < all ? rows : all) + warps - 1) / warps;
-    const dim3 grid(static_cast<unsigned>(want < 1 ? 1 : (want > 4 * ctas ? 4 * ctas : want)));
+cudaError_t launch_kv_join_few(const KvAttendParams& p, int head_dim, int dtype, int ctas, cudaStream_t st) {
     return by_type(dtype, [&](auto t) {
         using T = decltype(t);
-        return head_dim == 64 ? kv_launch(kv_join_kernel<T, 64>, grid, kJoinThreads, 0, st, true, p, ctas, slot_rows)
-                              : kv_launch(kv_join_kernel<T, 128>, grid, kJoinThreads, 0, st, true, p, ctas, slot_rows);
+        return kv_launch(head_dim == 64 ? kv_join_few_kernel<T, 64> : kv_join_few_kernel<T, 128>, dim3(ctas - 1), kJoinFewThreads, 0, st, true, p);
     });
 }
 
-cudaError_t launch_kv_merge(const KvMergeParams& p, int head_dim, int part_dtype, int out_dtype, int num_sms, bool chained,
-                            cudaStream_t st) {
+cudaError_t launch_kv_join_many(const KvAttendParams& p, int head_dim, int dtype, int ctas, cudaStream_t st) {
+    return by_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        auto* f = p.shared_pass ? (head_dim == 64 ? kv_join_many_kernel<T, 64, true> : kv_join_many_kernel<T, 128, true>)
+                                : (head_dim == 64 ? kv_join_many_kernel<T, 64, false> : kv_join_many_kernel<T, 128, false>);
+        return kv_launch(f, dim3(ctas - 1, kKvManyRows / 32), kJoinManyThreads, 0, st, true, p);
+    });
+}
+
+cudaError_t launch_kv_merge(const KvMergeParams& p, int head_dim, int part_dtype, int out_dtype, int num_sms, cudaStream_t st) {
     const int64_t per_cta = kMergeThreads / (head_dim / 8);
     const int64_t want = (static_cast<int64_t>(p.rows) * p.heads + per_cta - 1) / per_cta;
     const dim3 grid(static_cast<unsigned>(want > 16ll * num_sms ? 16ll * num_sms : want));
@@ -336,8 +365,8 @@ cudaError_t launch_kv_merge(const KvMergeParams& p, int head_dim, int part_dtype
         return by_any_type(out_dtype, [&](auto o) {
             using T = decltype(t);
             using O = decltype(o);
-            return head_dim == 64 ? kv_launch(kv_merge_kernel<T, O, 64>, grid, kMergeThreads, 0, st, chained, p)
-                                  : kv_launch(kv_merge_kernel<T, O, 128>, grid, kMergeThreads, 0, st, chained, p);
+            return head_dim == 64 ? kv_launch(kv_merge_kernel<T, O, 64>, grid, kMergeThreads, 0, st, false, p)
+                                  : kv_launch(kv_merge_kernel<T, O, 128>, grid, kMergeThreads, 0, st, false, p);
         });
     });
 }

@@ -42,21 +42,27 @@ struct KvAppendParams {
     int32_t q_heads, rot_dim, interleaved;
 };
 
-// Where a CTA's stretch of the line of tiles begins (KvCuts), left for the joining kernel.
+// Where a CTA's stretch of the line of tiles begins (KvCuts).
 struct KvPlace {
-    int64_t total;    // tiles of the line
-    int64_t begin;    // the unit's first tile on the line
-    int32_t t, count; // tile t of the unit's `count`
-    int32_t row0;     // first row of its sequence
+    int64_t begin;            // the unit's first tile on the line
+    int32_t t, count;         // tile t of the unit's `count`
+    int32_t row0;             // first row of its sequence
     int32_t packed0, packed;  // packed rows [packed0, packed0 + packed) of the sequence
-    int32_t h;        // KV head
-    int32_t s, _pad;
+    int32_t h, s;             // KV head, sequence
 };
 
-// A launch's places (one per CTA) and partial results (two slots per CTA: [rows][D] sums, then
-// the rows' base and weight sum).
+// What the joining kernel finds for a CTA: the rows of the unit that the CTA's cut is the first to
+// divide, left in parts: slot 1 of the CTA before it, slot 0 of this one and the next ones.
+struct KvCut {
+    int32_t parts;  // 0: nothing to join
+    int32_t row0, packed0, packed, h;
+};
+
+// A launch's cuts (one per CTA) and partial results, two slots per CTA: the sums of kRows packed rows
+// ([rows][D] of kv_decode, [D / 4][rows][4] of kv_prompt, so that its threads of neighbouring rows
+// write side by side), then the rows' base and weight sum.
 struct KvLine {
-    KvPlace* places;
+    KvCut* cuts;
     float* slots;
 };
 
@@ -78,7 +84,10 @@ struct KvAttendParams {
     float cap_x;     // scale / softcap
     float cap2;      // softcap in base 2
     int32_t out_f32;
-    int32_t shared_pass;  // kv_prompt: all rows against the shared prefix
+    int32_t few_rows;  // sequences of at most so many packed rows are kv_decode's
+    int32_t shared_pass;   // kv_prompt: all rows against the shared prefix, joined with
+    const float* own_out;  // what was found over the own keys, [rows][q_heads][D]
+    const float* own_lse;  // and its lse
     KvLine line;
 };
 
@@ -92,14 +101,13 @@ struct KvMergeParams {
     KvRowsView out;
     float* lse;
     int32_t rows, heads, part_count;
-    int32_t last_marks;  // rows whose last part's lse still holds kKvUnwritten are left alone
 };
-constexpr uint32_t kKvUnwritten = 0xffffffffu;
 
 // dtype: GFD_* of the cache.  chained: the launch may start before the one before it on the stream has
 // ended (it was made by the same call and touches nothing of this one's, or waits for it).
 cudaError_t launch_kv_append(const KvAppendParams& p, int head_dim, int dtype, int num_sms, cudaStream_t st);
-cudaError_t launch_kv_join(const KvAttendParams& p, int head_dim, int dtype, int ctas, int slot_rows, cudaStream_t st);
+cudaError_t launch_kv_join_few(const KvAttendParams& p, int head_dim, int dtype, int ctas, cudaStream_t st);
+cudaError_t launch_kv_join_many(const KvAttendParams& p, int head_dim, int dtype, int ctas, cudaStream_t st);
 int kv_decode_ctas(int num_sms);
 int kv_prompt_ctas(int num_sms);
 // cuTensorMapEncodeTiled, resolved through the runtime (libcuda is not linked)
@@ -110,13 +118,12 @@ cudaError_t launch_kv_decode(const KvAttendParams& p, int head_dim, int dtype, i
 
 // Bytes of a line's places and slots, and the line laid out in them.
 inline size_t kv_line_bytes(int ctas, int slot_rows, int head_dim) {
-    return (sizeof(KvPlace) * ctas + 255) / 256 * 256 +
+    return (sizeof(KvCut) * ctas + 255) / 256 * 256 +
            (static_cast<size_t>(ctas) * 2 * (static_cast<size_t>(slot_rows) * head_dim + 2 * slot_rows) * sizeof(float) + 255) / 256 * 256;
 }
 inline KvLine kv_line_at(void* p, int ctas) {
-    return KvLine{static_cast<KvPlace*>(p), reinterpret_cast<float*>(static_cast<char*>(p) + (sizeof(KvPlace) * ctas + 255) / 256 * 256)};
+    return KvLine{static_cast<KvCut*>(p), reinterpret_cast<float*>(static_cast<char*>(p) + (sizeof(KvCut) * ctas + 255) / 256 * 256)};
 }
-cudaError_t launch_kv_merge(const KvMergeParams& p, int head_dim, int part_dtype, int out_dtype, int num_sms, bool chained,
-                            cudaStream_t st);
+cudaError_t launch_kv_merge(const KvMergeParams& p, int head_dim, int part_dtype, int out_dtype, int num_sms, cudaStream_t st);
 
 }  // namespace gfdb

@@ -75,10 +75,10 @@ uint64_t table_bytes(const gfd_kv_batch& b) {
 
 // An attention call's kernels and where each keeps its intermediate results in the workspace.
 struct AttendPlan {
-    bool few, many;       // sequences of few / many rows may be among the batch's
+    bool few, many;       // kv_decode takes the sequences of few rows, kv_prompt the others
     size_t few_line, many_line, prefix_line;  // offsets of the kernels' lines
-    size_t parts, part_lse;                   // behind a shared prefix: results over it and over the own keys
-    size_t part_elems, bytes;
+    size_t own_out, own_lse;                  // behind a shared prefix: results over the own keys
+    size_t bytes;
 };
 
 AttendPlan plan_attend(const gfd_ctx* ctx, const gfd_kv_cache& c, const gfd_kv_batch& b, const gfd_kv_attend_args& a, int64_t shared_len) {
@@ -86,8 +86,11 @@ AttendPlan plan_attend(const gfd_ctx* ctx, const gfd_kv_cache& c, const gfd_kv_b
     if (b.rows <= 0 || b.seqs <= 0 || a.q_heads <= 0) return r;
     const int64_t group = a.q_heads / c.heads > 0 ? a.q_heads / c.heads : 1;
     const int64_t most = a.max_q_len > 0 && a.max_q_len < b.rows ? a.max_q_len : b.rows;  // rows of a sequence
-    r.few = group <= kKvFewRows;
     r.many = most * group > kKvFewRows;
+    // Where every sequence has many rows (no row left over: one has at least what the others cannot
+    // have), kv_prompt takes them all, whatever they turn out to be: two launches less, 10 us.
+    const int64_t least = b.rows - (b.seqs - 1) * most;
+    r.few = group <= kKvFewRows && (!r.many || least * group <= kKvFewRows);
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t here = at;
@@ -99,9 +102,8 @@ AttendPlan plan_attend(const gfd_ctx* ctx, const gfd_kv_cache& c, const gfd_kv_b
     if (r.many) r.many_line = take(many_bytes);
     if (shared_len > 0) {
         r.prefix_line = take(many_bytes);
-        r.part_elems = static_cast<size_t>(b.rows) * a.q_heads * c.head_dim;
-        r.parts = take(2 * r.part_elems * sizeof(float));
-        r.part_lse = take(2 * static_cast<size_t>(b.rows) * a.q_heads * sizeof(float));
+        r.own_out = take(static_cast<size_t>(b.rows) * a.q_heads * c.head_dim * sizeof(float));
+        r.own_lse = take(static_cast<size_t>(b.rows) * a.q_heads * sizeof(float));
     }
     r.bytes = at;
     return r;
@@ -216,6 +218,7 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
     p.cap_x = a->softcap > 0.0f ? a->scale / a->softcap : 0.0f;
     p.cap2 = a->softcap * 1.4426950408889634f;
     p.out_f32 = a->out_dtype == GFD_FP32;
+    p.few_rows = plan.few ? kKvFewRows : 0;
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
     char* ws = static_cast<char*>(a->workspace);
     const KvEncodeFn encode = driver().tensor_map;
@@ -223,15 +226,13 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
         return set_error(ctx, GFD_ERR_UNSUPPORTED, "%s: the driver has no cuTensorMapEncodeTiled", call);
     KvAttendParams own = p;
     if (shared_len > 0) {
-        // the results over the prefix and over the own keys go to the workspace in 32 bits
-        own.out = KvRowsView{ws + plan.parts + plan.part_elems * sizeof(float), static_cast<int64_t>(a->q_heads) * c->head_dim * 4,
-                             static_cast<int64_t>(c->head_dim) * 4};
-        own.lse = reinterpret_cast<float*>(ws + plan.part_lse) + b->rows * a->q_heads;
+        // the results over the own keys go to the workspace in 32 bits, the pass over the prefix finishes
+        own.out = KvRowsView{ws + plan.own_out, static_cast<int64_t>(a->q_heads) * c->head_dim * 4, static_cast<int64_t>(c->head_dim) * 4};
+        own.lse = reinterpret_cast<float*>(ws + plan.own_lse);
         own.out_f32 = 1;
     }
     cudaError_t e = cudaSuccess;
-    bool chained = false;  // kernels of this call behind one another: they share nothing until the last
-    if (shared_len > 0) e = cudaMemsetAsync(own.lse, 0xff, static_cast<size_t>(b->rows) * a->q_heads * sizeof(float), st);
+    bool chained = false;  // launches of this call overlap
     if (e == cudaSuccess && plan.few) {
         own.line = kv_line_at(ws + plan.few_line, kv_decode_ctas(ctx->num_sms));
         e = launch_kv_decode(own, c->head_dim, c->dtype, ctx->num_sms, chained, st);
@@ -243,27 +244,12 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
         chained = true;
     }
     if (e == cudaSuccess && shared_len > 0) {
-        KvAttendParams pre = own;
-        pre.out.data = ws + plan.parts;
-        pre.lse = reinterpret_cast<float*>(ws + plan.part_lse);
+        KvAttendParams pre = p;
         pre.shared_pass = 1;
+        pre.own_out = reinterpret_cast<const float*>(ws + plan.own_out);
+        pre.own_lse = own.lse;
         pre.line = kv_line_at(ws + plan.prefix_line, kv_prompt_ctas(ctx->num_sms));
         e = launch_kv_prompt(pre, c->head_dim, c->dtype, ctx->num_sms, encode, chained, st);
-    }
-    if (e == cudaSuccess && shared_len > 0) {
-        KvMergeParams m;
-        std::memset(&m, 0, sizeof(m));
-        m.parts = own.out;
-        m.parts.data = ws + plan.parts;
-        m.part_stride = static_cast<int64_t>(plan.part_elems * sizeof(float));
-        m.part_lse = reinterpret_cast<float*>(ws + plan.part_lse);
-        m.out = p.out;
-        m.lse = p.lse;
-        m.rows = p.batch.rows;
-        m.heads = a->q_heads;
-        m.part_count = 2;
-        m.last_marks = 1;
-        e = launch_kv_merge(m, c->head_dim, GFD_FP32, a->out_dtype, ctx->num_sms, true, st);
     }
     return e == cudaSuccess ? GFD_OK : cuda_error(ctx, e, "kv_attend: kernel launch");
 }
@@ -296,7 +282,7 @@ int merge(gfd_ctx* ctx, const gfd_kv_merge_args* a, void* stream) {
     p.heads = a->heads;
     p.part_count = a->part_count;
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
-    const cudaError_t e = launch_kv_merge(p, a->head_dim, a->part_dtype, a->out_dtype, ctx->num_sms, false, st);
+    const cudaError_t e = launch_kv_merge(p, a->head_dim, a->part_dtype, a->out_dtype, ctx->num_sms, st);
     return e == cudaSuccess ? GFD_OK : cuda_error(ctx, e, "kv_merge: kernel launch");
 }
 

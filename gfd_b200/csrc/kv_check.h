@@ -94,6 +94,16 @@ struct KvCuts {
     }
     GFD_HD int n() const { return static_cast<int>(ctas); }
     GFD_HD int64_t at(uint32_t c) const { return each * c + more * c / ctas; }  // more * c < 2^32: ctas < 2^16
+    // The last cut before position `end` of the line, c being one.
+    GFD_HD uint32_t last_before(uint32_t c, int64_t end) const {
+        uint32_t hi = ctas - 1;
+        while (c < hi) {
+            const uint32_t mid = c + (hi - c + 1) / 2;
+            if (at(mid) < end) c = mid;
+            else hi = mid - 1;
+        }
+        return c;
+    }
 };
 
 // ---------------------------------------------------------------------------

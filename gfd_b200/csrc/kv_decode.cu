@@ -5,7 +5,7 @@
 // so memory bounds it.  All (sequence, KV head) units are laid out as one line of 64-key tiles
 // and every CTA takes an equal stretch (KvCuts): a batch of mixed lengths, one long context and
 // a hundred short ones keep every SM equally busy, with nothing known on the host.  A unit
-// that a cut divides leaves partial sums in the workspace, joined by kv_join_kernel.
+// that a cut divides leaves partial sums in the workspace, joined by kv_join_few_kernel.
 //
 // Inside a CTA each of the 4 warps owns the 16 keys (one page or part of it) w of a tile and runs
 // alone: its own ring of stages filled with 16-byte cp.async (a page id per stage, ids fetched
@@ -78,7 +78,7 @@ __device__ __forceinline__ Seq few_seq(const KvAttendParams& p, int s) {
     Seq r;
     r.q = kv_seq(b.row_start[s], b.row_start[s + 1], b.kv_len[s], b.capacity, p.max_q_len);
     r.bad = !r.q.ok;
-    if (r.bad || r.q.rows * p.group > kRows) r.q.rows = r.q.keys = 0;
+    if (r.bad || static_cast<int64_t>(r.q.rows) * p.group > kRows) r.q.rows = r.q.keys = 0;
     r.all = KvSpan{0, 0, 0};
     r.tiles = KvTiles{0, 0, 0};
     if (r.q.rows > 0) {
@@ -201,10 +201,9 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
     const KvBatchView& b = p.batch;
 
     kv_let_next();
-    if (t == 0) s_place = KvPlace{};
     if (!kv_starts_ok(b)) {
         if (blockIdx.x == 0 && t == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
-        if (t == 0) p.line.places[blockIdx.x] = s_place;
+        if (t == 0) p.line.cuts[blockIdx.x].parts = 0;
         kv_wait_last();
         return;
     }
@@ -216,17 +215,13 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
     });
     const KvCuts cuts(total, gridDim.x);
     if (static_cast<int>(blockIdx.x) >= cuts.n()) {
-        if (t == 0) p.line.places[blockIdx.x].total = total;
+        if (t == 0) p.line.cuts[blockIdx.x].parts = 0;
         kv_wait_last();
         return;
     }
     const int64_t at = cuts.at(blockIdx.x), to = cuts.at(blockIdx.x + 1);
     find_place(p, mine, at, &s_place);
     __syncthreads();
-    if (t == 0) {
-        s_place.total = total;
-        p.line.places[blockIdx.x] = s_place;
-    }
 
     Cursor load, use;
     load.enter(p, s_place.s, s_place.h, s_place.t, to - at);
@@ -288,6 +283,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
     };
 #pragma unroll
     for (int i = 0; i < S::kStages - 1; ++i) issue();
+    if (t == 0) p.line.cuts[blockIdx.x] = kv_cut(cuts, blockIdx.x, s_place);  // while the first keys are on their way
 
     // ---- units ----
     int get = 0;
@@ -502,7 +498,7 @@ cudaError_t launch(const KvAttendParams& p, int ctas, bool chained, cudaStream_t
     const cudaError_t e = kv_launch(plain ? kv_decode_kernel<T, D, true> : kv_decode_kernel<T, D, false>, dim3(ctas), kThreads,
                                     Shape<D>::kSmem, st, chained, p);
     if (e != cudaSuccess) return e;
-    return launch_kv_join(p, D, std::is_same<T, __half>::value ? GFD_FP16 : GFD_BF16, ctas, kRows, st);
+    return launch_kv_join_few(p, D, std::is_same<T, __half>::value ? GFD_FP16 : GFD_BF16, ctas, st);
 }
 
 }  // namespace

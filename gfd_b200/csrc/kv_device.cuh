@@ -125,6 +125,48 @@ __device__ __forceinline__ void kv_store_out(const KvAttendParams& p, int64_t ro
     }
 }
 
+// What CTA c's cut leaves to join, for the CTA whose stretch begins at `at`.
+__device__ __forceinline__ KvCut kv_cut(const KvCuts& cuts, uint32_t c, const KvPlace& at) {
+    KvCut k{0, at.row0, at.packed0, at.packed, at.h};
+    if (c > 0 && at.t > 0 && cuts.at(c - 1) <= at.begin) k.parts = static_cast<int32_t>(cuts.last_before(c, at.begin + at.count) - c) + 2;
+    return k;
+}
+
+// The row belongs to a sequence that is worked on (the starts rise).
+__device__ __forceinline__ bool kv_row_ok(const KvAttendParams& p, int32_t row) {
+    const KvBatchView& b = p.batch;
+    int lo = 0, hi = b.seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (b.row_start[mid] <= row) lo = mid;
+        else hi = mid - 1;
+    }
+    return kv_seq(b.row_start[lo], b.row_start[lo + 1], b.kv_len[lo], b.capacity, p.max_q_len).ok;
+}
+
+// What becomes of a row's sums (relative to 2^base, weights adding up to sum): multiplied by `scale`
+// they are the result; behind a shared prefix the result over the own keys, times `own`, is
+// added (place: of the row and head there).  base and sum: of both together.
+struct KvFinish {
+    float scale, own, base, sum;
+};
+template <bool kShared>
+__device__ __forceinline__ KvFinish kv_finish(const KvAttendParams& p, float base, float sum, int64_t place) {
+    KvFinish f{0.0f, 0.0f, base, sum};
+    float own = -INFINITY;
+    if (kShared) own = p.own_lse[place] * kLog2e;
+    if (own == -INFINITY) {
+        if (sum != 0.0f) f.scale = 1.0f / sum;
+        return f;
+    }
+    f.base = fmaxf(base, own);
+    const float a = base == -INFINITY ? (sum == 0.0f ? 0.0f : 1.0f) : fast_exp2(base - f.base), b = fast_exp2(own - f.base);
+    f.sum = (sum == 0.0f ? 0.0f : sum * a) + b;
+    f.scale = a / f.sum;
+    f.own = b / f.sum;
+    return f;
+}
+
 // Pairs of 32-bit numbers, one instruction for both.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;

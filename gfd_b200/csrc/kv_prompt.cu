@@ -17,7 +17,7 @@
 // is in the next unit; 12 issues the products, 13 loads K and V (TMA boxes of 16 tokens x 64
 // elements, so that every page is found by its id), 14 loads Q, 15 walks the units.  Units lie
 // on one line of tiles that the CTAs (one per SM) share evenly; a cut unit leaves partial sums
-// for kv_join_kernel, as in kv_decode.cu.
+// for kv_join_many_kernel, as in kv_decode.cu.
 
 #include <cuda.h>
 
@@ -180,16 +180,17 @@ struct Many {
     bool bad;
 };
 
+template <bool kShared>
 __device__ __forceinline__ Many many_seq(const KvAttendParams& p, int s) {
     const KvBatchView& b = p.batch;
     Many r;
-    if (p.shared_pass) {
+    if (kShared) {
         r.q = KvSeq{b.row_start[0], b.row_start[b.seqs] - b.row_start[0], p.shared_len, true};
         r.bad = false;
     } else {
         r.q = kv_seq(b.row_start[s], b.row_start[s + 1], b.kv_len[s], b.capacity, p.max_q_len);
         r.bad = !r.q.ok;
-        if (r.bad || r.q.rows * p.group <= kKvFewRows) r.q.rows = r.q.keys = 0;
+        if (r.bad || static_cast<int64_t>(r.q.rows) * p.group <= p.few_rows) r.q.rows = r.q.keys = 0;
     }
     r.tiles = static_cast<int32_t>((static_cast<int64_t>(r.q.rows) * p.group + kRows - 1) / kRows);
     return r;
@@ -201,12 +202,13 @@ struct Unit {
     int32_t packed0, packed;
 };
 
+template <bool kShared>
 __device__ __forceinline__ Unit many_unit(const KvAttendParams& p, int s, const KvSeq& q, int rt) {
     Unit u;
     const int64_t packed = static_cast<int64_t>(q.rows) * p.group;
     u.packed0 = rt * kRows;
     u.packed = static_cast<int32_t>(min(static_cast<int64_t>(kRows), packed - u.packed0));
-    if (p.shared_pass) {
+    if (kShared) {
         // every row stands behind the prefix; with a window the rows nearest to it see most
         u.all = KvSpan{0, 0, p.shared_len};
         if (p.window > 0 && p.prefix_len == nullptr) u.all.lo = min(p.shared_len, max(0, p.shared_len + 1 - p.window));
@@ -224,6 +226,7 @@ __device__ __forceinline__ Unit many_unit(const KvAttendParams& p, int s, const 
     return u;
 }
 
+template <bool kShared>
 struct Cursor {
     Many m;
     Unit u;
@@ -238,8 +241,8 @@ struct Cursor {
         t = at.t;
         begin = at.begin;
         to = to_;
-        m = many_seq(p, s);
-        u = many_unit(p, s, m.q, rt);
+        m = many_seq<kShared>(p, s);
+        u = many_unit<kShared>(p, s, m.q, rt);
         clamp();
     }
     __device__ __forceinline__ void clamp() {
@@ -257,14 +260,14 @@ struct Cursor {
         if (++rt >= m.tiles) {
             rt = 0;
             do {
-                if (++s >= (p.shared_pass ? 1 : p.batch.seqs)) {
+                if (++s >= (kShared ? 1 : p.batch.seqs)) {
                     s = 0;
                     ++h;
                 }
-                m = many_seq(p, s);
+                m = many_seq<kShared>(p, s);
             } while (m.tiles == 0);
         }
-        u = many_unit(p, s, m.q, rt);
+        u = many_unit<kShared>(p, s, m.q, rt);
         clamp();
     }
 };
@@ -284,6 +287,29 @@ struct Desc {
         return (t < npre ? t : t - npre + first) * kTile;
     }
 };
+
+// Tiles [t0, t1) of a unit; none when t1 <= t0.
+template <bool kShared>
+__device__ __forceinline__ Desc describe(const KvAttendParams& p, int s, int h, int t0, int t1, const KvSeq& q, const Unit& u) {
+    Desc d;
+    d.s = s;
+    d.h = h;
+    d.t0 = t0;
+    d.nt = max(t1 - t0, 0);
+    d.count = u.tiles.count;
+    d.npre = u.tiles.npre;
+    d.first = u.tiles.first;
+    d.pre = u.all.pre;
+    d.lo = u.all.lo;
+    d.hi = u.all.hi;
+    d.packed0 = u.packed0;
+    d.packed = u.packed;
+    d.row0 = q.row0;
+    d.rows = q.rows;
+    d.keys = q.keys;
+    d.prefix = !kShared && p.prefix_len != nullptr ? p.prefix_len[s] : 0;
+    return d;
+}
 
 // Inclusive sum over the CTA's threads.
 __device__ __forceinline__ int64_t cta_scan(int64_t v, int64_t* warps, int64_t* total) {
@@ -338,13 +364,14 @@ constexpr float kGrow = 8.0f;
 
 // Position of row r of the unit and what it sees of this pass's keys; rows that do not exist see
 // everything.  `exact`: the position itself is needed, not only the span.
+template <bool kShared>
 __device__ __forceinline__ KvSpan row_span(const KvAttendParams& p, const Desc& u, int r, int32_t* pos, bool exact) {
     *pos = 0;
     if (r >= u.packed) return KvSpan{0x7fffffff, 0, 0};
     const int32_t of = kv_div_group(p, u.packed0 + r);
     int32_t n = p.shared_len + u.keys, prefix = u.prefix;
     *pos = n - u.rows + of;
-    if (p.shared_pass) {
+    if (kShared) {
         // all rows of the batch: the position is that of the row's own sequence, and without a
         // window, a prefix mask or a bias it does not matter
         const KvBatchView& b = p.batch;
@@ -363,7 +390,7 @@ __device__ __forceinline__ KvSpan row_span(const KvAttendParams& p, const Desc& 
             prefix = p.prefix_len != nullptr ? p.prefix_len[lo] : 0;
         }
     }
-    return kv_clip(kv_span(*pos, n, prefix, p.window, p.causal != 0), p.shared_pass ? 0 : p.shared_len, u.keys);
+    return kv_clip(kv_span(*pos, n, prefix, p.window, p.causal != 0), kShared ? 0 : p.shared_len, u.keys);
 }
 
 // the n lowest bits, n clamped to 0 .. 32
@@ -375,7 +402,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-template <typename T, int D, bool kPlain>
+// kShared: the pass over a shared prefix
+template <typename T, int D, bool kPlain, bool kShared>
 __global__ void __launch_bounds__(kThreads, 1)
     kv_prompt_kernel(const KvAttendParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
     using S = Shape<D>;
@@ -395,7 +423,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     kv_let_next();
     if (t == 0) {
-        s_place = KvPlace{};
         s_gave_up = 0;
         for (int i = 0; i < S::kSlots; ++i) {
             bar_init(smem_addr(&bars.full[i]), 1);
@@ -420,31 +447,52 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
 
-    // ---- this CTA's stretch of the line ----
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(S::kColumns)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (t == 13 * 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+    }
+
+    // ---- this CTA's stretch of the line, its first unit for all roles ----
     int64_t stretch_end = 0;
     {
-        const bool ok = kv_starts_ok(b);  // syncs
-        if (!ok && blockIdx.x == 0 && t == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
-        const int seqs = !ok ? 0 : (p.shared_pass ? 1 : b.seqs);
-        // first row tile of every sequence, kept where the operands will lie
+        // the sequences' row tiles; each sequence's first one is kept where the operands will lie
         int32_t* first = reinterpret_cast<int32_t*>(smem);
-        const int per = (seqs + kThreads - 1) / kThreads;
+        const int per = (b.seqs + kThreads - 1) / kThreads, s_lo = min(t * per, b.seqs), s_hi = min(s_lo + per, b.seqs);
         int64_t mine = 0, row_tiles = 0;
-        for (int s = t * per; s < min((t + 1) * per, seqs); ++s) {
-            const Many m = many_seq(p, s);
+        bool bad_starts = false;
+        for (int s = s_lo; s < s_hi; ++s) {
+            const int32_t from = b.row_start[s], to = b.row_start[s + 1];
+            bad_starts |= from < 0 || from > to || to > b.rows;
+            if (kShared) continue;
+            const Many m = many_seq<kShared>(p, s);
             if (m.bad && blockIdx.x == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
             mine += m.tiles;
         }
-        int64_t run = cta_scan(mine, s_warps, &row_tiles) - mine;
-        for (int s = t * per; s < min((t + 1) * per, seqs); ++s) {
-            first[s] = static_cast<int32_t>(run);
-            run += many_seq(p, s).tiles;
+        const bool ok = __syncthreads_or(bad_starts) == 0;
+        if (!ok && blockIdx.x == 0 && t == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
+        const int seqs = !ok ? 0 : (kShared ? 1 : b.seqs);
+        if (kShared) {
+            first[0] = 0;
+            row_tiles = ok ? many_seq<kShared>(p, 0).tiles : 0;
+        } else {
+            int64_t run = cta_scan(mine, s_warps, &row_tiles) - mine;
+            if (!ok) row_tiles = 0;
+            for (int s = s_lo; s < s_hi; ++s) {
+                first[s] = static_cast<int32_t>(run);
+                if (per > 1) run += many_seq<kShared>(p, s).tiles;
+            }
         }
         __syncthreads();
         // tiles of this thread's row tiles, then where the stretch begins
         const int64_t each = (row_tiles + kThreads - 1) / kThreads;
         const int64_t u0 = min(t * each, row_tiles), u1 = min(u0 + each, row_tiles);
         int s0 = 0;
+        Many m0{};
         if (u0 < u1) {
             int lo = 0, hi = seqs - 1;
             while (lo < hi) {
@@ -453,64 +501,59 @@ __global__ void __launch_bounds__(kThreads, 1)
                 else hi = mid - 1;
             }
             s0 = lo;
+            m0 = many_seq<kShared>(p, s0);
         }
-        int64_t per_head = 0, total = 0, at = 0;
-        bool none = false;
+        int64_t per_head = 0, total = 0, want = -1, head = 0;
         for (int pass = 0; pass < 2; ++pass) {
             int s = s0;
-            Many m{};
-            if (u0 < u1) m = many_seq(p, s);
-            int64_t sum = 0;
+            Many m = m0;
+            int64_t here = pass == 0 ? 0 : mine;
             for (int64_t u = u0; u < u1; ++u) {
-                while (u - first[s] >= m.tiles) m = many_seq(p, ++s);
+                while (u - first[s] >= m.tiles) m = many_seq<kShared>(p, ++s);
                 const int rt = static_cast<int>(u - first[s]);
-                const Unit x = many_unit(p, s, m.q, rt);
-                if (pass == 1 && !none) {
-                    const int64_t want = at % per_head, here = mine + sum;
-                    if (want >= here && want < here + x.tiles.count + kUnitCost) {
-                        s_place.s = s;
-                        s_place.h = static_cast<int32_t>(at / per_head);
-                        s_place.t = static_cast<int32_t>(max(want - here - kUnitCost, static_cast<int64_t>(0)));
-                        s_place.count = x.tiles.count;
-                        s_place.begin = at - (want - here) + kUnitCost;
-                        s_place.row0 = m.q.row0;
-                        s_place.packed0 = x.packed0;
-                        s_place.packed = x.packed;
-                    }
+                const Unit x = many_unit<kShared>(p, s, m.q, rt);
+                if (want >= here && want < here + x.tiles.count + kUnitCost) {
+                    const int64_t begin = head * per_head + here + kUnitCost;
+                    const int32_t t0 = static_cast<int32_t>(max(want - here - kUnitCost, static_cast<int64_t>(0)));
+                    s_place.s = s;
+                    s_place.h = static_cast<int32_t>(head);
+                    s_place.t = t0;
+                    s_place.count = x.tiles.count;
+                    s_place.begin = begin;
+                    s_place.row0 = m.q.row0;
+                    s_place.packed0 = x.packed0;
+                    s_place.packed = x.packed;
+                    const int64_t t1 = min(static_cast<int64_t>(x.tiles.count), max(stretch_end - begin, static_cast<int64_t>(0)));
+                    s_unit[0] = describe<kShared>(p, s, static_cast<int32_t>(head), t0, static_cast<int32_t>(t1), m.q, x);
                 }
-                sum += x.tiles.count + kUnitCost;
+                here += x.tiles.count + kUnitCost;
             }
             if (pass == 0) {
-                mine = cta_scan(sum, s_warps, &per_head) - sum;
+                mine = cta_scan(here, s_warps, &per_head) - here;
                 total = per_head * p.cache.heads;
                 const KvCuts cuts(total, gridDim.x);
-                none = static_cast<int>(blockIdx.x) >= cuts.n();
-                if (!none) {
-                    at = cuts.at(blockIdx.x);
+                if (static_cast<int>(blockIdx.x) < cuts.n()) {
+                    const int64_t at = cuts.at(blockIdx.x);
                     stretch_end = cuts.at(blockIdx.x + 1);
+                    head = at / per_head;
+                    want = at - head * per_head;
                 }
             }
         }
+        // (threads of CTAs without a stretch have found no place)
         __syncthreads();
-        if (t == 0) {
-            s_place.total = total;
-            p.line.places[blockIdx.x] = s_place;
-        }
-    }
-    if (stretch_end == 0) {
-        kv_wait_last();
-        return;
-    }
-
-    if (warp == 12) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(S::kColumns)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (t == kThreads - 1)
+            p.line.cuts[blockIdx.x] = stretch_end > 0 ? kv_cut(KvCuts(total, gridDim.x), blockIdx.x, s_place) : KvCut{};
     }
     tm_before();
     __syncthreads();
     tm_after();
     const uint32_t tmem = s_tmem;
+    if (stretch_end == 0) {
+        if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns) : "memory");
+        kv_wait_last();
+        return;
+    }
     const uint32_t sq = smem_addr(smem), ring = sq + 2 * S::kOperand;
     volatile int* gave_up = &s_gave_up;
     // The next unit, read by a whole warp (every role takes every unit, in order).
@@ -532,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int rr = t & (kHalf - 1);                                        // row of the half
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;  // this warp's lanes of tensor memory
         const uint32_t ts = tmem + lanes + x * kTile, to = tmem + lanes + S::kO + x * D;
-        const int32_t base_key = p.shared_pass ? 0 : p.shared_len;
+        const int32_t base_key = kShared ? 0 : p.shared_len;
         uint32_t s_phase = 0, ml_phase = 0;
         int seen = 0;
         Desc u;
@@ -542,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 continue;
             }
             int32_t pos;
-            const KvSpan sp = row_span(p, u, x * kHalf + rr, &pos, !kPlain);
+            const KvSpan sp = row_span<kShared>(p, u, x * kHalf + rr, &pos, !kPlain);
             float slope = 0.0f;
             if (!kPlain && p.alibi != nullptr) slope = p.alibi[u.h * p.group + (u.packed0 + x * kHalf + rr) % p.group] * kLog2e;
             const float scale = kPlain ? p.scale2 : 1.0f;
@@ -664,24 +707,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t o_phase = 0;  // bit x
             Desc u;
             bool good = true;
+            if (kShared) kv_wait_last();  // the results over the own keys, which finish here
             while (good && take(&u)) {
                 const bool whole = u.nt == u.count;
                 float* slot = p.line.slots + (2 * static_cast<int64_t>(blockIdx.x) + (u.t0 == 0 ? 1 : 0)) * (static_cast<int64_t>(kRows) * (D + 2));
-                const bool wide = !whole || p.out_f32;  // 32-bit results
                 for (int x = 0; x * kHalf < u.packed; ++x) {
                     const int rr = (warp & 3) * 32 + lane, r = x * kHalf + rr;
-                    const bool valid = r < u.packed;
-                    const int32_t packed = u.packed0 + (valid ? r : 0);
+                    const int32_t packed = u.packed0 + (r < u.packed ? r : 0);
                     const int32_t of = kv_div_group(p, packed);
                     const int64_t row = u.row0 + of;
                     const int32_t head = u.h * p.group + packed - of * p.group;
+                    const bool valid = r < u.packed && (!whole || !kShared || kv_row_ok(p, static_cast<int32_t>(row)));
                     uint64_t dst = 0;
-                    if (valid)
-                        dst = whole ? reinterpret_cast<uint64_t>(p.out.data + row * p.out.row_stride + head * p.out.head_stride)
-                                    : reinterpret_cast<uint64_t>(slot + static_cast<int64_t>(r) * D);
-                    uint64_t to_row[4];  // this lane writes rows lane / 4 + 8 i
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) to_row[i] = __shfl_sync(0xffffffffu, dst, lane / 4 + 8 * i);
+                    if (valid && whole) dst = reinterpret_cast<uint64_t>(p.out.data + row * p.out.row_stride + head * p.out.head_stride);
                     const uint32_t phase = (o_phase >> x) & 1u;
                     o_phase ^= 1u << x;
                     good = bar_wait(smem_addr(&bars.ml[x]), phase, gave_up) && bar_wait(smem_addr(&bars.o[x]), phase, gave_up);
@@ -690,8 +728,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float base = s_base[x][rr], l = s_sum[x][rr];
                     __syncwarp();
                     if (lane == 0) bar_arrive(smem_addr(&bars.ml_read[x]));
-                    const float inv = !whole ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
-                    float odd = 0.0f;  // NaN once a sum is not finite
+                    float odd = 0.0f;                // NaN once a sum is not finite
+                    KvFinish f{1.0f, 0.0f, base, l};  // what becomes of the sums
+                    const float* own = nullptr;
+                    if (whole) {
+                        f = kv_finish<kShared>(p, base, l, row * p.q_heads + head);
+                        if (kShared && valid && f.own != 0.0f) own = p.own_out + (row * p.q_heads + head) * D;
+                    }
+                    uint64_t to_row[4];  // this lane writes rows lane / 4 + 8 i
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) to_row[i] = __shfl_sync(0xffffffffu, dst, lane / 4 + 8 * i);
 #pragma unroll 1
                     for (int k = 0; k < D; k += 32) {
                         uint32_t o[32];
@@ -704,17 +750,34 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
-                            const float f = __uint_as_float(o[e]);
-                            odd = fmaf(f, 0.0f, odd);
-                            o[e] = __float_as_uint(f * inv);
+                            const float v = __uint_as_float(o[e]);
+                            odd = fmaf(v, 0.0f, odd);
+                            o[e] = __float_as_uint(v * f.scale);
                         }
+                        if (!whole) {
+                            // partial sums: 4 elements of 32 rows side by side
+                            if (valid)
+#pragma unroll
+                                for (int e = 0; e < 32; e += 4)
+                                    *reinterpret_cast<uint4*>(slot + (static_cast<int64_t>((k + e) / 4) * kRows + r) * 4) =
+                                        make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                            continue;
+                        }
+                        if (kShared && own != nullptr)
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) {
+                                const float4 y = *reinterpret_cast<const float4*>(own + k + e);
+                                o[e] = __float_as_uint(fmaf(y.x, f.own, __uint_as_float(o[e])));
+                                o[e + 1] = __float_as_uint(fmaf(y.y, f.own, __uint_as_float(o[e + 1])));
+                                o[e + 2] = __float_as_uint(fmaf(y.z, f.own, __uint_as_float(o[e + 2])));
+                                o[e + 3] = __float_as_uint(fmaf(y.w, f.own, __uint_as_float(o[e + 3])));
+                            }
                         // 64 bytes of every row at a time through shared memory, so that 4 lanes write
                         // them side by side
-                        const int steps = wide ? 2 : 1;
-                        if (!wide)
+                        if (!p.out_f32)
 #pragma unroll
                             for (int e = 0; e < 16; ++e) o[e] = Pack<T>::pair(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
-                        for (int st = 0; st < steps; ++st) {
+                        for (int st = 0; st < (p.out_f32 ? 2 : 1); ++st) {
 #pragma unroll
                             for (int y = 0; y < 4; ++y) {
                                 const uint32_t* w = o + 4 * y;
@@ -732,14 +795,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                                              : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                                              : "r"(stage + rw * 64 + (((lane & 3) ^ ((rw >> 1) & 3)) << 4))
                                              : "memory");
-                                if (to_row[i] != 0) *reinterpret_cast<uint4*>(to_row[i] + (wide ? 4 : 2) * k + 64 * st + 16 * (lane & 3)) = v;
+                                if (to_row[i] != 0)
+                                    *reinterpret_cast<uint4*>(to_row[i] + (p.out_f32 ? 4 : 2) * k + 64 * st + 16 * (lane & 3)) = v;
                             }
                             __syncwarp();
                         }
                     }
                     if (valid) {
                         if (whole) {
-                            if (p.lse != nullptr) p.lse[row * p.q_heads + head] = l == 0.0f ? -INFINITY : base * kLn2 + logf(l);
+                            if (p.lse != nullptr) p.lse[row * p.q_heads + head] = f.sum == 0.0f ? -INFINITY : f.base * kLn2 + logf(f.sum);
                         } else {
                             slot[static_cast<int64_t>(kRows) * D + r] = base;
                             slot[static_cast<int64_t>(kRows) * D + kRows + r] = l;
@@ -748,24 +812,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (uint32_t redo = __ballot_sync(0xffffffffu, valid && odd != 0.0f); redo != 0; redo &= redo - 1) {
                         const int src = __ffs(redo) - 1;
                         KvExact y;
-                        y.table = p.shared_pass ? p.shared_table : b.table + u.s * b.table_stride;
+                        y.table = kShared ? p.shared_table : b.table + u.s * b.table_stride;
                         y.tiles = KvTiles{u.npre, u.first, u.count};
-                        y.seen = row_span(p, u, x * kHalf + (warp & 3) * 32 + src, &y.pos, true);
-                        y.base = p.shared_pass ? 0 : p.shared_len;
+                        const int rs = x * kHalf + (warp & 3) * 32 + src;
+                        y.seen = row_span<kShared>(p, u, rs, &y.pos, true);
+                        y.base = kShared ? 0 : p.shared_len;
                         y.t0 = u.t0;
                         y.t1 = u.t0 + u.nt;
                         y.size = kTile;
                         y.row = __shfl_sync(0xffffffffu, row, src);
                         y.head = __shfl_sync(0xffffffffu, head, src);
                         y.kvh = u.h;
-                        const float rb = __shfl_sync(0xffffffffu, base, src), ri = __shfl_sync(0xffffffffu, inv, src);
+                        const float rb = __shfl_sync(0xffffffffu, base, src), rf = __shfl_sync(0xffffffffu, f.scale, src);
+                        const float ro = __shfl_sync(0xffffffffu, f.own, src);
                         const uint64_t rd = __shfl_sync(0xffffffffu, dst, src);
                         constexpr int kEach = D / 32;
                         float part[kEach];
                         kv_exact_row<T, D, kPlain>(p, y, rb, part);
                         for (int e = 0; e < kEach; ++e) {
-                            if (wide) reinterpret_cast<float*>(rd)[lane * kEach + e] = part[e] * ri;
-                            else reinterpret_cast<T*>(rd)[lane * kEach + e] = static_cast<T>(part[e] * ri);
+                            const int d = lane * kEach + e;
+                            float v = part[e] * rf;
+                            if (kShared && ro != 0.0f) v = fmaf(p.own_out[(y.row * p.q_heads + y.head) * D + d], ro, v);
+                            if (!whole) slot[(static_cast<int64_t>(d / 4) * kRows + rs) * 4 + d % 4] = v;
+                            else if (p.out_f32) reinterpret_cast<float*>(rd)[d] = v;
+                            else reinterpret_cast<T*>(rd)[d] = static_cast<T>(v);
                         }
                     }
                 }
@@ -862,7 +932,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             Desc u;
             bool good = true;
             while (good && take(&u)) {
-                const int32_t* table = p.shared_pass ? p.shared_table : b.table + u.s * b.table_stride;
+                const int32_t* table = kShared ? p.shared_table : b.table + u.s * b.table_stride;
                 const int32_t n = u.keys;
                 for (int i = 0; good && i < u.nt; ++i, ++seen) {
                     const int32_t j0 = u.key(i);
@@ -969,38 +1039,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         } else {
-            // ---- the units of the stretch ----
-            Cursor c;
+            // ---- the units of the stretch; the first one is there ----
+            if (lane == 0) bar_arrive(smem_addr(&bars.unit[0]));
+            Cursor<kShared> c;
             c.enter(p, s_place, stretch_end);
-            for (int i = 0;; ++i) {
+            for (int i = 1; !c.done; ++i) {
+                c.next(p);
                 const int k = i % kUnitRing;
                 if (!bar_wait(smem_addr(&bars.unit_read[k]), ((i / kUnitRing) & 1) ^ 1, gave_up)) break;
                 if (lane == 0) {
-                    Desc d{};
-                    if (!c.done) {
-                        d.s = c.s;
-                        d.h = c.h;
-                        d.t0 = c.t;
-                        d.nt = c.end - c.t;
-                        d.count = c.u.tiles.count;
-                        d.npre = c.u.tiles.npre;
-                        d.first = c.u.tiles.first;
-                        d.pre = c.u.all.pre;
-                        d.lo = c.u.all.lo;
-                        d.hi = c.u.all.hi;
-                        d.packed0 = c.u.packed0;
-                        d.packed = c.u.packed;
-                        d.row0 = c.m.q.row0;
-                        d.rows = c.m.q.rows;
-                        d.keys = c.m.q.keys;
-                        d.prefix = !p.shared_pass && p.prefix_len != nullptr ? p.prefix_len[c.s] : 0;
-                    }
-                    s_unit[k] = d;
+                    s_unit[k] = describe<kShared>(p, c.s, c.h, c.t, c.done ? c.t : c.end, c.m.q, c.u);
                     bar_arrive(smem_addr(&bars.unit[k]));
                 }
                 __syncwarp();
-                if (c.done) break;
-                c.next(p);
             }
         }
     }
@@ -1032,10 +1083,11 @@ bool make_map(CUtensorMap* map, const KvAttendParams& p, const char* base, int h
 template <typename T, int D>
 cudaError_t launch(const KvAttendParams& p, const CUtensorMap& k, const CUtensorMap& v, int ctas, bool chained, cudaStream_t st) {
     const bool plain = p.softcap == 0.0f && p.alibi == nullptr && p.scale2 > 0.0f;
-    const cudaError_t e = kv_launch(plain ? kv_prompt_kernel<T, D, true> : kv_prompt_kernel<T, D, false>, dim3(ctas), kThreads,
-                                    Shape<D>::kSmem, st, chained, p, k, v);
+    auto* f = p.shared_pass ? (plain ? kv_prompt_kernel<T, D, true, true> : kv_prompt_kernel<T, D, false, true>)
+                            : (plain ? kv_prompt_kernel<T, D, true, false> : kv_prompt_kernel<T, D, false, false>);
+    const cudaError_t e = kv_launch(f, dim3(ctas), kThreads, Shape<D>::kSmem, st, chained, p, k, v);
     if (e != cudaSuccess) return e;
-    return launch_kv_join(p, D, std::is_same<T, __half>::value ? GFD_FP16 : GFD_BF16, ctas, kRows, st);
+    return launch_kv_join_many(p, D, std::is_same<T, __half>::value ? GFD_FP16 : GFD_BF16, ctas, st);
 }
 
 }  // namespace
