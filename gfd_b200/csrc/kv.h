@@ -42,7 +42,7 @@ struct KvAppendParams {
     int32_t q_heads, rot_dim, interleaved;
 };
 
-// Where a CTA's stretch of the line of tiles begins (KvCuts).
+// Where a stretch of the line of tiles begins (KvCuts).
 struct KvPlace {
     int64_t begin;            // the unit's first tile on the line
     int32_t t, count;         // tile t of the unit's `count`
@@ -51,14 +51,14 @@ struct KvPlace {
     int32_t h, s;             // KV head, sequence
 };
 
-// What the joining kernel finds for a CTA: the rows of the unit that the CTA's cut is the first to
-// divide, left in parts: slot 1 of the CTA before it, slot 0 of this one and the next ones.
+// What the joining kernel finds for a stretch: the rows of the unit that the stretch's cut is the first
+// to divide, left in parts: slot 1 of the stretch before it, slot 0 of this one and the next ones.
 struct KvCut {
     int32_t parts;  // 0: nothing to join
     int32_t row0, packed0, packed, h;
 };
 
-// A launch's cuts (one per CTA) and partial results, two slots per CTA: the sums of kRows packed rows
+// A launch's cuts and partial results, one and two slots per stretch: the sums of kRows packed rows
 // ([rows][D] of kv_decode, [D / 4][rows][4] of kv_prompt, so that its threads of neighbouring rows
 // write side by side), then the rows' base and weight sum.
 struct KvLine {
@@ -108,7 +108,7 @@ struct KvMergeParams {
 cudaError_t launch_kv_append(const KvAppendParams& p, int head_dim, int dtype, int num_sms, cudaStream_t st);
 cudaError_t launch_kv_join_few(const KvAttendParams& p, int head_dim, int dtype, int ctas, cudaStream_t st);
 cudaError_t launch_kv_join_many(const KvAttendParams& p, int head_dim, int dtype, int ctas, cudaStream_t st);
-int kv_decode_ctas(int num_sms);
+int kv_decode_workers(int num_sms);  // each with a stretch of the line
 int kv_prompt_ctas(int num_sms);
 // cuTensorMapEncodeTiled, resolved through the runtime (libcuda is not linked)
 using KvEncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,

@@ -80,10 +80,10 @@ GFD_HD KvTiles kv_tiles(KvSpan s, int32_t size) {
     return t;
 }
 
-// All tiles of a launch form one line, unit after unit; CTA c takes [at(c), at(c + 1)), at least
-// one tile each: CTAs beyond n() have none.  A unit that lies in one CTA is finished there.  One
-// that is cut leaves partial results, one in each CTA it touches, in slot 1 of the CTA where it
-// begins and slot 0 of the others; the first cut inside a unit names the one who joins them.
+// All tiles of a launch form one line, unit after unit; stretch c is [at(c), at(c + 1)), at least one
+// tile each, n() of them.  A unit inside one stretch is finished there.  One that is cut leaves
+// partial results, one in each stretch it touches, in slot 1 of the one where it begins and slot 0
+// of the others; they are joined at the first cut inside the unit.
 struct KvCuts {
     int64_t each;
     uint32_t more, ctas;
@@ -93,7 +93,7 @@ struct KvCuts {
         more = ctas > 0 ? static_cast<uint32_t>(total - each * ctas) : 0;
     }
     GFD_HD int n() const { return static_cast<int>(ctas); }
-    GFD_HD int64_t at(uint32_t c) const { return each * c + more * c / ctas; }  // more * c < 2^32: ctas < 2^16
+    GFD_HD int64_t at(uint32_t c) const { return each * c + more * c / ctas; }  // more * c < 2^32: ctas <= 2^16
     // The last cut before position `end` of the line, c being one.
     GFD_HD uint32_t last_before(uint32_t c, int64_t end) const {
         uint32_t hi = ctas - 1;

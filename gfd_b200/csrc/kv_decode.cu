@@ -2,15 +2,16 @@
 // per KV head, where a packed row is one (row, query head) pair of the head's group.
 //
 // The work is reading the cache once: 4 D bytes per key and KV head against 4 D * 16 operations,
-// so memory bounds it.  All (sequence, KV head) units are laid out as one line of 64-key tiles
-// and every CTA takes an equal stretch (KvCuts): a batch of mixed lengths, one long context and
-// a hundred short ones keep every SM equally busy, with nothing known on the host.  A unit
-// that a cut divides leaves partial sums in the workspace, joined by kv_join_few_kernel.
+// so memory bounds it.  All (sequence, KV head) units are laid out as one line of 16-key tiles (one
+// page or part of one) and every warp takes an equal stretch (KvCuts): a batch of mixed lengths,
+// one long context and a hundred short ones keep every SM equally busy, with nothing known on
+// the host.  A unit that a cut divides leaves partial sums in the workspace, joined by
+// kv_join_few_kernel.
 //
-// Inside a CTA each of the 4 warps owns the 16 keys (one page or part of it) w of a tile and runs
-// alone: its own ring of stages filled with 16-byte cp.async (a page id per stage, ids fetched
-// 32 stages at a time), its own running maximum and sum, scores and sums by mma.m16n8k16 from
-// ldmatrix fragments.  No barrier between tiles; the warps join once per unit.
+// The warps run alone: each has its own ring of stages filled with 16-byte cp.async (8 KB a stage,
+// 192 KB in flight on an SM; block ids fetched 32 stages at a time), its own running maximum and
+// sum, scores and sums by mma.m16n8k16 from ldmatrix fragments, and writes its rows from
+// registers.  After the stretches are found there is no barrier.
 
 #include <type_traits>
 
@@ -21,7 +22,8 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kTile = kKvPage * kWarps;  // keys a CTA takes per step
+constexpr int kTile = kKvPage;  // keys a warp takes per step
+constexpr int kLeast = 2;       // tiles of a stretch, where there are enough: a part costs its joining about as much
 constexpr int kRows = kKvFewRows;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -94,52 +96,65 @@ __device__ __forceinline__ Seq few_seq(const KvAttendParams& p, int s) {
     return r;
 }
 
-template <typename F>
-__device__ __forceinline__ int64_t line_total(const KvAttendParams& p, int64_t* mine, F count) {
+// Where the stretches of this CTA's warps begin on the line, found together.  *cuts: the line's cuts;
+// false: the row starts do not rise.
+__device__ __forceinline__ bool find_places(const KvAttendParams& p, KvCuts* cuts, KvPlace* places) {
     __shared__ int64_t s_warp[kWarps];
+    const KvBatchView& b = p.batch;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int per = (p.batch.seqs + kThreads - 1) / kThreads;
+    const int per = (b.seqs + kThreads - 1) / kThreads, s_lo = min(t * per, b.seqs), s_hi = min(s_lo + per, b.seqs);
     int64_t sum = 0;
-    for (int s = t * per; s < min((t + 1) * per, p.batch.seqs); ++s) sum += count(s);
+    bool bad = false;
+    Seq q;
+    for (int s = s_lo; s < s_hi; ++s) {
+        const int32_t from = b.row_start[s], to = b.row_start[s + 1];
+        bad |= from < 0 || from > to || to > b.rows;
+        q = few_seq(p, s);
+        if (q.bad && blockIdx.x == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
+        sum += static_cast<int64_t>(q.tiles.count) * p.cache.heads;
+    }
     int64_t incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += y;
     }
-    __syncthreads();
     if (lane == 31) s_warp[warp] = incl;
-    __syncthreads();
-    int64_t before = 0, total = 0;
+    if (__syncthreads_or(bad) != 0) {
+        if (blockIdx.x == 0 && t == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
+        return false;
+    }
+    int64_t run = incl - sum, total = 0;
     for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += s_warp[w];
+        if (w < warp) run += s_warp[w];
         total += s_warp[w];
     }
-    *mine = before + incl - sum;
-    return total;
-}
-
-// Position `at` of the line, found by the CTA together.
-__device__ __forceinline__ void find_place(const KvAttendParams& p, int64_t mine, int64_t at, KvPlace* out) {
-    const int per = (p.batch.seqs + kThreads - 1) / kThreads;
-    const int t = threadIdx.x;
-    int64_t run = mine;
-    for (int s = t * per; s < min((t + 1) * per, p.batch.seqs); ++s) {
-        const Seq q = few_seq(p, s);
+    const int64_t most = (total + kLeast - 1) / kLeast;
+    *cuts = KvCuts(total, static_cast<uint32_t>(min(static_cast<int64_t>(kWarps) * gridDim.x, most)));
+    for (int s = s_lo; s < s_hi; ++s) {
+        if (per > 1) q = few_seq(p, s);
         const int32_t n = q.tiles.count;
         const int64_t here = static_cast<int64_t>(n) * p.cache.heads;
-        if (n > 0 && at >= run && at < run + here) {
-            out->s = s;
-            out->h = static_cast<int32_t>((at - run) / n);
-            out->t = static_cast<int32_t>((at - run) % n);
-            out->count = n;
-            out->begin = run + static_cast<int64_t>(out->h) * n;
-            out->row0 = q.q.row0;
-            out->packed0 = 0;
-            out->packed = q.q.rows * p.group;
-        }
+        if (n > 0)
+            for (int w = 0; w < kWarps; ++w) {
+                const int worker = w * gridDim.x + blockIdx.x;
+                if (worker >= cuts->n()) break;
+                const int64_t at = cuts->at(worker) - run;
+                if (at < 0 || at >= here) continue;
+                KvPlace& x = places[w];
+                x.s = s;
+                x.h = static_cast<int32_t>(at / n);
+                x.t = static_cast<int32_t>(at - static_cast<int64_t>(x.h) * n);
+                x.count = n;
+                x.begin = run + static_cast<int64_t>(x.h) * n;
+                x.row0 = q.q.row0;
+                x.packed0 = 0;
+                x.packed = q.q.rows * p.group;
+            }
         run += here;
     }
+    __syncthreads();
+    return true;
 }
 
 // Walks the units of a stretch.
@@ -180,12 +195,15 @@ struct Cursor {
 template <int D>
 struct Shape {
     static constexpr int kStages = D == 128 ? 3 : 6;
-    static constexpr int kRow = 2 * D;               // bytes of a key
+    static constexpr int kRow = 2 * D;                 // bytes of a key
     static constexpr int kStage = 2 * kKvPage * kRow;  // K and V of 16 keys
     static constexpr int kRing = kStages * kStage;
-    static constexpr int kJoin = kWarps * 8 * D * 4;  // 8 rows of every warp
-    static constexpr int kSmem = kWarps * kRing + kJoin;
+    static constexpr int kSmem = kWarps * kRing;
 };
+
+// fp16 weights reach 2^8, which keeps the small ones clear of that type's coarse steps below 2^-14.
+template <typename T>
+constexpr float kShift = std::is_same<T, __half>::value ? 8.0f : 0.0f;
 
 template <typename T, int D, bool kPlain>
 __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendParams p) {
@@ -193,38 +211,21 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
     constexpr int kSteps = D / 16;   // k-steps of the scores, pairs of n-tiles of the sums
     constexpr int kChunks = D / 8;   // 16-byte pieces of a key
     extern __shared__ __align__(128) char smem[];
-    __shared__ KvPlace s_place;
-    __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
-    __shared__ uint32_t s_odd;
-    float* s_join = reinterpret_cast<float*>(smem + kWarps * S::kRing);
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    __shared__ KvPlace s_place[kWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // neighbouring stretches lie on different SMs, so that a short line is spread over all of them
+    const int worker = warp * gridDim.x + blockIdx.x;
     const KvBatchView& b = p.batch;
 
     kv_let_next();
-    if (!kv_starts_ok(b)) {
-        if (blockIdx.x == 0 && t == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
-        if (t == 0) p.line.cuts[blockIdx.x].parts = 0;
+    KvCuts cuts(0, 0);
+    if (!find_places(p, &cuts, s_place) || worker >= cuts.n()) {
+        if (lane == 0) p.line.cuts[worker].parts = 0;
         kv_wait_last();
         return;
     }
-    int64_t mine;
-    const int64_t total = line_total(p, &mine, [&](int s) {
-        const Seq q = few_seq(p, s);
-        if (q.bad && blockIdx.x == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
-        return static_cast<int64_t>(q.tiles.count) * p.cache.heads;
-    });
-    const KvCuts cuts(total, gridDim.x);
-    if (static_cast<int>(blockIdx.x) >= cuts.n()) {
-        if (t == 0) p.line.cuts[blockIdx.x].parts = 0;
-        kv_wait_last();
-        return;
-    }
-    const int64_t at = cuts.at(blockIdx.x), to = cuts.at(blockIdx.x + 1);
-    find_place(p, mine, at, &s_place);
-    __syncthreads();
-
     Cursor load, use;
-    load.enter(p, s_place.s, s_place.h, s_place.t, to - at);
+    load.enter(p, s_place[warp].s, s_place[warp].h, s_place[warp].t, cuts.at(worker + 1) - cuts.at(worker));
     use = load;
 
     // ---- stages ----
@@ -240,12 +241,19 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
         if (!load.done) {
             const KvSpan& a = load.q.all;
             if (!ids_ok || load.t >= ids_from + 32) {
+                if (!ids_ok && lane < 2 * kRows) {
+                    // a new unit: its rows of Q set out as well
+                    const int r = lane / 2, of = kv_div_group(p, r);
+                    if (r < load.q.q.rows * p.group && (D == 128 || lane % 2 == 0))
+                        asm volatile("prefetch.global.L1 [%0];" ::"l"(p.q.data + (load.q.q.row0 + of) * p.q.row_stride +
+                                                                      (load.h * p.group + r - of * p.group) * p.q.head_stride + 128 * (lane % 2)));
+                }
                 ids_from = load.t;
                 ids_ok = true;
                 const int32_t i = ids_from + lane;
                 ids = -1;
                 if (i < load.end) {
-                    const int32_t j = load.q.tiles.at(i) * kTile + warp * kKvPage;
+                    const int32_t j = load.q.tiles.at(i) * kTile;
                     if (j < a.pre || (j + kKvPage > a.lo && j < a.hi)) {
                         ids = b.table[load.s * b.table_stride + j / kKvPage / pages];
                         if (ids < 0 || ids >= p.cache.blocks) {
@@ -258,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
             const int32_t id = __shfl_sync(0xffffffffu, ids, load.t - ids_from);
             if (id >= 0) {
                 live |= 1u;
-                const int32_t j = load.q.tiles.at(load.t) * kTile + warp * kKvPage;
+                const int32_t j = load.q.tiles.at(load.t) * kTile;
                 const int32_t place = (j / kKvPage % pages) * kKvPage;
                 const int64_t base = id * p.cache.block_stride + place * p.cache.token_stride + load.h * p.cache.head_stride;
                 const uint32_t dst = ring + put * S::kStage;
@@ -283,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
     };
 #pragma unroll
     for (int i = 0; i < S::kStages - 1; ++i) issue();
-    if (t == 0) p.line.cuts[blockIdx.x] = kv_cut(cuts, blockIdx.x, s_place);  // while the first keys are on their way
+    if (lane == 0) p.line.cuts[worker] = kv_cut(cuts, worker, s_place[warp]);  // while the first keys are on their way
 
     // ---- units ----
     int get = 0;
@@ -299,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int r = row_a + 8 * x;
-            const int i = r / p.group, head = use.h * p.group + r % p.group;
+            const int i = kv_div_group(p, r), head = use.h * p.group + r - i * p.group;
             pos[x] = n - use.q.q.rows + i;
             sp[x] = KvSpan{0, 0, 0};
             if (r < rows) {
@@ -313,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
                 qf[k][2 + x] = r < rows ? *reinterpret_cast<const uint32_t*>(src + 32 * k + 16) : 0u;
             }
         }
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // the weights' base (2^m) and sum
         float acc[2 * kSteps][4];
 #pragma unroll
         for (int i = 0; i < 2 * kSteps; ++i)
@@ -337,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
                     mma<T>(z[0], qf[k], f[0], f[1]);
                     mma<T>(z[1], qf[k], f[2], f[3]);
                 }
-                const int32_t j0 = use.q.tiles.at(use.t) * kTile + warp * kKvPage + 2 * (lane & 3);
+                const int32_t j0 = use.q.tiles.at(use.t) * kTile + 2 * (lane & 3);
                 float mx[2] = {-INFINITY, -INFINITY};
                 if (!kPlain) kv_cap<8>(p, reinterpret_cast<uint32_t*>(&z[0][0]));
 #pragma unroll
@@ -356,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
-                    mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
+                    mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2)) - kShift<T>;
                     grew |= mx[x] > m[x];
                     mx[x] = fmaxf(mx[x], m[x]);
                     base[x] = mx[x] == -INFINITY ? 0.0f : mx[x];
@@ -398,93 +406,64 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
             get = get + 1 == S::kStages ? 0 : get + 1;
         }
 
-        // ---- the warps join ----
+        // ---- the unit's rows ----
+        const bool whole = t0 == 0 && use.end == use.q.tiles.count;
+        float* slot = p.line.slots + (2 * static_cast<int64_t>(worker) + (t0 == 0 ? 1 : 0)) * (kRows * D + 2 * kRows);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
+            if (8 * x >= rows) break;
             l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
             l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-            if ((lane & 3) == 0) {
-                s_m[warp][row_a + 8 * x] = m[x];
-                s_l[warp][row_a + 8 * x] = l[x];
-            }
-        }
-        const bool whole = t0 == 0 && use.end == use.q.tiles.count;
-        float* slot = p.line.slots + (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0)) * (kRows * D + 2 * kRows);
-        for (int half = 0; half < 2 && 8 * half < rows; ++half) {
-            if (t == 0) s_odd = 0;
-            __syncthreads();
-            const int r = row_a + 8 * half;
-            const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-            const float keep = m[half] == -INFINITY ? 0.0f : fast_exp2(m[half] - top);
-            float* w = s_join + (warp * 8 + row_a) * D + 2 * (lane & 3);
+            const int r = row_a + 8 * x, i = kv_div_group(p, r), head = use.h * p.group + r - i * p.group;
+            const int64_t row = use.q.q.row0 + i;
+            const float inv = !whole ? 1.0f : (l[x] == 0.0f ? 0.0f : 1.0f / l[x]);
+            char* dst = whole ? p.out.data + row * p.out.row_stride + head * p.out.head_stride : reinterpret_cast<char*>(slot + r * D);
+            const bool wide = !whole || p.out_f32;
+            float odd = 0.0f;  // NaN once a sum is not finite
 #pragma unroll
-            for (int i = 0; i < 2 * kSteps; ++i)
-                *reinterpret_cast<float2*>(w + 8 * i) = make_float2(acc[i][2 * half] * keep, acc[i][2 * half + 1] * keep);
-            __syncthreads();
-            // 16 threads a row, D / 16 elements each
-            constexpr int kEach = D / 16;
-            const int jr = t >> 4, d0 = (t & 15) * kEach, rr = jr + 8 * half;
-            float sum[kEach] = {}, ml = 0.0f, mt = -INFINITY;
-#pragma unroll
-            for (int x = 0; x < kWarps; ++x) mt = fmaxf(mt, s_m[x][rr]);
-#pragma unroll
-            for (int x = 0; x < kWarps; ++x) {
-                if (s_m[x][rr] != -INFINITY) ml += s_l[x][rr] * fast_exp2(s_m[x][rr] - mt);
-                else ml += s_l[x][rr];  // 0, or NaN from scores that are NaN
-#pragma unroll
-                for (int e = 0; e < kEach; ++e) sum[e] += s_join[(x * 8 + jr) * D + d0 + e];
-            }
-            bool odd = false;
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) odd |= !(fabsf(sum[e]) < INFINITY);
-            if (odd && rr < rows) atomicOr(&s_odd, 1u << jr);
-            __syncthreads();
-            const uint32_t redo = s_odd;
-            for (int x = warp; x < 8; x += kWarps)
-                if ((redo >> x) & 1u) {
-                    const int r = x + 8 * half, i = r / p.group;
-                    const float mm = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-                    KvExact y;
-                    y.table = b.table + use.s * b.table_stride;
-                    y.tiles = use.q.tiles;
-                    y.pos = n - use.q.q.rows + i;
-                    y.seen = kv_clip(kv_span(y.pos, n, prefix, p.window, p.causal != 0), p.shared_len, use.q.q.keys);
-                    y.base = p.shared_len;
-                    y.t0 = t0;
-                    y.t1 = use.end;
-                    y.size = kTile;
-                    y.row = use.q.q.row0 + i;
-                    y.head = use.h * p.group + r % p.group;
-                    y.kvh = use.h;
-                    float part[D / 32];
-                    kv_exact_row<T, D, kPlain>(p, y, mm, part);
-                    for (int e = 0; e < D / 32; ++e) s_join[x * D + lane * (D / 32) + e] = part[e];
-                }
-            if (redo != 0) __syncthreads();
-            if ((redo >> jr) & 1u)
-#pragma unroll
-                for (int e = 0; e < kEach; ++e) sum[e] = s_join[jr * D + d0 + e];
-            if (rr < rows) {
-                if (whole) {
-                    const int64_t row = use.q.q.row0 + rr / p.group;
-                    const int head = use.h * p.group + rr % p.group;
-                    const float inv = ml == 0.0f ? 0.0f : 1.0f / ml;
-#pragma unroll
-                    for (int e = 0; e < kEach; ++e) sum[e] = ml == 0.0f ? 0.0f : sum[e] * inv;
-                    kv_store_out<T>(p, row, head, d0, sum, kEach);
-                    if (p.lse != nullptr && d0 == 0)
-                        p.lse[row * p.q_heads + head] = ml == 0.0f ? -INFINITY : mt * kLn2 + logf(ml);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < kEach; e += 4)
-                        *reinterpret_cast<float4*>(slot + rr * D + d0 + e) = *reinterpret_cast<float4*>(sum + e);
-                    if (d0 == 0) {
-                        slot[kRows * D + rr] = mt;
-                        slot[kRows * D + kRows + rr] = ml;
-                    }
+            for (int y = 0; y < 2 * kSteps; ++y) {
+                odd = fmaf(acc[y][2 * x], 0.0f, odd);
+                odd = fmaf(acc[y][2 * x + 1], 0.0f, odd);
+                if (r < rows) {
+                    const float v0 = acc[y][2 * x] * inv, v1 = acc[y][2 * x + 1] * inv;
+                    if (wide) reinterpret_cast<float2*>(dst)[4 * y + (lane & 3)] = make_float2(v0, v1);
+                    else reinterpret_cast<uint32_t*>(dst)[4 * y + (lane & 3)] = Pack<T>::pair(v0, v1);
                 }
             }
-            __syncthreads();
+            if (r < rows && (lane & 3) == 0) {
+                if (!whole) {
+                    slot[kRows * D + r] = m[x];
+                    slot[kRows * D + kRows + r] = l[x];
+                } else if (p.lse != nullptr) {
+                    p.lse[row * p.q_heads + head] = l[x] == 0.0f ? -INFINITY : m[x] * kLn2 + logf(l[x]);
+                }
+            }
+            for (uint32_t redo = __ballot_sync(0xffffffffu, r < rows && odd != 0.0f); redo != 0;) {
+                const int src = (__ffs(redo) - 1) & ~3;
+                redo &= ~(15u << src);
+                KvExact y;
+                y.table = b.table + use.s * b.table_stride;
+                y.tiles = use.q.tiles;
+                y.seen = KvSpan{__shfl_sync(0xffffffffu, sp[x].pre, src), __shfl_sync(0xffffffffu, sp[x].lo, src),
+                                __shfl_sync(0xffffffffu, sp[x].hi, src)};
+                y.pos = __shfl_sync(0xffffffffu, pos[x], src);
+                y.base = p.shared_len;
+                y.t0 = t0;
+                y.t1 = use.end;
+                y.size = kTile;
+                y.row = __shfl_sync(0xffffffffu, row, src);
+                y.head = __shfl_sync(0xffffffffu, head, src);
+                y.kvh = use.h;
+                const float rb = __shfl_sync(0xffffffffu, m[x], src), ri = __shfl_sync(0xffffffffu, inv, src);
+                const uint64_t rd = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), src);
+                constexpr int kEach = D / 32;
+                float part[kEach];
+                kv_exact_row<T, D, kPlain>(p, y, rb, part);
+                for (int e = 0; e < kEach; ++e) {
+                    if (wide) reinterpret_cast<float*>(rd)[lane * kEach + e] = part[e] * ri;
+                    else reinterpret_cast<T*>(rd)[lane * kEach + e] = static_cast<T>(part[e] * ri);
+                }
+            }
         }
         use.next_unit(p);
     }
@@ -498,15 +477,15 @@ cudaError_t launch(const KvAttendParams& p, int ctas, bool chained, cudaStream_t
     const cudaError_t e = kv_launch(plain ? kv_decode_kernel<T, D, true> : kv_decode_kernel<T, D, false>, dim3(ctas), kThreads,
                                     Shape<D>::kSmem, st, chained, p);
     if (e != cudaSuccess) return e;
-    return launch_kv_join_few(p, D, std::is_same<T, __half>::value ? GFD_FP16 : GFD_BF16, ctas, st);
+    return launch_kv_join_few(p, D, std::is_same<T, __half>::value ? GFD_FP16 : GFD_BF16, kWarps * ctas, st);
 }
 
 }  // namespace
 
-int kv_decode_ctas(int num_sms) { return 2 * num_sms; }
+int kv_decode_workers(int num_sms) { return 2 * num_sms * kWarps; }
 
 cudaError_t launch_kv_decode(const KvAttendParams& p, int head_dim, int dtype, int num_sms, bool chained, cudaStream_t st) {
-    const int ctas = kv_decode_ctas(num_sms);
+    const int ctas = 2 * num_sms;
     if (dtype == GFD_BF16)
         return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, ctas, chained, st) : launch<__nv_bfloat16, 128>(p, ctas, chained, st);
     return head_dim == 64 ? launch<__half, 64>(p, ctas, chained, st) : launch<__half, 128>(p, ctas, chained, st);

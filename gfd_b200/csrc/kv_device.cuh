@@ -268,7 +268,7 @@ __device__ __forceinline__ void kv_exact_row(const KvAttendParams& p, const KvEx
             const int32_t j = x.tiles.at(t) * x.size + c + lane;
             int64_t at = -1;
             float w = 0.0f;
-            if (j < x.seen.pre || (j >= x.seen.lo && j < x.seen.hi)) {
+            if (c + lane < x.size && (j < x.seen.pre || (j >= x.seen.lo && j < x.seen.hi))) {
                 const int32_t id = x.table[j / p.cache.block_tokens];
                 if (id >= 0 && id < p.cache.blocks) {
                     at = id * p.cache.block_stride + j % p.cache.block_tokens * p.cache.token_stride + x.kvh * p.cache.head_stride;
