@@ -176,110 +176,164 @@ __device__ __forceinline__ void part_weight(float base, float top, float* w, flo
     if (base != -INFINITY) *l *= *w;
 }
 
-// Of kv_decode, with up to hundreds of parts of a few rows: a warp per row, whose lanes weigh 32 parts
-// at a time and then sum D / 32 elements each over the parts, in their order.
-constexpr int kJoinFewThreads = 128;
+// Of kv_decode, with up to hundreds of parts of a few rows: a CTA takes 4 rows at a time and 128 parts:
+// its threads weigh them, then each warp sums every 8th part (D / 32 elements a lane), and the warps'
+// sums are added in their order.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinWarps = kJoinThreads / 32;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinFewThreads) kv_join_few_kernel(const KvAttendParams p) {
-    constexpr int kEach = D / 32, kSlot = kKvFewRows * (D + 2);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x + 1;
+__global__ void __launch_bounds__(kJoinThreads) kv_join_few_kernel(const KvAttendParams p) {
+    constexpr int kEach = D / 32, kSlot = kKvFewRows * (D + 2), kParts = 128;
+    __shared__ float s_w[kParts][4];
+    __shared__ float s_top[kJoinWarps][2], s_sum[kJoinWarps][2];
+    __shared__ float s_acc[kJoinWarps][4][D];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, c = blockIdx.x + 1;
     kv_let_next();
     kv_wait_last();
     const KvCut u = p.line.cuts[c];
     if (u.parts == 0) return;
     const float* slots = p.line.slots + 2 * static_cast<int64_t>(c - 1) * kSlot;  // part x: slot 1 for 0, else 2 x
-    for (int r = warp; r < u.packed; r += kJoinFewThreads / 32) {
-        float m = -INFINITY, l = 0.0f, sum[kEach] = {};
-        for (int x0 = 0; x0 < u.parts; x0 += 32) {
-            const int x = x0 + lane, n = min(32, u.parts - x0);
-            const float* slot = slots + static_cast<int64_t>(x == 0 ? 1 : 2 * x) * kSlot + kKvFewRows * D + r;
-            float pm = -INFINITY, pl = 0.0f;
-            if (lane < n) {
-                pm = slot[0];
-                pl = slot[kKvFewRows];
-            }
-            float top = pm;
+    for (int r0 = 0; r0 < u.packed; r0 += 4) {
+        const int nr = min(4, u.packed - r0);
+        float m[4], l[4], acc[4][kEach];
 #pragma unroll
-            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            top = fmaxf(top, m);
-            float keep, w;
-            part_weight(m, top, &keep, &l);
-            part_weight(pm, top, &w, &pl);
+        for (int r = 0; r < 4; ++r) {
+            m[r] = -INFINITY;
+            l[r] = 0.0f;
 #pragma unroll
-            for (int o = 16; o; o >>= 1) pl += __shfl_xor_sync(0xffffffffu, pl, o);
-            l += pl;
-            m = top;
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) sum[e] *= keep;
-#pragma unroll 8
-            for (int y = 0; y < n; ++y) {
-                const float wy = __shfl_sync(0xffffffffu, w, y);
-                const float* v = slots + static_cast<int64_t>(x0 + y == 0 ? 1 : 2 * (x0 + y)) * kSlot + r * D + lane * kEach;
-                float f[kEach];
-                if constexpr (kEach == 4) *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(v);
-                else *reinterpret_cast<float2*>(f) = *reinterpret_cast<const float2*>(v);
-                if (wy != 0.0f)
-#pragma unroll
-                    for (int e = 0; e < kEach; ++e) sum[e] = fmaf(f[e], wy, sum[e]);
-            }
+            for (int e = 0; e < kEach; ++e) acc[r][e] = 0.0f;
         }
-        const int32_t of = kv_div_group(p, r);
-        const int64_t row = u.row0 + of;
-        const int head = u.h * p.group + r - of * p.group;
-        const KvFinish f = kv_finish<false>(p, m, l, 0);
+        for (int x0 = 0; x0 < u.parts; x0 += kParts) {
+            const int n = min(kParts, u.parts - x0);
+            // thread t: part t % 128, rows 2 (t / 128) and the next
+            const int x = x0 + t % kParts, pair = t / kParts * 2;
+            float pm[2] = {-INFINITY, -INFINITY}, pl[2] = {0.0f, 0.0f};
+            const float* slot = slots + static_cast<int64_t>(x == 0 ? 1 : 2 * x) * kSlot + kKvFewRows * D + r0 + pair;
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) sum[e] *= f.scale;
-        char* at = p.out.data + row * p.out.row_stride + head * p.out.head_stride;
-        if (p.out_f32) {
-            if constexpr (kEach == 4) reinterpret_cast<float4*>(at)[lane] = *reinterpret_cast<const float4*>(sum);
-            else reinterpret_cast<float2*>(at)[lane] = *reinterpret_cast<const float2*>(sum);
-        } else {
-            if constexpr (kEach == 4) reinterpret_cast<uint2*>(at)[lane] = make_uint2(Pack<T>::pair(sum[0], sum[1]), Pack<T>::pair(sum[2], sum[3]));
-            else reinterpret_cast<uint32_t*>(at)[lane] = Pack<T>::pair(sum[0], sum[1]);
+            for (int y = 0; y < 2; ++y)
+                if (t % kParts < n && pair + y < nr) {
+                    pm[y] = slot[y];
+                    pl[y] = slot[kKvFewRows + y];
+                }
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                float top = pm[y];
+#pragma unroll
+                for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                if (lane == 0) s_top[warp][y] = top;
+            }
+            __syncthreads();
+            float top[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                top[r] = m[r];
+#pragma unroll
+                for (int w = 0; w < 4; ++w) top[r] = fmaxf(top[r], s_top[r / 2 * 4 + w][r & 1]);
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                float w;
+                part_weight(pm[y], pair == 0 ? top[y] : top[2 + y], &w, &pl[y]);
+                s_w[t % kParts][pair + y] = w;
+#pragma unroll
+                for (int o = 16; o; o >>= 1) pl[y] += __shfl_xor_sync(0xffffffffu, pl[y], o);
+                if (lane == 0) s_sum[warp][y] = pl[y];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float keep;
+                part_weight(m[r], top[r], &keep, &l[r]);
+                m[r] = top[r];
+#pragma unroll
+                for (int w = 0; w < 4; ++w) l[r] += s_sum[r / 2 * 4 + w][r & 1];
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) acc[r][e] *= keep;
+            }
+#pragma unroll 2
+            for (int y = warp; y < n; y += kJoinWarps) {
+                const float* v = slots + static_cast<int64_t>(x0 + y == 0 ? 1 : 2 * (x0 + y)) * kSlot + r0 * D + lane * kEach;
+                float f[4][kEach];
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (r < nr) {
+                        if constexpr (kEach == 4) *reinterpret_cast<float4*>(f[r]) = *reinterpret_cast<const float4*>(v + r * D);
+                        else *reinterpret_cast<float2*>(f[r]) = *reinterpret_cast<const float2*>(v + r * D);
+                    }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float w = s_w[y][r];
+                    if (r < nr && w != 0.0f)
+#pragma unroll
+                        for (int e = 0; e < kEach; ++e) acc[r][e] = fmaf(f[r][e], w, acc[r][e]);
+                }
+            }
+            __syncthreads();
         }
-        if (p.lse != nullptr && lane == 0) p.lse[row * p.q_heads + head] = f.sum == 0.0f ? -INFINITY : f.base * kLn2 + logf(f.sum);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) s_acc[warp][r][lane * kEach + e] = acc[r][e];
+        __syncthreads();
+        for (int i = t; i < nr * (D / 2); i += kJoinThreads) {
+            const int r = i / (D / 2), d = i % (D / 2) * 2;
+            float a = 0.0f, b = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kJoinWarps; ++w) {
+                a += s_acc[w][r][d];
+                b += s_acc[w][r][d + 1];
+            }
+            const float mr = r < 2 ? (r == 0 ? m[0] : m[1]) : (r == 2 ? m[2] : m[3]);
+            const float lr = r < 2 ? (r == 0 ? l[0] : l[1]) : (r == 2 ? l[2] : l[3]);
+            const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
+            const int32_t of = kv_div_group(p, r0 + r);
+            const int64_t row = u.row0 + of;
+            const int head = u.h * p.group + r0 + r - of * p.group;
+            char* at = p.out.data + row * p.out.row_stride + head * p.out.head_stride;
+            if (p.out_f32) *reinterpret_cast<float2*>(at + 4 * d) = make_float2(a * inv, b * inv);
+            else *reinterpret_cast<uint32_t*>(at + 2 * d) = Pack<T>::pair(a * inv, b * inv);
+            if (p.lse != nullptr && d == 0) p.lse[row * p.q_heads + head] = lr == 0.0f ? -INFINITY : mr * kLn2 + logf(lr);
+        }
+        __syncthreads();
     }
 }
 
-// Of kv_prompt, with many rows of mostly two parts: a CTA takes 32 rows, a lane per row and D / 8
-// elements a warp, so that the parts are read as they were written; the results go through shared
-// memory to be written row by row.
-constexpr int kJoinManyThreads = 256;
-
+// Of kv_prompt, with many rows: a CTA takes kRows rows, a thread one of them and 4 elements, so that the
+// parts are read as they were written; the results go through shared memory to be written row by row.
 template <typename T, int D, bool kShared>
-__global__ void __launch_bounds__(kJoinManyThreads) kv_join_many_kernel(const KvAttendParams p) {
-    constexpr int kEach = D / 8;  // elements of a thread
+__global__ void __launch_bounds__(kJoinThreads) kv_join_many_kernel(const KvAttendParams p) {
+    constexpr int kRows = kJoinThreads * 4 / D;  // 8 or 16
     constexpr int64_t kSlot = static_cast<int64_t>(kKvManyRows) * (D + 2);
-    __shared__ float s_out[32][D + 4];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x + 1;
+    __shared__ float s_out[kRows][D + 4];
+    __shared__ bool s_ok[kRows];
+    const int c = blockIdx.x + 1, t = threadIdx.x;
     kv_let_next();
     kv_wait_last();
     const KvCut u = p.line.cuts[c];
-    const int r0 = blockIdx.y * 32;
+    const int r0 = blockIdx.y * kRows;
     if (u.parts == 0 || r0 >= u.packed) return;
     const float* slots = p.line.slots + 2 * (c - 1) * kSlot;
-    const int r = r0 + lane;
+    const int r = r0 + t % kRows, d = t / kRows * 4;
     const bool live = r < u.packed;
-    float m = -INFINITY, l = 0.0f, sum[kEach] = {};
+    float m = -INFINITY, l = 0.0f, sum[4] = {};
     if (live)
-#pragma unroll 2
+#pragma unroll 4
         for (int x = 0; x < u.parts; ++x) {
             const float* slot = slots + (x == 0 ? 1 : 2 * x) * kSlot;
             const float pm = slot[kKvManyRows * D + r];
             float pl = slot[kKvManyRows * D + kKvManyRows + r];
-            float f[kEach];
-#pragma unroll
-            for (int e = 0; e < kEach; e += 4)
-                *reinterpret_cast<float4*>(f + e) = *reinterpret_cast<const float4*>(slot + (static_cast<int64_t>(warp * kEach + e) / 4 * kKvManyRows + r) * 4);
+            const float4 f = *reinterpret_cast<const float4*>(slot + (static_cast<int64_t>(d) / 4 * kKvManyRows + r) * 4);
             const float top = fmaxf(m, pm);
             float keep, w;
             part_weight(m, top, &keep, &l);
             part_weight(pm, top, &w, &pl);
             l += pl;
             m = top;
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) sum[e] = w != 0.0f ? fmaf(f[e], w, sum[e] * keep) : sum[e] * keep;
+            sum[0] = w != 0.0f ? fmaf(f.x, w, sum[0] * keep) : sum[0] * keep;
+            sum[1] = w != 0.0f ? fmaf(f.y, w, sum[1] * keep) : sum[1] * keep;
+            sum[2] = w != 0.0f ? fmaf(f.z, w, sum[2] * keep) : sum[2] * keep;
+            sum[3] = w != 0.0f ? fmaf(f.w, w, sum[3] * keep) : sum[3] * keep;
         }
     const int32_t packed = u.packed0 + (live ? r : r0), of = kv_div_group(p, packed);
     const int64_t row = u.row0 + of;
@@ -287,36 +341,31 @@ __global__ void __launch_bounds__(kJoinManyThreads) kv_join_many_kernel(const Kv
     const bool valid = live && (!kShared || kv_row_ok(p, static_cast<int32_t>(row)));
     if (valid) {
         const KvFinish f = kv_finish<kShared>(p, m, l, row * p.q_heads + head);
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) sum[e] *= f.scale;
         if (kShared && f.own != 0.0f) {
-            const float* own = p.own_out + (row * p.q_heads + head) * D + warp * kEach;
+            const float4 y = *reinterpret_cast<const float4*>(p.own_out + (row * p.q_heads + head) * D + d);
+            sum[0] = fmaf(y.x, f.own, sum[0] * f.scale);
+            sum[1] = fmaf(y.y, f.own, sum[1] * f.scale);
+            sum[2] = fmaf(y.z, f.own, sum[2] * f.scale);
+            sum[3] = fmaf(y.w, f.own, sum[3] * f.scale);
+        } else {
 #pragma unroll
-            for (int e = 0; e < kEach; e += 4) {
-                const float4 y = *reinterpret_cast<const float4*>(own + e);
-                sum[e] = fmaf(y.x, f.own, sum[e]);
-                sum[e + 1] = fmaf(y.y, f.own, sum[e + 1]);
-                sum[e + 2] = fmaf(y.z, f.own, sum[e + 2]);
-                sum[e + 3] = fmaf(y.w, f.own, sum[e + 3]);
-            }
+            for (int e = 0; e < 4; ++e) sum[e] *= f.scale;
         }
-        if (p.lse != nullptr && warp == 0) p.lse[row * p.q_heads + head] = f.sum == 0.0f ? -INFINITY : f.base * kLn2 + logf(f.sum);
-#pragma unroll
-        for (int e = 0; e < kEach; e += 4) *reinterpret_cast<float4*>(&s_out[lane][warp * kEach + e]) = *reinterpret_cast<const float4*>(sum + e);
+        if (p.lse != nullptr && d == 0) p.lse[row * p.q_heads + head] = f.sum == 0.0f ? -INFINITY : f.base * kLn2 + logf(f.sum);
+        *reinterpret_cast<float4*>(&s_out[t % kRows][d]) = *reinterpret_cast<const float4*>(sum);
     }
-    const unsigned ok = __ballot_sync(0xffffffffu, valid);  // the same rows in every warp
+    if (d == 0) s_ok[t % kRows] = valid;
     __syncthreads();
     constexpr int kLanes = D / 8;
-    for (int i = threadIdx.x / kLanes; i < 32; i += kJoinManyThreads / kLanes) {
-        if (!((ok >> i) & 1u)) continue;
+    const int i = t / kLanes, e = t % kLanes * 8;
+    if (i < kRows && s_ok[i]) {
         const int32_t pk = u.packed0 + r0 + i, o = kv_div_group(p, pk);
         char* at = p.out.data + static_cast<int64_t>(u.row0 + o) * p.out.row_stride + (u.h * p.group + pk - o * p.group) * p.out.head_stride;
-        const int d = threadIdx.x % kLanes * 8;
         float f[8];
-        *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(&s_out[i][d]);
-        *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(&s_out[i][d + 4]);
-        if (p.out_f32) Pack<float>::store(at + 4 * d, f);
-        else Pack<T>::store(at + 2 * d, f);
+        *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(&s_out[i][e]);
+        *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(&s_out[i][e + 4]);
+        if (p.out_f32) Pack<float>::store(at + 4 * e, f);
+        else Pack<T>::store(at + 2 * e, f);
     }
 }
 
@@ -344,7 +393,7 @@ cudaError_t launch_kv_append(const KvAppendParams& p, int head_dim, int dtype, i
 cudaError_t launch_kv_join_few(const KvAttendParams& p, int head_dim, int dtype, int ctas, cudaStream_t st) {
     return by_type(dtype, [&](auto t) {
         using T = decltype(t);
-        return kv_launch(head_dim == 64 ? kv_join_few_kernel<T, 64> : kv_join_few_kernel<T, 128>, dim3(ctas - 1), kJoinFewThreads, 0, st, true, p);
+        return kv_launch(head_dim == 64 ? kv_join_few_kernel<T, 64> : kv_join_few_kernel<T, 128>, dim3(ctas - 1), kJoinThreads, 0, st, true, p);
     });
 }
 
@@ -353,7 +402,7 @@ cudaError_t launch_kv_join_many(const KvAttendParams& p, int head_dim, int dtype
         using T = decltype(t);
         auto* f = p.shared_pass ? (head_dim == 64 ? kv_join_many_kernel<T, 64, true> : kv_join_many_kernel<T, 128, true>)
                                 : (head_dim == 64 ? kv_join_many_kernel<T, 64, false> : kv_join_many_kernel<T, 128, false>);
-        return kv_launch(f, dim3(ctas - 1, kKvManyRows / 32), kJoinManyThreads, 0, st, true, p);
+        return kv_launch(f, dim3(ctas - 1, kKvManyRows / (kJoinThreads * 4 / head_dim)), kJoinThreads, 0, st, true, p);
     });
 }
 

@@ -84,12 +84,17 @@ GFD_HD KvTiles kv_tiles(KvSpan s, int32_t size) {
 // tile each, n() of them.  A unit inside one stretch is finished there.  One that is cut leaves
 // partial results, one in each stretch it touches, in slot 1 of the one where it begins and slot 0
 // of the others; they are joined at the first cut inside the unit.
+// a / b for a >= 0, b > 0; the 64-bit division costs several times the 32-bit one.
+GFD_HD int64_t kv_div(int64_t a, int64_t b) {
+    return ((a | b) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+
 struct KvCuts {
     int64_t each;
     uint32_t more, ctas;
     GFD_HD KvCuts(int64_t total, uint32_t most) {
         ctas = total < static_cast<int64_t>(most) ? static_cast<uint32_t>(total) : most;
-        each = ctas > 0 ? total / ctas : 0;
+        each = ctas > 0 ? kv_div(total, ctas) : 0;
         more = ctas > 0 ? static_cast<uint32_t>(total - each * ctas) : 0;
     }
     GFD_HD int n() const { return static_cast<int>(ctas); }

@@ -143,7 +143,7 @@ __device__ __forceinline__ bool find_places(const KvAttendParams& p, KvCuts* cut
                 if (at < 0 || at >= here) continue;
                 KvPlace& x = places[w];
                 x.s = s;
-                x.h = static_cast<int32_t>(at / n);
+                x.h = static_cast<int32_t>(kv_div(at, n));
                 x.t = static_cast<int32_t>(at - static_cast<int64_t>(x.h) * n);
                 x.count = n;
                 x.begin = run + static_cast<int64_t>(x.h) * n;

@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (static_cast<int>(blockIdx.x) < cuts.n()) {
                     const int64_t at = cuts.at(blockIdx.x);
                     stretch_end = cuts.at(blockIdx.x + 1);
-                    head = at / per_head;
+                    head = kv_div(at, per_head);
                     want = at - head * per_head;
                 }
             }
