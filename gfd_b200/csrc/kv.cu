@@ -316,6 +316,15 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_many_kernel(const KvAtte
     const float* slots = p.line.slots + 2 * (c - 1) * kSlot;
     const int r = r0 + t % kRows, d = t / kRows * 4;
     const bool live = r < u.packed;
+    const int32_t packed = u.packed0 + (live ? r : r0), of = kv_div_group(p, packed);
+    const int64_t row = u.row0 + of;
+    const int head = u.h * p.group + packed - of * p.group;
+    float own_lse = -INFINITY;
+    float4 own = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (kShared) {
+        own_lse = p.own_lse[row * p.q_heads + head];
+        own = *reinterpret_cast<const float4*>(p.own_out + (row * p.q_heads + head) * D + d);
+    }
     float m = -INFINITY, l = 0.0f, sum[4] = {};
     if (live)
 #pragma unroll 4
@@ -335,21 +344,16 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_many_kernel(const KvAtte
             sum[2] = w != 0.0f ? fmaf(f.z, w, sum[2] * keep) : sum[2] * keep;
             sum[3] = w != 0.0f ? fmaf(f.w, w, sum[3] * keep) : sum[3] * keep;
         }
-    const int32_t packed = u.packed0 + (live ? r : r0), of = kv_div_group(p, packed);
-    const int64_t row = u.row0 + of;
-    const int head = u.h * p.group + packed - of * p.group;
-    const bool valid = live && (!kShared || kv_row_ok(p, static_cast<int32_t>(row)));
+    const bool valid = live && (!kShared || __float_as_uint(own_lse) != kKvSkipped);
     if (valid) {
-        const KvFinish f = kv_finish<kShared>(p, m, l, row * p.q_heads + head);
-        if (kShared && f.own != 0.0f) {
-            const float4 y = *reinterpret_cast<const float4*>(p.own_out + (row * p.q_heads + head) * D + d);
-            sum[0] = fmaf(y.x, f.own, sum[0] * f.scale);
-            sum[1] = fmaf(y.y, f.own, sum[1] * f.scale);
-            sum[2] = fmaf(y.z, f.own, sum[2] * f.scale);
-            sum[3] = fmaf(y.w, f.own, sum[3] * f.scale);
-        } else {
+        const KvFinish f = kv_finish<kShared>(m, l, own_lse);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] *= f.scale;
+        for (int e = 0; e < 4; ++e) sum[e] *= f.scale;
+        if (kShared && f.own != 0.0f) {
+            sum[0] = fmaf(own.x, f.own, sum[0]);
+            sum[1] = fmaf(own.y, f.own, sum[1]);
+            sum[2] = fmaf(own.z, f.own, sum[2]);
+            sum[3] = fmaf(own.w, f.own, sum[3]);
         }
         if (p.lse != nullptr && d == 0) p.lse[row * p.q_heads + head] = f.sum == 0.0f ? -INFINITY : f.base * kLn2 + logf(f.sum);
         *reinterpret_cast<float4*>(&s_out[t % kRows][d]) = *reinterpret_cast<const float4*>(sum);

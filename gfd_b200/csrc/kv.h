@@ -66,6 +66,8 @@ struct KvLine {
     float* slots;
 };
 
+constexpr uint32_t kKvSkipped = 0xffffffffu;  // a NaN that no sum leaves
+
 struct KvAttendParams {
     KvCacheView cache;
     KvBatchView batch;
@@ -87,7 +89,8 @@ struct KvAttendParams {
     int32_t few_rows;  // sequences of at most so many packed rows are kv_decode's
     int32_t shared_pass;   // kv_prompt: all rows against the shared prefix, joined with
     const float* own_out;  // what was found over the own keys, [rows][q_heads][D]
-    const float* own_lse;  // and its lse
+    const float* own_lse;  // and its lse; kKvSkipped for rows of skipped sequences
+    float* skipped_lse;    // where the passes over the own keys leave those marks; null: nowhere
     KvLine line;
 };
 
@@ -113,7 +116,11 @@ int kv_prompt_ctas(int num_sms);
 // cuTensorMapEncodeTiled, resolved through the runtime (libcuda is not linked)
 using KvEncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-cudaError_t launch_kv_prompt(const KvAttendParams& p, int head_dim, int dtype, int num_sms, KvEncodeFn encode, bool chained, cudaStream_t st);
+struct KvMaps {
+    CUtensorMap k, v;  // the cache as kv_prompt reads it
+};
+bool kv_make_maps(KvMaps* maps, const KvCacheView& cache, int head_dim, int dtype, KvEncodeFn encode);
+cudaError_t launch_kv_prompt(const KvAttendParams& p, int head_dim, int dtype, int num_sms, const KvMaps& maps, bool chained, cudaStream_t st);
 cudaError_t launch_kv_decode(const KvAttendParams& p, int head_dim, int dtype, int num_sms, bool chained, cudaStream_t st);
 
 // Bytes of a line's places and slots, and the line laid out in them.

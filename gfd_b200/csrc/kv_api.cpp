@@ -222,13 +222,18 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
     char* ws = static_cast<char*>(a->workspace);
     const KvEncodeFn encode = driver().tensor_map;
-    if ((plan.many || shared_len > 0) && encode == nullptr)
-        return set_error(ctx, GFD_ERR_UNSUPPORTED, "%s: the driver has no cuTensorMapEncodeTiled", call);
+    KvMaps maps;
+    if (plan.many || shared_len > 0) {
+        if (encode == nullptr) return set_error(ctx, GFD_ERR_UNSUPPORTED, "%s: the driver has no cuTensorMapEncodeTiled", call);
+        if (!kv_make_maps(&maps, p.cache, c->head_dim, c->dtype, encode))
+            return set_error(ctx, GFD_ERR_INVALID, "%s: the cache's shape does not fit a tensor map", call);
+    }
     KvAttendParams own = p;
     if (shared_len > 0) {
         // the results over the own keys go to the workspace in 32 bits, the pass over the prefix finishes
         own.out = KvRowsView{ws + plan.own_out, static_cast<int64_t>(a->q_heads) * c->head_dim * 4, static_cast<int64_t>(c->head_dim) * 4};
         own.lse = reinterpret_cast<float*>(ws + plan.own_lse);
+        own.skipped_lse = own.lse;
         own.out_f32 = 1;
     }
     cudaError_t e = cudaSuccess;
@@ -240,7 +245,7 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
     }
     if (e == cudaSuccess && plan.many) {
         own.line = kv_line_at(ws + plan.many_line, kv_prompt_ctas(ctx->num_sms));
-        e = launch_kv_prompt(own, c->head_dim, c->dtype, ctx->num_sms, encode, chained, st);
+        e = launch_kv_prompt(own, c->head_dim, c->dtype, ctx->num_sms, maps, chained, st);
         chained = true;
     }
     if (e == cudaSuccess && shared_len > 0) {
@@ -249,7 +254,7 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
         pre.own_out = reinterpret_cast<const float*>(ws + plan.own_out);
         pre.own_lse = own.lse;
         pre.line = kv_line_at(ws + plan.prefix_line, kv_prompt_ctas(ctx->num_sms));
-        e = launch_kv_prompt(pre, c->head_dim, c->dtype, ctx->num_sms, encode, chained, st);
+        e = launch_kv_prompt(pre, c->head_dim, c->dtype, ctx->num_sms, maps, chained, st);
     }
     return e == cudaSuccess ? GFD_OK : cuda_error(ctx, e, "kv_attend: kernel launch");
 }

@@ -110,7 +110,10 @@ __device__ __forceinline__ bool find_places(const KvAttendParams& p, KvCuts* cut
         const int32_t from = b.row_start[s], to = b.row_start[s + 1];
         bad |= from < 0 || from > to || to > b.rows;
         q = few_seq(p, s);
-        if (q.bad && blockIdx.x == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
+        if (q.bad && blockIdx.x == 0) {
+            kv_report(p.status, GFD_KV_BAD_LENGTH);
+            if (from >= 0 && to <= b.rows) kv_mark_skipped(p, s);
+        }
         sum += static_cast<int64_t>(q.tiles.count) * p.cache.heads;
     }
     int64_t incl = sum;

@@ -132,29 +132,23 @@ __device__ __forceinline__ KvCut kv_cut(const KvCuts& cuts, uint32_t c, const Kv
     return k;
 }
 
-// The row belongs to a sequence that is worked on (the starts rise).
-__device__ __forceinline__ bool kv_row_ok(const KvAttendParams& p, int32_t row) {
-    const KvBatchView& b = p.batch;
-    int lo = 0, hi = b.seqs - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (b.row_start[mid] <= row) lo = mid;
-        else hi = mid - 1;
-    }
-    return kv_seq(b.row_start[lo], b.row_start[lo + 1], b.kv_len[lo], b.capacity, p.max_q_len).ok;
+// Marks the rows of a sequence that is skipped, for the pass over the shared prefix (one thread calls).
+__device__ __forceinline__ void kv_mark_skipped(const KvAttendParams& p, int s) {
+    if (p.skipped_lse == nullptr) return;
+    const int64_t from = static_cast<int64_t>(p.batch.row_start[s]) * p.q_heads, to = static_cast<int64_t>(p.batch.row_start[s + 1]) * p.q_heads;
+    for (int64_t i = from; i < to; ++i) reinterpret_cast<uint32_t*>(p.skipped_lse)[i] = kKvSkipped;
 }
 
 // What becomes of a row's sums (relative to 2^base, weights adding up to sum): multiplied by `scale`
 // they are the result; behind a shared prefix the result over the own keys, times `own`, is
-// added (place: of the row and head there).  base and sum: of both together.
+// added.  base and sum: of both together.
 struct KvFinish {
     float scale, own, base, sum;
 };
 template <bool kShared>
-__device__ __forceinline__ KvFinish kv_finish(const KvAttendParams& p, float base, float sum, int64_t place) {
+__device__ __forceinline__ KvFinish kv_finish(float base, float sum, float own_lse) {
     KvFinish f{0.0f, 0.0f, base, sum};
-    float own = -INFINITY;
-    if (kShared) own = p.own_lse[place] * kLog2e;
+    const float own = kShared ? own_lse * kLog2e : -INFINITY;
     if (own == -INFINITY) {
         if (sum != 0.0f) f.scale = 1.0f / sum;
         return f;

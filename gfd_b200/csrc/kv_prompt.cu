@@ -470,7 +470,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             bad_starts |= from < 0 || from > to || to > b.rows;
             if (kShared) continue;
             const Many m = many_seq<kShared>(p, s);
-            if (m.bad && blockIdx.x == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
+            if (m.bad && blockIdx.x == 0) {
+                kv_report(p.status, GFD_KV_BAD_LENGTH);
+                if (from >= 0 && to <= b.rows) kv_mark_skipped(p, s);
+            }
             mine += m.tiles;
         }
         const bool ok = __syncthreads_or(bad_starts) == 0;
@@ -717,7 +720,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int32_t of = kv_div_group(p, packed);
                     const int64_t row = u.row0 + of;
                     const int32_t head = u.h * p.group + packed - of * p.group;
-                    const bool valid = r < u.packed && (!whole || !kShared || kv_row_ok(p, static_cast<int32_t>(row)));
+                    const float own_lse = kShared ? p.own_lse[row * p.q_heads + head] : -INFINITY;
+                    const bool valid = r < u.packed && (!whole || !kShared || __float_as_uint(own_lse) != kKvSkipped);
                     uint64_t dst = 0;
                     if (valid && whole) dst = reinterpret_cast<uint64_t>(p.out.data + row * p.out.row_stride + head * p.out.head_stride);
                     const uint32_t phase = (o_phase >> x) & 1u;
@@ -732,7 +736,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     KvFinish f{1.0f, 0.0f, base, l};  // what becomes of the sums
                     const float* own = nullptr;
                     if (whole) {
-                        f = kv_finish<kShared>(p, base, l, row * p.q_heads + head);
+                        f = kv_finish<kShared>(base, l, own_lse);
                         if (kShared && valid && f.own != 0.0f) own = p.own_out + (row * p.q_heads + head) * D;
                     }
                     uint64_t to_row[4];  // this lane writes rows lane / 4 + 8 i
@@ -1066,26 +1070,25 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // The cache's K or V as [blocks][tokens][heads][D], read in boxes of 16 tokens x 64 elements.
-bool make_map(CUtensorMap* map, const KvAttendParams& p, const char* base, int head_dim, int dtype, KvEncodeFn encode) {
+bool make_map(CUtensorMap* map, const KvCacheView& c, const char* base, int head_dim, int dtype, KvEncodeFn encode) {
     const cuuint64_t row = static_cast<cuuint64_t>(head_dim) * 2;
-    cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(p.cache.heads),
-                          static_cast<cuuint64_t>(p.cache.block_tokens), static_cast<cuuint64_t>(p.cache.blocks)};
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(c.heads), static_cast<cuuint64_t>(c.block_tokens),
+                                static_cast<cuuint64_t>(c.blocks)};
     // the stride of a dimension of one is not used, but has to be one that the map takes
-    cuuint64_t strides[3] = {p.cache.heads > 1 ? static_cast<cuuint64_t>(p.cache.head_stride) : row,
-                             static_cast<cuuint64_t>(p.cache.token_stride),
-                             p.cache.blocks > 1 ? static_cast<cuuint64_t>(p.cache.block_stride) : row};
-    cuuint32_t box[4] = {64, 1, kKvPage, 1}, ones[4] = {1, 1, 1, 1};
+    const cuuint64_t strides[3] = {c.heads > 1 ? static_cast<cuuint64_t>(c.head_stride) : row, static_cast<cuuint64_t>(c.token_stride),
+                                   c.blocks > 1 ? static_cast<cuuint64_t>(c.block_stride) : row};
+    const cuuint32_t box[4] = {64, 1, kKvPage, 1}, ones[4] = {1, 1, 1, 1};
     return encode(map, dtype == GFD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<char*>(base),
                   dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, int D>
-cudaError_t launch(const KvAttendParams& p, const CUtensorMap& k, const CUtensorMap& v, int ctas, bool chained, cudaStream_t st) {
+cudaError_t launch(const KvAttendParams& p, const KvMaps& maps, int ctas, bool chained, cudaStream_t st) {
     const bool plain = p.softcap == 0.0f && p.alibi == nullptr && p.scale2 > 0.0f;
     auto* f = p.shared_pass ? (plain ? kv_prompt_kernel<T, D, true, true> : kv_prompt_kernel<T, D, false, true>)
                             : (plain ? kv_prompt_kernel<T, D, true, false> : kv_prompt_kernel<T, D, false, false>);
-    const cudaError_t e = kv_launch(f, dim3(ctas), kThreads, Shape<D>::kSmem, st, chained, p, k, v);
+    const cudaError_t e = kv_launch(f, dim3(ctas), kThreads, Shape<D>::kSmem, st, chained, p, maps.k, maps.v);
     if (e != cudaSuccess) return e;
     return launch_kv_join_many(p, D, std::is_same<T, __half>::value ? GFD_FP16 : GFD_BF16, ctas, st);
 }
@@ -1094,15 +1097,14 @@ cudaError_t launch(const KvAttendParams& p, const CUtensorMap& k, const CUtensor
 
 int kv_prompt_ctas(int num_sms) { return num_sms; }
 
-cudaError_t launch_kv_prompt(const KvAttendParams& p, int head_dim, int dtype, int num_sms, KvEncodeFn encode, bool chained,
-                             cudaStream_t st) {
-    CUtensorMap k, v;
-    if (!make_map(&k, p, p.cache.k, head_dim, dtype, encode) || !make_map(&v, p, p.cache.v, head_dim, dtype, encode))
-        return cudaErrorInvalidValue;
+bool kv_make_maps(KvMaps* maps, const KvCacheView& cache, int head_dim, int dtype, KvEncodeFn encode) {
+    return make_map(&maps->k, cache, cache.k, head_dim, dtype, encode) && make_map(&maps->v, cache, cache.v, head_dim, dtype, encode);
+}
+
+cudaError_t launch_kv_prompt(const KvAttendParams& p, int head_dim, int dtype, int num_sms, const KvMaps& maps, bool chained, cudaStream_t st) {
     const int ctas = kv_prompt_ctas(num_sms);
-    if (dtype == GFD_BF16)
-        return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, k, v, ctas, chained, st) : launch<__nv_bfloat16, 128>(p, k, v, ctas, chained, st);
-    return head_dim == 64 ? launch<__half, 64>(p, k, v, ctas, chained, st) : launch<__half, 128>(p, k, v, ctas, chained, st);
+    if (dtype == GFD_BF16) return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, maps, ctas, chained, st) : launch<__nv_bfloat16, 128>(p, maps, ctas, chained, st);
+    return head_dim == 64 ? launch<__half, 64>(p, maps, ctas, chained, st) : launch<__half, 128>(p, maps, ctas, chained, st);
 }
 
 }  // namespace gfdb

@@ -17,6 +17,7 @@ default stream is passed as the legacy default stream).
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import numpy as np
 
@@ -62,10 +63,33 @@ class _Merge(ctypes.Structure):
         (n, ctypes.c_int32) for n in ("part_count", "heads", "head_dim", "part_dtype", "out_dtype", "_pad")]
 
 
-def _stream(s) -> _VP:
+def _format(c) -> str:
+    """struct format of a ctypes structure (all fields aligned, so nothing is padded)."""
+    one = {_VP: "Q", ctypes.c_size_t: "Q", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f"}
+    return "".join(one[t] if t in one else _format(t) for _, t in c._fields_)
+
+
+def _packer(c):
+    p = struct.Struct("=" + _format(c))
+    assert p.size == ctypes.sizeof(c)
+
+    def pack(*values) -> bytes:
+        try:
+            return p.pack(*values)
+        except (struct.error, OverflowError) as e:
+            raise ValueError(f"an argument is out of range: {e}") from None
+
+    return pack
+
+
+# A call packs its arguments in one go: a ctypes structure, field by field, costs as much as the launch.
+_pack_batch, _pack_append, _pack_attend, _pack_merge = (_packer(c) for c in (_Batch, _Append, _Attend, _Merge))
+
+
+def _stream(s) -> int:
     if isinstance(s, int):
-        return _VP(s)
-    return _VP(s.cuda_stream or 1)  # 1: the legacy default stream, which torch calls 0
+        return s
+    return s.cuda_stream or 1  # 1: the legacy default stream, which torch calls 0
 
 
 _codes = {}  # dtype object -> code or None: naming a type costs as much as a whole call
@@ -84,22 +108,23 @@ def _dtype(x, what: str) -> int:
     return d
 
 
-def _rows(x, what: str, rows: int, heads: int, dim: int, dtype: int) -> _Rows:
+def _rows(x, what: str, rows: int, heads: int, dim: int, dtype: int):
+    """Address, row stride and head stride of a row array."""
     if x.shape != (rows, heads, dim):
         raise ValueError(f"{what}: shape {tuple(x.shape)}, expected {(rows, heads, dim)}")
     if _code(x.dtype) != dtype:
         raise ValueError(f"{what}: type {x.dtype} does not match")
-    st = x.stride()
-    if st[2] != 1:
+    row, head, one = x.stride()
+    if one != 1:
         raise ValueError(f"{what}: the elements of a head must be contiguous")
-    return _Rows(x.data_ptr(), st[0] if rows > 1 else 0, st[1] if heads > 1 else 0)
+    return x.data_ptr(), row if rows > 1 else 0, head if heads > 1 else 0
 
 
-def _vector(x, what: str, shape, dtype: str) -> int:
-    """Address of a contiguous vector or matrix (None: NULL)."""
+def _vector(x, what: str, shape, dtype) -> int:
+    """Address of a contiguous vector or matrix (None: 0)."""
     if x is None:
-        return None
-    if x.shape != tuple(shape) or _code(x.dtype) != dtype or not x.is_contiguous():
+        return 0
+    if x.shape != shape or _code(x.dtype) != dtype or not x.is_contiguous():
         raise ValueError(f"{what}: expected contiguous {'torch.float32' if dtype == FP32 else dtype} of shape {tuple(shape)}, "
                          f"got {x.dtype} {tuple(x.shape)}")
     return x.data_ptr()
@@ -117,14 +142,12 @@ class Batch:
             raise ValueError("table: the entries of a row must be contiguous")
         self.arrays = (row_start, kv_len, table)
         self.seqs = seqs
-        self._c = _Batch(_vector(row_start, "row_start", (seqs + 1,), "torch.int32"),
-                         _vector(kv_len, "kv_len", (seqs,), "torch.int32"), table.data_ptr() or None,
-                         table.stride(0) if seqs > 1 else table.shape[1], 0, seqs, table.shape[1])
+        self._head = (_vector(row_start, "row_start", (seqs + 1,), "torch.int32"), _vector(kv_len, "kv_len", (seqs,), "torch.int32"),
+                      table.data_ptr(), table.stride(0) if seqs > 1 else table.shape[1])
+        self._tail = (seqs, table.shape[1])
 
-    def _rows(self, rows: int) -> _Batch:
-        c = _Batch.from_buffer_copy(self._c)
-        c.rows = rows
-        return c
+    def _c(self, rows: int) -> bytes:
+        return _pack_batch(*self._head, rows, *self._tail)
 
 
 class PagedCache:
@@ -141,8 +164,8 @@ class PagedCache:
         self.blocks, self.block_tokens, self.heads, self.head_dim = k.shape
         self.dtype = _dtype(k, "k")
         st = k.stride()
-        self._c = _Cache(k.data_ptr(), v.data_ptr(), self.blocks, st[0], st[1], st[2] if self.heads > 1 else 0,
-                         self.block_tokens, self.heads, self.head_dim, self.dtype)
+        self._c = bytes(_Cache(k.data_ptr(), v.data_ptr(), self.blocks, st[0], st[1], st[2] if self.heads > 1 else 0,
+                               self.block_tokens, self.heads, self.head_dim, self.dtype))
 
     # -- moving blocks between host memory and the cache ----------------------------------
     def _block_entries(self, host_ptr: int, host_ids, block_ids, to_host: bool) -> np.ndarray:
@@ -168,68 +191,59 @@ class PagedCache:
         """Gathers host blocks (block h: K then V of all its tokens, at host_ptr + h * block bytes
         in pinned memory) into the cache's blocks, asynchronously on `stream`."""
         e = self._block_entries(host_ptr, host_ids, block_ids, False)
-        self.ctx._check(self.ctx.gather(e, _stream(stream).value or 0))
+        self.ctx._check(self.ctx.gather(e, _stream(stream)))
 
     def offload(self, host_ptr: int, host_ids, block_ids, stream=0):
         """The reverse of fetch: cache blocks to host blocks."""
         e = self._block_entries(host_ptr, host_ids, block_ids, True)
-        self.ctx._check(self.ctx.scatter(e, _stream(stream).value or 0))
+        self.ctx._check(self.ctx.scatter(e, _stream(stream)))
 
     # -- operators ------------------------------------------------------------------------
     def append(self, batch: Batch, k, v, q=None, q_out=None, inv_freq=None, interleaved: bool = False, positions=None,
                status=None, stream=0):
         """gfd_kv_append: stores k, v [rows, heads, dim] at the ends of the sequences, k (and q
         into q_out) rotated by position when inv_freq [rot_dim / 2] is given."""
-        rows, a = k.shape[0], _Append()
-        a.k = _rows(k, "k", rows, self.heads, self.head_dim, self.dtype)
-        a.v = _rows(v, "v", rows, self.heads, self.head_dim, self.dtype)
+        rows, heads, dim, dtype = k.shape[0], self.heads, self.head_dim, self.dtype
         if (q is None) != (q_out is None):
             raise ValueError("q and q_out go together")
+        q_heads, q_args, out_args = 0, (0, 0, 0), (0, 0, 0)
         if q is not None:
-            a.q_heads = q.shape[1]
-            a.q = _rows(q, "q", rows, a.q_heads, self.head_dim, self.dtype)
-            a.q_out = _rows(q_out, "q_out", rows, a.q_heads, self.head_dim, self.dtype)
-        if inv_freq is not None:
-            a.rot_dim = 2 * inv_freq.shape[0]
-            a.inv_freq = _vector(inv_freq, "inv_freq", (inv_freq.shape[0],), FP32)
-        a.interleaved = bool(interleaved)
-        a.positions = _vector(positions, "positions", (rows,), "torch.int32")
-        a.status = _vector(status, "status", (1,), "torch.int32")
-        b = batch._rows(rows)
-        self.ctx._check(self.ctx.lib.gfd_kv_append(self.ctx.handle, ctypes.byref(self._c), ctypes.byref(b),
-                                                   ctypes.byref(a), _stream(stream)))
+            q_heads = q.shape[1]
+            q_args = _rows(q, "q", rows, q_heads, dim, dtype)
+            out_args = _rows(q_out, "q_out", rows, q_heads, dim, dtype)
+        half = 0 if inv_freq is None else inv_freq.shape[0]
+        a = _pack_append(*_rows(k, "k", rows, heads, dim, dtype), *_rows(v, "v", rows, heads, dim, dtype), *q_args, *out_args,
+                         _vector(inv_freq, "inv_freq", (half,), FP32), _vector(positions, "positions", (rows,), "torch.int32"),
+                         _vector(status, "status", (1,), "torch.int32"), q_heads, 2 * half, bool(interleaved), 0)
+        ctx = self.ctx
+        ctx._check(ctx.lib.gfd_kv_append(ctx.handle, self._c, batch._c(rows), a, _stream(stream)))
 
     def workspace_bytes(self, rows: int, q_heads: int, seqs: int, max_q_len: int = 0, shared_len: int = 0) -> int:
         """Bytes of workspace that attend / attend_shared need for these shapes."""
         b, a, n = _Batch(rows=rows, seqs=seqs), _Attend(q_heads=q_heads, max_q_len=max_q_len), ctypes.c_size_t()
-        self.ctx._check(self.ctx.lib.gfd_kv_attend_workspace(self.ctx.handle, ctypes.byref(self._c), ctypes.byref(b),
+        self.ctx._check(self.ctx.lib.gfd_kv_attend_workspace(self.ctx.handle, self._c, ctypes.byref(b),
                                                              ctypes.byref(a), shared_len, ctypes.byref(n)))
         return n.value
 
     def _attend(self, batch, q, out, lse, scale, causal, window, softcap, alibi, prefix_len, max_q_len, workspace, status):
-        rows, heads = q.shape[0], q.shape[1]
-        a = _Attend()
-        a.q_heads = heads
-        a.q = _rows(q, "q", rows, heads, self.head_dim, self.dtype)
-        a.out_dtype = _dtype(out, "out")
-        a.out = _rows(out, "out", rows, heads, self.head_dim, a.out_dtype)
-        a.lse = _vector(lse, "lse", (rows, heads), FP32)
-        a.alibi = _vector(alibi, "alibi", (heads,), FP32)
-        a.prefix_len = _vector(prefix_len, "prefix_len", (batch.seqs,), "torch.int32")
+        rows, heads, dim = q.shape[0], q.shape[1], self.head_dim
+        out_dtype = _dtype(out, "out")
+        room, room_bytes = 0, 0
         if workspace is not None:
-            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        a.status = _vector(status, "status", (1,), "torch.int32")
-        a.max_q_len, a.causal, a.window = max_q_len or 0, bool(causal), window
-        a.scale = self.head_dim ** -0.5 if scale is None else scale
-        a.softcap = softcap
-        return batch._rows(rows), a
+            room, room_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        return batch._c(rows), _pack_attend(
+            *_rows(q, "q", rows, heads, dim, self.dtype), *_rows(out, "out", rows, heads, dim, out_dtype),
+            _vector(lse, "lse", (rows, heads), FP32), _vector(alibi, "alibi", (heads,), FP32),
+            _vector(prefix_len, "prefix_len", (batch.seqs,), "torch.int32"), room, room_bytes,
+            _vector(status, "status", (1,), "torch.int32"), heads, out_dtype, max_q_len or 0, bool(causal), window,
+            dim ** -0.5 if scale is None else scale, softcap, 0)
 
     def attend(self, batch: Batch, q, out, lse=None, scale=None, causal: bool = True, window: int = 0, softcap: float = 0.0,
                alibi=None, prefix_len=None, max_q_len=None, workspace=None, status=None, stream=0):
         """gfd_kv_attend: q [rows, q_heads, dim] over the cache into out (and lse [rows, q_heads])."""
         b, a = self._attend(batch, q, out, lse, scale, causal, window, softcap, alibi, prefix_len, max_q_len, workspace, status)
-        self.ctx._check(self.ctx.lib.gfd_kv_attend(self.ctx.handle, ctypes.byref(self._c), ctypes.byref(b), ctypes.byref(a),
-                                                   _stream(stream)))
+        ctx = self.ctx
+        ctx._check(ctx.lib.gfd_kv_attend(ctx.handle, self._c, b, a, _stream(stream)))
 
     def attend_shared(self, batch: Batch, shared_table, shared_len: int, q, out, lse=None, scale=None, causal: bool = True,
                       window: int = 0, softcap: float = 0.0, alibi=None, prefix_len=None, max_q_len=None, workspace=None,
@@ -241,8 +255,8 @@ class PagedCache:
         if shared_table.dim() != 1 or shared_table.shape[0] < need:
             raise ValueError(f"shared_table: {need} block ids needed for {shared_len} tokens")
         table = _vector(shared_table, "shared_table", shared_table.shape, "torch.int32")
-        self.ctx._check(self.ctx.lib.gfd_kv_attend_shared(self.ctx.handle, ctypes.byref(self._c), ctypes.byref(b), _VP(table),
-                                                          shared_len, ctypes.byref(a), _stream(stream)))
+        ctx = self.ctx
+        ctx._check(ctx.lib.gfd_kv_attend_shared(ctx.handle, self._c, b, table, shared_len, a, _stream(stream)))
 
 
 def merge(ctx: Context, parts, part_lse, out, lse=None, stream=0):
@@ -250,12 +264,9 @@ def merge(ctx: Context, parts, part_lse, out, lse=None, stream=0):
     if parts.dim() != 4 or parts.stride(3) != 1:
         raise ValueError("parts must be [parts, rows, heads, dim], the elements of a head contiguous")
     n, rows, heads, dim = parts.shape
-    a, st = _Merge(), parts.stride()
-    a.parts = _Rows(parts.data_ptr(), st[1] if rows > 1 else 0, st[2] if heads > 1 else 0)
-    a.part_stride = st[0] if n > 1 else 0
-    a.part_lse = _vector(part_lse, "part_lse", (n, rows, heads), FP32)
-    a.part_dtype, a.out_dtype = _dtype(parts, "parts"), _dtype(out, "out")
-    a.out = _rows(out, "out", rows, heads, dim, a.out_dtype)
-    a.lse = _vector(lse, "lse", (rows, heads), FP32)
-    a.rows, a.part_count, a.heads, a.head_dim = rows, n, heads, dim
-    ctx._check(ctx.lib.gfd_kv_merge(ctx.handle, ctypes.byref(a), _stream(stream)))
+    part, row, head, _ = parts.stride()
+    out_dtype = _dtype(out, "out")
+    a = _pack_merge(parts.data_ptr(), row if rows > 1 else 0, head if heads > 1 else 0, part if n > 1 else 0,
+                    _vector(part_lse, "part_lse", (n, rows, heads), FP32), *_rows(out, "out", rows, heads, dim, out_dtype),
+                    _vector(lse, "lse", (rows, heads), FP32), rows, n, heads, dim, _dtype(parts, "parts"), out_dtype, 0)
+    ctx._check(ctx.lib.gfd_kv_merge(ctx.handle, a, _stream(stream)))

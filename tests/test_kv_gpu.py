@@ -448,6 +448,23 @@ def test_shared_masks_poison_and_bad_pages(gpu_ctx):
     oracle.check_attend(got, lse, s.want())
 
 
+@pytest.mark.parametrize("q_lens", [[1, 2, 1], [1, 2, 60], [300, 2, 60]])
+def test_shared_bad_lengths_skip_the_sequence(gpu_ctx, q_lens):
+    torch = torch_()
+    s = Setup(gpu_ctx, "bf16", 2, 4, 64, 16, q_lens, [n + 9 for n in q_lens], seed=16, spare_rows=1, shared_len=700)
+    want = s.want()
+    s.lens[1] = 1  # fewer keys than rows
+    got, lse = s.attend()
+    torch.cuda.synchronize()
+    a, b = s.row_start[1], s.row_start[2]
+    assert int(s.status) == kv.BAD_LENGTH and bool((got[a:b] == 7).all()) and bool((lse[a:b] == 7).all())
+    oracle.check_attend(got, lse, want, [r for r in range(s.row_start[-1]) if not a <= r < b])
+    s.starts[1] = s.rows + 5
+    got, lse = s.attend()
+    torch.cuda.synchronize()
+    assert bool((got == 7).all()) and bool((lse == 7).all())
+
+
 # ---------------------------------------------------------------------------
 # merge
 # ---------------------------------------------------------------------------
