@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_few_kernel(const KvAtten
             char* at = p.out.data + row * p.out.row_stride + head * p.out.head_stride;
             if (p.out_f32) *reinterpret_cast<float2*>(at + 4 * d) = make_float2(a * inv, b * inv);
             else *reinterpret_cast<uint32_t*>(at + 2 * d) = Pack<T>::pair(a * inv, b * inv);
-            if (p.lse != nullptr && d == 0) p.lse[row * p.q_heads + head] = lr == 0.0f ? -INFINITY : mr * kLn2 + logf(lr);
+            if (p.lse != nullptr && d == 0) p.lse[row * p.q_heads + head] = kv_lse(p, mr, lr);
         }
         __syncthreads();
     }
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_many_kernel(const KvAtte
         }
     const bool valid = live && (!kShared || __float_as_uint(own_lse) != kKvSkipped);
     if (valid) {
-        const KvFinish f = kv_finish<kShared>(m, l, own_lse);
+        const KvFinish f = kv_finish<kShared>(p, m, l, own_lse);
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[e] *= f.scale;
         if (kShared && f.own != 0.0f) {
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_many_kernel(const KvAtte
             sum[2] = fmaf(own.z, f.own, sum[2]);
             sum[3] = fmaf(own.w, f.own, sum[3]);
         }
-        if (p.lse != nullptr && d == 0) p.lse[row * p.q_heads + head] = f.sum == 0.0f ? -INFINITY : f.base * kLn2 + logf(f.sum);
+        if (p.lse != nullptr && d == 0) p.lse[row * p.q_heads + head] = kv_lse(p, f.base, f.sum);
         *reinterpret_cast<float4*>(&s_out[t % kRows][d]) = *reinterpret_cast<const float4*>(sum);
     }
     if (d == 0) s_ok[t % kRows] = valid;

@@ -85,6 +85,7 @@ struct KvAttendParams {
     float scale2;    // scale in base 2
     float cap_x;     // scale / softcap
     float cap2;      // softcap in base 2
+    float to_ln;     // from the kernels' base-2 scores to natural ones: ln 2, and what rounded off scale2 or cap_x and cap2
     int32_t out_f32;
     int32_t few_rows;  // sequences of at most so many packed rows are kv_decode's
     int32_t shared_pass;   // kv_prompt: all rows against the shared prefix, joined with

@@ -217,6 +217,9 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
     p.scale2 = a->scale * 1.4426950408889634f;
     p.cap_x = a->softcap > 0.0f ? a->scale / a->softcap : 0.0f;
     p.cap2 = a->softcap * 1.4426950408889634f;
+    // scores of 10 and more would show the rounding of these factors in lse
+    const double factor = a->softcap > 0.0f ? static_cast<double>(p.cap_x) * p.cap2 : static_cast<double>(p.scale2);
+    p.to_ln = static_cast<float>(a->alibi != nullptr || factor == 0.0 ? 0.6931471805599453 : a->scale / factor);
     p.out_f32 = a->out_dtype == GFD_FP32;
     p.few_rows = plan.few ? kKvFewRows : 0;
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;

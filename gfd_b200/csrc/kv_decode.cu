@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
                     slot[kRows * D + r] = m[x];
                     slot[kRows * D + kRows + r] = l[x];
                 } else if (p.lse != nullptr) {
-                    p.lse[row * p.q_heads + head] = l[x] == 0.0f ? -INFINITY : m[x] * kLn2 + logf(l[x]);
+                    p.lse[row * p.q_heads + head] = kv_lse(p, m[x], l[x]);
                 }
             }
             for (uint32_t redo = __ballot_sync(0xffffffffu, r < rows && odd != 0.0f); redo != 0;) {

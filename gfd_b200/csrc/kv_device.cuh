@@ -12,7 +12,6 @@
 namespace gfdb {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 // 2^x by the hardware instruction: within 2^-22 of the value, results below 2^-126 are 0
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -139,6 +138,10 @@ __device__ __forceinline__ void kv_mark_skipped(const KvAttendParams& p, int s) 
     for (int64_t i = from; i < to; ++i) reinterpret_cast<uint32_t*>(p.skipped_lse)[i] = kKvSkipped;
 }
 
+__device__ __forceinline__ float kv_lse(const KvAttendParams& p, float base, float sum) {
+    return sum == 0.0f ? -INFINITY : fmaf(base, p.to_ln, logf(sum));
+}
+
 // What becomes of a row's sums (relative to 2^base, weights adding up to sum): multiplied by `scale`
 // they are the result; behind a shared prefix the result over the own keys, times `own`, is
 // added.  base and sum: of both together.
@@ -146,9 +149,9 @@ struct KvFinish {
     float scale, own, base, sum;
 };
 template <bool kShared>
-__device__ __forceinline__ KvFinish kv_finish(float base, float sum, float own_lse) {
+__device__ __forceinline__ KvFinish kv_finish(const KvAttendParams& p, float base, float sum, float own_lse) {
     KvFinish f{0.0f, 0.0f, base, sum};
-    const float own = kShared ? own_lse * kLog2e : -INFINITY;
+    const float own = kShared ? own_lse / p.to_ln : -INFINITY;
     if (own == -INFINITY) {
         if (sum != 0.0f) f.scale = 1.0f / sum;
         return f;
@@ -192,25 +195,25 @@ __device__ __forceinline__ float kv_tanh2(const KvAttendParams& p, float x) {
 }
 
 // N products of queries and keys to scores in base 2: scaled, capped where the call has a cap.
-// Where the warp's products all lie within the cap (|x| <= 1, the usual case) tanh x is x P(x^2)
-// on the FMA units, P of degree 5 by least largest error (2^-22; 2^-21.6 with the roundings):
-// the special-function unit, which the exponentials need, is left out.
+// Where the warp's products all lie within three quarters of the cap (the usual case) tanh x is
+// x P(x^2) on the FMA units, P = 1 + ... of degree 5 by least largest relative error (2^-24.9;
+// 2^-22.9 with the roundings): the special-function unit, which the exponentials need, is left out.
 template <int N>
 __device__ __forceinline__ void kv_cap(const KvAttendParams& p, uint32_t* z) {
     if (p.softcap > 0.0f) {
         float m = 0.0f;
 #pragma unroll
         for (int e = 0; e < N; ++e) m = fmaxf(m, fabsf(__uint_as_float(z[e])));
-        if (__all_sync(0xffffffffu, m * fabsf(p.cap_x) <= 1.0f)) {
+        if (__all_sync(0xffffffffu, m * fabsf(p.cap_x) <= 0.75f)) {
             const uint64_t sx = pack2(p.cap_x, p.cap_x), amp = pack2(p.cap2, p.cap2);
 #pragma unroll
             for (int e = 0; e < N; e += 2) {
                 const uint64_t x = mul2(pack2(__uint_as_float(z[e]), __uint_as_float(z[e + 1])), sx), y = mul2(x, x);
-                uint64_t q = fma2(y, pack2(-0.0028394656255841255f, -0.0028394656255841255f), pack2(0.01611418090760708f, 0.01611418090760708f));
-                q = fma2(q, y, pack2(-0.05097286403179169f, -0.05097286403179169f));
-                q = fma2(q, y, pack2(0.13253524899482727f, 0.13253524899482727f));
-                q = fma2(q, y, pack2(-0.3332400321960449f, -0.3332400321960449f));
-                q = fma2(q, y, pack2(0.9999968409538269f, 0.9999968409538269f));
+                uint64_t q = fma2(y, pack2(-0.004769490100443363f, -0.004769490100443363f), pack2(0.019664913415908813f, 0.019664913415908813f));
+                q = fma2(q, y, pack2(-0.0533902570605278f, -0.0533902570605278f));
+                q = fma2(q, y, pack2(0.13326521217823029f, 0.13326521217823029f));
+                q = fma2(q, y, pack2(-0.3333306908607483f, -0.3333306908607483f));
+                q = fma2(q, y, pack2(1.0f, 1.0f));
                 float a, b;
                 unpack2(mul2(mul2(q, x), amp), a, b);
                 z[e] = __float_as_uint(a);

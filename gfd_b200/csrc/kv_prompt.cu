@@ -736,7 +736,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     KvFinish f{1.0f, 0.0f, base, l};  // what becomes of the sums
                     const float* own = nullptr;
                     if (whole) {
-                        f = kv_finish<kShared>(base, l, own_lse);
+                        f = kv_finish<kShared>(p, base, l, own_lse);
                         if (kShared && valid && f.own != 0.0f) own = p.own_out + (row * p.q_heads + head) * D;
                     }
                     uint64_t to_row[4];  // this lane writes rows lane / 4 + 8 i
@@ -807,7 +807,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (valid) {
                         if (whole) {
-                            if (p.lse != nullptr) p.lse[row * p.q_heads + head] = f.sum == 0.0f ? -INFINITY : f.base * kLn2 + logf(f.sum);
+                            if (p.lse != nullptr) p.lse[row * p.q_heads + head] = kv_lse(p, f.base, f.sum);
                         } else {
                             slot[static_cast<int64_t>(kRows) * D + r] = base;
                             slot[static_cast<int64_t>(kRows) * D + kRows + r] = l;
