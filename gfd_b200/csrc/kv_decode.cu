@@ -348,35 +348,50 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
                     mma<T>(z[0], qf[k], f[0], f[1]);
                     mma<T>(z[1], qf[k], f[2], f[3]);
                 }
-                const int32_t j0 = use.q.tiles.at(use.t) * kTile + 2 * (lane & 3);
-                float mx[2] = {-INFINITY, -INFINITY};
-                if (!kPlain) kv_cap<8>(p, reinterpret_cast<uint32_t*>(&z[0][0]));
-#pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int x = e >> 1;
-                        const int32_t j = j0 + 8 * nt + (e & 1);
-                        const bool seen = j < sp[x].pre || (j >= sp[x].lo && j < sp[x].hi);
-                        const float v = kPlain ? z[nt][e] * p.scale2 : fmaf(slope[x], static_cast<float>(p.shared_len + j - pos[x]), z[nt][e]);
-                        z[nt][e] = seen ? v : -INFINITY;
-                        mx[x] = fmaxf(mx[x], z[nt][e]);
-                    }
-                float base[2];
+                const int32_t j0 = use.q.tiles.at(use.t) * kTile;
+                // z[nt][2 x + e]: row row_a + 8 x, key j0 + 8 nt + 2 (lane % 4) + e.  Up to 8 rows the second half idles.
+                float base[2] = {0.0f, 0.0f}, top[2] = {m[0], m[1]};
                 bool grew = false;
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
-                    mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2)) - kShift<T>;
-                    grew |= mx[x] > m[x];
-                    mx[x] = fmaxf(mx[x], m[x]);
-                    base[x] = mx[x] == -INFINITY ? 0.0f : mx[x];
+                    if (8 * x >= rows) break;
+                    uint32_t y[4] = {__float_as_uint(z[0][2 * x]), __float_as_uint(z[0][2 * x + 1]), __float_as_uint(z[1][2 * x]),
+                                     __float_as_uint(z[1][2 * x + 1])};
+                    const int32_t j = j0 + 2 * (lane & 3);
+                    if (!kPlain) {
+                        kv_cap<4>(p, y);
+                        if (p.alibi != nullptr) {
+                            const float d = static_cast<float>(p.shared_len + j - pos[x]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                y[e] = __float_as_uint(fmaf(slope[x], d + static_cast<float>(8 * (e >> 1) + (e & 1)), __uint_as_float(y[e])));
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * p.scale2);
+                    }
+                    const bool inside = (j0 >= sp[x].lo && j0 + kTile <= sp[x].hi) || j0 + kTile <= sp[x].pre;
+                    if (__any_sync(0xffffffffu, !inside)) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int32_t k = j + 8 * (e >> 1) + (e & 1);
+                            if (!(k < sp[x].pre || (k >= sp[x].lo && k < sp[x].hi))) y[e] = 0xff800000u;
+                        }
+                    }
+                    float mx = fmaxf(fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])), fmaxf(__uint_as_float(y[2]), __uint_as_float(y[3])));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) - kShift<T>;
+                    grew |= mx > m[x];
+                    top[x] = fmaxf(mx, m[x]);
+                    base[x] = top[x] == -INFINITY ? 0.0f : top[x];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) z[e >> 1][2 * x + (e & 1)] = __uint_as_float(y[e]);
                 }
                 if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const float keep = fast_exp2(m[x] - base[x]);
-                        m[x] = mx[x];
+                        m[x] = top[x];
                         l[x] *= keep;
 #pragma unroll
                         for (int i = 0; i < 2 * kSteps; ++i) {
@@ -387,12 +402,19 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
                 }
                 // weights: summed in 32 bits, rounded to the cache's type for the product with V
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        z[nt][e] = fast_exp2(z[nt][e] - base[e >> 1]);
-                        l[e >> 1] += z[nt][e];
+                for (int x = 0; x < 2; ++x) {
+                    if (8 * x >= rows) {
+                        z[0][2] = z[0][3] = z[1][2] = z[1][3] = 0.0f;
+                        break;
                     }
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                        for (int e = 2 * x; e < 2 * x + 2; ++e) {
+                            z[nt][e] = fast_exp2(z[nt][e] - base[x]);
+                            l[x] += z[nt][e];
+                        }
+                }
                 const uint32_t pf[4] = {Pack<T>::pair(z[0][0], z[0][1]), Pack<T>::pair(z[0][2], z[0][3]),
                                         Pack<T>::pair(z[1][0], z[1][1]), Pack<T>::pair(z[1][2], z[1][3])};
                 const int vrow = (lane & 7) + (((lane >> 3) & 1) << 3);
