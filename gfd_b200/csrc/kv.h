@@ -80,6 +80,7 @@ struct KvAttendParams {
     int32_t shared_len;
     int32_t q_heads, group;
     uint64_t group_magic;  // ceil(2^44 / group), see kv_div_group
+    uint64_t page_magic;   // ceil(2^32 / pages of a block), see kv_div_pages
     int32_t max_q_len, causal, window;
     float scale, softcap;
     float scale2;    // scale in base 2
@@ -112,7 +113,7 @@ struct KvMergeParams {
 cudaError_t launch_kv_append(const KvAppendParams& p, int head_dim, int dtype, int num_sms, cudaStream_t st);
 cudaError_t launch_kv_join_few(const KvAttendParams& p, int head_dim, int dtype, int ctas, cudaStream_t st);
 cudaError_t launch_kv_join_many(const KvAttendParams& p, int head_dim, int dtype, int ctas, cudaStream_t st);
-int kv_decode_workers(int num_sms);  // each with a stretch of the line
+int kv_decode_workers(int num_sms, int head_dim);  // each with a stretch of the line
 int kv_prompt_ctas(int num_sms);
 // cuTensorMapEncodeTiled, resolved through the runtime (libcuda is not linked)
 using KvEncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,

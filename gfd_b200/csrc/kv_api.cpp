@@ -98,7 +98,7 @@ AttendPlan plan_attend(const gfd_ctx* ctx, const gfd_kv_cache& c, const gfd_kv_b
         return here;
     };
     const size_t many_bytes = kv_line_bytes(kv_prompt_ctas(ctx->num_sms), kKvManyRows, c.head_dim);
-    if (r.few) r.few_line = take(kv_line_bytes(kv_decode_workers(ctx->num_sms), kKvFewRows, c.head_dim));
+    if (r.few) r.few_line = take(kv_line_bytes(kv_decode_workers(ctx->num_sms, c.head_dim), kKvFewRows, c.head_dim));
     if (r.many) r.many_line = take(many_bytes);
     if (shared_len > 0) {
         r.prefix_line = take(many_bytes);
@@ -209,6 +209,8 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
     p.q_heads = a->q_heads;
     p.group = a->q_heads / c->heads;
     p.group_magic = ((1ull << 44) + p.group - 1) / p.group;
+    const uint32_t pages = c->block_tokens / kKvPage;
+    p.page_magic = ((1ull << 32) + pages - 1) / pages;
     p.max_q_len = a->max_q_len;
     p.causal = a->causal != 0;
     p.window = a->window;
@@ -242,7 +244,7 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
     cudaError_t e = cudaSuccess;
     bool chained = false;  // launches of this call overlap
     if (e == cudaSuccess && plan.few) {
-        own.line = kv_line_at(ws + plan.few_line, kv_decode_workers(ctx->num_sms));
+        own.line = kv_line_at(ws + plan.few_line, kv_decode_workers(ctx->num_sms, c->head_dim));
         e = launch_kv_decode(own, c->head_dim, c->dtype, ctx->num_sms, chained, st);
         chained = true;
     }

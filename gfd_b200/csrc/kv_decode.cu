@@ -22,7 +22,8 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kTile = kKvPage;  // keys a warp takes per step
+template <int D>
+constexpr int kPerSm = D == 64 ? 3 : 2;  // CTAs of an SM
 constexpr int kLeast = 2;       // tiles of a stretch, where there are enough: a part costs its joining about as much
 constexpr int kRows = kKvFewRows;
 
@@ -89,7 +90,7 @@ __device__ __forceinline__ Seq few_seq(const KvAttendParams& p, int s) {
         const KvSpan first = kv_clip(kv_span(n - r.q.rows, n, prefix, p.window, p.causal != 0), p.shared_len, r.q.keys);
         const KvSpan last = kv_clip(kv_span(n - 1, n, prefix, p.window, p.causal != 0), p.shared_len, r.q.keys);
         r.all = KvSpan{first.pre, first.lo, last.hi};
-        r.tiles = kv_tiles(r.all, kTile);
+        r.tiles = kv_tiles(r.all, kKvPage);
         // a sequence that sees none of its own keys still has rows to write
         if (r.tiles.count == 0) r.tiles = KvTiles{1, 0, 1};
     }
@@ -197,8 +198,8 @@ struct Cursor {
 
 template <int D>
 struct Shape {
-    static constexpr int kStages = D == 128 ? 3 : 6;
-    static constexpr int kRow = 2 * D;                 // bytes of a key
+    static constexpr int kStages = D == 64 ? 3 : 3;
+    static constexpr int kRow = 2 * D;                   // bytes of a key
     static constexpr int kStage = 2 * kKvPage * kRow;  // K and V of 16 keys
     static constexpr int kRing = kStages * kStage;
     static constexpr int kSmem = kWarps * kRing;
@@ -209,10 +210,11 @@ template <typename T>
 constexpr float kShift = std::is_same<T, __half>::value ? 8.0f : 0.0f;
 
 template <typename T, int D, bool kPlain>
-__global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendParams p) {
+__global__ void __launch_bounds__(kThreads, kPerSm<D>) kv_decode_kernel(const KvAttendParams p) {
     using S = Shape<D>;
     constexpr int kSteps = D / 16;   // k-steps of the scores, pairs of n-tiles of the sums
     constexpr int kChunks = D / 8;   // 16-byte pieces of a key
+    constexpr int kTile = kKvPage;   // keys of a tile
     extern __shared__ __align__(128) char smem[];
     __shared__ KvPlace s_place[kWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -239,6 +241,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
     bool ids_ok = false;
     uint32_t live = 0;      // bit i: the stage issued i stages ago holds keys
     int put = 0;
+    // lane i of a step copies piece i % kChunks of key i / kChunks, kStep keys a step
+    constexpr int kStep = 32 / kChunks;
+    const int64_t lane_off = lane / kChunks * p.cache.token_stride + 16 * (lane % kChunks);
+    const int64_t step_off = kStep * p.cache.token_stride;
+    const uint32_t lane_to = ring + lane / kChunks * S::kRow + ((lane % kChunks ^ lane / kChunks) << 4);
     auto issue = [&]() {
         live <<= 1;
         if (!load.done) {
@@ -257,8 +264,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
                 ids = -1;
                 if (i < load.end) {
                     const int32_t j = load.q.tiles.at(i) * kTile;
-                    if (j < a.pre || (j + kKvPage > a.lo && j < a.hi)) {
-                        ids = b.table[load.s * b.table_stride + j / kKvPage / pages];
+                    if (j < a.pre || (j + kTile > a.lo && j < a.hi)) {
+                        ids = b.table[load.s * b.table_stride + kv_div_pages(p, j / kTile)];
                         if (ids < 0 || ids >= p.cache.blocks) {
                             kv_report(p.status, GFD_KV_BAD_PAGE);
                             ids = -1;
@@ -269,19 +276,33 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
             const int32_t id = __shfl_sync(0xffffffffu, ids, load.t - ids_from);
             if (id >= 0) {
                 live |= 1u;
-                const int32_t j = load.q.tiles.at(load.t) * kTile;
-                const int32_t place = (j / kKvPage % pages) * kKvPage;
-                const int64_t base = id * p.cache.block_stride + place * p.cache.token_stride + load.h * p.cache.head_stride;
-                const uint32_t dst = ring + put * S::kStage;
+                const int32_t page = load.q.tiles.at(load.t), j = page * kTile;
+                const int32_t place = (page - kv_div_pages(p, page) * pages) * kKvPage;
+                const int64_t off = id * p.cache.block_stride + place * p.cache.token_stride + load.h * p.cache.head_stride + lane_off;
+                const char* k = p.cache.k + off;
+                const char* v = p.cache.v + off;
+                const uint32_t to = lane_to + put * S::kStage;
+                if ((j >= a.lo && j + kTile <= a.hi) || j + kTile <= a.pre) {
 #pragma unroll
-                for (int i = 0; i < kKvPage * kChunks / 32; ++i) {
-                    const int r = (i * 32 + lane) / kChunks, c = lane % kChunks;
-                    const int64_t off = base + r * p.cache.token_stride + 16 * c;
+                    for (int i = 0; i < kKvPage / kStep; ++i) {
+                        const uint32_t at = (to ^ (((i * kStep) & 7) << 4)) + i * kStep * S::kRow;
+                        copy16(at, k, true);
+                        copy16(at + kTile * S::kRow, v, true);
+                        k += step_off;
+                        v += step_off;
+                    }
+                } else {
                     // keys no row sees stay zero, so that what lies there cannot reach a sum
-                    const bool take = j + r < a.pre || (j + r >= a.lo && j + r < a.hi);
-                    const uint32_t o = r * S::kRow + ((c ^ (r & 7)) << 4);
-                    copy16(dst + o, p.cache.k + off, take);
-                    copy16(dst + kKvPage * S::kRow + o, p.cache.v + off, take);
+#pragma unroll 1
+                    for (int i = 0; i < kKvPage / kStep; ++i) {
+                        const int32_t key = j + i * kStep + lane / kChunks;
+                        const bool take = key < a.pre || (key >= a.lo && key < a.hi);
+                        const uint32_t at = (to ^ (((i * kStep) & 7) << 4)) + i * kStep * S::kRow;
+                        copy16(at, k, take);
+                        copy16(at + kTile * S::kRow, v, take);
+                        k += step_off;
+                        v += step_off;
+                    }
                 }
             }
             if (++load.t == load.end) {
@@ -337,14 +358,16 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
             copy_wait<S::kStages - 1>();
             __syncwarp();
             if ((live >> (S::kStages - 1)) & 1u) {
-                const uint32_t kb = ring + get * S::kStage, vb = kb + kKvPage * S::kRow;
+                const uint32_t kb = ring + get * S::kStage, vb = kb + kTile * S::kRow;
                 float z[2][4] = {};
-                const int row = (lane & 7) + ((lane >> 4) << 3);
+                // piece 2 k + b of row r lies at (2 k + b) ^ (r % 8): k only flips bits of the address
+                const int krow = (lane & 7) + ((lane >> 4) << 3), vrow = (lane & 7) + (((lane >> 3) & 1) << 3);
+                const uint32_t ka = kb + krow * S::kRow + ((((lane >> 3) & 1) ^ (krow & 7)) << 4);
+                const uint32_t va = vb + vrow * S::kRow + (((lane >> 4) ^ (vrow & 7)) << 4);
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
                     uint32_t f[4];
-                    const int c = 2 * k + ((lane >> 3) & 1);
-                    ldsm4(f, kb + row * S::kRow + ((c ^ (row & 7)) << 4));
+                    ldsm4(f, ka ^ (k << 5));
                     mma<T>(z[0], qf[k], f[0], f[1]);
                     mma<T>(z[1], qf[k], f[2], f[3]);
                 }
@@ -355,8 +378,9 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     if (8 * x >= rows) break;
-                    uint32_t y[4] = {__float_as_uint(z[0][2 * x]), __float_as_uint(z[0][2 * x + 1]), __float_as_uint(z[1][2 * x]),
-                                     __float_as_uint(z[1][2 * x + 1])};
+                    uint32_t y[4];  // y[2 nt + e]
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = __float_as_uint(z[e / 2][2 * x + (e & 1)]);
                     const int32_t j = j0 + 2 * (lane & 3);
                     if (!kPlain) {
                         kv_cap<4>(p, y);
@@ -364,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
                             const float d = static_cast<float>(p.shared_len + j - pos[x]);
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                y[e] = __float_as_uint(fmaf(slope[x], d + static_cast<float>(8 * (e >> 1) + (e & 1)), __uint_as_float(y[e])));
+                                y[e] = __float_as_uint(fmaf(slope[x], d + static_cast<float>(8 * (e / 2) + (e & 1)), __uint_as_float(y[e])));
                         }
                     } else {
 #pragma unroll
@@ -374,18 +398,20 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
                     if (__any_sync(0xffffffffu, !inside)) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const int32_t k = j + 8 * (e >> 1) + (e & 1);
+                            const int32_t k = j + 8 * (e / 2) + (e & 1);
                             if (!(k < sp[x].pre || (k >= sp[x].lo && k < sp[x].hi))) y[e] = 0xff800000u;
                         }
                     }
-                    float mx = fmaxf(fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])), fmaxf(__uint_as_float(y[2]), __uint_as_float(y[3])));
+                    float mx = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+#pragma unroll
+                    for (int e = 2; e < 4; ++e) mx = fmaxf(mx, __uint_as_float(y[e]));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) - kShift<T>;
                     grew |= mx > m[x];
                     top[x] = fmaxf(mx, m[x]);
                     base[x] = top[x] == -INFINITY ? 0.0f : top[x];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) z[e >> 1][2 * x + (e & 1)] = __uint_as_float(y[e]);
+                    for (int e = 0; e < 4; ++e) z[e / 2][2 * x + (e & 1)] = __uint_as_float(y[e]);
                 }
                 if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
@@ -403,26 +429,21 @@ __global__ void __launch_bounds__(kThreads, 2) kv_decode_kernel(const KvAttendPa
                 // weights: summed in 32 bits, rounded to the cache's type for the product with V
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    if (8 * x >= rows) {
-                        z[0][2] = z[0][3] = z[1][2] = z[1][3] = 0.0f;
-                        break;
-                    }
+                    const bool some = 8 * x < rows;
 #pragma unroll
                     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
                         for (int e = 2 * x; e < 2 * x + 2; ++e) {
-                            z[nt][e] = fast_exp2(z[nt][e] - base[x]);
+                            z[nt][e] = some ? fast_exp2(z[nt][e] - base[x]) : 0.0f;
                             l[x] += z[nt][e];
                         }
                 }
-                const uint32_t pf[4] = {Pack<T>::pair(z[0][0], z[0][1]), Pack<T>::pair(z[0][2], z[0][3]),
-                                        Pack<T>::pair(z[1][0], z[1][1]), Pack<T>::pair(z[1][2], z[1][3])};
-                const int vrow = (lane & 7) + (((lane >> 3) & 1) << 3);
+                const uint32_t pf[4] = {Pack<T>::pair(z[0][0], z[0][1]), Pack<T>::pair(z[0][2], z[0][3]), Pack<T>::pair(z[1][0], z[1][1]),
+                                        Pack<T>::pair(z[1][2], z[1][3])};
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i) {
                     uint32_t f[4];
-                    const int c = 2 * i + (lane >> 4);
-                    ldsm4t(f, vb + vrow * S::kRow + ((c ^ (vrow & 7)) << 4));
+                    ldsm4t(f, va ^ (i << 5));
                     mma<T>(acc[2 * i], pf, f[0], f[1]);
                     mma<T>(acc[2 * i + 1], pf, f[2], f[3]);
                 }
@@ -507,10 +528,10 @@ cudaError_t launch(const KvAttendParams& p, int ctas, bool chained, cudaStream_t
 
 }  // namespace
 
-int kv_decode_workers(int num_sms) { return 2 * num_sms * kWarps; }
+int kv_decode_workers(int num_sms, int head_dim) { return num_sms * kWarps * (head_dim == 64 ? kPerSm<64> : kPerSm<128>); }
 
 cudaError_t launch_kv_decode(const KvAttendParams& p, int head_dim, int dtype, int num_sms, bool chained, cudaStream_t st) {
-    const int ctas = 2 * num_sms;
+    const int ctas = num_sms * (head_dim == 64 ? kPerSm<64> : kPerSm<128>);
     if (dtype == GFD_BF16)
         return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, ctas, chained, st) : launch<__nv_bfloat16, 128>(p, ctas, chained, st);
     return head_dim == 64 ? launch<__half, 64>(p, ctas, chained, st) : launch<__half, 128>(p, ctas, chained, st);

@@ -85,6 +85,11 @@ __device__ __forceinline__ int32_t kv_div_group(const KvAttendParams& p, int32_t
     return static_cast<int32_t>(__umul64hi(static_cast<uint64_t>(n) << 20, p.group_magic));
 }
 
+// n / (pages of a block) for 0 <= n < 2^26 and up to 64 pages: n times pages stays below 2^32.
+__device__ __forceinline__ int32_t kv_div_pages(const KvAttendParams& p, int32_t n) {
+    return static_cast<int32_t>(static_cast<uint64_t>(n) * p.page_magic >> 32);
+}
+
 // row_start rises from >= 0 to <= rows (every thread of the CTA calls; same answer for all).
 __device__ __forceinline__ bool kv_starts_ok(const KvBatchView& b) {
     bool bad = false;
@@ -292,7 +297,7 @@ __device__ __forceinline__ void kv_exact_row(const KvAttendParams& p, const KvEx
 
 template <typename... P, typename... A>
 cudaError_t kv_launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, bool chained, A... args) {
-    if (smem > 48 * 1024) {
+    if (smem > 32 * 1024) {  // with the static part more than 48 KB
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
         if (e != cudaSuccess) return e;
     }

@@ -945,14 +945,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     int32_t id = p.cache.blocks;  // a block outside the map: loads as zeros
                     bool bad = false;
                     if ((j < u.pre || (j + kKvPage > u.lo && j < u.hi)) && j < n) {
-                        id = table[j / kKvPage / pages];
+                        id = table[kv_div_pages(p, j / kKvPage)];
                         if (id < 0 || id >= p.cache.blocks) {
                             bad = true;
                             id = p.cache.blocks;
                             kv_report(p.status, GFD_KV_BAD_PAGE);
                         }
                     }
-                    const int32_t in_block = (j / kKvPage % pages) * kKvPage;
+                    const int32_t in_block = (j / kKvPage - kv_div_pages(p, j / kKvPage) * pages) * kKvPage;
                     const uint32_t bad_pages = __ballot_sync(0xffffffffu, bad) & 0xffu;
                     // a page that the sequence ends in: V's tokens behind the end are kept out by hand,
                     // whatever lies there would meet weights of zero
