@@ -11,16 +11,18 @@ namespace {
 // ---------------------------------------------------------------------------
 // A head is cut into items of 16 elements that one thread moves: item i < rot_dim / 16
 // holds the 8 pairs that rotate together (two 16-byte pieces rot_dim / 2 apart, or 16
-// neighbours when interleaved), the items above copy.  A CTA takes kRows rows: their
-// places and the sines and cosines of their rot_dim / 2 angles are formed once in shared
-// memory and serve all K and Q heads.  Angles: p * inv_freq is exact in 64 bits up to
+// neighbours when interleaved), the items above copy.  A thread keeps its item for all heads, so the
+// sines and cosines of its 8 angles stay in registers while it walks the heads of a row, 2 of them
+// in flight at a time.  Memory bounds the kernel: 8.5 thousand rows of 32 + 8 + 8 heads of 128 take 51 us,
+// 5.1 TB/s (4 heads in flight and 8 rows a CTA: 76 us; 3 or 5 CTAs an SM: 60, 89).  A CTA takes
+// kMaxRows rows (one where there are few) and forms their places and angles once.  Angles: p * inv_freq is exact in 64 bits up to
 // p = 2^29, and a turn is taken off in 64 bits before the 32-bit sine, so a position of a
 // million is as accurate as a small one.
 constexpr int kAppendThreads = 256;
+constexpr int kMaxRows = 4;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvAppendParams p, int rows_per_cta) {
-    constexpr int kMaxRows = 4;
+__global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const KvAppendParams p, int rows_per_cta) {
     __shared__ float s_cos[kMaxRows][D / 2], s_sin[kMaxRows][D / 2];
     __shared__ int32_t s_seq[kMaxRows], s_block[kMaxRows], s_place[kMaxRows], s_pos[kMaxRows];
     const KvBatchView& b = p.batch;
@@ -28,7 +30,12 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvAppen
     const int32_t row0 = blockIdx.x * rows_per_cta;
     const int nrows = min(rows_per_cta, b.rows - row0);
     if (t < kMaxRows) s_seq[t] = -1;
-    if (!kv_starts_ok(b)) {  // syncs
+    bool bad = false;
+    for (int s = t; s < b.seqs; s += kAppendThreads) {
+        const int32_t a = b.row_start[s], e = b.row_start[s + 1];
+        bad |= a < 0 || a > e || e > b.rows;
+    }
+    if (__syncthreads_or(bad) != 0) {
         if (blockIdx.x == 0 && t == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
         return;
     }
@@ -42,91 +49,105 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const KvAppen
         }
         for (int i = max(a - row0, 0); i < min(e - row0, nrows); ++i) {
             const int32_t pos = q.keys - q.rows + (row0 + i - a);
-            int32_t place;
-            const int32_t block = kv_block(b, s, pos, p.cache.block_tokens, nullptr, 0, &place);
             s_seq[i] = s;
-            s_place[i] = place;
-            s_block[i] = block >= 0 && block < p.cache.blocks ? block : -1;
-            if (s_block[i] < 0) kv_report(p.status, GFD_KV_BAD_PAGE);
+            s_place[i] = pos;
             s_pos[i] = p.positions != nullptr ? p.positions[row0 + i] : pos;
         }
     }
     __syncthreads();
     const int half = p.rot_dim / 2;
-    for (int i = t; i < nrows * half; i += kAppendThreads) {
-        const int r = i / half, f = i % half;
-        if (s_seq[r] < 0) continue;
-        constexpr double kPerTurn = 0.15915494309189535;  // 1 / (2 pi)
-        double turns = static_cast<double>(s_pos[r]) * static_cast<double>(p.inv_freq[f]) * kPerTurn;
-        turns -= rint(turns);
-        float sn, cs;
-        sincospif(static_cast<float>(2.0 * turns), &sn, &cs);
-        s_cos[r][f] = cs;
-        s_sin[r][f] = sn;
+    // the places, by the last warp, while the others form the angles
+    if (t >= kAppendThreads - 32) {
+        const int r = t - (kAppendThreads - 32);
+        if (r < nrows && s_seq[r] >= 0) {
+            int32_t place;
+            const int32_t block = kv_block(b, s_seq[r], s_place[r], p.cache.block_tokens, nullptr, 0, &place);
+            s_place[r] = place;
+            s_block[r] = block >= 0 && block < p.cache.blocks ? block : -1;
+            if (s_block[r] < 0) kv_report(p.status, GFD_KV_BAD_PAGE);
+        }
+    } else {
+        for (int i = t; i < nrows * half; i += kAppendThreads - 32) {
+            const int r = i / half, f = i % half;
+            if (s_seq[r] < 0) continue;
+            constexpr double kPerTurn = 0.15915494309189535;  // 1 / (2 pi)
+            double turns = static_cast<double>(s_pos[r]) * static_cast<double>(p.inv_freq[f]) * kPerTurn;
+            turns -= rint(turns);
+            float sn, cs;
+            sincospif(static_cast<float>(2.0 * turns), &sn, &cs);
+            s_cos[r][f] = cs;
+            s_sin[r][f] = sn;
+        }
     }
     __syncthreads();
 
-    constexpr int kItems = D / 16;
-    const int kvh = p.cache.heads;
-    const int per_row = (p.q_heads + 2 * kvh) * kItems;
-    for (int i = t; i < nrows * per_row; i += kAppendThreads) {
-        const int r = i / per_row, rest = i % per_row;
+    constexpr int kItems = D / 16, kHeads = kAppendThreads / kItems, kAhead = 2;  // heads of a step, steps in flight
+    const int it = t % kItems, kvh = p.cache.heads, heads = p.q_heads + 2 * kvh;
+    const bool turns = it < p.rot_dim / 16;
+    const int e0 = turns && !p.interleaved ? it * 8 : it * 16, e1 = turns && !p.interleaved ? e0 + half : e0 + 8;
+    for (int r = 0; r < nrows; ++r) {
         if (s_seq[r] < 0) continue;
-        int h = rest / kItems;
-        const int it = rest % kItems;
         const int64_t row = row0 + r;
-        const char* src;
-        char* dst;
-        bool turn = it < p.rot_dim / 16;
-        if (h < p.q_heads) {
-            src = p.q.data + row * p.q.row_stride + h * p.q.head_stride;
-            dst = p.q_out.data + row * p.q_out.row_stride + h * p.q_out.head_stride;
-        } else {
-            h -= p.q_heads;
-            const bool is_v = h >= kvh;
-            if (is_v) h -= kvh;
-            const KvRowsView& x = is_v ? p.v : p.k;
-            if (s_block[r] < 0) continue;
-            src = x.data + row * x.row_stride + h * x.head_stride;
-            dst = const_cast<char*>(is_v ? p.cache.v : p.cache.k) + s_block[r] * p.cache.block_stride +
-                  s_place[r] * p.cache.token_stride + h * p.cache.head_stride;
-            turn = turn && !is_v;
+        float cs[8], sn[8];
+        if (turns) {
+            Pack<float>::load(reinterpret_cast<const char*>(&s_cos[r][it * 8]), cs);
+            Pack<float>::load(reinterpret_cast<const char*>(&s_sin[r][it * 8]), sn);
         }
-        if (!turn) {
-            const int e = it * 16;
-            // the pairs of the split form lie rot_dim / 2 apart; what is copied is contiguous
-            const uint4 x0 = *reinterpret_cast<const uint4*>(src + 2 * e), x1 = *reinterpret_cast<const uint4*>(src + 2 * e + 16);
-            *reinterpret_cast<uint4*>(dst + 2 * e) = x0;
-            *reinterpret_cast<uint4*>(dst + 2 * e + 16) = x1;
-            continue;
-        }
-        const int e0 = p.interleaved ? it * 16 : it * 8;
-        const int e1 = p.interleaved ? e0 + 8 : e0 + half;
-        float a[8], c[8];
-        Pack<T>::load(src + 2 * e0, a);
-        Pack<T>::load(src + 2 * e1, c);
-        const float* cs = &s_cos[r][it * 8];
-        const float* sn = &s_sin[r][it * 8];
-        if (p.interleaved) {
+        const int64_t cell = s_block[r] >= 0 ? s_block[r] * p.cache.block_stride + s_place[r] * p.cache.token_stride : -1;
+        for (int h0 = t / kItems; h0 < heads; h0 += kHeads * kAhead) {
+            uint4 a[kAhead], c[kAhead];
+            char* dst[kAhead];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float x = a[2 * j], y = a[2 * j + 1];
-                a[2 * j] = x * cs[j] - y * sn[j];
-                a[2 * j + 1] = x * sn[j] + y * cs[j];
-                const float u = c[2 * j], w = c[2 * j + 1];
-                c[2 * j] = u * cs[4 + j] - w * sn[4 + j];
-                c[2 * j + 1] = u * sn[4 + j] + w * cs[4 + j];
+            for (int y = 0; y < kAhead; ++y) {
+                const int h = h0 + y * kHeads;
+                const char* src = nullptr;
+                dst[y] = nullptr;
+                if (h < p.q_heads) {
+                    src = p.q.data + row * p.q.row_stride + h * p.q.head_stride;
+                    dst[y] = p.q_out.data + row * p.q_out.row_stride + h * p.q_out.head_stride;
+                } else if (h < heads && cell >= 0) {
+                    const bool is_v = h >= p.q_heads + kvh;
+                    const int k = h - p.q_heads - (is_v ? kvh : 0);
+                    src = is_v ? p.v.data + row * p.v.row_stride + k * p.v.head_stride : p.k.data + row * p.k.row_stride + k * p.k.head_stride;
+                    dst[y] = const_cast<char*>(is_v ? p.cache.v : p.cache.k) + cell + k * p.cache.head_stride;
+                }
+                if (src == nullptr) continue;
+                // V is copied: the same pieces as the rotation's, wherever they lie
+                a[y] = *reinterpret_cast<const uint4*>(src + 2 * e0);
+                c[y] = *reinterpret_cast<const uint4*>(src + 2 * e1);
             }
-        } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = a[j], y = c[j];
-                a[j] = x * cs[j] - y * sn[j];
-                c[j] = x * sn[j] + y * cs[j];
+            for (int y = 0; y < kAhead; ++y) {
+                if (dst[y] == nullptr) continue;
+                if (!turns || h0 + y * kHeads >= p.q_heads + kvh) {
+                    *reinterpret_cast<uint4*>(dst[y] + 2 * e0) = a[y];
+                    *reinterpret_cast<uint4*>(dst[y] + 2 * e1) = c[y];
+                    continue;
+                }
+                float u[8], w[8];
+                Pack<T>::load(reinterpret_cast<const char*>(&a[y]), u);
+                Pack<T>::load(reinterpret_cast<const char*>(&c[y]), w);
+                if (p.interleaved) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float x0 = u[2 * j], y0 = u[2 * j + 1], x1 = w[2 * j], y1 = w[2 * j + 1];
+                        u[2 * j] = x0 * cs[j] - y0 * sn[j];
+                        u[2 * j + 1] = x0 * sn[j] + y0 * cs[j];
+                        w[2 * j] = x1 * cs[4 + j] - y1 * sn[4 + j];
+                        w[2 * j + 1] = x1 * sn[4 + j] + y1 * cs[4 + j];
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float x0 = u[j], y0 = w[j];
+                        u[j] = x0 * cs[j] - y0 * sn[j];
+                        w[j] = x0 * sn[j] + y0 * cs[j];
+                    }
+                }
+                Pack<T>::store(dst[y] + 2 * e0, u);
+                Pack<T>::store(dst[y] + 2 * e1, w);
             }
         }
-        Pack<T>::store(dst + 2 * e0, a);
-        Pack<T>::store(dst + 2 * e1, c);
     }
 }
 
@@ -167,8 +188,10 @@ __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const KvMergePa
 }
 
 // ---------------------------------------------------------------------------
-// Join of an attention launch's partial results: CTA x (times gridDim.y) sees to cut x + 1.
+// Join of an attention launch's partial results.
 // ---------------------------------------------------------------------------
+constexpr int kJoinThreads = 256;
+constexpr int kJoinWarps = kJoinThreads / 32;
 // Weight of a part whose sums are relative to 2^base, and its share of the weight sum: a part without
 // keys (-inf) adds nothing but a NaN that its scores left.
 __device__ __forceinline__ void part_weight(float base, float top, float* w, float* l) {
@@ -176,12 +199,9 @@ __device__ __forceinline__ void part_weight(float base, float top, float* w, flo
     if (base != -INFINITY) *l *= *w;
 }
 
-// Of kv_decode, with up to hundreds of parts of a few rows: a CTA takes 4 rows at a time and 128 parts:
+// Of kv_decode, with up to hundreds of parts of a few rows: a CTA per cut takes 4 rows at a time and 128 parts:
 // its threads weigh them, then each warp sums every 8th part (D / 32 elements a lane), and the warps'
 // sums are added in their order.
-constexpr int kJoinThreads = 256;
-constexpr int kJoinWarps = kJoinThreads / 32;
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_few_kernel(const KvAttendParams p) {
     constexpr int kEach = D / 32, kSlot = kKvFewRows * (D + 2), kParts = 128;
@@ -299,77 +319,93 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_few_kernel(const KvAtten
     }
 }
 
-// Of kv_prompt, with many rows: a CTA takes kRows rows, a thread one of them and 4 elements, so that the
-// parts are read as they were written; the results go through shared memory to be written row by row.
+// Of kv_prompt, with many rows: a CTA takes 32 rows of a cut, a lane one of them and a warp D / 8
+// elements, so that the parts are read as they were written, 4 at a time; the results go through shared
+// memory to be written row by row.
 template <typename T, int D, bool kShared>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_many_kernel(const KvAttendParams p) {
-    constexpr int kRows = kJoinThreads * 4 / D;  // 8 or 16
+    constexpr int kEach = D / 8, kBatch = 4;  // elements of a thread, parts side by side
     constexpr int64_t kSlot = static_cast<int64_t>(kKvManyRows) * (D + 2);
-    __shared__ float s_out[kRows][D + 4];
-    __shared__ bool s_ok[kRows];
-    const int c = blockIdx.x + 1, t = threadIdx.x;
+    __shared__ float s_out[32][D + 4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x + 1;
     kv_let_next();
     kv_wait_last();
     const KvCut u = p.line.cuts[c];
-    const int r0 = blockIdx.y * kRows;
+    const int r0 = blockIdx.y * 32;
     if (u.parts == 0 || r0 >= u.packed) return;
-    const float* slots = p.line.slots + 2 * (c - 1) * kSlot;
-    const int r = r0 + t % kRows, d = t / kRows * 4;
-    const bool live = r < u.packed;
-    const int32_t packed = u.packed0 + (live ? r : r0), of = kv_div_group(p, packed);
+    const float* slots = p.line.slots + 2 * (c - 1) * kSlot;  // part x: slot 1 for 0, else 2 x
+    const bool live = r0 + lane < u.packed;
+    const int r = live ? r0 + lane : r0;
+    const int32_t packed = u.packed0 + r, of = kv_div_group(p, packed);
     const int64_t row = u.row0 + of;
     const int head = u.h * p.group + packed - of * p.group;
-    float own_lse = -INFINITY;
-    float4 own = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (kShared) {
-        own_lse = p.own_lse[row * p.q_heads + head];
-        own = *reinterpret_cast<const float4*>(p.own_out + (row * p.q_heads + head) * D + d);
-    }
-    float m = -INFINITY, l = 0.0f, sum[4] = {};
-    if (live)
-#pragma unroll 4
-        for (int x = 0; x < u.parts; ++x) {
+    const int64_t place = row * p.q_heads + head;
+    const float own_lse = kShared ? p.own_lse[place] : -INFINITY;
+    float m = -INFINITY, l = 0.0f, sum[kEach] = {};
+    for (int x0 = 0; x0 < u.parts; x0 += kBatch) {
+        float pm[kBatch], pl[kBatch], f[kBatch][kEach];
+#pragma unroll
+        for (int y = 0; y < kBatch; ++y) {
+            const int x = x0 + y;
+            pm[y] = -INFINITY;
+            pl[y] = 0.0f;
+            if (x >= u.parts) continue;
             const float* slot = slots + (x == 0 ? 1 : 2 * x) * kSlot;
-            const float pm = slot[kKvManyRows * D + r];
-            float pl = slot[kKvManyRows * D + kKvManyRows + r];
-            const float4 f = *reinterpret_cast<const float4*>(slot + (static_cast<int64_t>(d) / 4 * kKvManyRows + r) * 4);
-            const float top = fmaxf(m, pm);
-            float keep, w;
-            part_weight(m, top, &keep, &l);
-            part_weight(pm, top, &w, &pl);
-            l += pl;
-            m = top;
-            sum[0] = w != 0.0f ? fmaf(f.x, w, sum[0] * keep) : sum[0] * keep;
-            sum[1] = w != 0.0f ? fmaf(f.y, w, sum[1] * keep) : sum[1] * keep;
-            sum[2] = w != 0.0f ? fmaf(f.z, w, sum[2] * keep) : sum[2] * keep;
-            sum[3] = w != 0.0f ? fmaf(f.w, w, sum[3] * keep) : sum[3] * keep;
+            pm[y] = slot[kKvManyRows * D + r];
+            pl[y] = slot[kKvManyRows * D + kKvManyRows + r];
+#pragma unroll
+            for (int e = 0; e < kEach; e += 4)
+                *reinterpret_cast<float4*>(f[y] + e) =
+                    *reinterpret_cast<const float4*>(slot + (static_cast<int64_t>(warp * kEach + e) / 4 * kKvManyRows + r) * 4);
         }
+        float top = m, keep;
+#pragma unroll
+        for (int y = 0; y < kBatch; ++y) top = fmaxf(top, pm[y]);
+        part_weight(m, top, &keep, &l);
+        m = top;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) sum[e] *= keep;
+#pragma unroll
+        for (int y = 0; y < kBatch; ++y) {
+            float w;
+            part_weight(pm[y], top, &w, &pl[y]);
+            l += pl[y];
+            if (w != 0.0f)
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) sum[e] = fmaf(f[y][e], w, sum[e]);
+        }
+    }
     const bool valid = live && (!kShared || __float_as_uint(own_lse) != kKvSkipped);
     if (valid) {
         const KvFinish f = kv_finish<kShared>(p, m, l, own_lse);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] *= f.scale;
-        if (kShared && f.own != 0.0f) {
-            sum[0] = fmaf(own.x, f.own, sum[0]);
-            sum[1] = fmaf(own.y, f.own, sum[1]);
-            sum[2] = fmaf(own.z, f.own, sum[2]);
-            sum[3] = fmaf(own.w, f.own, sum[3]);
-        }
-        if (p.lse != nullptr && d == 0) p.lse[row * p.q_heads + head] = kv_lse(p, f.base, f.sum);
-        *reinterpret_cast<float4*>(&s_out[t % kRows][d]) = *reinterpret_cast<const float4*>(sum);
+        for (int e = 0; e < kEach; ++e) sum[e] *= f.scale;
+        if (kShared && f.own != 0.0f)
+#pragma unroll
+            for (int e = 0; e < kEach; e += 4) {
+                const float4 y = *reinterpret_cast<const float4*>(p.own_out + place * D + warp * kEach + e);
+                sum[e] = fmaf(y.x, f.own, sum[e]);
+                sum[e + 1] = fmaf(y.y, f.own, sum[e + 1]);
+                sum[e + 2] = fmaf(y.z, f.own, sum[e + 2]);
+                sum[e + 3] = fmaf(y.w, f.own, sum[e + 3]);
+            }
+        if (p.lse != nullptr && warp == 0) p.lse[place] = kv_lse(p, f.base, f.sum);
+#pragma unroll
+        for (int e = 0; e < kEach; e += 4) *reinterpret_cast<float4*>(&s_out[lane][warp * kEach + e]) = *reinterpret_cast<const float4*>(sum + e);
     }
-    if (d == 0) s_ok[t % kRows] = valid;
+    const unsigned ok = __ballot_sync(0xffffffffu, valid);  // the same rows in every warp
     __syncthreads();
     constexpr int kLanes = D / 8;
-    const int i = t / kLanes, e = t % kLanes * 8;
-    if (i < kRows && s_ok[i]) {
+    for (int i = threadIdx.x / kLanes; i < 32; i += kJoinThreads / kLanes) {
+        if (!((ok >> i) & 1u)) continue;
         const int32_t pk = u.packed0 + r0 + i, o = kv_div_group(p, pk);
         char* at = p.out.data + static_cast<int64_t>(u.row0 + o) * p.out.row_stride + (u.h * p.group + pk - o * p.group) * p.out.head_stride;
+        const int d = threadIdx.x % kLanes * 8;
         float f[8];
-        *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(&s_out[i][e]);
-        *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(&s_out[i][e + 4]);
-        if (p.out_f32) Pack<float>::store(at + 4 * e, f);
-        else Pack<T>::store(at + 2 * e, f);
+        *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(&s_out[i][d]);
+        *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(&s_out[i][d + 4]);
+        if (p.out_f32) Pack<float>::store(at + 4 * d, f);
+        else Pack<T>::store(at + 2 * d, f);
     }
 }
 
@@ -385,7 +421,7 @@ cudaError_t by_any_type(int dtype, F f) {
 }  // namespace
 
 cudaError_t launch_kv_append(const KvAppendParams& p, int head_dim, int dtype, int num_sms, cudaStream_t st) {
-    const int rows_per_cta = p.batch.rows > 8 * num_sms ? 4 : 1;
+    const int rows_per_cta = p.batch.rows > 4 * num_sms ? kMaxRows : 1;
     const dim3 grid((p.batch.rows + rows_per_cta - 1) / rows_per_cta);
     return by_type(dtype, [&](auto t) {
         using T = decltype(t);
@@ -394,19 +430,19 @@ cudaError_t launch_kv_append(const KvAppendParams& p, int head_dim, int dtype, i
     });
 }
 
-cudaError_t launch_kv_join_few(const KvAttendParams& p, int head_dim, int dtype, int ctas, cudaStream_t st) {
+cudaError_t launch_kv_join_few(const KvAttendParams& p, int head_dim, int dtype, int stretches, cudaStream_t st) {
     return by_type(dtype, [&](auto t) {
         using T = decltype(t);
-        return kv_launch(head_dim == 64 ? kv_join_few_kernel<T, 64> : kv_join_few_kernel<T, 128>, dim3(ctas - 1), kJoinThreads, 0, st, true, p);
+        return kv_launch(head_dim == 64 ? kv_join_few_kernel<T, 64> : kv_join_few_kernel<T, 128>, dim3(stretches - 1), kJoinThreads, 0, st, true, p);
     });
 }
 
-cudaError_t launch_kv_join_many(const KvAttendParams& p, int head_dim, int dtype, int ctas, cudaStream_t st) {
+cudaError_t launch_kv_join_many(const KvAttendParams& p, int head_dim, int dtype, int stretches, cudaStream_t st) {
     return by_type(dtype, [&](auto t) {
         using T = decltype(t);
         auto* f = p.shared_pass ? (head_dim == 64 ? kv_join_many_kernel<T, 64, true> : kv_join_many_kernel<T, 128, true>)
                                 : (head_dim == 64 ? kv_join_many_kernel<T, 64, false> : kv_join_many_kernel<T, 128, false>);
-        return kv_launch(f, dim3(ctas - 1, kKvManyRows / (kJoinThreads * 4 / head_dim)), kJoinThreads, 0, st, true, p);
+        return kv_launch(f, dim3(stretches - 1, kKvManyRows / 32), kJoinThreads, 0, st, true, p);
     });
 }
 

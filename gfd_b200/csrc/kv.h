@@ -111,8 +111,8 @@ struct KvMergeParams {
 // dtype: GFD_* of the cache.  chained: the launch may start before the one before it on the stream has
 // ended (it was made by the same call and touches nothing of this one's, or waits for it).
 cudaError_t launch_kv_append(const KvAppendParams& p, int head_dim, int dtype, int num_sms, cudaStream_t st);
-cudaError_t launch_kv_join_few(const KvAttendParams& p, int head_dim, int dtype, int ctas, cudaStream_t st);
-cudaError_t launch_kv_join_many(const KvAttendParams& p, int head_dim, int dtype, int ctas, cudaStream_t st);
+cudaError_t launch_kv_join_few(const KvAttendParams& p, int head_dim, int dtype, int stretches, cudaStream_t st);
+cudaError_t launch_kv_join_many(const KvAttendParams& p, int head_dim, int dtype, int stretches, cudaStream_t st);
 int kv_decode_workers(int num_sms, int head_dim);  // each with a stretch of the line
 int kv_prompt_ctas(int num_sms);
 // cuTensorMapEncodeTiled, resolved through the runtime (libcuda is not linked)

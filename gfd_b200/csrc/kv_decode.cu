@@ -518,7 +518,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) kv_decode_kernel(const Kv
 }
 
 template <typename T, int D>
-cudaError_t launch(const KvAttendParams& p, int ctas, bool chained, cudaStream_t st) {
+cudaError_t launch(const KvAttendParams& p, int num_sms, bool chained, cudaStream_t st) {
+    const int ctas = num_sms * kPerSm<D>;
     const bool plain = p.softcap == 0.0f && p.alibi == nullptr;
     const cudaError_t e = kv_launch(plain ? kv_decode_kernel<T, D, true> : kv_decode_kernel<T, D, false>, dim3(ctas), kThreads,
                                     Shape<D>::kSmem, st, chained, p);
@@ -531,10 +532,9 @@ cudaError_t launch(const KvAttendParams& p, int ctas, bool chained, cudaStream_t
 int kv_decode_workers(int num_sms, int head_dim) { return num_sms * kWarps * (head_dim == 64 ? kPerSm<64> : kPerSm<128>); }
 
 cudaError_t launch_kv_decode(const KvAttendParams& p, int head_dim, int dtype, int num_sms, bool chained, cudaStream_t st) {
-    const int ctas = num_sms * (head_dim == 64 ? kPerSm<64> : kPerSm<128>);
     if (dtype == GFD_BF16)
-        return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, ctas, chained, st) : launch<__nv_bfloat16, 128>(p, ctas, chained, st);
-    return head_dim == 64 ? launch<__half, 64>(p, ctas, chained, st) : launch<__half, 128>(p, ctas, chained, st);
+        return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, num_sms, chained, st) : launch<__nv_bfloat16, 128>(p, num_sms, chained, st);
+    return head_dim == 64 ? launch<__half, 64>(p, num_sms, chained, st) : launch<__half, 128>(p, num_sms, chained, st);
 }
 
 }  // namespace gfdb
