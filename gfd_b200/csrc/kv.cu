@@ -152,38 +152,52 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const KvAp
 }
 
 // ---------------------------------------------------------------------------
-// Merge: one group of D / 8 threads per (row, head), 8 elements a thread
+// Merge: one group of D / 8 threads per (row, head), 8 elements a thread, 4 parts in flight at a time.
+// Memory bounds it.
 // ---------------------------------------------------------------------------
 constexpr int kMergeThreads = 256;
 
 template <typename T, typename O, int D>
 __global__ void __launch_bounds__(kMergeThreads) kv_merge_kernel(const KvMergeParams p) {
-    constexpr int kLanes = D / 8;
+    constexpr int kLanes = D / 8, kBatch = 4;
     const int64_t n = static_cast<int64_t>(p.rows) * p.heads;
     const int lane = threadIdx.x % kLanes;
     const int64_t step = static_cast<int64_t>(gridDim.x) * (kMergeThreads / kLanes);
     for (int64_t u = blockIdx.x * static_cast<int64_t>(kMergeThreads / kLanes) + threadIdx.x / kLanes; u < n; u += step) {
-        const int64_t row = u / p.heads, h = u % p.heads;
-        float m = -INFINITY;
-        for (int i = 0; i < p.part_count; ++i) m = fmaxf(m, p.part_lse[i * n + u]);
-        const float base = m == -INFINITY ? 0.0f : m;
-        float acc[8] = {}, total = 0.0f;
+        const int64_t row = kv_div(u, p.heads), h = u - row * p.heads;
+        float m = -INFINITY, total = 0.0f, acc[8] = {};
         const char* src = p.parts.data + row * p.parts.row_stride + h * p.parts.head_stride + lane * 8 * sizeof(T);
-        for (int i = 0; i < p.part_count; ++i) {
-            const float l = p.part_lse[i * n + u];
-            if (l == -INFINITY) continue;
-            const float w = expf(l - base);
-            total += w;
-            float f[8];
-            Pack<T>::load(src + i * p.part_stride, f);
+        for (int i0 = 0; i0 < p.part_count; i0 += kBatch) {
+            float l[kBatch], f[kBatch][8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, f[e], acc[e]);
+            for (int i = 0; i < kBatch; ++i) {
+                l[i] = -INFINITY;
+                if (i0 + i >= p.part_count) continue;
+                l[i] = p.part_lse[(i0 + i) * n + u];
+                Pack<T>::load(src + (i0 + i) * p.part_stride, f[i]);
+            }
+            float top = m;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) top = fmaxf(top, l[i]);
+            const float keep = m == -INFINITY ? 0.0f : expf(m - top);
+            m = top;
+            total *= keep;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] *= keep;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                if (l[i] == -INFINITY) continue;  // whatever its output holds
+                const float w = expf(l[i] - top);
+                total += w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, f[i][e], acc[e]);
+            }
         }
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = total == 0.0f ? 0.0f : acc[e] * inv;
+        for (int e = 0; e < 8; ++e) acc[e] *= inv;
         Pack<O>::store(p.out.data + row * p.out.row_stride + h * p.out.head_stride + lane * 8 * sizeof(O), acc);
-        if (lane == 0 && p.lse != nullptr) p.lse[u] = total == 0.0f ? -INFINITY : base + logf(total);
+        if (lane == 0 && p.lse != nullptr) p.lse[u] = total == 0.0f ? -INFINITY : m + logf(total);
     }
 }
 
