@@ -484,22 +484,28 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) kv_decode_kernel(const Kv
                     p.lse[row * p.q_heads + head] = kv_lse(p, m[x], l[x]);
                 }
             }
-            for (uint32_t redo = __ballot_sync(0xffffffffu, r < rows && odd != 0.0f); redo != 0;) {
-                const int src = (__ffs(redo) - 1) & ~3;
-                redo &= ~(15u << src);
-                KvExact y;
+            // (a weight sum that is not finite makes the row NaN as it is)
+            uint32_t redo = __ballot_sync(0xffffffffu, r < rows && odd != 0.0f && l[x] < INFINITY);
+            KvExact y;
+            if (redo != 0) {
                 y.table = b.table + use.s * b.table_stride;
                 y.tiles = use.q.tiles;
-                y.seen = KvSpan{__shfl_sync(0xffffffffu, sp[x].pre, src), __shfl_sync(0xffffffffu, sp[x].lo, src),
-                                __shfl_sync(0xffffffffu, sp[x].hi, src)};
-                y.pos = __shfl_sync(0xffffffffu, pos[x], src);
                 y.base = p.shared_len;
                 y.t0 = t0;
                 y.t1 = use.end;
                 y.size = kTile;
+                y.kvh = use.h;
+                y.seen = sp[x];
+                redo = kv_to_redo<T, D>(p, y, use.q.q.keys, redo);
+            }
+            while (redo != 0) {
+                const int src = (__ffs(redo) - 1) & ~3;  // the row's first lane
+                redo &= ~(15u << src);
+                y.seen = KvSpan{__shfl_sync(0xffffffffu, sp[x].pre, src), __shfl_sync(0xffffffffu, sp[x].lo, src),
+                                __shfl_sync(0xffffffffu, sp[x].hi, src)};
+                y.pos = __shfl_sync(0xffffffffu, pos[x], src);
                 y.row = __shfl_sync(0xffffffffu, row, src);
                 y.head = __shfl_sync(0xffffffffu, head, src);
-                y.kvh = use.h;
                 const float rb = __shfl_sync(0xffffffffu, m[x], src), ri = __shfl_sync(0xffffffffu, inv, src);
                 const uint64_t rd = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), src);
                 constexpr int kEach = D / 32;

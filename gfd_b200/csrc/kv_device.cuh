@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "kv.h"
 
@@ -254,10 +255,63 @@ struct KvExact {
     int32_t head, kvh;
 };
 
+// Which rows (a lane each, bits of `odd`: their sums by matrix products are not finite) have to be summed
+// key by key: those with an element that is NaN or infinite in values which the row does not see
+// (0 * inf and 0 * NaN reached the sum) and in none that it sees.  Everything else is as it should be: a
+// seen NaN, or an overflow.  A row that sees such values in every element needs no further search.
+// keys: of the sequence; x.seen: of this lane's row.
+template <typename T, int D>
+__device__ __forceinline__ uint32_t kv_to_redo(const KvAttendParams& p, const KvExact& x, int32_t keys, uint32_t odd) {
+    constexpr uint32_t kMax = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;  // exponent of NaN and infinity
+    constexpr int kWords = D / 32;
+    const int lane = threadIdx.x & 31;
+    uint32_t in[kWords] = {}, out[kWords] = {};  // a bit an element: bad among seen values, among the others
+    for (int t = x.t0; t < x.t1; ++t)
+        for (int c = 0; c < x.size; c += 32) {
+            const int32_t j = x.tiles.at(t) * x.size + c + lane;
+            uint32_t bad[kWords] = {}, any = 0;
+            if (c + lane < x.size && j < keys) {
+                const int32_t id = x.table[j / p.cache.block_tokens];
+                if (id >= 0 && id < p.cache.blocks) {
+                    const char* v = p.cache.v + id * p.cache.block_stride + j % p.cache.block_tokens * p.cache.token_stride +
+                                    x.kvh * p.cache.head_stride;
+#pragma unroll
+                    for (int e = 0; e < D; e += 8) {
+                        const uint4 q = *reinterpret_cast<const uint4*>(v + 2 * e);
+                        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                        for (int y = 0; y < 4; ++y) {
+                            if ((w[y] & kMax) == kMax) bad[e / 32] |= 1u << (e % 32 + 2 * y);
+                            if ((w[y] >> 16 & kMax) == kMax) bad[e / 32] |= 2u << (e % 32 + 2 * y);
+                        }
+                        any |= bad[e / 32];
+                    }
+                }
+            }
+            for (uint32_t ball = __ballot_sync(0xffffffffu, any != 0); ball != 0; ball &= ball - 1) {
+                const int src = __ffs(ball) - 1;
+                const int32_t k = __shfl_sync(0xffffffffu, j, src);
+                const bool sees = k < x.seen.pre || (k >= x.seen.lo && k < x.seen.hi);
+                uint32_t all = 0xffffffffu;
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) {
+                    const uint32_t w = __shfl_sync(0xffffffffu, bad[i], src);
+                    in[i] |= sees ? w : 0u;
+                    out[i] |= sees ? 0u : w;
+                    all &= in[i];
+                }
+                odd &= __ballot_sync(0xffffffffu, all != 0xffffffffu);
+                if (odd == 0) return 0;
+            }
+        }
+    uint32_t hit = 0;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) hit |= out[i] & ~in[i];
+    return odd & __ballot_sync(0xffffffffu, hit != 0);
+}
+
 // The sum of the row's weights times values, key by key and only over keys that it sees, by one
-// warp; lane i gets elements [i D / 32, (i + 1) D / 32).  For rows whose sum by matrix products
-// met a NaN or an infinity, which a key that only other rows see may have put there (0 * inf).
-// m: what the weights are relative to, in base 2.
+// warp; lane i gets elements [i D / 32, (i + 1) D / 32).  m: what the weights are relative to,
+// in base 2.
 template <typename T, int D, bool kPlain>
 __device__ __forceinline__ void kv_exact_row(const KvAttendParams& p, const KvExact& x, float m, float* acc) {
     constexpr int kEach = D / 32;

@@ -813,20 +813,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                             slot[static_cast<int64_t>(kRows) * D + kRows + r] = l;
                         }
                     }
-                    for (uint32_t redo = __ballot_sync(0xffffffffu, valid && odd != 0.0f); redo != 0; redo &= redo - 1) {
-                        const int src = __ffs(redo) - 1;
-                        KvExact y;
+                    // (a weight sum that is not finite makes the row NaN as it is)
+                    uint32_t redo = __ballot_sync(0xffffffffu, valid && odd != 0.0f && l < INFINITY);
+                    KvExact y;
+                    if (redo != 0) {
                         y.table = kShared ? p.shared_table : b.table + u.s * b.table_stride;
                         y.tiles = KvTiles{u.npre, u.first, u.count};
-                        const int rs = x * kHalf + (warp & 3) * 32 + src;
-                        y.seen = row_span<kShared>(p, u, rs, &y.pos, true);
                         y.base = kShared ? 0 : p.shared_len;
                         y.t0 = u.t0;
                         y.t1 = u.t0 + u.nt;
                         y.size = kTile;
+                        y.kvh = u.h;
+                        y.seen = row_span<kShared>(p, u, r, &y.pos, true);
+                        redo = kv_to_redo<T, D>(p, y, u.keys, redo);
+                    }
+                    for (; redo != 0; redo &= redo - 1) {
+                        const int src = __ffs(redo) - 1;
+                        const int rs = x * kHalf + (warp & 3) * 32 + src;
+                        y.seen = row_span<kShared>(p, u, rs, &y.pos, true);
                         y.row = __shfl_sync(0xffffffffu, row, src);
                         y.head = __shfl_sync(0xffffffffu, head, src);
-                        y.kvh = u.h;
                         const float rb = __shfl_sync(0xffffffffu, base, src), rf = __shfl_sync(0xffffffffu, f.scale, src);
                         const float ro = __shfl_sync(0xffffffffu, f.own, src);
                         const uint64_t rd = __shfl_sync(0xffffffffu, dst, src);

@@ -318,6 +318,81 @@ def test_attend_ignores_what_is_masked(gpu_ctx, shape, poison):
     assert not bool(torch.isfinite(got[last].float()).any())
 
 
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1], [3000, 500]), ([2000, 40], [2100, 300])])
+def test_attend_nan_that_is_seen(gpu_ctx, q_lens, kv_lens):
+    """A NaN or an infinity that rows see makes those rows NaN or infinite and no others, and does
+    not cost more than a few times the call."""
+    torch = torch_()
+    s = Setup(gpu_ctx, "bf16", 2, 4, 64, 16, q_lens, kv_lens, seed=17)
+    want = s.want(window=700)
+    n = s.row_start[-1]
+    s.q[q_lens[0] // 2] = float("nan")
+    got, lse = s.attend(window=700)
+    torch.cuda.synchronize()
+    assert bool(torch.isnan(got[q_lens[0] // 2].float()).all()) and bool(torch.isnan(lse[q_lens[0] // 2]).all())
+    oracle.check_attend(got, lse, want, [r for r in range(n) if r != q_lens[0] // 2])
+    s.q[:] = torch.where(torch.isnan(s.q), torch.zeros_like(s.q), s.q)
+    want = s.want(window=700)
+    j = kv_lens[0] - q_lens[0] // 2 - 650  # seen by some rows only
+    s.v[int(s.table[0, j // 16]), j % 16, :, 5] = float("nan")
+    got, lse = s.attend(window=700)
+    torch.cuda.synchronize()
+    assert int(s.status) == 0
+    sees = [r for r in range(q_lens[0]) if j <= kv_lens[0] - q_lens[0] + r < j + 700]
+    assert sees and bool(torch.isnan(got[sees][:, :, 5].float()).all())
+    oracle.check_attend(got[:, :, 6:], lse, tuple(x[:, :, 6:] if x.dim() == 3 else x for x in want))
+    oracle.check_attend(got, lse, want, [r for r in range(n) if r not in set(sees)])
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", [([3], [500]), ([400], [700])])
+def test_attend_nan_seen_in_one_element_and_masked_in_another(gpu_ctx, q_lens, kv_lens):
+    torch = torch_()
+    s = Setup(gpu_ctx, "fp16", 2, 4, 128, 16, q_lens, kv_lens, seed=23)
+    want = s.want()
+    s.v[int(s.table[0, 1]), 3, :, 5] = float("nan")  # every row sees it
+    j = kv_lens[0] - 1  # the last row alone sees it
+    s.v[int(s.table[0, j // 16]), j % 16, :, 77] = float("inf")
+    got, lse = s.attend()
+    torch.cuda.synchronize()
+    assert bool(torch.isnan(got[:, :, 5].float()).all()) and bool(torch.isinf(got[-1, :, 77].float()).all())
+    n = q_lens[0]
+    keep = [d for d in range(128) if d not in (5, 77)]
+    cut = lambda x, d: x[:, :, d] if x.dim() == 3 else x
+    oracle.check_attend(got[:, :, keep], lse, tuple(cut(x, keep) for x in want))
+    oracle.check_attend(got[:, :, 77:78], lse, tuple(cut(x, [77]) for x in want), list(range(n - 1)))
+
+
+def test_attend_all_values_nan_is_not_slow(gpu_ctx):
+    torch = torch_()
+    s = Setup(gpu_ctx, "bf16", 2, 4, 128, 16, [4000], [4000], seed=18)
+    s.v[:] = float("nan")
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    s.attend()
+    a.record()
+    got, _ = s.attend()
+    b.record()
+    torch.cuda.synchronize()
+    assert bool(torch.isnan(got.float()).all()) and int(s.status) == 0
+    assert a.elapsed_time(b) < 100  # the call itself takes 0.3 ms
+
+
+@pytest.mark.parametrize("shape", [1, 4, 6])
+def test_attend_pages_behind_the_window_may_be_gone(gpu_ctx, shape):
+    """Block ids of pages that no row sees are not looked at."""
+    torch = torch_()
+    s = Setup(gpu_ctx, *SHAPES[shape], seed=19)
+    bt = s.k.shape[1]
+    want = s.want(window=20)
+    for i, n in enumerate(s.kv_lens):
+        first = max(0, n - s.q_lens[i] - 19) // bt
+        s.table[i, :first] = -1
+        s.table[i, -(-n // bt):] = 2 ** 31 - 1
+    got, lse = s.attend(window=20)
+    torch.cuda.synchronize()
+    assert int(s.status) == 0
+    oracle.check_attend(got, lse, want)
+
+
 def test_attend_bad_pages_are_masked(gpu_ctx):
     torch = torch_()
     for shape in (1, 6):
