@@ -742,10 +742,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
             const uint32_t stage = sq + (2 + S::kSlots) * S::kOperand + (warp & 3) * kStageBytes;
             uint32_t o_phase = 0;  // bit x
-            Desc u;
             bool good = true;
             if (kShared) kv_wait_last();  // the results over the own keys, which finish here
-            while (good && take(&u)) {
+            // The unit is read where it lies, and given back when its rows are written: with a copy of it
+            // in registers this loop's spilled, and with 2/3 of the SM's memory taken by
+            // operands, what is spilled comes back from L2.
+            for (; good; ++unit) {
+                const Desc& u = s_unit[unit % kUnitRing];
+                if (!bar_wait(smem_addr(&bars.unit[unit % kUnitRing]), (unit / kUnitRing) & 1, gave_up) || u.nt <= 0) break;
                 const bool whole = u.nt == u.count;
                 float* slot = p.line.slots + (2 * static_cast<int64_t>(blockIdx.x) + (u.t0 == 0 ? 1 : 0)) * (static_cast<int64_t>(kRows) * (D + 2));
                 for (int x = 0; x * kHalf < u.packed; ++x) {
@@ -773,9 +777,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                         f = kv_finish<kShared>(p, base, l, own_lse);
                         if (kShared && valid && f.own != 0.0f) own = p.own_out + (row * p.q_heads + head) * D;
                     }
-                    uint64_t to_row[4];  // this lane writes rows lane / 4 + 8 i
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) to_row[i] = __shfl_sync(0xffffffffu, dst, lane / 4 + 8 * i);
 #pragma unroll 1
                     for (int k = 0; k < D; k += 32) {
                         uint32_t o[32];
@@ -833,8 +834,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                                              : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                                              : "r"(stage + rw * 64 + (((lane & 3) ^ ((rw >> 1) & 3)) << 4))
                                              : "memory");
-                                if (to_row[i] != 0)
-                                    *reinterpret_cast<uint4*>(to_row[i] + (p.out_f32 ? 4 : 2) * k + 64 * st + 16 * (lane & 3)) = v;
+                                const uint64_t to_row = __shfl_sync(0xffffffffu, dst, rw);
+                                if (to_row != 0)
+                                    *reinterpret_cast<uint4*>(to_row + (p.out_f32 ? 4 : 2) * k + 64 * st + 16 * (lane & 3)) = v;
                             }
                             __syncwarp();
                         }
@@ -883,6 +885,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
+                __syncwarp();
+                if (lane == 0) bar_arrive(smem_addr(&bars.unit_read[unit % kUnitRing]));
             }
         } else if (warp == 12) {
             // ---- products: the whole warp walks, one thread issues ----
