@@ -89,6 +89,7 @@ struct KvAttendParams {
     float to_ln;     // from the kernels' base-2 scores to natural ones: ln 2, and what rounded off scale2 or cap_x and cap2
     int32_t out_f32;
     int32_t few_rows;  // sequences of at most so many packed rows are kv_decode's
+    int32_t q_mapped;      // kv_prompt: Q comes by its tensor map
     int32_t shared_pass;   // kv_prompt: all rows against the shared prefix, joined with
     const float* own_out;  // what was found over the own keys, [rows][q_heads][D]
     const float* own_lse;  // and its lse; kKvSkipped for rows of skipped sequences
@@ -120,8 +121,10 @@ using KvEncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, v
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 struct KvMaps {
     CUtensorMap k, v;  // the cache as kv_prompt reads it
+    CUtensorMap q;     // and the rows, where `q_mapped`
+    bool q_mapped;
 };
-bool kv_make_maps(KvMaps* maps, const KvCacheView& cache, int head_dim, int dtype, KvEncodeFn encode);
+bool kv_make_maps(KvMaps* maps, const KvAttendParams& p, int head_dim, int dtype, KvEncodeFn encode);
 cudaError_t launch_kv_prompt(const KvAttendParams& p, int head_dim, int dtype, int num_sms, const KvMaps& maps, bool chained, cudaStream_t st);
 cudaError_t launch_kv_decode(const KvAttendParams& p, int head_dim, int dtype, int num_sms, bool chained, cudaStream_t st);
 

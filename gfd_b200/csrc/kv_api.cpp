@@ -230,8 +230,9 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
     KvMaps maps;
     if (plan.many || shared_len > 0) {
         if (encode == nullptr) return set_error(ctx, GFD_ERR_UNSUPPORTED, "%s: the driver has no cuTensorMapEncodeTiled", call);
-        if (!kv_make_maps(&maps, p.cache, c->head_dim, c->dtype, encode))
+        if (!kv_make_maps(&maps, p, c->head_dim, c->dtype, encode))
             return set_error(ctx, GFD_ERR_INVALID, "%s: the cache's shape does not fit a tensor map", call);
+        p.q_mapped = maps.q_mapped;
     }
     KvAttendParams own = p;
     if (shared_len > 0) {

@@ -168,6 +168,15 @@ __device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, i
         "l"(map), "r"(x), "r"(head), "r"(place), "r"(block), "r"(bar)
         : "memory");
 }
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int head, int row, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(head), "r"(row), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_rows_ahead(const CUtensorMap* map, int x, int head, int row) {  // into L2
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"(map), "r"(x), "r"(head), "r"(row) : "memory");
+}
 
 // ---------------------------------------------------------------------------
 // Units
@@ -435,7 +444,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // kShared: the pass over a shared prefix
 template <typename T, int D, bool kPlain, bool kShared>
 __global__ void __launch_bounds__(kThreads, 1)
-    kv_prompt_kernel(const KvAttendParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    kv_prompt_kernel(const KvAttendParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                     const __grid_constant__ CUtensorMap map_q) {
     using S = Shape<D>;
     extern __shared__ char smem_raw[];
     __shared__ Bars bars;
@@ -485,6 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (t == 13 * 32) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+        if (p.q_mapped) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
     }
 
     // ---- this CTA's stretch of the line, its first unit for all roles ----
@@ -579,6 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             p.line.cuts[blockIdx.x] = stretch_end > 0 ? kv_cut(KvCuts(total, gridDim.x), blockIdx.x, s_place) : KvCut{};
     }
     tm_before();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // `first` lay where Q goes
     __syncthreads();
     tm_after();
     const uint32_t tmem = s_tmem;
@@ -1046,13 +1058,43 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         } else if (warp == 14) {
-            // ---- Q: every row by neighbouring lanes, zeros for rows that do not exist ----
+            // ---- Q ----
+            uint32_t phase = 0;  // bit x
+            if (p.q_mapped) {
+                // a box of [64 elements][heads of the group][rows]: packed rows in order.  Rows behind
+                // the sequence's last one bring whatever follows it into rows that nothing is written for.
+                Desc u;
+                bool good = true;
+                while (good && take(&u)) {
+                    const int head = u.h * p.group, row = u.row0 + kv_div_group(p, u.packed0), by = kHalf / p.group;
+                    if (lane < 2 * S::kBlocks && lane / S::kBlocks * kHalf < u.packed)
+                        tma_rows_ahead(&map_q, lane % S::kBlocks * 64, head, row + lane / S::kBlocks * by);
+                    for (int x = 0; good && x * kHalf < u.packed; ++x) {
+                        good = bar_wait(smem_addr(&bars.q_read[x]), ((phase >> x) & 1u) ^ 1u, gave_up);
+                        if (!good) break;
+                        phase ^= 1u << x;
+                        const uint32_t there = smem_addr(&bars.q[x]);
+                        if (lane == 0) bar_expect(there, S::kOperand);
+                        __syncwarp();
+                        if (lane < S::kBlocks)
+                            tma_rows(sq + x * S::kOperand + lane * S::kBlock, &map_q, lane * 64, head, row + x * by, there);
+                    }
+                }
+                if (*gave_up != 0) {
+                    // the copies in flight land before the block ends
+                    for (int x = 0; x < 2; ++x) {
+                        const uint64_t t0 = clock_ns();
+                        while (!bar_try(smem_addr(&bars.q[x]), ((phase >> x) & 1u) ^ 1u) && clock_ns() - t0 < kWaitLimitNs) {
+                        }
+                    }
+                }
+            }
+            // groups and strides that no box has: every row by neighbouring lanes, zeros for rows that do not exist
             constexpr int kLanes = D / 8, kPer = 32 / kLanes;  // lanes of a row, rows a step
             const int ch = lane % kLanes, sub = lane / kLanes;
             const uint32_t to = sq + (ch / 8) * S::kBlock + sub * 128;
-            uint32_t phase = 0;                                // bit x
             Desc u;
-            bool good = true;
+            bool good = !p.q_mapped;
             while (good && take(&u)) {
                 // where the unit's rows lie, and a start on bringing them into L2
                 __syncwarp();
@@ -1127,12 +1169,27 @@ bool make_map(CUtensorMap* map, const KvCacheView& c, const char* base, int head
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Q as [rows][heads][D], read in boxes of 128 packed rows x 64 elements.  Not where a group's heads do
+// not divide 128, nor with strides that no map takes (rows or heads that are one and the same, say).
+bool make_rows_map(CUtensorMap* map, const KvAttendParams& p, int head_dim, int dtype, KvEncodeFn encode) {
+    const cuuint64_t row = static_cast<cuuint64_t>(head_dim) * 2;
+    if (p.group > kHalf || kHalf % p.group != 0 || (p.q_heads > 1 && p.q.head_stride == 0) || (p.batch.rows > 1 && p.q.row_stride == 0))
+        return false;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(p.q_heads), static_cast<cuuint64_t>(p.batch.rows)};
+    const cuuint64_t strides[2] = {p.q_heads > 1 ? static_cast<cuuint64_t>(p.q.head_stride) : row,
+                                   p.batch.rows > 1 ? static_cast<cuuint64_t>(p.q.row_stride) : row};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(kHalf / p.group)}, ones[3] = {1, 1, 1};
+    return encode(map, dtype == GFD_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p.q.data, dims, strides, box,
+                  ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D>
 cudaError_t launch(const KvAttendParams& p, const KvMaps& maps, int ctas, bool chained, cudaStream_t st) {
     const bool plain = p.softcap == 0.0f && p.alibi == nullptr && p.scale2 > 0.0f;
     auto* f = p.shared_pass ? (plain ? kv_prompt_kernel<T, D, true, true> : kv_prompt_kernel<T, D, false, true>)
                             : (plain ? kv_prompt_kernel<T, D, true, false> : kv_prompt_kernel<T, D, false, false>);
-    const cudaError_t e = kv_launch(f, dim3(ctas), kThreads, Shape<D>::kSmem, st, chained, p, maps.k, maps.v);
+    const cudaError_t e = kv_launch(f, dim3(ctas), kThreads, Shape<D>::kSmem, st, chained, p, maps.k, maps.v, maps.q);
     if (e != cudaSuccess) return e;
     return launch_kv_join_many(p, D, std::is_same<T, __half>::value ? GFD_FP16 : GFD_BF16, ctas, st);
 }
@@ -1141,8 +1198,10 @@ cudaError_t launch(const KvAttendParams& p, const KvMaps& maps, int ctas, bool c
 
 int kv_prompt_ctas(int num_sms) { return num_sms; }
 
-bool kv_make_maps(KvMaps* maps, const KvCacheView& cache, int head_dim, int dtype, KvEncodeFn encode) {
-    return make_map(&maps->k, cache, cache.k, head_dim, dtype, encode) && make_map(&maps->v, cache, cache.v, head_dim, dtype, encode);
+bool kv_make_maps(KvMaps* maps, const KvAttendParams& p, int head_dim, int dtype, KvEncodeFn encode) {
+    *maps = KvMaps{};
+    maps->q_mapped = make_rows_map(&maps->q, p, head_dim, dtype, encode);
+    return make_map(&maps->k, p.cache, p.cache.k, head_dim, dtype, encode) && make_map(&maps->v, p.cache, p.cache.v, head_dim, dtype, encode);
 }
 
 cudaError_t launch_kv_prompt(const KvAttendParams& p, int head_dim, int dtype, int num_sms, const KvMaps& maps, bool chained, cudaStream_t st) {
