@@ -34,7 +34,6 @@ constexpr int kTile = 128;          // keys of a step
 constexpr int kPages = kTile / kKvPage;
 constexpr int kThreads = 512;
 constexpr int kAux = 80, kMain = 176;  // registers of the helpers' and the softmax warps: 256 x (80 + 176) = 64 K
-constexpr int kStageBytes = 32 * 64; // a softmax warp's room for results on their way out
 // On the line every unit is as much longer than its tiles: what beginning and finishing one costs.
 constexpr int kUnitCost = 3;
 constexpr int kBadRing = 8;         // tiles whose bad pages are remembered
@@ -167,6 +166,17 @@ __device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, i
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
         "l"(map), "r"(x), "r"(head), "r"(place), "r"(block), "r"(bar)
         : "memory");
+}
+// 32 bytes; `wide`: both ends of them on 32
+__device__ __forceinline__ void store8(uint64_t to, const uint32_t* r, bool wide) {
+    if (wide) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+                     "r"(r[5]), "r"(r[6]), "r"(r[7])
+                     : "memory");
+    } else {
+        *reinterpret_cast<uint4*>(to) = make_uint4(r[0], r[1], r[2], r[3]);
+        *reinterpret_cast<uint4*>(to + 16) = make_uint4(r[4], r[5], r[6], r[7]);
+    }
 }
 __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int x, int head, int row, uint32_t bar) {
     asm volatile(
@@ -349,7 +359,7 @@ struct Shape {
     static constexpr int kOperand = kHalf * D * 2;        // bytes of Q of a half, K or V of a tile
     static constexpr int kBlock = kHalf * 128;            // bytes of a 64-element block of one
     static constexpr int kSlots = 4;                      // K and V tiles in flight
-    static constexpr int kSmem = 2 * kOperand + kSlots * kOperand + 4 * kStageBytes + 1024;
+    static constexpr int kSmem = 2 * kOperand + kSlots * kOperand + 1024;
     static constexpr uint32_t kColumns = 512;             // S, S, O, O
     static constexpr uint32_t kO = 256;                   // O of half A
 };
@@ -752,7 +762,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp < 12) {
             // ---- finished rows ----
             const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-            const uint32_t stage = sq + (2 + S::kSlots) * S::kOperand + (warp & 3) * kStageBytes;
+            // rows that begin on 32 bytes are written 32 bytes at a time
+            const bool wide = ((reinterpret_cast<uint64_t>(p.out.data) | p.out.row_stride | p.out.head_stride) & 31) == 0;
             uint32_t o_phase = 0;  // bit x
             bool good = true;
             if (kShared) kv_wait_last();  // the results over the own keys, which finish here
@@ -782,7 +793,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float base = s_base[x][rr], l = s_sum[x][rr];
                     __syncwarp();
                     if (lane == 0) bar_arrive(smem_addr(&bars.ml_read[x]));
-                    float odd = 0.0f;                // NaN once a sum is not finite
+                    uint64_t odd0 = 0, odd1 = 0;      // pairs of 0.0f, NaN once a sum is not finite
                     KvFinish f{1.0f, 0.0f, base, l};  // what becomes of the sums
                     const float* own = nullptr;
                     if (whole) {
@@ -799,11 +810,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                             __syncwarp();
                             if (lane == 0) bar_arrive(smem_addr(&bars.o_read[x]));
                         }
+                        const uint64_t by = pack2(f.scale, f.scale);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const float v = __uint_as_float(o[e]);
-                            odd = fmaf(v, 0.0f, odd);
-                            o[e] = __float_as_uint(v * f.scale);
+                        for (int e = 0; e < 32; e += 2) {
+                            const uint64_t v = pack2(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
+                            uint64_t& odd = e & 2 ? odd1 : odd0;
+                            odd = fma2(v, 0, odd);
+                            float a, c;
+                            unpack2(mul2(v, by), a, c);
+                            o[e] = __float_as_uint(a);
+                            o[e + 1] = __float_as_uint(c);
                         }
                         if (!whole) {
                             // partial sums: 4 elements of 32 rows side by side
@@ -823,34 +839,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 o[e + 2] = __float_as_uint(fmaf(y.z, f.own, __uint_as_float(o[e + 2])));
                                 o[e + 3] = __float_as_uint(fmaf(y.w, f.own, __uint_as_float(o[e + 3])));
                             }
-                        // 64 bytes of every row at a time through shared memory, so that 4 lanes write
-                        // them side by side
-                        if (!p.out_f32)
+                        if (dst == 0) continue;
+                        if (p.out_f32) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8) store8(dst + 4 * (k + e), o + e, wide);
+                        } else {
 #pragma unroll
                             for (int e = 0; e < 16; ++e) o[e] = Pack<T>::pair(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
-                        for (int st = 0; st < (p.out_f32 ? 2 : 1); ++st) {
-#pragma unroll
-                            for (int y = 0; y < 4; ++y) {
-                                const uint32_t* w = o + 4 * y;
-                                const bool up = st == 1;
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((y ^ ((lane >> 1) & 3)) << 4)),
-                                             "r"(up ? w[16] : w[0]), "r"(up ? w[17] : w[1]), "r"(up ? w[18] : w[2]), "r"(up ? w[19] : w[3])
-                                             : "memory");
-                            }
-                            __syncwarp();
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int rw = lane / 4 + 8 * i;
-                                uint4 v;
-                                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                             : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                                             : "r"(stage + rw * 64 + (((lane & 3) ^ ((rw >> 1) & 3)) << 4))
-                                             : "memory");
-                                const uint64_t to_row = __shfl_sync(0xffffffffu, dst, rw);
-                                if (to_row != 0)
-                                    *reinterpret_cast<uint4*>(to_row + (p.out_f32 ? 4 : 2) * k + 64 * st + 16 * (lane & 3)) = v;
-                            }
-                            __syncwarp();
+                            store8(dst + 2 * k, o, wide);
+                            store8(dst + 2 * k + 32, o + 8, wide);
                         }
                     }
                     if (valid) {
@@ -861,6 +858,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                             slot[static_cast<int64_t>(kRows) * D + kRows + r] = l;
                         }
                     }
+                    float odd, odd_c;
+                    unpack2(add2(odd0, odd1), odd, odd_c);
+                    odd += odd_c;
                     // (a weight sum that is not finite makes the row NaN as it is)
                     uint32_t redo = __ballot_sync(0xffffffffu, valid && odd != 0.0f && l < INFINITY);
                     KvExact y;
