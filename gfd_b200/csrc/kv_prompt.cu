@@ -34,8 +34,9 @@ constexpr int kTile = 128;          // keys of a step
 constexpr int kPages = kTile / kKvPage;
 constexpr int kThreads = 512;
 constexpr int kAux = 80, kMain = 176;  // registers of the helpers' and the softmax warps: 256 x (80 + 176) = 64 K
-// On the line every unit is as much longer than its tiles: what beginning and finishing one costs.
-constexpr int kUnitCost = 3;
+// On the line every unit is as much longer than its tiles: what beginning and finishing one costs
+// (1 to 3 come out alike within 2 %, 5 and 8 slower).
+constexpr int kUnitCost = 2;
 constexpr int kBadRing = 8;         // tiles whose bad pages are remembered
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
