@@ -271,7 +271,6 @@ int merge(gfd_ctx* ctx, const gfd_kv_merge_args* a, void* stream) {
     const char* why = kv_check_merge(*a);
     if (!why && a->rows > 0) why = kv_check_rows(a->parts, a->rows, a->heads, a->head_dim, a->part_dtype, false, &pb);
     if (!why && a->rows > 0) why = kv_check_rows(a->out, a->rows, a->heads, a->head_dim, a->out_dtype, true, &ob);
-    if (!why && a->part_count > 1 && a->part_stride > (1ll << 40)) why = "part_stride is too large";
     if (why) return set_error(ctx, GFD_ERR_INVALID, "kv_merge: %s", why);
     if (a->rows == 0) return GFD_OK;
     pb += static_cast<uint64_t>(a->part_count - 1) * a->part_stride * kv_elt(a->part_dtype);

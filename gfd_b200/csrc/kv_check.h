@@ -80,15 +80,15 @@ GFD_HD KvTiles kv_tiles(KvSpan s, int32_t size) {
     return t;
 }
 
-// All tiles of a launch form one line, unit after unit; stretch c is [at(c), at(c + 1)), at least one
-// tile each, n() of them.  A unit inside one stretch is finished there.  One that is cut leaves
-// partial results, one in each stretch it touches, in slot 1 of the one where it begins and slot 0
-// of the others; they are joined at the first cut inside the unit.
 // a / b for a >= 0, b > 0; the 64-bit division costs several times the 32-bit one.
 GFD_HD int64_t kv_div(int64_t a, int64_t b) {
     return ((a | b) >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
 }
 
+// All tiles of a launch form one line, unit after unit; stretch c is [at(c), at(c + 1)), at least one
+// tile each, n() of them.  A unit inside one stretch is finished there.  One that is cut leaves
+// partial results, one in each stretch it touches, in slot 1 of the one where it begins and slot 0
+// of the others; they are joined at the first cut inside the unit.
 struct KvCuts {
     int64_t each;
     uint32_t more, ctas;
@@ -213,7 +213,7 @@ inline const char* kv_check_attend(const gfd_kv_attend_args& a, const gfd_kv_cac
     if (!std::isfinite(a.scale)) return "scale is not finite";
     if (!std::isfinite(a.softcap) || a.softcap < 0.0f) return "softcap must be finite and not negative";
     if (a.softcap > 0.0f && (!std::isfinite(a.scale / a.softcap) || a.softcap > 1e30f)) return "softcap is out of range";
-    if (a.q.data == a.out.data) return "out must not be q";
+    if (a.q.data == a.out.data && a.q.data != nullptr) return "out must not be q";  // (no rows, no pointers)
     if (!kv_aligned(a.lse, 4) || !kv_aligned(a.alibi, 4) || !kv_aligned(a.prefix_len, 4) || !kv_aligned(a.status, 4))
         return "lse, alibi, prefix_len or status is not 4-byte aligned";
     return nullptr;
@@ -227,6 +227,7 @@ inline const char* kv_check_merge(const gfd_kv_merge_args& a) {
     for (int32_t t : {a.part_dtype, a.out_dtype})
         if (t != GFD_BF16 && t != GFD_FP16 && t != GFD_FP32) return "unknown type";
     if (a.part_stride < 0 || a.part_stride % 8 != 0) return "part_stride must be a multiple of 8, not negative";
+    if (a.part_count > 1 && a.part_stride > (1ll << 40)) return "part_stride is too large";
     if ((a.rows > 0 && a.part_lse == nullptr) || !kv_aligned(a.part_lse, 4) || !kv_aligned(a.lse, 4)) return "part_lse is NULL, or part_lse or lse not 4-byte aligned";
     if (a.rows > 0)
         for (int i = 0; i < a.part_count; ++i)

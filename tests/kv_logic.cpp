@@ -25,6 +25,18 @@ int gfdt_kv_seq(int32_t start, int32_t end, int32_t len, int64_t capacity, int32
     out[0] = q.row0, out[1] = q.rows, out[2] = q.keys;
     return q.ok;
 }
+void gfdt_kv_tiles(const int32_t* span, int32_t base, int32_t len, int32_t size, int32_t* out) {
+    const KvTiles t = kv_tiles(kv_clip(KvSpan{span[0], span[1], span[2]}, base, len), size);
+    out[0] = t.npre, out[1] = t.first, out[2] = t.count;
+}
+// at(0) .. at(n), n returned
+int gfdt_kv_cuts(int64_t total, uint32_t most, int64_t* at) {
+    const KvCuts c(total, most);
+    for (int i = 0; i <= c.n() && c.n() > 0; ++i) at[i] = c.at(i);
+    return c.n();
+}
+uint32_t gfdt_kv_last_before(int64_t total, uint32_t most, uint32_t c, int64_t end) { return KvCuts(total, most).last_before(c, end); }
+int64_t gfdt_kv_div(int64_t a, int64_t b) { return kv_div(a, b); }
 // sizes and last offsets of the argument structures
 void gfdt_kv_layout(uint64_t* out) {
     const uint64_t v[] = {sizeof(gfd_kv_cache),       offsetof(gfd_kv_cache, dtype),

@@ -253,3 +253,77 @@ def test_block_entries():
     c = kv.PagedCache(None, apart[0].transpose(1, 2), apart[1].transpose(1, 2))
     with pytest.raises(ValueError):
         c.fetch(0, [0], [0])
+
+
+def test_tiles_hold_every_visible_key_and_no_other(lib):
+    """Against a walk over keys: tiles with a key of [0, pre) or of [lo, hi), each once, in order."""
+    rng = np.random.default_rng(5)
+    lib.gfdt_kv_tiles.argtypes = [_VP, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _VP]
+    cases = [(0, 0, 0, 0, 0), (0, 0, 1, 0, 1), (5, 5, 5, 0, 9), (3, 700, 701, 0, 701), (16, 16, 32, 16, 16), (900, 900, 900, 128, 400)]
+    for _ in range(400):
+        pre, lo, n = sorted(rng.integers(0, 700, 3).tolist())
+        cases.append((pre, lo, int(rng.integers(lo, 701)), int(rng.integers(0, 300)), int(rng.integers(0, 500))))
+    for pre, lo, hi, base, length in cases:
+        for size in (16, 128):
+            span, out = (ctypes.c_int32 * 3)(pre, lo, hi), (ctypes.c_int32 * 3)()
+            lib.gfdt_kv_tiles(span, base, length, size, out)
+            npre, first, count = out
+            got = [i if i < npre else i - npre + first for i in range(count)]
+            keys = [j - base for j in range(base, base + length) if j < pre or lo <= j < hi]
+            assert got == sorted({j // size for j in keys}), (pre, lo, hi, base, length, size)
+
+
+def test_cuts_share_the_line_evenly(lib):
+    lib.gfdt_kv_cuts.argtypes = [ctypes.c_int64, ctypes.c_uint32, _VP]
+    lib.gfdt_kv_last_before.argtypes = [ctypes.c_int64, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_int64]
+    lib.gfdt_kv_last_before.restype = ctypes.c_uint32
+    lib.gfdt_kv_div.argtypes, lib.gfdt_kv_div.restype = [ctypes.c_int64] * 2, ctypes.c_int64
+    rng = np.random.default_rng(6)
+    at = (ctypes.c_int64 * 2049)()
+    assert lib.gfdt_kv_cuts(0, 148, at) == 0
+    for total, most in [(1, 148), (147, 148), (148, 148), (149, 148), (2 ** 40 + 7, 1776), (2 ** 31, 2048), (2 ** 33 - 1, 1184)] + \
+            [(int(rng.integers(1, 5000)), int(rng.integers(1, 2048))) for _ in range(200)]:
+        n = lib.gfdt_kv_cuts(total, most, at)
+        a = list(at[:n + 1])
+        sizes = np.diff(a)
+        assert n == min(total, most) and a[0] == 0 and a[n] == total and sizes.min() >= 1 and sizes.max() - sizes.min() <= 1
+        for c in {0, n // 3, n - 1}:
+            for end in {a[c] + 1, a[c + 1], a[c + 1] + 1, total, (a[c] + total) // 2 + 1}:
+                want = max(i for i in range(n) if i == c or (i > c and a[i] < end))
+                assert lib.gfdt_kv_last_before(total, most, c, end) == want, (total, most, c, end)
+    for a, b in ((0, 1), (2 ** 32 - 1, 1), (2 ** 32, 3), (2 ** 40 + 1, 2 ** 33), (17, 2 ** 34), (2 ** 62, 7), (2 ** 32 - 1, 2 ** 32 - 1)):
+        assert lib.gfdt_kv_div(a, b) == a // b
+
+
+def test_reciprocals_divide_exactly():
+    """The kernels divide packed rows by the group, and pages by a block's, with a multiplication: the
+    same magic numbers and shifts, at the quotients' edges."""
+    for group in list(range(1, 130)) + [255, 256, 1000, 4095, 8191, 8192]:
+        magic = -(-2 ** 44 // group)
+        for k in (1, 2, 1000, (2 ** 31 - 1) // group):
+            for n in (k * group - 1, k * group, k * group + group - 1):
+                if 0 <= n < 2 ** 31:
+                    assert (n << 20) * magic >> 64 == n // group
+    for pages in range(1, 65):
+        magic = -(-2 ** 32 // pages)
+        for k in (1, 77, (2 ** 26 - 1) // pages):
+            for n in (k * pages - 1, k * pages, k * pages + pages - 1):
+                if 0 <= n < 2 ** 26:
+                    assert n * magic >> 32 == n // pages
+
+
+def test_attend_parameters_out_of_range(lib):
+    c = cache()
+
+    def check(**kw):
+        a = kv._Attend(q_heads=32, scale=0.1, out_dtype=kv.BF16)
+        a.q.data, a.out.data = 1 << 24, 1 << 25
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return lib.gfdt_kv_attend(ctypes.byref(a), ctypes.byref(c))
+    assert check() is None and check(softcap=30.0) is None and check(scale=0.0) is None and check(scale=-1.0) is None
+    no_rows = kv._Attend(q_heads=32, scale=0.1, out_dtype=kv.BF16)  # whose tensors have no address
+    assert lib.gfdt_kv_attend(ctypes.byref(no_rows), ctypes.byref(c)) is None
+    for kw in (dict(q_heads=0), dict(q_heads=12), dict(q_heads=8 * 1024 + 8), dict(scale=float("nan")), dict(scale=float("inf")),
+               dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=float("inf")), dict(window=-1), dict(max_q_len=-1)):
+        assert check(**kw) is not None, kw
