@@ -91,16 +91,6 @@ __device__ __forceinline__ int32_t kv_div_pages(const KvAttendParams& p, int32_t
     return static_cast<int32_t>(static_cast<uint64_t>(n) * p.page_magic >> 32);
 }
 
-// row_start rises from >= 0 to <= rows (every thread of the CTA calls; same answer for all).
-__device__ __forceinline__ bool kv_starts_ok(const KvBatchView& b) {
-    bool bad = false;
-    for (int i = threadIdx.x; i < b.seqs; i += blockDim.x) {
-        const int32_t a = b.row_start[i], e = b.row_start[i + 1];
-        bad |= a < 0 || a > e || e > b.rows;
-    }
-    return __syncthreads_or(bad) == 0;
-}
-
 __device__ __forceinline__ void kv_report(uint32_t* status, uint32_t bits) {
     if (status != nullptr && bits != 0) atomicOr(status, bits);
 }
@@ -115,19 +105,6 @@ __device__ __forceinline__ int32_t kv_block(const KvBatchView& b, int s, int32_t
     }
     *place = j % bt;
     return t[j / bt];
-}
-
-template <typename T>
-__device__ __forceinline__ void kv_store_out(const KvAttendParams& p, int64_t row, int head, int d0, const float* v, int n) {
-    char* at = p.out.data + row * p.out.row_stride + head * p.out.head_stride;
-    if (p.out_f32) {
-        float* o = reinterpret_cast<float*>(at) + d0;
-        for (int i = 0; i < n; i += 4) *reinterpret_cast<float4*>(o + i) = *reinterpret_cast<const float4*>(v + i);
-    } else {
-        uint32_t* o = reinterpret_cast<uint32_t*>(at + 2 * d0);
-        for (int i = 0; i < n; i += 4)
-            *reinterpret_cast<uint2*>(o + i / 2) = make_uint2(Pack<T>::pair(v[i], v[i + 1]), Pack<T>::pair(v[i + 2], v[i + 3]));
-    }
 }
 
 // What CTA c's cut leaves to join, for the CTA whose stretch begins at `at`.

@@ -381,7 +381,6 @@ struct Shift {  // weights reach 2^(shift + 8): fp16 keeps them clear of its sma
 };
 constexpr float kGrow = 8.0f;
 
-
 // Position of row r of the unit and what it sees of this pass's keys; rows that do not exist see
 // everything.  `exact`: the position itself is needed, not only the span.
 template <bool kShared>
@@ -415,6 +414,7 @@ __device__ __forceinline__ KvSpan row_span(const KvAttendParams& p, const Desc& 
 
 // the n lowest bits, n clamped to 0 .. 32
 __device__ __forceinline__ uint32_t below(int32_t n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
+
 // 2^x of both, without the special function unit: 2^n from the exponent's bits, n the nearest whole
 // number, times a polynomial of degree 5 in x - n (least relative error on [-1/2, 1/2], 1 at 0; off by
 // at most 2^-22.5 in 32-bit arithmetic).  Below -126 it falls to 0, and from -127 on, -infinity

@@ -739,3 +739,117 @@ def test_refusals(gpu_ctx):
     assert "out must not be a part" in refused(kv.merge, gpu_ctx, parts, torch.zeros(2, 1, 1, device="cuda"), parts[1])
     torch.cuda.synchronize()
     assert bool((out == 7).all())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,group", [(3, 1), (2, 3), (1, 7), (2, 16), (1, 128), (1, 160)])
+def test_attend_prompt_groups(gpu_ctx, heads, group, d):
+    """Units of 128 packed rows of a half begin inside a token's heads or not, with the next
+    sequence's rows behind the last one: NaN there reaches nothing."""
+    rows = [max(2, 300 // group), 1, max(3, 520 // group + 1)]
+    s = Setup(gpu_ctx, "bf16", heads, group, d, 16, rows, [n + 45 for n in rows], seed=29)
+    s.check()
+    s.q[rows[0]:] = float("nan")
+    got, lse = s.attend()
+    torch_().cuda.synchronize()
+    assert bool(torch_().isnan(got[rows[0]:].float()).all())
+    s.q[rows[0]:] = 0
+    oracle.check_attend(got, lse, s.want(), slice(0, rows[0]))
+
+
+@pytest.mark.parametrize("kind", ["heads_first", "broadcast_rows", "broadcast_heads", "gap"])
+def test_attend_prompt_q_strides(gpu_ctx, kind):
+    torch = torch_()
+    s = Setup(gpu_ctx, "fp16", 2, 4, 128, 16, [200, 70], [300, 70], seed=31)
+    n, h = s.q.shape[:2]
+    if kind == "heads_first":
+        q = s.normal(h, n, 128).transpose(0, 1)
+    elif kind == "broadcast_rows":
+        q = s.normal(1, h, 128).expand(n, h, 128)
+    elif kind == "broadcast_heads":
+        q = s.normal(n, 1, 128).expand(n, h, 128)
+    else:
+        q = s.normal(n, h + 1, 136)[:, 1:, 8:]
+    got, lse = s.attend(q=q)
+    torch.cuda.synchronize()
+    oracle.check_attend(got, lse, s.want(q=q))
+
+
+@pytest.mark.parametrize("out_dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_prompt_rows_off_32_bytes(gpu_ctx, d, out_dtype):
+    """Result rows that begin on 16 bytes and not on 32."""
+    torch = torch_()
+    s = Setup(gpu_ctx, "bf16", 2, 4, d, 32, [150, 20], [150, 333], seed=37)
+    e = 4 if out_dtype == "fp32" else 8
+    big = torch.full((s.rows, s.hq, d + 2 * e), 7.0, device="cuda", dtype=types()[out_dtype])
+    out = big[:, :, e:e + d]
+    assert out.data_ptr() % 32 == 16
+    got, lse = s.attend(out=out)
+    torch.cuda.synchronize()
+    oracle.check_attend(got, lse, s.want())
+    assert bool((big[:, :, :e] == 7).all()) and bool((big[:, :, e + d:] == 7).all())
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 4], [700, 40]), ([130, 60], [400, 60])])
+def test_attend_cap_of_large_scores(gpu_ctx, q_lens, kv_lens):
+    """Scores far above the cap next to ones below it."""
+    s = Setup(gpu_ctx, "bf16", 2, 4, 64, 16, q_lens, kv_lens, seed=41)
+    s.q[:, ::2] *= 6
+    s.check(softcap=2.0)
+    s.check(softcap=500.0, scale=-0.25)
+
+
+def test_attend_padded_batch(gpu_ctx):
+    """Empty sequences before, between and behind, whatever their lengths and tables say, and rows of none."""
+    torch = torch_()
+    q_lens, kv_lens = [0, 90, 0, 0, 1, 0, 3, 0], [0, 90, 0, 0, 50, 0, 64, 0]
+    s = Setup(gpu_ctx, "bf16", 2, 4, 128, 16, q_lens, kv_lens, seed=43, spare_rows=9)
+    empty = [i for i, n in enumerate(q_lens) if n == 0]
+    s.lens[empty] = torch.tensor([0, -5, 10 ** 9, 7, 1], dtype=torch.int32, device="cuda")
+    s.table[empty] = -1
+    s.check()
+    none = kv.Batch(torch.zeros(1, dtype=torch.int32, device="cuda"), s.lens[:0], s.table[:0])
+    out = torch.full_like(s.q, 7.0)
+    s.cache.attend(none, s.q, out, workspace=s.workspace(), status=s.status)
+    s.cache.attend(s.batch, s.q[:0], out[:0], workspace=s.workspace(), status=s.status)
+    torch.cuda.synchronize()
+    assert bool((out == 7).all()) and int(s.status) in (0, kv.BAD_LENGTH)
+
+
+def test_attend_4096_sequences(gpu_ctx):
+    rng = np.random.default_rng(47)
+    q_lens = [int(x) for x in rng.integers(0, 3, 4096)]
+    q_lens[1000], q_lens[4095] = 70, 33
+    s = Setup(gpu_ctx, "fp16", 1, 2, 64, 16, q_lens, [n + int(x) for n, x in zip(q_lens, rng.integers(0, 30, 4096))], seed=47)
+    s.check()
+
+
+def test_shared_on_two_streams_and_in_a_graph(gpu_ctx):
+    """Two calls at once, each with its workspace, and one replayed behind a changed prefix."""
+    torch = torch_()
+    a = Setup(gpu_ctx, "bf16", 2, 4, 128, 16, [1, 5, 1], [9, 70, 33], seed=53, shared_len=500)
+    b = Setup(gpu_ctx, "bf16", 2, 4, 128, 16, [40, 2], [60, 2], seed=54, shared_len=260)
+    st = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    res = []
+    for _ in range(20):
+        res = []
+        for s, x in zip((a, b), st):
+            with torch.cuda.stream(x):  # the results and workspaces are filled there too
+                res.append(s.attend())
+    torch.cuda.synchronize()
+    for s, (out, lse) in zip((a, b), res):
+        oracle.check_attend(out, lse, s.want())
+    out, lse, ws = torch.empty_like(a.q), torch.empty(a.rows, a.hq, device="cuda"), a.workspace(5)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        a.cache.attend_shared(a.batch, a.shared_table, a.shared_len, a.q, out, lse=lse, max_q_len=5, workspace=ws, status=a.status,
+                              stream=torch.cuda.current_stream())
+    a.q.normal_(generator=a.gen)
+    a.shared_table[:] = a.shared_table.flip(0)
+    a.lens[1] = a.kv_lens[1] = 12
+    g.replay()
+    torch.cuda.synchronize()
+    oracle.check_attend(out, lse, a.want())
+    assert int(a.status) == 0
