@@ -12,6 +12,11 @@
 // 192 KB in flight on an SM; block ids fetched 32 stages at a time), its own running maximum and
 // sum, scores and sums by mma.m16n8k16 from ldmatrix fragments, and writes its rows from
 // registers.  After the stretches are found there is no barrier.
+//
+// Measured: 64 sequences of up to 8192 tokens, 8 heads of 128, in 170 us with their join, 6.0 TB/s; two of
+// 131 thousand, 24 query heads of 64 behind a cap, in 102 us, 5.0 TB/s (there 12 rows' scores and the cap's
+// polynomial fill half of the issue slots).  128 elements a head take 252 registers, two CTAs an SM; 64 take
+// 168, and the third is worth 123 -> 102 us.
 
 #include <type_traits>
 

@@ -12,10 +12,16 @@
 // the weights are at most 2^8 and the sums stay in tensor memory untouched, so the rescaling
 // of O is rare.  Sums and maxima are 32-bit; the weights' rounding to the 16-bit type for the
 // second product is the only one before the result's.
+// With 128 elements a head the softmax between the two products bounds a tile (the tensor pipe is
+// active 58 % of the time, both halves' 256 exponentials a key take as long as their products): 881 us for
+// 8192 rows on 8192 keys and 32 heads, 1248 TFLOP/s, 484 us causal.  With 64 the special function unit
+// alone does: 715 us, 770 TFLOP/s.  Short units wait for O to be written before the next one's sums begin:
+// 16 prompts of 512 rows take 96 us, 716 TFLOP/s.
 //
 // Roles: warps 0-3 softmax of half A, 4-7 of half B; 8-11 write finished rows while the softmax
 // is in the next unit; 12 issues the products, 13 loads K and V (TMA boxes of 16 tokens x 64
-// elements, so that every page is found by its id), 14 loads Q, 15 walks the units.  Units lie
+// elements, so that every page is found by its id), 14 loads Q (a box of the group's heads x rows where
+// the heads divide 128), 15 walks the units.  Units lie
 // on one line of tiles that the CTAs (one per SM) share evenly; a cut unit leaves partial sums
 // for kv_join_many_kernel, as in kv_decode.cu.
 
