@@ -234,33 +234,39 @@ struct KvExact {
 
 // Which rows (a lane each, bits of `odd`: their sums by matrix products are not finite) have to be summed
 // key by key: those with an element that is NaN or infinite in values which the row does not see
-// (0 * inf and 0 * NaN reached the sum) and in none that it sees.  Everything else is as it should be: a
-// seen NaN, or an overflow.  A row that sees such values in every element needs no further search.
+// (0 * inf and 0 * NaN reached the sum), unless the values that it sees make that element NaN by themselves: a
+// NaN among them, or infinities of both signs.  (One infinity, or several of one sign, is a result of its own,
+// which a masked value must not turn into NaN.)  A row that is NaN in every element needs no further search.
 // keys: of the sequence; x.seen: of this lane's row.
 template <typename T, int D>
 __device__ __forceinline__ uint32_t kv_to_redo(const KvAttendParams& p, const KvExact& x, int32_t keys, uint32_t odd) {
     constexpr uint32_t kMax = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;  // exponent of NaN and infinity
     constexpr int kWords = D / 32;
     const int lane = threadIdx.x & 31;
-    uint32_t in[kWords] = {}, out[kWords] = {};  // a bit an element: bad among seen values, among the others
+    // a bit an element: infinities of one sign and the other among seen values (a NaN counts as both), any of
+    // them among the others
+    uint32_t plus[kWords] = {}, minus[kWords] = {}, out[kWords] = {};
     for (int t = x.t0; t < x.t1; ++t)
         for (int c = 0; c < x.size; c += 32) {
             const int32_t j = x.tiles.at(t) * x.size + c + lane;
-            uint32_t bad[kWords] = {}, any = 0;
+            uint32_t up[kWords] = {}, down[kWords] = {}, any = 0;
             if (c + lane < x.size && j < keys) {
                 const int32_t id = x.table[j / p.cache.block_tokens];
                 if (id >= 0 && id < p.cache.blocks) {
                     const char* v = p.cache.v + id * p.cache.block_stride + j % p.cache.block_tokens * p.cache.token_stride +
                                     x.kvh * p.cache.head_stride;
 #pragma unroll
-                    for (int e = 0; e < D; e += 8) {
-                        const uint4 q = *reinterpret_cast<const uint4*>(v + 2 * e);
-                        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-                        for (int y = 0; y < 4; ++y) {
-                            if ((w[y] & kMax) == kMax) bad[e / 32] |= 1u << (e % 32 + 2 * y);
-                            if ((w[y] >> 16 & kMax) == kMax) bad[e / 32] |= 2u << (e % 32 + 2 * y);
+                    for (int e = 0; e < D; e += 2) {
+                        const uint32_t w = *reinterpret_cast<const uint32_t*>(v + 2 * e);
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            const uint32_t h = w >> (16 * y) & 0xffffu, bit = 1u << (e % 32 + y);
+                            if ((h & kMax) != kMax) continue;
+                            const bool nan = (h & 0x7fffu) != kMax;
+                            if (nan || h == kMax) up[e / 32] |= bit;
+                            if (nan || h != kMax) down[e / 32] |= bit;
                         }
-                        any |= bad[e / 32];
+                        any |= up[e / 32] | down[e / 32];
                     }
                 }
             }
@@ -271,10 +277,11 @@ __device__ __forceinline__ uint32_t kv_to_redo(const KvAttendParams& p, const Kv
                 uint32_t all = 0xffffffffu;
 #pragma unroll
                 for (int i = 0; i < kWords; ++i) {
-                    const uint32_t w = __shfl_sync(0xffffffffu, bad[i], src);
-                    in[i] |= sees ? w : 0u;
-                    out[i] |= sees ? 0u : w;
-                    all &= in[i];
+                    const uint32_t u = __shfl_sync(0xffffffffu, up[i], src), d = __shfl_sync(0xffffffffu, down[i], src);
+                    plus[i] |= sees ? u : 0u;
+                    minus[i] |= sees ? d : 0u;
+                    out[i] |= sees ? 0u : u | d;
+                    all &= plus[i] & minus[i];
                 }
                 odd &= __ballot_sync(0xffffffffu, all != 0xffffffffu);
                 if (odd == 0) return 0;
@@ -282,7 +289,7 @@ __device__ __forceinline__ uint32_t kv_to_redo(const KvAttendParams& p, const Kv
         }
     uint32_t hit = 0;
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) hit |= out[i] & ~in[i];
+    for (int i = 0; i < kWords; ++i) hit |= out[i] & ~(plus[i] & minus[i]);
     return odd & __ballot_sync(0xffffffffu, hit != 0);
 }
 

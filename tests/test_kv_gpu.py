@@ -853,3 +853,74 @@ def test_shared_on_two_streams_and_in_a_graph(gpu_ctx):
     torch.cuda.synchronize()
     oracle.check_attend(out, lse, a.want())
     assert int(a.status) == 0
+
+
+def put(s, i, j, e, value):
+    """V of key j of sequence i, element(s) e of every head."""
+    bt = s.k.shape[1]
+    s.v[int(s.table[i, j // bt]), j % bt, :, e] = value
+
+
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.mark.parametrize("seen", [INF, -INF])
+@pytest.mark.parametrize("masked", [NAN, INF, -INF])
+@pytest.mark.parametrize("dtype,d,q_lens,kv_lens", [("bf16", 64, [4], [45]), ("fp16", 128, [3], [500]), ("fp16", 64, [150], [200]),
+                                                    ("bf16", 128, [70], [1000])])
+def test_attend_seen_infinity_beside_a_masked_value(gpu_ctx, dtype, d, q_lens, kv_lens, seen, masked):
+    """An infinity that a row sees is its result in that element, whatever the same element of a masked key holds."""
+    torch = torch_()
+    s = Setup(gpu_ctx, dtype, 2, 4, d, 16, q_lens, kv_lens, seed=61)
+    want = s.want()
+    n, keys = q_lens[0], kv_lens[0]
+    put(s, 0, keys - n, 9, seen)          # every row sees it
+    put(s, 0, keys - 1, 9, masked)        # the last row alone sees this one
+    put(s, 0, keys - n // 2, 33, -seen)   # the rows of the first half do not see this one
+    put(s, 0, keys - 1, 33, masked)
+    put(s, 0, keys - n, d - 1, seen)      # NaN by what every row sees
+    put(s, 0, keys - n, d - 2, NAN)
+    put(s, 0, max(0, keys - n - 1), d - 1, -seen)
+    put(s, 0, keys - 1, d - 1, masked)
+    got, lse = s.attend()
+    torch.cuda.synchronize()
+    assert int(s.status) == 0
+    rows = list(range(n - 1))             # all but the last
+    g = got.float()
+    assert bool((g[rows, :, 9] == seen).all())
+    last = seen if masked == seen else NAN
+    assert bool((g[n - 1, :, 9] == last).all() if last == seen else torch.isnan(g[n - 1, :, 9]).all())
+    half = [r for r in rows if r >= n - n // 2]  # row i stands at keys - n + i
+    assert bool((g[half, :, 33] == -seen).all())
+    assert bool(torch.isnan(g[:, :, d - 2:]).all())
+    keep = [e for e in range(d) if e not in (9, 33, d - 1, d - 2)]
+    oracle.check_attend(got[:, :, keep], lse, tuple(x[:, :, keep] if x.dim() == 3 else x for x in want))
+    before = [r for r in rows if r < n - n // 2]
+    oracle.check_attend(got[:, :, 33:34], lse, tuple(x[:, :, 33:34] if x.dim() == 3 else x for x in want), before)
+
+
+@pytest.mark.parametrize("masked", [NAN, INF, -INF])
+@pytest.mark.parametrize("d,q_lens", [(64, [2, 5, 1]), (128, [2, 130, 3])])
+def test_shared_seen_infinity_beside_a_masked_value(gpu_ctx, d, q_lens, masked):
+    """The same in a shared prefix: a window hides its first keys from some rows only."""
+    torch = torch_()
+    kv_lens = [n + 7 for n in q_lens]
+    s = Setup(gpu_ctx, "bf16", 2, 4, d, 16, q_lens, kv_lens, seed=62, shared_len=200)
+    window = 60  # both values in the same keys of a tile
+    want = s.want(window=window)
+    first = [200 + n - m + i - window + 1 for n, m in zip(kv_lens, q_lens) for i in range(m)]  # first key each row sees
+    at = int(s.shared_table[199 // 16])
+    s.v[at, 199 % 16, :, 9] = INF                         # seen by all rows whose window reaches back so far
+    j = min(first)                                        # seen by the row that sees furthest back
+    s.v[int(s.shared_table[j // 16]), j % 16, :, 9] = masked
+    got, lse = s.attend(window=window)
+    torch.cuda.synchronize()
+    assert int(s.status) == 0
+    g = got.float()
+    sees = [r for r, f in enumerate(first) if j < f <= 199]
+    none = [r for r, f in enumerate(first) if f > 199]
+    assert sees and bool((g[sees, :, 9] == INF).all())
+    keep = [e for e in range(d) if e != 9]
+    oracle.check_attend(got[:, :, keep], lse, tuple(x[:, :, keep] if x.dim() == 3 else x for x in want))
+    if none:
+        oracle.check_attend(got, lse, want, none)
