@@ -503,6 +503,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) kv_decode_kernel(const Kv
                 y.seen = sp[x];
                 redo = kv_to_redo<T, D>(p, y, use.q.q.keys, redo);
             }
+            // (other lanes write those rows again, behind the ordinary stores)
+            __syncwarp();
             while (redo != 0) {
                 const int src = (__ffs(redo) - 1) & ~3;  // the row's first lane
                 redo &= ~(15u << src);

@@ -882,6 +882,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         y.seen = row_span<kShared>(p, u, r, &y.pos, true);
                         redo = kv_to_redo<T, D>(p, y, u.keys, redo);
                     }
+                    // (other lanes write those rows again, behind the ordinary stores)
+                    __syncwarp();
                     for (; redo != 0; redo &= redo - 1) {
                         const int src = __ffs(redo) - 1;
                         const int rs = x * kHalf + (warp & 3) * 32 + src;

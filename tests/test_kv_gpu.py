@@ -924,3 +924,25 @@ def test_shared_seen_infinity_beside_a_masked_value(gpu_ctx, d, q_lens, masked):
     oracle.check_attend(got[:, :, keep], lse, tuple(x[:, :, keep] if x.dim() == 3 else x for x in want))
     if none:
         oracle.check_attend(got, lse, want, none)
+
+
+@pytest.mark.parametrize("out_dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("d,q_lens,kv_lens", [(64, [4, 3], [60, 900]), (128, [3, 4], [2000, 21]), (64, [90, 2], [300, 33]),
+                                              (128, [130], [3000])])
+def test_attend_rows_summed_again_replace_the_first_sums(gpu_ctx, d, q_lens, kv_lens, out_dtype):
+    """Rows that a masked NaN reached are written twice; the second time is what stays, call after call."""
+    torch = torch_()
+    s = Setup(gpu_ctx, "bf16", 2, 4, d, 16, q_lens, kv_lens, seed=63)
+    want = s.want()
+    ends = [b - 1 for b in s.row_start[1:]]
+    for i, n in enumerate(kv_lens):
+        put(s, i, n - 1, slice(None), NAN)  # the last row of each sequence alone sees it
+    rows = [r for r in range(s.rows) if r not in ends]
+    first = None
+    for _ in range(30):
+        got, lse = s.attend(out_dtype=out_dtype)
+        torch.cuda.synchronize()
+        first = got.clone() if first is None else first
+        assert torch.equal(got[rows], first[rows])
+    oracle.check_attend(got, lse, want, rows)
+    assert bool(torch.isnan(got[ends].float()).all())
