@@ -170,14 +170,13 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
     const bool empty = b->rows == 0 || b->seqs == 0;
     if (!why && !empty) why = kv_check_rows(a->q, b->rows, a->q_heads, c->head_dim, c->dtype, false, &qb);
     if (!why && !empty) why = kv_check_rows(a->out, b->rows, a->q_heads, c->head_dim, a->out_dtype, true, &ob);
-    const AttendPlan plan = plan_attend(ctx, *c, *b, *a, shared_len);
-    const size_t need = plan.bytes;
-    if (!why && !empty && need > 0) {
-        if (a->workspace == nullptr || !kv_aligned(a->workspace, 256)) why = "workspace is NULL or not 256-byte aligned";
-        else if (a->workspace_bytes < need) why = "workspace is smaller than gfd_kv_attend_workspace says";
-    }
     if (why) return set_error(ctx, GFD_ERR_INVALID, "%s: %s", call, why);
     if (empty) return GFD_OK;
+    const AttendPlan plan = plan_attend(ctx, *c, *b, *a, shared_len);  // (divides by the heads: after the checks)
+    const size_t need = plan.bytes;
+    if (need > 0 && (a->workspace == nullptr || !kv_aligned(a->workspace, 256))) why = "workspace is NULL or not 256-byte aligned";
+    else if (a->workspace_bytes < need) why = "workspace is smaller than gfd_kv_attend_workspace says";
+    if (why) return set_error(ctx, GFD_ERR_INVALID, "%s: %s", call, why);
     const uint64_t shared_blocks = (static_cast<uint64_t>(shared_len) + c->block_tokens - 1) / c->block_tokens;
     const Region regions[] = {{c->k, cache_bytes, "the cache's K"},
                               {c->v, cache_bytes, "the cache's V"},

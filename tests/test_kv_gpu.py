@@ -946,3 +946,35 @@ def test_attend_rows_summed_again_replace_the_first_sums(gpu_ctx, d, q_lens, kv_
         assert torch.equal(got[rows], first[rows])
     oracle.check_attend(got, lse, want, rows)
     assert bool(torch.isnan(got[ends].float()).all())
+
+
+@pytest.mark.parametrize("field,value", [("heads", 0), ("heads", -3), ("heads", 1025), ("head_dim", 0), ("block_tokens", 0), ("blocks", 0),
+                                         ("dtype", 7)])
+def test_entry_points_refuse_a_cache_of_no_shape(gpu_ctx, field, value):
+    """Through the C entry points: nothing is worked out from a shape before it is checked."""
+    s = Setup(gpu_ctx, "bf16", 2, 2, 64, 16, [1, 1], [20, 30], seed=64)
+    c = kv._Cache.from_buffer_copy(s.cache._c)
+    setattr(c, field, value)
+    l, h, b = gpu_ctx.lib, gpu_ctx.handle, s.batch._c(2)
+    out, ws = torch_().full_like(s.q, 7.0), s.workspace(1)
+    a = kv._Attend(q=kv._Rows(s.q.data_ptr(), 256, 64), out=kv._Rows(out.data_ptr(), 256, 64), workspace=ws.data_ptr(),
+                   workspace_bytes=ws.numel(), q_heads=4, scale=0.1, out_dtype=kv.BF16)
+    n = ctypes.c_size_t()
+    assert l.gfd_kv_attend(h, bytes(c), b, bytes(a), 0) == GFD_ERR_INVALID
+    assert l.gfd_kv_attend_shared(h, bytes(c), b, s.starts.data_ptr(), 16, bytes(a), 0) == GFD_ERR_INVALID
+    assert l.gfd_kv_attend_workspace(h, bytes(c), b, bytes(a), 0, ctypes.byref(n)) == GFD_ERR_INVALID
+    assert l.gfd_kv_append(h, bytes(c), b, bytes(kv._Append()), 0) == GFD_ERR_INVALID
+    torch_().cuda.synchronize()
+    assert bool((out == 7).all())
+
+
+def test_a_cache_without_heads_is_refused(gpu_ctx):
+    """The same through the Python layer, whose tensors may have a dimension of nothing."""
+    torch = torch_()
+    s = Setup(gpu_ctx, "bf16", 2, 2, 64, 16, [1, 1], [20, 30], seed=65)
+    cache = kv.PagedCache(gpu_ctx, s.k[:, :, :0], s.v[:, :, :0])
+    with pytest.raises(GfdError) as e:
+        cache.attend(s.batch, s.q, torch.empty_like(s.q), workspace=s.workspace(1))
+    assert e.value.code == GFD_ERR_INVALID
+    with pytest.raises(GfdError):
+        cache.append(s.batch, s.normal(2, 0, 64), s.normal(2, 0, 64))
