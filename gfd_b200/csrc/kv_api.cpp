@@ -69,10 +69,6 @@ KvRowsView view(const gfd_kv_rows& r, int64_t rows, int64_t heads, int elt) {
     return KvRowsView{static_cast<char*>(r.data), rows > 1 ? r.row_stride * elt : 0, heads > 1 ? r.head_stride * elt : 0};
 }
 
-uint64_t table_bytes(const gfd_kv_batch& b) {
-    return b.table_width == 0 ? 0 : (static_cast<uint64_t>(b.seqs - 1) * b.table_stride + b.table_width) * sizeof(int32_t);
-}
-
 // An attention call's kernels and where each keeps its intermediate results in the workspace.
 struct AttendPlan {
     bool few, many;       // kv_decode takes the sequences of few rows, kv_prompt the others
@@ -132,7 +128,7 @@ int append(gfd_ctx* ctx, const gfd_kv_cache* c, const gfd_kv_batch* b, const gfd
                               {a->q_out.data, qob, "q_out"},
                               {b->row_start, (static_cast<uint64_t>(b->seqs) + 1) * 4, "row_start"},
                               {b->kv_len, static_cast<uint64_t>(b->seqs) * 4, "kv_len"},
-                              {b->table, table_bytes(*b), "table"},
+                              {b->table, kv_table_bytes(*b), "table"},
                               {a->inv_freq, static_cast<uint64_t>(a->rot_dim) * 2, "inv_freq"},
                               {a->positions, static_cast<uint64_t>(b->rows) * 4, "positions"},
                               {a->status, 4, "status"}};
@@ -184,7 +180,7 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
                               {a->out.data, ob, "out"},
                               {b->row_start, (static_cast<uint64_t>(b->seqs) + 1) * 4, "row_start"},
                               {b->kv_len, static_cast<uint64_t>(b->seqs) * 4, "kv_len"},
-                              {b->table, table_bytes(*b), "table"},
+                              {b->table, kv_table_bytes(*b), "table"},
                               {shared_table, shared_blocks * 4, "shared_table"},
                               {a->lse, static_cast<uint64_t>(b->rows) * a->q_heads * 4, "lse"},
                               {a->alibi, static_cast<uint64_t>(a->q_heads) * 4, "alibi"},

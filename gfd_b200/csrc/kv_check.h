@@ -180,11 +180,18 @@ inline const char* kv_check_cache(const gfd_kv_cache& c, bool write, uint64_t* b
     return nullptr;
 }
 
+// Bytes of the block table of a batch that was checked.
+inline uint64_t kv_table_bytes(const gfd_kv_batch& b) {
+    const int64_t n[1] = {b.seqs}, st[1] = {b.seqs > 1 ? b.table_stride : 0};
+    return b.table_width == 0 ? 0 : kv_extent(n, st, 1, b.table_width, sizeof(int32_t));
+}
+
 inline const char* kv_check_batch(const gfd_kv_batch& b, const gfd_kv_cache& c, int64_t shared_len) {
     if (b.rows < 0 || b.rows > 0x3fffffffll) return "bad number of rows";
     if (b.seqs < 0 || b.seqs > GFD_KV_MAX_SEQS) return "bad number of sequences";
     if (b.rows == 0 || b.seqs == 0) return nullptr;
     if (b.table_width < 0 || b.table_stride < 0 || (b.seqs > 1 && b.table_stride < b.table_width)) return "bad block table shape";
+    if (b.table_width > 0 && kv_table_bytes(b) == 0) return "the block table is too large";
     if (shared_len < 0 || shared_len + static_cast<int64_t>(b.table_width) * c.block_tokens > kKvMaxTokens)
         return "more than 2^30 tokens in a sequence's table";
     if (b.row_start == nullptr || b.kv_len == nullptr || (b.table == nullptr && b.table_width > 0))

@@ -10,6 +10,7 @@ extern "C" {
 
 const char* gfdt_kv_cache(const gfd_kv_cache* c, int write, uint64_t* bytes) { return kv_check_cache(*c, write != 0, bytes); }
 const char* gfdt_kv_batch(const gfd_kv_batch* b, const gfd_kv_cache* c, int64_t shared) { return kv_check_batch(*b, *c, shared); }
+uint64_t gfdt_kv_table_bytes(const gfd_kv_batch* b) { return kv_table_bytes(*b); }
 const char* gfdt_kv_append(const gfd_kv_append_args* a, const gfd_kv_cache* c) { return kv_check_append(*a, *c); }
 const char* gfdt_kv_attend(const gfd_kv_attend_args* a, const gfd_kv_cache* c) { return kv_check_attend(*a, *c); }
 const char* gfdt_kv_merge(const gfd_kv_merge_args* a) { return kv_check_merge(*a); }

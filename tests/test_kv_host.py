@@ -327,3 +327,20 @@ def test_attend_parameters_out_of_range(lib):
     for kw in (dict(q_heads=0), dict(q_heads=12), dict(q_heads=8 * 1024 + 8), dict(scale=float("nan")), dict(scale=float("inf")),
                dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=float("inf")), dict(window=-1), dict(max_q_len=-1)):
         assert check(**kw) is not None, kw
+
+
+def test_table_extent(lib):
+    """The table's bytes are counted without wrapping: what is checked is what the kernels read."""
+    lib.gfdt_kv_table_bytes.argtypes, lib.gfdt_kv_table_bytes.restype = [_VP], ctypes.c_uint64
+    c = cache()
+
+    def check(seqs, width, stride):
+        b = kv._Batch(row_start=64, kv_len=128, table=256, table_stride=stride, rows=7, seqs=seqs, table_width=width)
+        return lib.gfdt_kv_batch(ctypes.byref(b), ctypes.byref(c), 0), lib.gfdt_kv_table_bytes(ctypes.byref(b))
+
+    for seqs, width, stride in ((1, 5, 0), (1, 5, 1 << 62), (3, 5, 5), (3, 5, 9), (4096, 1000, 1 << 20), (2, 1, (1 << 60) - 2)):
+        why, n = check(seqs, width, stride)
+        assert why is None and n == 4 * ((seqs - 1) * (stride if seqs > 1 else 0) + width), (seqs, width, stride)
+    for seqs, width, stride in ((5, 5, 1 << 62), (2, 5, 1 << 62), (2, 1, 1 << 60), (4096, 1, 1 << 51), (3, 7, (1 << 63) - 1)):
+        assert check(seqs, width, stride)[0] is not None, (seqs, width, stride)
+    assert check(3, 0, 1 << 62) == (None, 0)  # a table of no width is not read
