@@ -51,13 +51,6 @@ struct KvPlace {
     int32_t h, s;             // KV head, sequence
 };
 
-// What the joining kernel finds for a stretch: the rows of the unit that the stretch's cut is the first
-// to divide, left in parts: slot 1 of the stretch before it, slot 0 of this one and the next ones.
-struct KvCut {
-    int32_t parts;  // 0: nothing to join
-    int32_t row0, packed0, packed, h;
-};
-
 // A launch's cuts and partial results, one and two slots per stretch: the sums of kRows packed rows
 // ([rows][D] of kv_decode, [D / 4][rows][4] of kv_prompt, so that its threads of neighbouring rows
 // write side by side), then the rows' base and weight sum.
@@ -97,9 +90,6 @@ struct KvAttendParams {
     KvLine line;
 };
 
-constexpr int kKvManyRows = 256;  // packed rows of a unit of kv_prompt
-constexpr int kKvFewRows = 16;  // packed rows (rows x group) up to which kv_decode takes a sequence
-
 struct KvMergeParams {
     KvRowsView parts;
     int64_t part_stride;  // bytes
@@ -128,11 +118,7 @@ bool kv_make_maps(KvMaps* maps, const KvAttendParams& p, int head_dim, int dtype
 cudaError_t launch_kv_prompt(const KvAttendParams& p, int head_dim, int dtype, int num_sms, const KvMaps& maps, bool chained, cudaStream_t st);
 cudaError_t launch_kv_decode(const KvAttendParams& p, int head_dim, int dtype, int num_sms, bool chained, cudaStream_t st);
 
-// Bytes of a line's places and slots, and the line laid out in them.
-inline size_t kv_line_bytes(int ctas, int slot_rows, int head_dim) {
-    return (sizeof(KvCut) * ctas + 255) / 256 * 256 +
-           (static_cast<size_t>(ctas) * 2 * (static_cast<size_t>(slot_rows) * head_dim + 2 * slot_rows) * sizeof(float) + 255) / 256 * 256;
-}
+// A line laid out in the kv_line_bytes at p.
 inline KvLine kv_line_at(void* p, int ctas) {
     return KvLine{static_cast<KvCut*>(p), reinterpret_cast<float*>(static_cast<char*>(p) + (sizeof(KvCut) * ctas + 255) / 256 * 256)};
 }

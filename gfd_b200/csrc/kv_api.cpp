@@ -69,40 +69,8 @@ KvRowsView view(const gfd_kv_rows& r, int64_t rows, int64_t heads, int elt) {
     return KvRowsView{static_cast<char*>(r.data), rows > 1 ? r.row_stride * elt : 0, heads > 1 ? r.head_stride * elt : 0};
 }
 
-// An attention call's kernels and where each keeps its intermediate results in the workspace.
-struct AttendPlan {
-    bool few, many;       // kv_decode takes the sequences of few rows, kv_prompt the others
-    size_t few_line, many_line, prefix_line;  // offsets of the kernels' lines
-    size_t own_out, own_lse;                  // behind a shared prefix: results over the own keys
-    size_t bytes;
-};
-
-AttendPlan plan_attend(const gfd_ctx* ctx, const gfd_kv_cache& c, const gfd_kv_batch& b, const gfd_kv_attend_args& a, int64_t shared_len) {
-    AttendPlan r{};
-    if (b.rows <= 0 || b.seqs <= 0 || a.q_heads <= 0) return r;
-    const int64_t group = a.q_heads / c.heads > 0 ? a.q_heads / c.heads : 1;
-    const int64_t most = a.max_q_len > 0 && a.max_q_len < b.rows ? a.max_q_len : b.rows;  // rows of a sequence
-    r.many = most * group > kKvFewRows;
-    // Where every sequence has many rows (no row left over: one has at least what the others cannot
-    // have), kv_prompt takes them all, whatever they turn out to be: two launches less, 10 us.
-    const int64_t least = b.rows - (b.seqs - 1) * most;
-    r.few = group <= kKvFewRows && (!r.many || least * group <= kKvFewRows);
-    size_t at = 0;
-    auto take = [&](size_t n) {
-        const size_t here = at;
-        at += (n + 255) / 256 * 256;
-        return here;
-    };
-    const size_t many_bytes = kv_line_bytes(kv_prompt_ctas(ctx->num_sms), kKvManyRows, c.head_dim);
-    if (r.few) r.few_line = take(kv_line_bytes(kv_decode_workers(ctx->num_sms, c.head_dim), kKvFewRows, c.head_dim));
-    if (r.many) r.many_line = take(many_bytes);
-    if (shared_len > 0) {
-        r.prefix_line = take(many_bytes);
-        r.own_out = take(static_cast<size_t>(b.rows) * a.q_heads * c.head_dim * sizeof(float));
-        r.own_lse = take(static_cast<size_t>(b.rows) * a.q_heads * sizeof(float));
-    }
-    r.bytes = at;
-    return r;
+KvPlan plan_attend(const gfd_ctx* ctx, const gfd_kv_cache& c, const gfd_kv_batch& b, const gfd_kv_attend_args& a, int64_t shared_len) {
+    return kv_plan(c, b, a, shared_len, kv_decode_workers(ctx->num_sms, c.head_dim), kv_prompt_ctas(ctx->num_sms));
 }
 
 int append(gfd_ctx* ctx, const gfd_kv_cache* c, const gfd_kv_batch* b, const gfd_kv_append_args* a, void* stream) {
@@ -168,7 +136,7 @@ int attend(gfd_ctx* ctx, const char* call, const gfd_kv_cache* c, const gfd_kv_b
     if (!why && !empty) why = kv_check_rows(a->out, b->rows, a->q_heads, c->head_dim, a->out_dtype, true, &ob);
     if (why) return set_error(ctx, GFD_ERR_INVALID, "%s: %s", call, why);
     if (empty) return GFD_OK;
-    const AttendPlan plan = plan_attend(ctx, *c, *b, *a, shared_len);  // (divides by the heads: after the checks)
+    const KvPlan plan = plan_attend(ctx, *c, *b, *a, shared_len);  // (divides by the heads: after the checks)
     const size_t need = plan.bytes;
     if (need > 0 && (a->workspace == nullptr || !kv_aligned(a->workspace, 256))) why = "workspace is NULL or not 256-byte aligned";
     else if (a->workspace_bytes < need) why = "workspace is smaller than gfd_kv_attend_workspace says";

@@ -4,6 +4,7 @@
 // compile it with a plain C++ compiler.
 
 #include <cmath>
+#include <cstddef>
 #include <cstdint>
 #include <initializer_list>
 
@@ -110,6 +111,65 @@ struct KvCuts {
         return c;
     }
 };
+
+// What the joining kernel finds for a stretch: the rows of the unit that the stretch's cut is the first
+// to divide, left in parts: slot 1 of the stretch before it, slot 0 of this one and the next ones.
+struct KvCut {
+    int32_t parts;  // 0: nothing to join
+    int32_t row0, packed0, packed, h;
+};
+
+// ---------------------------------------------------------------------------
+// An attention call's kernels and workspace
+// ---------------------------------------------------------------------------
+constexpr int kKvManyRows = 256;  // packed rows of a unit of kv_prompt
+constexpr int kKvFewRows = 16;  // packed rows (rows x group) up to which kv_decode takes a sequence
+
+// Bytes of a line's cuts and slots.
+inline size_t kv_line_bytes(int ctas, int slot_rows, int head_dim) {
+    return (sizeof(KvCut) * ctas + 255) / 256 * 256 +
+           (static_cast<size_t>(ctas) * 2 * (static_cast<size_t>(slot_rows) * head_dim + 2 * slot_rows) * sizeof(float) + 255) / 256 * 256;
+}
+
+// Which kernels a call runs, and where each keeps its intermediate results in the workspace.
+struct KvPlan {
+    bool few, many;       // kv_decode takes the sequences of few rows, kv_prompt the others
+    size_t few_line, many_line, prefix_line;  // offsets of the kernels' lines
+    size_t own_out, own_lse;                  // behind a shared prefix: results over the own keys
+    size_t bytes;
+};
+
+// few_workers, many_ctas: the stretches of the two kernels on this GPU.  The cache has been checked.  A batch
+// of no more rows, sequences, rows a sequence and shared tokens never needs more bytes than one of more: the
+// kernels that run depend on how the rows can be spread over the sequences, the room does not.
+inline KvPlan kv_plan(const gfd_kv_cache& c, const gfd_kv_batch& b, const gfd_kv_attend_args& a, int64_t shared_len, int few_workers,
+                      int many_ctas) {
+    KvPlan r{};
+    if (b.rows <= 0 || b.seqs <= 0 || a.q_heads <= 0) return r;
+    const int64_t group = a.q_heads / c.heads > 0 ? a.q_heads / c.heads : 1;
+    const int64_t most = a.max_q_len > 0 && a.max_q_len < b.rows ? a.max_q_len : b.rows;  // rows of a sequence
+    r.many = most * group > kKvFewRows;
+    // Where every sequence has many rows (no row left over: one has at least what the others cannot
+    // have), kv_prompt takes them all, whatever they turn out to be: two launches less, 10 us.
+    const int64_t least = b.rows - (b.seqs - 1) * most;
+    r.few = group <= kKvFewRows && (!r.many || least * group <= kKvFewRows);
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        const size_t here = at;
+        at += (n + 255) / 256 * 256;
+        return here;
+    };
+    const size_t many_bytes = kv_line_bytes(many_ctas, kKvManyRows, c.head_dim);
+    if (group <= kKvFewRows) r.few_line = take(kv_line_bytes(few_workers, kKvFewRows, c.head_dim));
+    if (r.many) r.many_line = take(many_bytes);
+    if (shared_len > 0) {
+        r.prefix_line = take(many_bytes);
+        r.own_out = take(static_cast<size_t>(b.rows) * a.q_heads * c.head_dim * sizeof(float));
+        r.own_lse = take(static_cast<size_t>(b.rows) * a.q_heads * sizeof(float));
+    }
+    r.bytes = at;
+    return r;
+}
 
 // ---------------------------------------------------------------------------
 // Checks: each returns nullptr, or what is wrong

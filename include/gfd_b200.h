@@ -341,7 +341,9 @@ int gfd_kv_attend_shared(gfd_ctx* ctx, const gfd_kv_cache* cache, const gfd_kv_b
                          const gfd_kv_attend_args* args, void* stream);
 
 /* Bytes of workspace for a call of these shapes (only q_heads, max_q_len of args, rows and
- * seqs of batch, and the cache's shape are read; no array is touched). */
+ * seqs of batch, and the cache's shape are read; no array is touched).  Enough for every
+ * call of the same cache and q_heads with no more rows, seqs, max_q_len (0 is the most) and
+ * shared_len. */
 int gfd_kv_attend_workspace(gfd_ctx* ctx, const gfd_kv_cache* cache, const gfd_kv_batch* batch,
                             const gfd_kv_attend_args* args, int64_t shared_len, size_t* bytes);
 

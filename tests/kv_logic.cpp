@@ -10,6 +10,16 @@ extern "C" {
 
 const char* gfdt_kv_cache(const gfd_kv_cache* c, int write, uint64_t* bytes) { return kv_check_cache(*c, write != 0, bytes); }
 const char* gfdt_kv_batch(const gfd_kv_batch* b, const gfd_kv_cache* c, int64_t shared) { return kv_check_batch(*b, *c, shared); }
+// workspace of a call on a GPU of `sms`; kernels: bit 0 kv_decode, bit 1 kv_prompt
+uint64_t gfdt_kv_workspace(const gfd_kv_cache* c, int64_t rows, int32_t seqs, int32_t q_heads, int32_t max_q_len, int64_t shared, int sms,
+                           int* kernels) {
+    gfd_kv_batch b{};
+    gfd_kv_attend_args a{};
+    b.rows = rows, b.seqs = seqs, a.q_heads = q_heads, a.max_q_len = max_q_len;
+    const KvPlan p = kv_plan(*c, b, a, shared, sms * 4 * (c->head_dim == 64 ? 3 : 2), sms);
+    *kernels = (p.few ? 1 : 0) + (p.many ? 2 : 0);
+    return p.bytes;
+}
 uint64_t gfdt_kv_table_bytes(const gfd_kv_batch* b) { return kv_table_bytes(*b); }
 const char* gfdt_kv_append(const gfd_kv_append_args* a, const gfd_kv_cache* c) { return kv_check_append(*a, *c); }
 const char* gfdt_kv_attend(const gfd_kv_attend_args* a, const gfd_kv_cache* c) { return kv_check_attend(*a, *c); }

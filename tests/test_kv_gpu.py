@@ -978,3 +978,14 @@ def test_a_cache_without_heads_is_refused(gpu_ctx):
     assert e.value.code == GFD_ERR_INVALID
     with pytest.raises(GfdError):
         cache.append(s.batch, s.normal(2, 0, 64), s.normal(2, 0, 64))
+
+
+@pytest.mark.parametrize("shared_len", [0, 100])
+def test_workspace_of_the_largest_batch_serves_smaller_ones(gpu_ctx, shared_len):
+    """Sequences that all have many rows, then the same program's batches with short ones among them."""
+    ws = None
+    for q_lens in ([90] * 4, [90, 1, 2, 90], [1] * 4, [90, 90], [3]):
+        s = Setup(gpu_ctx, "bf16", 2, 4, 64, 16, q_lens, [n + 30 for n in q_lens], seed=66, shared_len=shared_len)
+        if ws is None:
+            ws = s.workspace(90)
+        s.check(max_q_len=90, workspace=ws)

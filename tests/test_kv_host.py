@@ -344,3 +344,27 @@ def test_table_extent(lib):
     for seqs, width, stride in ((5, 5, 1 << 62), (2, 5, 1 << 62), (2, 1, 1 << 60), (4096, 1, 1 << 51), (3, 7, (1 << 63) - 1)):
         assert check(seqs, width, stride)[0] is not None, (seqs, width, stride)
     assert check(3, 0, 1 << 62) == (None, 0)  # a table of no width is not read
+
+
+def test_workspace_of_a_larger_batch_holds_a_smaller_one(lib):
+    """Room asked for once, for the largest batch, serves every smaller one, whichever kernels that takes."""
+    f = lib.gfdt_kv_workspace
+    f.argtypes = [_VP, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int64, ctypes.c_int, ctypes.POINTER(ctypes.c_int)]
+    f.restype = ctypes.c_uint64
+    k = ctypes.c_int()
+
+    def room(rows, seqs, max_q, shared=0, heads=8, group=4, d=128):
+        c = cache(heads=heads, head_dim=d)
+        return f(ctypes.byref(c), rows, seqs, heads * group, max_q, shared, 148, ctypes.byref(k))
+
+    assert room(32768, 4, 8192) >= room(10000, 4, 8192)  # four whole prompts, then prompts among decode steps
+    assert k.value == 3 and room(32768, 4, 8192) and k.value == 2 and room(4, 4, 1) and k.value == 1
+    rng = np.random.default_rng(8)
+    for _ in range(3000):
+        group, d = int(rng.choice([1, 3, 4, 8, 16, 17, 40])), int(rng.choice([64, 128]))
+        rows, seqs = int(rng.integers(1, 40000)), int(rng.integers(1, 300))
+        max_q, shared = int(rng.choice([0, 1, 4, 16, 300, 50000])), int(rng.choice([0, 1, 5000]))
+        less = dict(rows=int(rng.integers(1, rows + 1)), seqs=int(rng.integers(1, seqs + 1)), shared=int(rng.integers(0, shared + 1)),
+                    max_q=int(rng.integers(0, 60000)) if max_q == 0 else int(rng.integers(1, max_q + 1)))
+        assert room(rows, seqs, max_q, shared, group=group, d=d) >= room(**less, group=group, d=d), (rows, seqs, max_q, shared, less)
+    assert room(0, 4, 1) == 0 and room(5, 0, 1) == 0
