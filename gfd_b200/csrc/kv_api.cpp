@@ -296,10 +296,11 @@ int gfd_kv_attend_shared(gfd_ctx* ctx, const gfd_kv_cache* cache, const gfd_kv_b
 int gfd_kv_attend_workspace(gfd_ctx* ctx, const gfd_kv_cache* cache, const gfd_kv_batch* batch,
                             const gfd_kv_attend_args* args, int64_t shared_len, size_t* bytes) {
     return guarded(ctx, [&] {
-        if (bytes == nullptr || cache == nullptr || batch == nullptr || args == nullptr || shared_len < 0)
+        if (bytes == nullptr || cache == nullptr || batch == nullptr || args == nullptr)
             return set_error(ctx, GFD_ERR_INVALID, "kv_attend_workspace: NULL argument");
         uint64_t unused = 0;
         const char* why = kv_check_cache(*cache, false, &unused);
+        if (!why) why = kv_check_workspace(*cache, *batch, *args, shared_len);
         if (why) return set_error(ctx, GFD_ERR_INVALID, "kv_attend_workspace: %s", why);
         *bytes = plan_attend(ctx, *cache, *batch, *args, shared_len).bytes;
         return static_cast<int>(GFD_OK);

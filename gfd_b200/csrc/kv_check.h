@@ -286,6 +286,17 @@ inline const char* kv_check_attend(const gfd_kv_attend_args& a, const gfd_kv_cac
     return nullptr;
 }
 
+// What gfd_kv_attend_workspace reads, within the limits of the calls themselves (so that nothing wraps).
+inline const char* kv_check_workspace(const gfd_kv_cache& c, const gfd_kv_batch& b, const gfd_kv_attend_args& a, int64_t shared_len) {
+    if (b.rows < 0 || b.rows > 0x3fffffffll) return "bad number of rows";
+    if (b.seqs < 0 || b.seqs > GFD_KV_MAX_SEQS) return "bad number of sequences";
+    if (a.q_heads < 1 || a.q_heads > 8 * kKvMaxHeads || a.q_heads % c.heads != 0)
+        return "query heads must be a multiple of the cache's heads";
+    if (a.max_q_len < 0) return "max_q_len is negative";
+    if (shared_len < 0 || shared_len > kKvMaxTokens) return "bad shared_len";
+    return nullptr;
+}
+
 inline const char* kv_check_merge(const gfd_kv_merge_args& a) {
     if (a.rows < 0 || a.rows > 0x3fffffffll) return "bad number of rows";
     if (a.part_count < 1 || a.part_count > kKvMaxParts) return "bad number of parts";

@@ -23,6 +23,9 @@ uint64_t gfdt_kv_workspace(const gfd_kv_cache* c, int64_t rows, int32_t seqs, in
 uint64_t gfdt_kv_table_bytes(const gfd_kv_batch* b) { return kv_table_bytes(*b); }
 const char* gfdt_kv_append(const gfd_kv_append_args* a, const gfd_kv_cache* c) { return kv_check_append(*a, *c); }
 const char* gfdt_kv_attend(const gfd_kv_attend_args* a, const gfd_kv_cache* c) { return kv_check_attend(*a, *c); }
+const char* gfdt_kv_check_workspace(const gfd_kv_cache* c, const gfd_kv_batch* b, const gfd_kv_attend_args* a, int64_t shared) {
+    return kv_check_workspace(*c, *b, *a, shared);
+}
 const char* gfdt_kv_merge(const gfd_kv_merge_args* a) { return kv_check_merge(*a); }
 const char* gfdt_kv_rows(const gfd_kv_rows* r, int64_t rows, int64_t heads, int64_t dim, int32_t dtype, int out, uint64_t* bytes) {
     return kv_check_rows(*r, rows, heads, dim, dtype, out != 0, bytes);

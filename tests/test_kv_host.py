@@ -368,3 +368,18 @@ def test_workspace_of_a_larger_batch_holds_a_smaller_one(lib):
                     max_q=int(rng.integers(0, 60000)) if max_q == 0 else int(rng.integers(1, max_q + 1)))
         assert room(rows, seqs, max_q, shared, group=group, d=d) >= room(**less, group=group, d=d), (rows, seqs, max_q, shared, less)
     assert room(0, 4, 1) == 0 and room(5, 0, 1) == 0
+
+
+def test_workspace_of_shapes_out_of_range_is_refused(lib):
+    f = lib.gfdt_kv_check_workspace
+    f.argtypes, f.restype = [_VP, _VP, _VP, ctypes.c_int64], ctypes.c_char_p
+    c = cache()
+
+    def check(rows=100, seqs=4, q_heads=32, max_q=9, shared=0):
+        b, a = kv._Batch(rows=rows, seqs=seqs), kv._Attend(q_heads=q_heads, max_q_len=max_q)
+        return f(ctypes.byref(c), ctypes.byref(b), ctypes.byref(a), shared)
+
+    assert check() is None and check(rows=0, seqs=0) is None and check(rows=(1 << 30) - 1, shared=1 << 30, q_heads=8192) is None
+    for kw in (dict(rows=-1), dict(rows=1 << 30), dict(rows=1 << 62), dict(seqs=-1), dict(seqs=4097), dict(q_heads=0), dict(q_heads=12),
+               dict(q_heads=8200), dict(q_heads=1 << 30), dict(max_q=-1), dict(shared=-1), dict(shared=(1 << 30) + 1)):
+        assert check(**kw) is not None, kw
