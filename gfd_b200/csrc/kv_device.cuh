@@ -178,16 +178,18 @@ __device__ __forceinline__ float kv_tanh2(const KvAttendParams& p, float x) {
 }
 
 // N products of queries and keys to scores in base 2: scaled, capped where the call has a cap.
-// Where the warp's products all lie within three quarters of the cap (the usual case) tanh x is
+// Where a thread's products all lie within three quarters of the cap (the usual case) tanh x is
 // x P(x^2) on the FMA units, P = 1 + ... of degree 5 by least largest relative error (2^-24.9;
 // 2^-22.9 with the roundings): the special-function unit, which the exponentials need, is left out.
+// Products of keys that the row does not see come as 0, so that the choice, and with it a result's last
+// bits, goes by what the row sees and not by its neighbours.
 template <int N>
 __device__ __forceinline__ void kv_cap(const KvAttendParams& p, uint32_t* z) {
     if (p.softcap > 0.0f) {
         float m = 0.0f;
 #pragma unroll
         for (int e = 0; e < N; ++e) m = fmaxf(m, fabsf(__uint_as_float(z[e])));
-        if (__all_sync(0xffffffffu, m * fabsf(p.cap_x) <= 0.75f)) {
+        if (m * fabsf(p.cap_x) <= 0.75f) {
             const uint64_t sx = pack2(p.cap_x, p.cap_x), amp = pack2(p.cap2, p.cap2);
 #pragma unroll
             for (int e = 0; e < N; e += 2) {
@@ -206,6 +208,7 @@ __device__ __forceinline__ void kv_cap(const KvAttendParams& p, uint32_t* z) {
 #pragma unroll
             for (int e = 0; e < N; ++e) z[e] = __float_as_uint(kv_tanh2(p, __uint_as_float(z[e]) * p.cap_x));
         }
+        __syncwarp();
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) z[e] = __float_as_uint(__uint_as_float(z[e]) * p.scale2);

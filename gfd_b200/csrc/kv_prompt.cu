@@ -667,7 +667,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int k = 0; k < kTile; k += 32) tm_ld32(ts + k, z + k);
 #pragma unroll
                 for (int k = 0; k < kTile; k += 32) tm_wait32(z + k);
+                // keys [j0 + k, j0 + k + 32) that the row sees, a bit each
+                auto sees = [&](int k) {
+                    const int32_t j = j0 + k;
+                    const uint32_t out = (((bad >> (k / kKvPage)) & 1u) ? 0x0000ffffu : 0u) | (((bad >> (k / kKvPage)) & 2u) ? 0xffff0000u : 0u);
+                    return (below(sp.pre - j) | (below(sp.hi - j) & ~below(sp.lo - j))) & ~out;
+                };
                 if (!kPlain) {
+                    if (masked && p.softcap > 0.0f)
+#pragma unroll
+                        for (int k = 0; k < kTile; k += 32) {
+                            const uint32_t some = sees(k);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) z[k + e] = (some & (1u << e)) != 0 ? z[k + e] : 0u;
+                        }
                     kv_cap<kTile>(p, z);
                     if (p.alibi != nullptr) {
                         const float d0 = static_cast<float>(base_key + j0 - pos);
@@ -685,11 +698,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (masked)
 #pragma unroll
                     for (int k = 0; k < kTile; k += 32) {
-                        const int32_t j = j0 + k;
-                        const uint32_t out = (((bad >> (k / kKvPage)) & 1u) ? 0x0000ffffu : 0u) | (((bad >> (k / kKvPage)) & 2u) ? 0xffff0000u : 0u);
-                        const uint32_t sees = (below(sp.pre - j) | (below(sp.hi - j) & ~below(sp.lo - j))) & ~out;
+                        const uint32_t some = sees(k);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) z[k + e] = (sees & (1u << e)) != 0 ? z[k + e] : 0xff800000u;
+                        for (int e = 0; e < 32; ++e) z[k + e] = (some & (1u << e)) != 0 ? z[k + e] : 0xff800000u;
                     }
                 float m8[8];
 #pragma unroll
@@ -705,9 +716,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float top = most * scale - Shift<T>::value;
                 const bool grew = top > base + kGrow || (base == -INFINITY && top > -INFINITY);
                 if (__any_sync(0xffffffffu, grew)) {
-                    const float to_base = fmaxf(base, top);
-                    const float keep = to_base == -INFINITY ? 1.0f : fast_exp2(base - to_base);
-                    base = to_base;
+                    // (a row's base moves by its own scores alone, so that its roundings do not go by its neighbours)
+                    const float keep = grew ? fast_exp2(base - top) : 1.0f;
+                    base = grew ? top : base;
                     l *= keep;
                     if (i > 0) {
 #pragma unroll 1

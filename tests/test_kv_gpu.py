@@ -989,3 +989,31 @@ def test_workspace_of_the_largest_batch_serves_smaller_ones(gpu_ctx, shared_len)
         if ws is None:
             ws = s.workspace(90)
         s.check(max_q_len=90, workspace=ws)
+
+
+@pytest.mark.parametrize("kw", [{}, dict(softcap=3.0), dict(softcap=50.0, window=40), dict(window=40)])
+@pytest.mark.parametrize("dtype,d,q_lens,kv_lens,shared", [
+    ("bf16", 64, [1, 4], [45, 300], 0), ("fp16", 128, [3, 2], [500, 33], 0), ("bf16", 128, [150, 70], [200, 700], 0),
+    ("fp16", 64, [200, 33], [400, 33], 0), ("bf16", 64, [2, 3, 1], [20, 40, 9], 300), ("bf16", 128, [1, 100], [9, 130], 150)])
+def test_attend_bits_do_not_depend_on_what_a_row_does_not_see(gpu_ctx, dtype, d, q_lens, kv_lens, shared, kw):
+    """Large keys and values where a row's mask hides them, and other rows' queries, leave every bit of it as it was."""
+    torch = torch_()
+    s = Setup(gpu_ctx, dtype, 2, 4, d, 16, q_lens, kv_lens, seed=67, shared_len=shared)
+    a, la = s.attend(out_dtype="fp32", **kw)
+    first = lambda i: max(0, kv_lens[i] - q_lens[i] - 39) if kw.get("window") else 0  # first own key that any row sees
+    for i, n in enumerate(kv_lens):
+        for j in list(range(first(i))) + [n - 1] + list(range(n, -(-n // 16) * 16)):  # the last key: the last row's alone
+            block, place = int(s.table[i, j // 16]), j % 16
+            s.k[block, place] *= 3000
+            s.v[block, place] *= 30
+    b, lb = s.attend(out_dtype="fp32", **kw)
+    ends = [x - 1 for x in s.row_start[1:]]
+    rows = [r for r in range(s.rows) if r not in ends]
+    torch.cuda.synchronize()
+    assert torch.equal(a[rows], b[rows]) and torch.equal(la[rows], lb[rows])
+    s.q[ends] *= 40
+    s.q[rows[::3]] *= 40
+    c, lc = s.attend(out_dtype="fp32", **kw)
+    rest = [r for r in rows if r not in rows[::3]]
+    torch.cuda.synchronize()
+    assert torch.equal(a[rest], c[rest]) and torch.equal(la[rest], lc[rest])
