@@ -388,19 +388,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) kv_decode_kernel(const Kv
                     for (int e = 0; e < 4; ++e) y[e] = __float_as_uint(z[e / 2][2 * x + (e & 1)]);
                     const int32_t j = j0 + 2 * (lane & 3);
                     const bool inside = (j0 >= sp[x].lo && j0 + kTile <= sp[x].hi) || j0 + kTile <= sp[x].pre;
-                    uint32_t hidden = 0;  // bit e: key of y[e] is masked
-                    if (__any_sync(0xffffffffu, !inside)) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int32_t k = j + 8 * (e / 2) + (e & 1);
-                            if (!(k < sp[x].pre || (k >= sp[x].lo && k < sp[x].hi))) hidden |= 1u << e;
-                        }
-                    }
+                    const bool masked = __any_sync(0xffffffffu, !inside);
+                    auto sees = [&](int e) {
+                        const int32_t k = j + 8 * (e / 2) + (e & 1);
+                        return k < sp[x].pre || (k >= sp[x].lo && k < sp[x].hi);
+                    };
                     if (!kPlain) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (hidden >> e & 1u) y[e] = 0;
-                        kv_cap<4>(p, y);
+                        kv_cap<4>(p, y, masked, [&](int) { return (sees(0) ? 1u : 0u) | (sees(1) ? 2u : 0u) | (sees(2) ? 4u : 0u) | (sees(3) ? 8u : 0u); });
                         if (p.alibi != nullptr) {
                             const float d = static_cast<float>(p.shared_len + j - pos[x]);
 #pragma unroll
@@ -411,9 +405,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) kv_decode_kernel(const Kv
 #pragma unroll
                         for (int e = 0; e < 4; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * p.scale2);
                     }
+                    if (masked) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (hidden >> e & 1u) y[e] = 0xff800000u;
+                        for (int e = 0; e < 4; ++e)
+                            if (!sees(e)) y[e] = 0xff800000u;
+                    }
                     float mx = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
 #pragma unroll
                     for (int e = 2; e < 4; ++e) mx = fmaxf(mx, __uint_as_float(y[e]));

@@ -181,14 +181,24 @@ __device__ __forceinline__ float kv_tanh2(const KvAttendParams& p, float x) {
 // Where a thread's products all lie within three quarters of the cap (the usual case) tanh x is
 // x P(x^2) on the FMA units, P = 1 + ... of degree 5 by least largest relative error (2^-24.9;
 // 2^-22.9 with the roundings): the special-function unit, which the exponentials need, is left out.
-// Products of keys that the row does not see come as 0, so that the choice, and with it a result's last
-// bits, goes by what the row sees and not by its neighbours.
-template <int N>
-__device__ __forceinline__ void kv_cap(const KvAttendParams& p, uint32_t* z) {
+// The choice, and with it a result's last bits, goes by what the row sees and not by its neighbours: products
+// beyond that bound are looked for among the keys that `sees` (of 32 keys a word, asked where `masked`).
+template <int N, typename F>
+__device__ __forceinline__ void kv_cap(const KvAttendParams& p, uint32_t* z, bool masked, F sees) {
     if (p.softcap > 0.0f) {
         float m = 0.0f;
 #pragma unroll
         for (int e = 0; e < N; ++e) m = fmaxf(m, fabsf(__uint_as_float(z[e])));
+        if (masked && m * fabsf(p.cap_x) > 0.75f) {
+            m = 0.0f;
+#pragma unroll
+            for (int k = 0; k < N; k += 32) {
+                const uint32_t some = sees(k);
+#pragma unroll
+                for (int e = k; e < k + 32 && e < N; ++e)
+                    if (some >> (e - k) & 1u) m = fmaxf(m, fabsf(__uint_as_float(z[e])));
+            }
+        }
         if (m * fabsf(p.cap_x) <= 0.75f) {
             const uint64_t sx = pack2(p.cap_x, p.cap_x), amp = pack2(p.cap2, p.cap2);
 #pragma unroll

@@ -674,14 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     return (below(sp.pre - j) | (below(sp.hi - j) & ~below(sp.lo - j))) & ~out;
                 };
                 if (!kPlain) {
-                    if (masked && p.softcap > 0.0f)
-#pragma unroll
-                        for (int k = 0; k < kTile; k += 32) {
-                            const uint32_t some = sees(k);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) z[k + e] = (some & (1u << e)) != 0 ? z[k + e] : 0u;
-                        }
-                    kv_cap<kTile>(p, z);
+                    kv_cap<kTile>(p, z, masked, sees);
                     if (p.alibi != nullptr) {
                         const float d0 = static_cast<float>(base_key + j0 - pos);
                         const uint64_t from = pack2(d0, d0), by = pack2(slope, slope);
