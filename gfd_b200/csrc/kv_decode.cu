@@ -10,17 +10,18 @@
 //
 // The warps run alone: each has its own ring of stages filled with 16-byte cp.async (8 KB a stage,
 // 192 KB in flight on an SM; block ids fetched 32 stages at a time), its own running maximum and
-// sum, scores and sums by mma.m16n8k16 from ldmatrix fragments, and writes its rows from
+// sum, scores and sums by mma.m16n8k16 from ldmatrix fragments (KvRows16), and writes its rows from
 // registers.  After the stretches are found there is no barrier.
 //
 // Measured: 64 sequences of up to 8192 tokens, 8 heads of 128, in 170 us with their join, 6.0 TB/s; two of
 // 131 thousand, 24 query heads of 64 behind a cap, in 102 us, 5.0 TB/s (there 12 rows' scores and the cap's
-// polynomial fill half of the issue slots).  128 elements a head take 252 registers, two CTAs an SM; 64 take
-// 168, and the third is worth 123 -> 102 us.
+// polynomial fill half of the issue slots).  128 elements a head take 217-221 registers, two CTAs an SM; 64
+// take 156-161, and the third is worth 123 -> 102 us.
 
 #include <type_traits>
 
-#include "kv_device.cuh"
+#include "kv_rows.cuh"
+#include "kv_wait.cuh"
 
 namespace gfdb {
 namespace {
@@ -32,8 +33,6 @@ constexpr int kPerSm = D == 64 ? 3 : 2;  // CTAs of an SM
 constexpr int kLeast = 2;       // tiles of a stretch, where there are enough: a part costs its joining about as much
 constexpr int kRows = kKvFewRows;
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-
 // 16 bytes into shared memory, zeros where !take
 __device__ __forceinline__ void copy16(uint32_t dst, const char* src, bool take) {
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
@@ -42,34 +41,6 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int N>
 __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
-
-template <typename T>
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // One sequence as this kernel sees it: its rows and, in the count of its own keys (behind the
@@ -203,21 +174,17 @@ struct Cursor {
 
 template <int D>
 struct Shape {
-    static constexpr int kStages = D == 64 ? 3 : 3;
+    static constexpr int kStages = 3;
     static constexpr int kRow = 2 * D;                   // bytes of a key
     static constexpr int kStage = 2 * kKvPage * kRow;  // K and V of 16 keys
     static constexpr int kRing = kStages * kStage;
     static constexpr int kSmem = kWarps * kRing;
 };
 
-// fp16 weights reach 2^8, which keeps the small ones clear of that type's coarse steps below 2^-14.
-template <typename T>
-constexpr float kShift = std::is_same<T, __half>::value ? 8.0f : 0.0f;
-
 template <typename T, int D, bool kPlain>
 __global__ void __launch_bounds__(kThreads, kPerSm<D>) kv_decode_kernel(const KvAttendParams p) {
     using S = Shape<D>;
-    constexpr int kSteps = D / 16;   // k-steps of the scores, pairs of n-tiles of the sums
+    constexpr int kSteps = D / 16;
     constexpr int kChunks = D / 8;   // 16-byte pieces of a key
     constexpr int kTile = kKvPage;   // keys of a tile
     extern __shared__ __align__(128) char smem[];
@@ -328,34 +295,21 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) kv_decode_kernel(const Kv
     while (!use.done) {
         const int32_t rows = use.q.q.rows * p.group;
         const int32_t n = p.shared_len + use.q.q.keys;
-        uint32_t qf[kSteps][4];
-        KvSpan sp[2];
-        int32_t pos[2];
-        float slope[2] = {0.0f, 0.0f};
+        KvRows16<T, D, kPlain> w;
+        w.begin(rows);
         const int prefix = p.prefix_len != nullptr ? p.prefix_len[use.s] : 0;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int r = row_a + 8 * x;
             const int i = kv_div_group(p, r), head = use.h * p.group + r - i * p.group;
-            pos[x] = n - use.q.q.rows + i;
-            sp[x] = KvSpan{0, 0, 0};
+            w.pos[x] = n - use.q.q.rows + i;
+            w.sp[x] = KvSpan{0, 0, 0};
             if (r < rows) {
-                sp[x] = kv_clip(kv_span(pos[x], n, prefix, p.window, p.causal != 0), p.shared_len, use.q.q.keys);
-                if (!kPlain && p.alibi != nullptr) slope[x] = p.alibi[head] * kLog2e;
+                w.sp[x] = kv_clip(kv_span(w.pos[x], n, prefix, p.window, p.causal != 0), p.shared_len, use.q.q.keys);
+                if (!kPlain && p.alibi != nullptr) w.slope[x] = p.alibi[head] * kLog2e;
             }
-            const char* src = p.q.data + (use.q.q.row0 + i) * p.q.row_stride + head * p.q.head_stride + 4 * (lane & 3);
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                qf[k][x] = r < rows ? *reinterpret_cast<const uint32_t*>(src + 32 * k) : 0u;
-                qf[k][2 + x] = r < rows ? *reinterpret_cast<const uint32_t*>(src + 32 * k + 16) : 0u;
-            }
+            w.load_q(x, p.q.data + (use.q.q.row0 + i) * p.q.row_stride + head * p.q.head_stride, r < rows);
         }
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // the weights' base (2^m) and sum
-        float acc[2 * kSteps][4];
-#pragma unroll
-        for (int i = 0; i < 2 * kSteps; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][e] = 0.0f;
         const int32_t t0 = use.t;
 
         for (; use.t < use.end; ++use.t) {
@@ -364,97 +318,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) kv_decode_kernel(const Kv
             __syncwarp();
             if ((live >> (S::kStages - 1)) & 1u) {
                 const uint32_t kb = ring + get * S::kStage, vb = kb + kTile * S::kRow;
-                float z[2][4] = {};
-                // piece 2 k + b of row r lies at (2 k + b) ^ (r % 8): k only flips bits of the address
-                const int krow = (lane & 7) + ((lane >> 4) << 3), vrow = (lane & 7) + (((lane >> 3) & 1) << 3);
-                const uint32_t ka = kb + krow * S::kRow + ((((lane >> 3) & 1) ^ (krow & 7)) << 4);
-                const uint32_t va = vb + vrow * S::kRow + (((lane >> 4) ^ (vrow & 7)) << 4);
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    uint32_t f[4];
-                    ldsm4(f, ka ^ (k << 5));
-                    mma<T>(z[0], qf[k], f[0], f[1]);
-                    mma<T>(z[1], qf[k], f[2], f[3]);
-                }
                 const int32_t j0 = use.q.tiles.at(use.t) * kTile;
-                // z[nt][2 x + e]: row row_a + 8 x, key j0 + 8 nt + 2 (lane % 4) + e.  Up to 8 rows the second half idles.
-                float base[2] = {0.0f, 0.0f}, top[2] = {m[0], m[1]};
-                bool grew = false;
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    if (8 * x >= rows) break;
-                    uint32_t y[4];  // y[2 nt + e]
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] = __float_as_uint(z[e / 2][2 * x + (e & 1)]);
-                    const int32_t j = j0 + 2 * (lane & 3);
-                    const bool inside = (j0 >= sp[x].lo && j0 + kTile <= sp[x].hi) || j0 + kTile <= sp[x].pre;
-                    const bool masked = __any_sync(0xffffffffu, !inside);
-                    auto sees = [&](int e) {
-                        const int32_t k = j + 8 * (e / 2) + (e & 1);
-                        return k < sp[x].pre || (k >= sp[x].lo && k < sp[x].hi);
-                    };
-                    if (!kPlain) {
-                        kv_cap<4>(p, y, masked, [&](int) { return (sees(0) ? 1u : 0u) | (sees(1) ? 2u : 0u) | (sees(2) ? 4u : 0u) | (sees(3) ? 8u : 0u); });
-                        if (p.alibi != nullptr) {
-                            const float d = static_cast<float>(p.shared_len + j - pos[x]);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                y[e] = __float_as_uint(fmaf(slope[x], d + static_cast<float>(8 * (e / 2) + (e & 1)), __uint_as_float(y[e])));
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * p.scale2);
-                    }
-                    if (masked) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (!sees(e)) y[e] = 0xff800000u;
-                    }
-                    float mx = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
-#pragma unroll
-                    for (int e = 2; e < 4; ++e) mx = fmaxf(mx, __uint_as_float(y[e]));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) - kShift<T>;
-                    grew |= mx > m[x];
-                    top[x] = fmaxf(mx, m[x]);
-                    base[x] = top[x] == -INFINITY ? 0.0f : top[x];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) z[e / 2][2 * x + (e & 1)] = __uint_as_float(y[e]);
-                }
-                if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const float keep = fast_exp2(m[x] - base[x]);
-                        m[x] = top[x];
-                        l[x] *= keep;
-#pragma unroll
-                        for (int i = 0; i < 2 * kSteps; ++i) {
-                            acc[i][2 * x] *= keep;
-                            acc[i][2 * x + 1] *= keep;
-                        }
-                    }
-                }
-                // weights: summed in 32 bits, rounded to the cache's type for the product with V
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const bool some = 8 * x < rows;
-#pragma unroll
-                    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                        for (int e = 2 * x; e < 2 * x + 2; ++e) {
-                            z[nt][e] = some ? fast_exp2(z[nt][e] - base[x]) : 0.0f;
-                            l[x] += z[nt][e];
-                        }
-                }
-                const uint32_t pf[4] = {Pack<T>::pair(z[0][0], z[0][1]), Pack<T>::pair(z[0][2], z[0][3]), Pack<T>::pair(z[1][0], z[1][1]),
-                                        Pack<T>::pair(z[1][2], z[1][3])};
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
-                    uint32_t f[4];
-                    ldsm4t(f, va ^ (i << 5));
-                    mma<T>(acc[2 * i], pf, f[0], f[1]);
-                    mma<T>(acc[2 * i + 1], pf, f[2], f[3]);
-                }
+                // (the rows of one token see the same keys, and the others are zeros)
+                const uint32_t odd = use.q.q.rows > 1 && w.cut(j0) ? w.odd_keys(vb) : 0u;
+                w.tile(p, kb, vb, j0, p.shared_len, odd, vb);
             }
             __syncwarp();
             get = get + 1 == S::kStages ? 0 : get + 1;
@@ -466,67 +333,31 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D>) kv_decode_kernel(const Kv
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             if (8 * x >= rows) break;
-            l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-            l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+            float l = w.l[x];
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
             const int r = row_a + 8 * x, i = kv_div_group(p, r), head = use.h * p.group + r - i * p.group;
             const int64_t row = use.q.q.row0 + i;
-            const float inv = !whole ? 1.0f : (l[x] == 0.0f ? 0.0f : 1.0f / l[x]);
+            if (r >= rows) continue;
+            const float inv = !whole ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
             char* dst = whole ? p.out.data + row * p.out.row_stride + head * p.out.head_stride : reinterpret_cast<char*>(slot + r * D);
             const bool wide = !whole || p.out_f32;
-            float odd = 0.0f;  // NaN once a sum is not finite
 #pragma unroll
             for (int y = 0; y < 2 * kSteps; ++y) {
-                odd = fmaf(acc[y][2 * x], 0.0f, odd);
-                odd = fmaf(acc[y][2 * x + 1], 0.0f, odd);
-                if (r < rows) {
-                    const float v0 = acc[y][2 * x] * inv, v1 = acc[y][2 * x + 1] * inv;
-                    if (wide) reinterpret_cast<float2*>(dst)[4 * y + (lane & 3)] = make_float2(v0, v1);
-                    else reinterpret_cast<uint32_t*>(dst)[4 * y + (lane & 3)] = Pack<T>::pair(v0, v1);
-                }
+                const float v0 = w.acc[y][2 * x] * inv, v1 = w.acc[y][2 * x + 1] * inv;
+                if (wide) reinterpret_cast<float2*>(dst)[4 * y + (lane & 3)] = make_float2(v0, v1);
+                else reinterpret_cast<uint32_t*>(dst)[4 * y + (lane & 3)] = Pack<T>::pair(v0, v1);
             }
-            if (r < rows && (lane & 3) == 0) {
+            if ((lane & 3) == 0) {
                 if (!whole) {
-                    slot[kRows * D + r] = m[x];
-                    slot[kRows * D + kRows + r] = l[x];
+                    slot[kRows * D + r] = w.m[x];
+                    slot[kRows * D + kRows + r] = l;
                 } else if (p.lse != nullptr) {
-                    p.lse[row * p.q_heads + head] = kv_lse(p, m[x], l[x]);
-                }
-            }
-            // (a weight sum that is not finite makes the row NaN as it is)
-            uint32_t redo = __ballot_sync(0xffffffffu, r < rows && odd != 0.0f && l[x] < INFINITY);
-            KvExact y;
-            if (redo != 0) {
-                y.table = b.table + use.s * b.table_stride;
-                y.tiles = use.q.tiles;
-                y.base = p.shared_len;
-                y.t0 = t0;
-                y.t1 = use.end;
-                y.size = kTile;
-                y.kvh = use.h;
-                y.seen = sp[x];
-                redo = kv_to_redo<T, D>(p, y, use.q.q.keys, redo);
-            }
-            // (other lanes write those rows again, behind the ordinary stores)
-            __syncwarp();
-            while (redo != 0) {
-                const int src = (__ffs(redo) - 1) & ~3;  // the row's first lane
-                redo &= ~(15u << src);
-                y.seen = KvSpan{__shfl_sync(0xffffffffu, sp[x].pre, src), __shfl_sync(0xffffffffu, sp[x].lo, src),
-                                __shfl_sync(0xffffffffu, sp[x].hi, src)};
-                y.pos = __shfl_sync(0xffffffffu, pos[x], src);
-                y.row = __shfl_sync(0xffffffffu, row, src);
-                y.head = __shfl_sync(0xffffffffu, head, src);
-                const float rb = __shfl_sync(0xffffffffu, m[x], src), ri = __shfl_sync(0xffffffffu, inv, src);
-                const uint64_t rd = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), src);
-                constexpr int kEach = D / 32;
-                float part[kEach];
-                kv_exact_row<T, D, kPlain>(p, y, rb, part);
-                for (int e = 0; e < kEach; ++e) {
-                    if (wide) reinterpret_cast<float*>(rd)[lane * kEach + e] = part[e] * ri;
-                    else reinterpret_cast<T*>(rd)[lane * kEach + e] = static_cast<T>(part[e] * ri);
+                    p.lse[row * p.q_heads + head] = kv_lse(p, w.m[x], l);
                 }
             }
         }
+        __syncwarp();
         use.next_unit(p);
     }
     copy_wait<0>();

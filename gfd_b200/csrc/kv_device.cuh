@@ -38,6 +38,10 @@ struct Pack<__nv_bfloat16> {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
+    static __device__ __forceinline__ void unpair(uint32_t w, float& a, float& b) {
+        a = __uint_as_float(w << 16);
+        b = __uint_as_float(w & 0xffff0000u);
+    }
     static __device__ __forceinline__ void store(char* p, const float (&f)[8]) {
         *reinterpret_cast<uint4*>(p) = make_uint4(pair(f[0], f[1]), pair(f[2], f[3]), pair(f[4], f[5]), pair(f[6], f[7]));
     }
@@ -57,6 +61,11 @@ struct Pack<__half> {
     static __device__ __forceinline__ uint32_t pair(float a, float b) {
         const __half2 h = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ void unpair(uint32_t w, float& a, float& b) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        a = v.x;
+        b = v.y;
     }
     static __device__ __forceinline__ void store(char* p, const float (&f)[8]) {
         *reinterpret_cast<uint4*>(p) = make_uint4(pair(f[0], f[1]), pair(f[2], f[3]), pair(f[4], f[5]), pair(f[6], f[7]));
@@ -177,173 +186,62 @@ __device__ __forceinline__ float kv_tanh2(const KvAttendParams& p, float x) {
     return fmaf(-2.0f * p.cap2, r, p.cap2);
 }
 
+// cap * tanh in base 2 of both products, |cap_x times them| up to 3/4: tanh x is x P(x^2) on the FMA units, P = 1 + ...
+// of degree 5 by least largest relative error (2^-24.9; 2^-22.9 with the roundings).
+__device__ __forceinline__ uint64_t kv_tanh2_small(const KvAttendParams& p, uint64_t z) {
+    const uint64_t x = mul2(z, pack2(p.cap_x, p.cap_x)), y = mul2(x, x);
+    uint64_t q = fma2(y, pack2(-0.004769490100443363f, -0.004769490100443363f), pack2(0.019664913415908813f, 0.019664913415908813f));
+    q = fma2(q, y, pack2(-0.0533902570605278f, -0.0533902570605278f));
+    q = fma2(q, y, pack2(0.13326521217823029f, 0.13326521217823029f));
+    q = fma2(q, y, pack2(-0.3333306908607483f, -0.3333306908607483f));
+    q = fma2(q, y, pack2(1.0f, 1.0f));
+    return mul2(mul2(q, x), pack2(p.cap2, p.cap2));
+}
+
 // N products of queries and keys to scores in base 2: scaled, capped where the call has a cap.
-// Where a thread's products all lie within three quarters of the cap (the usual case) tanh x is
-// x P(x^2) on the FMA units, P = 1 + ... of degree 5 by least largest relative error (2^-24.9;
-// 2^-22.9 with the roundings): the special-function unit, which the exponentials need, is left out.
-// The choice, and with it a result's last bits, goes by what the row sees and not by its neighbours: products
-// beyond that bound are looked for among the keys that `sees` (of 32 keys a word, asked where `masked`).
+// Where a thread's products all lie within three quarters of the cap tanh is a polynomial; usually those of the
+// whole warp do, and the special-function unit, which the exponentials need, is left out.  The choice, and
+// with it a result's last bits, goes by what the row sees and not by its neighbours: otherwise the largest
+// product is looked for among the keys that `sees` (of 32 keys a word, asked where `masked`).
 template <int N, typename F>
 __device__ __forceinline__ void kv_cap(const KvAttendParams& p, uint32_t* z, bool masked, F sees) {
     if (p.softcap > 0.0f) {
         float m = 0.0f;
 #pragma unroll
         for (int e = 0; e < N; ++e) m = fmaxf(m, fabsf(__uint_as_float(z[e])));
-        if (masked && m * fabsf(p.cap_x) > 0.75f) {
-            m = 0.0f;
-#pragma unroll
-            for (int k = 0; k < N; k += 32) {
-                const uint32_t some = sees(k);
-#pragma unroll
-                for (int e = k; e < k + 32 && e < N; ++e)
-                    if (some >> (e - k) & 1u) m = fmaxf(m, fabsf(__uint_as_float(z[e])));
-            }
-        }
-        if (m * fabsf(p.cap_x) <= 0.75f) {
-            const uint64_t sx = pack2(p.cap_x, p.cap_x), amp = pack2(p.cap2, p.cap2);
+        if (__all_sync(0xffffffffu, m * fabsf(p.cap_x) <= 0.75f)) {
 #pragma unroll
             for (int e = 0; e < N; e += 2) {
-                const uint64_t x = mul2(pack2(__uint_as_float(z[e]), __uint_as_float(z[e + 1])), sx), y = mul2(x, x);
-                uint64_t q = fma2(y, pack2(-0.004769490100443363f, -0.004769490100443363f), pack2(0.019664913415908813f, 0.019664913415908813f));
-                q = fma2(q, y, pack2(-0.0533902570605278f, -0.0533902570605278f));
-                q = fma2(q, y, pack2(0.13326521217823029f, 0.13326521217823029f));
-                q = fma2(q, y, pack2(-0.3333306908607483f, -0.3333306908607483f));
-                q = fma2(q, y, pack2(1.0f, 1.0f));
                 float a, b;
-                unpack2(mul2(mul2(q, x), amp), a, b);
+                unpack2(kv_tanh2_small(p, pack2(__uint_as_float(z[e]), __uint_as_float(z[e + 1]))), a, b);
                 z[e] = __float_as_uint(a);
                 z[e + 1] = __float_as_uint(b);
             }
         } else {
+            if (masked) {
+                m = 0.0f;
 #pragma unroll
-            for (int e = 0; e < N; ++e) z[e] = __float_as_uint(kv_tanh2(p, __uint_as_float(z[e]) * p.cap_x));
+                for (int k = 0; k < N; k += 32) {
+                    const uint32_t some = sees(k);
+#pragma unroll
+                    for (int e = k; e < k + 32 && e < N; ++e)
+                        if (some >> (e - k) & 1u) m = fmaxf(m, fabsf(__uint_as_float(z[e])));
+                }
+            }
+            const bool small = m * fabsf(p.cap_x) <= 0.75f;
+#pragma unroll
+            for (int e = 0; e < N; e += 2) {
+                const float x = __uint_as_float(z[e]), y = __uint_as_float(z[e + 1]);
+                float a, b;
+                unpack2(kv_tanh2_small(p, pack2(x, y)), a, b);
+                z[e] = __float_as_uint(small ? a : kv_tanh2(p, x * p.cap_x));
+                z[e + 1] = __float_as_uint(small ? b : kv_tanh2(p, y * p.cap_x));
+            }
         }
-        __syncwarp();
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) z[e] = __float_as_uint(__uint_as_float(z[e]) * p.scale2);
     }
-}
-
-// One score in base 2: scale and cap of the product, bias by distance.
-template <bool kPlain>
-__device__ __forceinline__ float kv_score2(const KvAttendParams& p, float dot, float slope, int32_t dist) {
-    if (kPlain) return dot * p.scale2;
-    const float z = p.softcap > 0.0f ? kv_tanh2(p, dot * p.cap_x) : dot * p.scale2;
-    return fmaf(slope * kLog2e, static_cast<float>(dist), z);
-}
-
-// A stretch of one sequence's keys that one packed row (row `row` of the batch at position
-// pos, query head `head`, KV head kvh) is summed over: keys [0, n) named by `table`, of which
-// key j stands at position base + j, in tiles [t0, t1) of `size` keys.
-struct KvExact {
-    const int32_t* table;
-    KvTiles tiles;
-    KvSpan seen;  // of this row
-    int32_t base, pos, t0, t1, size;
-    int64_t row;
-    int32_t head, kvh;
-};
-
-// Which rows (a lane each, bits of `odd`: their sums by matrix products are not finite) have to be summed
-// key by key: those with an element that is NaN or infinite in values which the row does not see
-// (0 * inf and 0 * NaN reached the sum), unless the values that it sees make that element NaN by themselves: a
-// NaN among them, or infinities of both signs.  (One infinity, or several of one sign, is a result of its own,
-// which a masked value must not turn into NaN.)  A row that is NaN in every element needs no further search.
-// keys: of the sequence; x.seen: of this lane's row.
-template <typename T, int D>
-__device__ __forceinline__ uint32_t kv_to_redo(const KvAttendParams& p, const KvExact& x, int32_t keys, uint32_t odd) {
-    constexpr uint32_t kMax = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;  // exponent of NaN and infinity
-    constexpr int kWords = D / 32;
-    const int lane = threadIdx.x & 31;
-    // a bit an element: infinities of one sign and the other among seen values (a NaN counts as both), any of
-    // them among the others
-    uint32_t plus[kWords] = {}, minus[kWords] = {}, out[kWords] = {};
-    for (int t = x.t0; t < x.t1; ++t)
-        for (int c = 0; c < x.size; c += 32) {
-            const int32_t j = x.tiles.at(t) * x.size + c + lane;
-            uint32_t up[kWords] = {}, down[kWords] = {}, any = 0;
-            if (c + lane < x.size && j < keys) {
-                const int32_t id = x.table[j / p.cache.block_tokens];
-                if (id >= 0 && id < p.cache.blocks) {
-                    const char* v = p.cache.v + id * p.cache.block_stride + j % p.cache.block_tokens * p.cache.token_stride +
-                                    x.kvh * p.cache.head_stride;
-#pragma unroll
-                    for (int e = 0; e < D; e += 2) {
-                        const uint32_t w = *reinterpret_cast<const uint32_t*>(v + 2 * e);
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            const uint32_t h = w >> (16 * y) & 0xffffu, bit = 1u << (e % 32 + y);
-                            if ((h & kMax) != kMax) continue;
-                            const bool nan = (h & 0x7fffu) != kMax;
-                            if (nan || h == kMax) up[e / 32] |= bit;
-                            if (nan || h != kMax) down[e / 32] |= bit;
-                        }
-                        any |= up[e / 32] | down[e / 32];
-                    }
-                }
-            }
-            for (uint32_t ball = __ballot_sync(0xffffffffu, any != 0); ball != 0; ball &= ball - 1) {
-                const int src = __ffs(ball) - 1;
-                const int32_t k = __shfl_sync(0xffffffffu, j, src);
-                const bool sees = k < x.seen.pre || (k >= x.seen.lo && k < x.seen.hi);
-                uint32_t all = 0xffffffffu;
-#pragma unroll
-                for (int i = 0; i < kWords; ++i) {
-                    const uint32_t u = __shfl_sync(0xffffffffu, up[i], src), d = __shfl_sync(0xffffffffu, down[i], src);
-                    plus[i] |= sees ? u : 0u;
-                    minus[i] |= sees ? d : 0u;
-                    out[i] |= sees ? 0u : u | d;
-                    all &= plus[i] & minus[i];
-                }
-                odd &= __ballot_sync(0xffffffffu, all != 0xffffffffu);
-                if (odd == 0) return 0;
-            }
-        }
-    uint32_t hit = 0;
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) hit |= out[i] & ~(plus[i] & minus[i]);
-    return odd & __ballot_sync(0xffffffffu, hit != 0);
-}
-
-// The sum of the row's weights times values, key by key and only over keys that it sees, by one
-// warp; lane i gets elements [i D / 32, (i + 1) D / 32).  m: what the weights are relative to,
-// in base 2.
-template <typename T, int D, bool kPlain>
-__device__ __forceinline__ void kv_exact_row(const KvAttendParams& p, const KvExact& x, float m, float* acc) {
-    constexpr int kEach = D / 32;
-    const int lane = threadIdx.x & 31;
-    const char* qrow = p.q.data + x.row * p.q.row_stride + x.head * p.q.head_stride;
-    const float slope = !kPlain && p.alibi != nullptr ? p.alibi[x.head] : 0.0f;
-    for (int e = 0; e < kEach; ++e) acc[e] = 0.0f;
-    for (int t = x.t0; t < x.t1; ++t)
-        for (int c = 0; c < x.size; c += 32) {
-            const int32_t j = x.tiles.at(t) * x.size + c + lane;
-            int64_t at = -1;
-            float w = 0.0f;
-            if (c + lane < x.size && (j < x.seen.pre || (j >= x.seen.lo && j < x.seen.hi))) {
-                const int32_t id = x.table[j / p.cache.block_tokens];
-                if (id >= 0 && id < p.cache.blocks) {
-                    at = id * p.cache.block_stride + j % p.cache.block_tokens * p.cache.token_stride + x.kvh * p.cache.head_stride;
-                    float dot = 0.0f;
-                    for (int e = 0; e < D; e += 8) {
-                        float a[8], b[8];
-                        Pack<T>::load(p.cache.k + at + 2 * e, a);
-                        Pack<T>::load(qrow + 2 * e, b);
-                        for (int y = 0; y < 8; ++y) dot = fmaf(a[y], b[y], dot);
-                    }
-                    const float z = kv_score2<kPlain>(p, dot, slope, x.base + j - x.pos);
-                    w = z == -INFINITY ? 0.0f : fast_exp2(z - m);
-                }
-            }
-            for (int y = 0; y < 32; ++y) {
-                const float wy = __shfl_sync(0xffffffffu, w, y);
-                const int64_t ay = __shfl_sync(0xffffffffu, at, y);
-                if (ay < 0 || wy == 0.0f) continue;
-                for (int e = 0; e < kEach; ++e)
-                    acc[e] = fmaf(wy, static_cast<float>(reinterpret_cast<const T*>(p.cache.v + ay)[lane * kEach + e]), acc[e]);
-            }
-        }
 }
 
 template <typename... P, typename... A>

@@ -21,7 +21,8 @@
 // Roles: warps 0-3 softmax of half A, 4-7 of half B; 8-11 write finished rows while the softmax
 // is in the next unit; 12 issues the products, 13 loads K and V (TMA boxes of 16 tokens x 64
 // elements, so that every page is found by its id), 14 loads Q (a box of the group's heads x rows where
-// the heads divide 128), 15 walks the units.  Units lie
+// the heads divide 128), 15 walks the units and watches over the others' waits.  Units whose values held a NaN
+// or an infinity are summed once more at the end (sum_again).  Units lie
 // on one line of tiles that the CTAs (one per SM) share evenly; a cut unit leaves partial sums
 // for kv_join_many_kernel, as in kv_decode.cu.
 
@@ -29,7 +30,8 @@
 
 #include <type_traits>
 
-#include "kv_device.cuh"
+#include "kv_rows.cuh"
+#include "kv_wait.cuh"
 
 namespace gfdb {
 namespace {
@@ -44,49 +46,7 @@ constexpr int kAux = 80, kMain = 176;  // registers of the helpers' and the soft
 // (1 to 3 come out alike within 2 %, 5 and 8 slower).
 constexpr int kUnitCost = 2;
 constexpr int kBadRing = 8;         // tiles whose bad pages are remembered
-
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-
-// ---- barriers: every wait is bounded ----
-__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n.reg .pred q;\nmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\nselp.u32 %0, 1, 0, q;\n}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-constexpr uint64_t kWaitLimitNs = 10000000000ull;  // rows summed key by key over a long cache keep others waiting
-__device__ __forceinline__ uint64_t clock_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
-// false: the wait ran out, or another warp's did
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-    uint64_t t0 = 0;
-    for (uint32_t i = 1; !bar_try(bar, parity); ++i) {
-        if ((i & 255u) != 0) continue;
-        if (*gave_up != 0) return false;
-        const uint64_t now = clock_ns();
-        if (t0 == 0) t0 = now;
-        if (now - t0 > kWaitLimitNs) {
-            *gave_up = 1;
-            return false;
-        }
-    }
-    return true;
-}
+constexpr int kOddUnits = 1024;     // units of a CTA that are marked one by one; the last mark is the others'
 
 // ---- tensor memory and products ----
 __device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t* r) {
@@ -379,6 +339,7 @@ struct Bars {
     uint64_t unit[kUnitRing], unit_read[kUnitRing];
     uint64_t q[2], q_read[2], s[2], p[2], p2[2];      // Q there / products with it done, scores, weights in two parts
     uint64_t o[2], o_read[2], ml[2], ml_read[2];      // sums done / taken, their base and weight sum
+    uint64_t done;                                    // all rows written
 };
 
 template <typename T>
@@ -458,6 +419,129 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
+// ---------------------------------------------------------------------------
+// Units whose sums met a NaN or an infinity
+// ---------------------------------------------------------------------------
+// A value that a row's mask hides reaches its sum as 0 * NaN, so units with sums that are not finite are summed
+// once more, by the softmax warps when the stretch is done and nothing waits: 128 rows at a time, 16 a warp, such
+// values taken out of the tile on its way into shared memory and added to the sums of the rows that see them
+// (KvRows16).  A result that is to be NaN or infinite comes out as that.  What a unit costs this way does not
+// depend on where such values lie.
+constexpr int kAgainThreads = 256;
+__device__ __forceinline__ void again_sync() { asm volatile("bar.sync 2, %0;" ::"n"(kAgainThreads) : "memory"); }
+
+template <typename T, int D, bool kPlain, bool kShared>
+__device__ __forceinline__ void sum_again(const KvAttendParams& p, const KvPlace& from, int64_t to, uint32_t smem, uint32_t* flags,
+                                          const uint8_t* marks) {
+    using Rows = KvRows16<T, D, kPlain>;
+    constexpr int kRow = 2 * D, kChunks = D / 8, kSub = kTile / kKvPage;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const uint32_t sk = smem, sv = sk + kTile * kRow, raw = sv + kTile * kRow;  // K, V without such values, V
+    const int pages = p.cache.block_tokens / kKvPage;
+    const int32_t base_key = kShared ? 0 : p.shared_len;
+    if (t < 2 * kSub) flags[t] = 0;
+    again_sync();
+    Cursor<kShared> c;
+    c.enter(p, from, to);
+    int turn = 0;
+    for (int i = 0; !c.done; ++i, c.next(p)) {
+        if (marks[min(i, kOddUnits - 1)] == 0) continue;
+        const Desc u = describe<kShared>(p, c.s, c.h, c.t, c.end, c.m.q, c.u);
+        const int32_t* table = kShared ? p.shared_table : p.batch.table + u.s * p.batch.table_stride;
+        const bool whole = u.nt == u.count;
+        for (int half = 0; half < u.packed; half += kHalf) {
+            const int first = half + warp * 16;
+            Rows w;
+            w.begin(max(0, min(16, u.packed - first)));
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int r = first + lane / 4 + 8 * x;
+                const int32_t packed = u.packed0 + (r < u.packed ? r : 0), of = kv_div_group(p, packed);
+                const int32_t head = u.h * p.group + packed - of * p.group;
+                w.sp[x] = row_span<kShared>(p, u, r, &w.pos[x], true);
+                if (!kPlain && p.alibi != nullptr) w.slope[x] = p.alibi[head] * kLog2e;
+                w.load_q(x, p.q.data + static_cast<int64_t>(u.row0 + of) * p.q.row_stride + head * p.q.head_stride, r < u.packed);
+            }
+            for (int k = 0; k < u.nt; ++k, turn ^= 1) {
+                const int32_t j0 = u.key(k);
+                uint32_t* flag = flags + turn * kSub;  // per 16 keys: bit 31 some are there, bit i key i's values are not all finite
+                for (int e = t; e < kTile * kChunks; e += kAgainThreads) {
+                    const int key = e / kChunks, piece = e % kChunks;
+                    const int32_t j = j0 + key, page = j / kKvPage;
+                    uint4 a = make_uint4(0, 0, 0, 0), v = a;
+                    if (j < u.pre || (j >= u.lo && j < u.hi)) {
+                        const int32_t in = kv_div_pages(p, page), id = table[in];
+                        if (id >= 0 && id < p.cache.blocks) {
+                            const int64_t at = id * p.cache.block_stride + ((page - in * pages) * kKvPage + j % kKvPage) * p.cache.token_stride +
+                                               u.h * p.cache.head_stride + 16 * piece;
+                            a = *reinterpret_cast<const uint4*>(p.cache.k + at);
+                            v = *reinterpret_cast<const uint4*>(p.cache.v + at);
+                            if (piece == 0) atomicOr(flag + key / kKvPage, 1u << 31);
+                            if ((kv_odd<T>(v.x) | kv_odd<T>(v.y) | kv_odd<T>(v.z) | kv_odd<T>(v.w)) != 0)
+                                atomicOr(flag + key / kKvPage, 1u << (key % kKvPage));
+                        }
+                    }
+                    const uint32_t to_piece = key * kRow + ((piece ^ (key & 7)) << 4);
+                    Rows::sts16(sk + to_piece, a.x, a.y, a.z, a.w);
+                    Rows::sts16(sv + to_piece, kv_finite<T>(v.x), kv_finite<T>(v.y), kv_finite<T>(v.z), kv_finite<T>(v.w));
+                    Rows::sts16(raw + to_piece, v.x, v.y, v.z, v.w);
+                }
+                again_sync();
+                if (t < kSub) flags[(turn ^ 1) * kSub + t] = 0;
+                if (w.rows > 0)
+                    for (int y = 0; y < kSub; ++y) {
+                        const uint32_t f = flag[y];
+                        if (f >> 31 == 0) continue;
+                        const uint32_t at = y * kKvPage * kRow;
+                        w.tile(p, sk + at, sv + at, j0 + y * kKvPage, base_key, f & 0xffffu, raw + at);
+                    }
+                again_sync();
+            }
+            float* slot = p.line.slots + (2 * static_cast<int64_t>(blockIdx.x) + (u.t0 == 0 ? 1 : 0)) * (static_cast<int64_t>(kRows) * (D + 2));
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                float l = w.l[x];
+                l += __shfl_xor_sync(0xffffffffu, l, 1);
+                l += __shfl_xor_sync(0xffffffffu, l, 2);
+                const int r = first + lane / 4 + 8 * x, d0 = 2 * (lane & 3);
+                if (r >= u.packed) continue;
+                if (!whole) {
+#pragma unroll
+                    for (int y = 0; y < D / 8; ++y) {
+                        const int d = 8 * y + d0;
+                        *reinterpret_cast<float2*>(slot + (static_cast<int64_t>(d / 4) * kRows + r) * 4 + d % 4) = make_float2(w.acc[y][2 * x], w.acc[y][2 * x + 1]);
+                    }
+                    if (d0 == 0) {
+                        slot[static_cast<int64_t>(kRows) * D + r] = w.m[x];
+                        slot[static_cast<int64_t>(kRows) * D + kRows + r] = l;
+                    }
+                    continue;
+                }
+                const int32_t packed = u.packed0 + r, of = kv_div_group(p, packed);
+                const int64_t row = u.row0 + of, place = row * p.q_heads + u.h * p.group + packed - of * p.group;
+                const int32_t head = u.h * p.group + packed - of * p.group;
+                const float own_lse = kShared ? p.own_lse[place] : -INFINITY;
+                if (kShared && __float_as_uint(own_lse) == kKvSkipped) continue;
+                const KvFinish f = kv_finish<kShared>(p, w.m[x], l, own_lse);
+                char* dst = p.out.data + row * p.out.row_stride + head * p.out.head_stride;
+#pragma unroll
+                for (int y = 0; y < D / 8; ++y) {
+                    const int d = 8 * y + d0;
+                    float a = w.acc[y][2 * x] * f.scale, b = w.acc[y][2 * x + 1] * f.scale;
+                    if (kShared && f.own != 0.0f) {
+                        const float2 o = *reinterpret_cast<const float2*>(p.own_out + place * D + d);
+                        a = fmaf(o.x, f.own, a);
+                        b = fmaf(o.y, f.own, b);
+                    }
+                    if (p.out_f32) *reinterpret_cast<float2*>(dst + 4 * d) = make_float2(a, b);
+                    else *reinterpret_cast<uint32_t*>(dst + 2 * d) = Pack<T>::pair(a, b);
+                }
+                if (p.lse != nullptr && d0 == 0) p.lse[place] = kv_lse(p, f.base, f.sum);
+            }
+        }
+    }
+}
+
 // kShared: the pass over a shared prefix
 template <typename T, int D, bool kPlain, bool kShared>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -469,8 +553,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ KvPlace s_place;
     __shared__ int64_t s_warps[kThreads / 32];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_gave_up;
+    __shared__ KvWaits s_waits;
     __shared__ uint32_t s_bad[kBadRing];
+    __shared__ uint8_t s_marks[kOddUnits];            // units to be summed again
+    __shared__ uint32_t s_flags[2 * kTile / kKvPage];  // of sum_again
     __shared__ Desc s_unit[kUnitRing];
     __shared__ float s_base[2][kHalf], s_sum[2][kHalf];
     __shared__ const char* s_rows[kRows];
@@ -480,7 +566,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     kv_let_next();
     if (t == 0) {
-        s_gave_up = 0;
+        s_waits.gave_up = 0;
+        s_waits.held = kShared;  // until the warps that write have waited for the passes over the own keys
+        s_waits.steps = 0;
         for (int i = 0; i < S::kSlots; ++i) {
             bar_init(smem_addr(&bars.full[i]), 1);
             bar_init(smem_addr(&bars.empty[i]), 1);
@@ -500,10 +588,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             bar_init(smem_addr(&bars.ml[i]), 4);
             bar_init(smem_addr(&bars.ml_read[i]), 4);
         }
+        bar_init(smem_addr(&bars.done), 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
 
+    for (int i = t; i < kOddUnits; i += kThreads) s_marks[i] = 0;
     if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(S::kColumns)
                      : "memory");
@@ -617,7 +707,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         return;
     }
     const uint32_t sq = smem_addr(smem), ring = sq + 2 * S::kOperand;
-    volatile int* gave_up = &s_gave_up;
+    volatile KvWaits* waits = &s_waits;
+    volatile int* gave_up = &s_waits.gave_up;
     // The next unit, read by a whole warp (every role takes every unit, in order).
     int unit = 0;
     auto take = [&](Desc* d) -> bool {
@@ -768,6 +859,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) bar_arrive(smem_addr(&bars.ml[x]));
         }
+        // the warps that write are done, and with them all copies and products
+        __syncwarp();
+        asm volatile("bar.sync 1, 384;" ::: "memory");
+        uint32_t some = 0;
+        for (int i = lane; i < kOddUnits; i += 32) some |= s_marks[i];
+        if (__any_sync(0xffffffffu, some != 0) && *gave_up == 0) {
+            if (kShared) kv_wait_last();
+            sum_again<T, D, kPlain, kShared>(p, s_place, stretch_end, sq, s_flags, s_marks);
+        }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAux));
         if (warp < 12) {
@@ -777,7 +877,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool wide = ((reinterpret_cast<uint64_t>(p.out.data) | p.out.row_stride | p.out.head_stride) & 31) == 0;
             uint32_t o_phase = 0;  // bit x
             bool good = true;
-            if (kShared) kv_wait_last();  // the results over the own keys, which finish here
+            if (kShared) {
+                kv_wait_last();  // the results over the own keys, which finish here
+                if (t == 8 * 32) waits->held = 0;
+            }
             // The unit is read where it lies, and given back when its rows are written: with a copy of it
             // in registers this loop's spilled, and with 2/3 of the SM's memory taken by
             // operands, what is spilled comes back from L2.
@@ -873,46 +976,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     unpack2(add2(odd0, odd1), odd, odd_c);
                     odd += odd_c;
                     // (a weight sum that is not finite makes the row NaN as it is)
-                    uint32_t redo = __ballot_sync(0xffffffffu, valid && odd != 0.0f && l < INFINITY);
-                    KvExact y;
-                    if (redo != 0) {
-                        y.table = kShared ? p.shared_table : b.table + u.s * b.table_stride;
-                        y.tiles = KvTiles{u.npre, u.first, u.count};
-                        y.base = kShared ? 0 : p.shared_len;
-                        y.t0 = u.t0;
-                        y.t1 = u.t0 + u.nt;
-                        y.size = kTile;
-                        y.kvh = u.h;
-                        y.seen = row_span<kShared>(p, u, r, &y.pos, true);
-                        redo = kv_to_redo<T, D>(p, y, u.keys, redo);
-                    }
-                    // (other lanes write those rows again, behind the ordinary stores)
-                    __syncwarp();
-                    for (; redo != 0; redo &= redo - 1) {
-                        const int src = __ffs(redo) - 1;
-                        const int rs = x * kHalf + (warp & 3) * 32 + src;
-                        y.seen = row_span<kShared>(p, u, rs, &y.pos, true);
-                        y.row = __shfl_sync(0xffffffffu, row, src);
-                        y.head = __shfl_sync(0xffffffffu, head, src);
-                        const float rb = __shfl_sync(0xffffffffu, base, src), rf = __shfl_sync(0xffffffffu, f.scale, src);
-                        const float ro = __shfl_sync(0xffffffffu, f.own, src);
-                        const uint64_t rd = __shfl_sync(0xffffffffu, dst, src);
-                        constexpr int kEach = D / 32;
-                        float part[kEach];
-                        kv_exact_row<T, D, kPlain>(p, y, rb, part);
-                        for (int e = 0; e < kEach; ++e) {
-                            const int d = lane * kEach + e;
-                            float v = part[e] * rf;
-                            if (kShared && ro != 0.0f) v = fmaf(p.own_out[(y.row * p.q_heads + y.head) * D + d], ro, v);
-                            if (!whole) slot[(static_cast<int64_t>(d / 4) * kRows + rs) * 4 + d % 4] = v;
-                            else if (p.out_f32) reinterpret_cast<float*>(rd)[d] = v;
-                            else reinterpret_cast<T*>(rd)[d] = static_cast<T>(v);
-                        }
-                    }
+                    const uint32_t again = __ballot_sync(0xffffffffu, valid && odd != 0.0f && l < INFINITY);
+                    if (again != 0 && lane == 0) *const_cast<volatile uint8_t*>(&s_marks[min(unit, kOddUnits - 1)]) = 1;
                 }
                 __syncwarp();
                 if (lane == 0) bar_arrive(smem_addr(&bars.unit_read[unit % kUnitRing]));
             }
+            __syncwarp();
+            if (lane == 0) bar_arrive(smem_addr(&bars.done));
+            asm volatile("bar.arrive 1, 384;" ::: "memory");
         } else if (warp == 12) {
             // ---- products: the whole warp walks, one thread issues ----
             int slot = 0;
@@ -933,6 +1005,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int j = j0; j < j1; ++j) mma_ts(tmem + S::kO + x * D, tmem + x * kTile + j * 8, c + j * (2048 >> 4), kPv, add || j > 0);
             };
+            uint32_t steps = 0;
             Desc u;
             bool good = true;
             while (good && take(&u)) {
@@ -995,6 +1068,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     slot = k;
                     if (more) slot = k + 1 == S::kSlots ? 0 : k + 1;
+                    if (lane == 0) waits->steps = ++steps;
                 }
             }
         } else if (warp == 13) {
@@ -1061,15 +1135,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-            if (*gave_up != 0) {
-                // the copies in flight land before the block ends: `full` flips once more for each slot
-                // that was filled and not yet waited for
-                for (int i = 0; i < S::kSlots; ++i) {
-                    const uint64_t t0 = clock_ns();
-                    while (!bar_try(smem_addr(&bars.full[i]), ((phase >> i) & 1u) ^ 1u) && clock_ns() - t0 < kWaitLimitNs) {
-                    }
-                }
-            }
+            // the copies in flight land before the block ends: `full` flips once more for each slot that was filled
+            for (int i = 0; *gave_up != 0 && i < S::kSlots; ++i) bar_drain(smem_addr(&bars.full[i]), ((phase >> i) & 1u) ^ 1u);
         } else if (warp == 14) {
             // ---- Q ----
             uint32_t phase = 0;  // bit x
@@ -1093,14 +1160,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             tma_rows(sq + x * S::kOperand + lane * S::kBlock, &map_q, lane * 64, head, row + x * by, there);
                     }
                 }
-                if (*gave_up != 0) {
-                    // the copies in flight land before the block ends
-                    for (int x = 0; x < 2; ++x) {
-                        const uint64_t t0 = clock_ns();
-                        while (!bar_try(smem_addr(&bars.q[x]), ((phase >> x) & 1u) ^ 1u) && clock_ns() - t0 < kWaitLimitNs) {
-                        }
-                    }
-                }
+                for (int x = 0; *gave_up != 0 && x < 2; ++x) bar_drain(smem_addr(&bars.q[x]), ((phase >> x) & 1u) ^ 1u);  // likewise
             }
             // groups and strides that no box has: every row by neighbouring lanes, zeros for rows that do not exist
             constexpr int kLanes = D / 8, kPer = 32 / kLanes;  // lanes of a row, rows a step
@@ -1142,20 +1202,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         } else {
-            // ---- the units of the stretch; the first one is there ----
+            // ---- the units of the stretch; the first one is there.  This warp watches over the others' waits ----
             if (lane == 0) bar_arrive(smem_addr(&bars.unit[0]));
             Cursor<kShared> c;
             c.enter(p, s_place, stretch_end);
             for (int i = 1; !c.done; ++i) {
                 c.next(p);
                 const int k = i % kUnitRing;
-                if (!bar_wait(smem_addr(&bars.unit_read[k]), ((i / kUnitRing) & 1) ^ 1, gave_up)) break;
+                if (!bar_watch(smem_addr(&bars.unit_read[k]), ((i / kUnitRing) & 1) ^ 1, waits)) break;
                 if (lane == 0) {
                     s_unit[k] = describe<kShared>(p, c.s, c.h, c.t, c.done ? c.t : c.end, c.m.q, c.u);
                     bar_arrive(smem_addr(&bars.unit[k]));
                 }
                 __syncwarp();
             }
+            bar_watch(smem_addr(&bars.done), 0, waits);
         }
     }
 
@@ -1163,7 +1224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tm_before();
     __syncthreads();
     tm_after();
-    if (t == 0 && s_gave_up != 0) kv_report(p.status, GFD_KV_GAVE_UP);
+    if (t == 0 && s_waits.gave_up != 0) kv_report(p.status, GFD_KV_GAVE_UP);
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns) : "memory");
     kv_wait_last();
 }

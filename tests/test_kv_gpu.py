@@ -1017,3 +1017,88 @@ def test_attend_bits_do_not_depend_on_what_a_row_does_not_see(gpu_ctx, dtype, d,
     rest = [r for r in rows if r not in rows[::3]]
     torch.cuda.synchronize()
     assert torch.equal(a[rest], c[rest]) and torch.equal(la[rest], lc[rest])
+
+
+@pytest.mark.parametrize("poison", [NAN, INF])
+@pytest.mark.parametrize("dtype,heads,group,d,rows,keys,kw", [
+    ("bf16", 1, 2, 64, 300, 200000, {}), ("fp16", 1, 4, 128, 40, 150000, dict(window=90000)),
+    ("bf16", 2, 3, 128, 20, 60000, dict(softcap=30.0, alibi=True)), ("fp16", 2, 4, 64, 4, 300000, {})])
+def test_attend_masked_nan_in_a_long_context(gpu_ctx, dtype, heads, group, d, rows, keys, kw, poison):
+    """The last keys, which only the last rows see, hold NaN or infinities: the other rows are summed as without
+    them, in a time of the same order, and no wait runs out."""
+    torch = torch_()
+    s = Setup(gpu_ctx, dtype, heads, group, d, 64, [rows], [keys], seed=68)
+    kw = dict(kw)
+    if kw.pop("alibi", False):
+        kw["alibi"] = s.slopes()
+    want = s.want(**kw)
+    out, ws = torch.empty(rows, s.hq, d, device="cuda", dtype=s.dt), s.workspace(rows)
+    a, b, c = (torch.cuda.Event(enable_timing=True) for _ in range(3))
+    s.attend(out=out, workspace=ws, **kw)
+    a.record()
+    s.attend(out=out, workspace=ws, **kw)
+    b.record()
+    torch.cuda.synchronize()
+    n = max(1, rows // 10)
+    for j in range(keys - n, keys):
+        put(s, 0, j, slice(None), poison)
+    b.record()
+    got, lse = s.attend(out=out, workspace=ws, **kw)
+    c.record()
+    torch.cuda.synchronize()
+    assert int(s.status) == 0
+    oracle.check_attend(got, lse, want, slice(0, rows - n))
+    assert not bool(torch.isfinite(got[rows - n:].float()).any())
+    assert bool(torch.isfinite(lse).all())
+    assert b.elapsed_time(c) < 200  # ms; without the NaN the calls take about one
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_mixed_units_with_and_without_nan(gpu_ctx, d):
+    """Units of one stretch: some met a masked NaN, some an infinity that rows see, most nothing of the kind."""
+    torch = torch_()
+    q_lens = [90, 3, 200, 64, 1, 130, 70, 300]
+    kv_lens = [100, 40, 700, 64, 90, 1000, 200, 300]
+    s = Setup(gpu_ctx, "fp16", 8, 4, d, 16, q_lens, kv_lens, seed=69)
+    want = s.want()
+    ends = [b - 1 for b in s.row_start[1:]]
+    for i in (0, 3, 5, 7):
+        put(s, i, kv_lens[i] - 1, slice(None), NAN)
+    at = kv_lens[2] - 100
+    put(s, 2, at, 7, INF)
+    got, lse = s.attend()
+    torch.cuda.synchronize()
+    assert int(s.status) == 0
+    inf_rows = [s.row_start[2] + r for r in range(200) if kv_lens[2] - 200 + r >= at]
+    bad = {ends[i] for i in (0, 3, 5, 7)}
+    rows = [r for r in range(s.rows) if r not in bad]
+    cut = lambda x, e: x[:, :, e] if x.dim() == 3 else x
+    keep = [e for e in range(d) if e != 7]
+    oracle.check_attend(got[:, :, keep], lse, tuple(cut(x, keep) for x in want), rows)
+    oracle.check_attend(got[:, :, 7:8], lse, tuple(cut(x, [7]) for x in want), [r for r in rows if r not in set(inf_rows)])
+    assert bool((got[inf_rows][:, :, 7] == INF).all()) and bool(torch.isnan(got[sorted(bad)].float()).all())
+
+
+@pytest.mark.parametrize("kw", [{}, dict(softcap=20.0)])
+@pytest.mark.parametrize("d,out_dtype", [(64, "fp32"), (128, None)])
+def test_shared_masked_nan(gpu_ctx, d, out_dtype, kw):
+    """A shared prefix whose first keys a window hides from most rows, and own keys that only the last rows see, hold NaN."""
+    torch = torch_()
+    q_lens, kv_lens = [1, 3, 90, 1, 200], [30, 12, 95, 1, 260]
+    s = Setup(gpu_ctx, "bf16", 2, 4, d, 16, q_lens, kv_lens, seed=70, shared_len=600)
+    window = 400
+    want = s.want(window=window, **kw)
+    first = [600 + n - m + i - window + 1 for n, m in zip(kv_lens, q_lens) for i in range(m)]
+    j = min(first) + 2
+    s.v[int(s.shared_table[j // 16]), j % 16] = NAN
+    for i in (1, 2, 4):
+        put(s, i, kv_lens[i] - 1, slice(None), INF)
+    got, lse = s.attend(out_dtype=out_dtype, window=window, **kw)
+    torch.cuda.synchronize()
+    assert int(s.status) == 0
+    ends = [s.row_start[i + 1] - 1 for i in (1, 2, 4)]
+    nan = [r for r, f in enumerate(first) if f <= j]
+    rows = [r for r in range(s.rows) if r not in set(ends) | set(nan)]
+    assert nan and rows
+    oracle.check_attend(got, lse, want, rows)
+    assert bool(torch.isnan(got[nan].float()).all()) and not bool(torch.isfinite(got[ends].float()).any())
