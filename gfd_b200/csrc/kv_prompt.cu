@@ -339,7 +339,7 @@ struct Bars {
     uint64_t unit[kUnitRing], unit_read[kUnitRing];
     uint64_t q[2], q_read[2], s[2], p[2], p2[2];      // Q there / products with it done, scores, weights in two parts
     uint64_t o[2], o_read[2], ml[2], ml_read[2];      // sums done / taken, their base and weight sum
-    uint64_t done;                                    // all rows written
+    uint64_t last, done;                              // all products done, all rows written
 };
 
 template <typename T>
@@ -588,6 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bar_init(smem_addr(&bars.ml[i]), 4);
             bar_init(smem_addr(&bars.ml_read[i]), 4);
         }
+        bar_init(smem_addr(&bars.last), 1);
         bar_init(smem_addr(&bars.done), 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1071,6 +1072,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) waits->steps = ++steps;
                 }
             }
+            // tensor memory and the operands stay until the last product is done
+            if (elect_one()) tm_commit(smem_addr(&bars.last));
+            __syncwarp();
+            bar_drain(smem_addr(&bars.last), 0);
         } else if (warp == 13) {
             // ---- K and V ----
             int slot = 0, seen = 0;  // seen: tiles so far
@@ -1136,7 +1141,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             // the copies in flight land before the block ends: `full` flips once more for each slot that was filled
-            for (int i = 0; *gave_up != 0 && i < S::kSlots; ++i) bar_drain(smem_addr(&bars.full[i]), ((phase >> i) & 1u) ^ 1u);
+            for (int i = 0; i < S::kSlots; ++i) bar_drain(smem_addr(&bars.full[i]), ((phase >> i) & 1u) ^ 1u);
         } else if (warp == 14) {
             // ---- Q ----
             uint32_t phase = 0;  // bit x
@@ -1160,7 +1165,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             tma_rows(sq + x * S::kOperand + lane * S::kBlock, &map_q, lane * 64, head, row + x * by, there);
                     }
                 }
-                for (int x = 0; *gave_up != 0 && x < 2; ++x) bar_drain(smem_addr(&bars.q[x]), ((phase >> x) & 1u) ^ 1u);  // likewise
+                for (int x = 0; x < 2; ++x) bar_drain(smem_addr(&bars.q[x]), ((phase >> x) & 1u) ^ 1u);  // likewise
             }
             // groups and strides that no box has: every row by neighbouring lanes, zeros for rows that do not exist
             constexpr int kLanes = D / 8, kPer = 32 / kLanes;  // lanes of a row, rows a step
