@@ -425,8 +425,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // A value that a row's mask hides reaches its sum as 0 * NaN, so units with sums that are not finite are summed
 // once more, by the softmax warps when the stretch is done and nothing waits: 128 rows at a time, 16 a warp, such
 // values taken out of the tile on its way into shared memory and added to the sums of the rows that see them
-// (KvRows16).  A result that is to be NaN or infinite comes out as that.  What a unit costs this way does not
-// depend on where such values lie.
+// (KvRows16).  A result that is to be NaN or infinite comes out as that.  8192 causal rows of 32 heads of 128 take
+// 1.8 ms when the last key alone holds a NaN and 5.3 ms when every unit meets one, 0.50 ms otherwise.
 constexpr int kAgainThreads = 256;
 __device__ __forceinline__ void again_sync() { asm volatile("bar.sync 2, %0;" ::"n"(kAgainThreads) : "memory"); }
 

@@ -65,9 +65,11 @@ struct KvRows16 {
     float m[2], l[2];              // the weights' base (2^m) and sum; l: this lane's share
     float acc[2 * kSteps][4];
     int32_t rows;                  // rows that exist
+    bool spent;                    // all their sums are NaN
 
     __device__ __forceinline__ void begin(int32_t rows_) {
         rows = rows_;
+        spent = false;
         m[0] = m[1] = -INFINITY;
         l[0] = l[1] = slope[0] = slope[1] = 0.0f;
 #pragma unroll
@@ -214,6 +216,7 @@ struct KvRows16 {
         return keys;
     }
     __device__ __forceinline__ void add_odd(uint32_t vb, int32_t j0, uint32_t keys) {
+        if (spent) return;
         for (; keys != 0; keys &= keys - 1) {
             const int k = __ffs(keys) - 1;
             const bool s0 = sees(0, j0 + k), s1 = sees(1, j0 + k);
@@ -231,6 +234,14 @@ struct KvRows16 {
                 if (s1) acc[i][2] += a, acc[i][3] += b;
             }
         }
+        bool left = false;
+        const int r = (threadIdx.x & 31) >> 2;
+#pragma unroll
+        for (int i = 0; i < 2 * kSteps; ++i) {
+            if (r < rows) left |= acc[i][0] == acc[i][0] || acc[i][1] == acc[i][1];
+            if (r + 8 < rows) left |= acc[i][2] == acc[i][2] || acc[i][3] == acc[i][3];
+        }
+        spent = !__any_sync(0xffffffffu, left);
     }
     static __device__ __forceinline__ void clear_odd(uint32_t vb) {
         for (int i = threadIdx.x & 31; i < kTile * kRow / 16; i += 32) {
