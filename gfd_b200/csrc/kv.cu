@@ -60,9 +60,8 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const KvAp
     if (t >= kAppendThreads - 32) {
         const int r = t - (kAppendThreads - 32);
         if (r < nrows && s_seq[r] >= 0) {
-            int32_t place;
-            const int32_t block = kv_block(b, s_seq[r], s_place[r], p.cache.block_tokens, nullptr, 0, &place);
-            s_place[r] = place;
+            const int32_t token = s_place[r], bt = p.cache.block_tokens, block = b.table[s_seq[r] * b.table_stride + token / bt];
+            s_place[r] = token % bt;
             s_block[r] = block >= 0 && block < p.cache.blocks ? block : -1;
             if (s_block[r] < 0) kv_report(p.status, GFD_KV_BAD_PAGE);
         }

@@ -104,18 +104,6 @@ __device__ __forceinline__ void kv_report(uint32_t* status, uint32_t bits) {
     if (status != nullptr && bits != 0) atomicOr(status, bits);
 }
 
-// Block id and place of token j of a sequence (its own table behind the shared prefix).
-__device__ __forceinline__ int32_t kv_block(const KvBatchView& b, int s, int32_t j, int32_t bt, const int32_t* shared_table,
-                                            int32_t shared_len, int32_t* place) {
-    const int32_t* t = shared_table;
-    if (j >= shared_len) {
-        t = b.table + s * b.table_stride;
-        j -= shared_len;
-    }
-    *place = j % bt;
-    return t[j / bt];
-}
-
 // What CTA c's cut leaves to join, for the CTA whose stretch begins at `at`.
 __device__ __forceinline__ KvCut kv_cut(const KvCuts& cuts, uint32_t c, const KvPlace& at) {
     KvCut k{0, at.row0, at.packed0, at.packed, at.h};
