@@ -158,6 +158,16 @@ __device__ __forceinline__ void tma_rows_ahead(const CUtensorMap* map, int x, in
 // ---------------------------------------------------------------------------
 // Units
 // ---------------------------------------------------------------------------
+// What the rows of sequence s see of the shared prefix together: the first of them sees furthest back.  All of it
+// behind the prefix or in a skipped or empty sequence: nothing.
+__device__ __forceinline__ KvSpan seen_of_prefix(const KvAttendParams& p, int s) {
+    const KvBatchView& b = p.batch;
+    const KvSeq q = kv_seq(b.row_start[s], b.row_start[s + 1], b.kv_len[s], b.capacity, p.max_q_len);
+    if (!q.ok || q.rows == 0) return KvSpan{0, p.shared_len, p.shared_len};
+    const int32_t n = p.shared_len + q.keys, prefix = p.prefix_len != nullptr ? p.prefix_len[s] : 0;
+    return kv_clip(kv_span(n - q.rows, n, prefix, p.window, p.causal != 0), 0, p.shared_len);
+}
+
 // What the launch walks over: the sequences with many rows, or (shared pass) all rows of the
 // batch as one sequence against the shared prefix.
 struct Many {
@@ -188,17 +198,15 @@ struct Unit {
     int32_t packed0, packed;
 };
 
+// seen: what the batch's rows see together of the shared prefix (shared pass)
 template <bool kShared>
-__device__ __forceinline__ Unit many_unit(const KvAttendParams& p, int s, const KvSeq& q, int rt) {
+__device__ __forceinline__ Unit many_unit(const KvAttendParams& p, int s, const KvSeq& q, int rt, const KvSpan& seen) {
     Unit u;
     const int64_t packed = static_cast<int64_t>(q.rows) * p.group;
     u.packed0 = rt * kRows;
     u.packed = static_cast<int32_t>(min(static_cast<int64_t>(kRows), packed - u.packed0));
     if (kShared) {
-        // every row stands behind the prefix; with a window the rows nearest to it see most
-        u.all = KvSpan{0, 0, p.shared_len};
-        if (p.window > 0 && p.prefix_len == nullptr) u.all.lo = min(p.shared_len, max(0, p.shared_len + 1 - p.window));
-        if (p.window > 0 && u.all.lo >= p.shared_len) u.all.hi = u.all.lo = p.shared_len;
+        u.all = seen;
     } else {
         const int32_t n = p.shared_len + q.keys, pos0 = n - q.rows;
         const int32_t prefix = p.prefix_len != nullptr ? p.prefix_len[s] : 0;
@@ -220,7 +228,7 @@ struct Cursor {
     int64_t begin, to;         // of the unit's first tile, and of the stretch's end, on the line
     bool done;
 
-    __device__ __forceinline__ void enter(const KvAttendParams& p, const KvPlace& at, int64_t to_) {
+    __device__ __forceinline__ void enter(const KvAttendParams& p, const KvPlace& at, int64_t to_, const KvSpan& seen) {
         s = at.s;
         h = at.h;
         rt = at.packed0 / kRows;
@@ -228,7 +236,7 @@ struct Cursor {
         begin = at.begin;
         to = to_;
         m = many_seq<kShared>(p, s);
-        u = many_unit<kShared>(p, s, m.q, rt);
+        u = many_unit<kShared>(p, s, m.q, rt, seen);
         clamp();
     }
     __device__ __forceinline__ void clamp() {
@@ -236,7 +244,7 @@ struct Cursor {
         done = t >= end;
     }
     // The line runs over KV heads, within a head over sequences, within a sequence over row tiles.
-    __device__ __forceinline__ void next(const KvAttendParams& p) {
+    __device__ __forceinline__ void next(const KvAttendParams& p, const KvSpan& seen) {
         begin += u.tiles.count + kUnitCost;
         if (begin >= to) {
             done = true;
@@ -253,7 +261,7 @@ struct Cursor {
                 m = many_seq<kShared>(p, s);
             } while (m.tiles == 0);
         }
-        u = many_unit<kShared>(p, s, m.q, rt);
+        u = many_unit<kShared>(p, s, m.q, rt, seen);
         clamp();
     }
 };
@@ -432,7 +440,7 @@ __device__ __forceinline__ void again_sync() { asm volatile("bar.sync 2, %0;" ::
 
 template <typename T, int D, bool kPlain, bool kShared>
 __device__ __forceinline__ void sum_again(const KvAttendParams& p, const KvPlace& from, int64_t to, uint32_t smem, uint32_t* flags,
-                                          const uint8_t* marks) {
+                                          const uint8_t* marks, const KvSpan& seen) {
     using Rows = KvRows16<T, D, kPlain>;
     constexpr int kRow = 2 * D, kChunks = D / 8, kSub = kTile / kKvPage;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -442,9 +450,9 @@ __device__ __forceinline__ void sum_again(const KvAttendParams& p, const KvPlace
     if (t < 2 * kSub) flags[t] = 0;
     again_sync();
     Cursor<kShared> c;
-    c.enter(p, from, to);
+    c.enter(p, from, to, seen);
     int turn = 0;
-    for (int i = 0; !c.done; ++i, c.next(p)) {
+    for (int i = 0; !c.done; ++i, c.next(p, seen)) {
         if (marks[min(i, kOddUnits - 1)] == 0) continue;
         const Desc u = describe<kShared>(p, c.s, c.h, c.t, c.end, c.m.q, c.u);
         const int32_t* table = kShared ? p.shared_table : p.batch.table + u.s * p.batch.table_stride;
@@ -551,6 +559,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ char smem_raw[];
     __shared__ Bars bars;
     __shared__ KvPlace s_place;
+    __shared__ KvSpan s_seen;                         // of the shared prefix, by the batch's rows together
+    __shared__ int32_t s_reach[kThreads / 32][2];
     __shared__ int64_t s_warps[kThreads / 32];
     __shared__ uint32_t s_tmem;
     __shared__ KvWaits s_waits;
@@ -614,10 +624,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int per = (b.seqs + kThreads - 1) / kThreads, s_lo = min(t * per, b.seqs), s_hi = min(s_lo + per, b.seqs);
         int64_t mine = 0, row_tiles = 0;
         bool bad_starts = false;
+        int32_t pre = 0, lo = p.shared_len;
         for (int s = s_lo; s < s_hi; ++s) {
             const int32_t from = b.row_start[s], to = b.row_start[s + 1];
             bad_starts |= from < 0 || from > to || to > b.rows;
-            if (kShared) continue;
+            if (kShared) {
+                if (p.window > 0) {
+                    const KvSpan x = seen_of_prefix(p, s);
+                    pre = max(pre, x.pre);
+                    lo = min(lo, x.lo);
+                }
+                continue;
+            }
             const Many m = many_seq<kShared>(p, s);
             if (m.bad && blockIdx.x == 0) {
                 kv_report(p.status, GFD_KV_BAD_LENGTH);
@@ -625,10 +643,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             mine += m.tiles;
         }
+        if (kShared) {
+            pre = __reduce_max_sync(0xffffffffu, pre);
+            lo = __reduce_min_sync(0xffffffffu, lo);
+            if (lane == 0) {
+                s_reach[warp][0] = pre;
+                s_reach[warp][1] = lo;
+            }
+        }
         const bool ok = __syncthreads_or(bad_starts) == 0;
         if (!ok && blockIdx.x == 0 && t == 0) kv_report(p.status, GFD_KV_BAD_LENGTH);
         const int seqs = !ok ? 0 : (kShared ? 1 : b.seqs);
         if (kShared) {
+            for (int w = 0; w < kThreads / 32; ++w) {
+                pre = max(pre, s_reach[w][0]);
+                lo = min(lo, s_reach[w][1]);
+            }
+            // (without a window every row sees all of it)
+            if (p.window == 0) lo = 0;
+            if (t == 0) s_seen = lo < p.shared_len ? KvSpan{pre, max(lo, pre), p.shared_len} : KvSpan{pre, pre, pre};
             first[0] = 0;
             row_tiles = ok ? many_seq<kShared>(p, 0).tiles : 0;
         } else {
@@ -663,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int64_t u = u0; u < u1; ++u) {
                 while (u - first[s] >= m.tiles) m = many_seq<kShared>(p, ++s);
                 const int rt = static_cast<int>(u - first[s]);
-                const Unit x = many_unit<kShared>(p, s, m.q, rt);
+                const Unit x = many_unit<kShared>(p, s, m.q, rt, s_seen);
                 if (want >= here && want < here + x.tiles.count + kUnitCost) {
                     const int64_t begin = head * per_head + here + kUnitCost;
                     const int32_t t0 = static_cast<int32_t>(max(want - here - kUnitCost, static_cast<int64_t>(0)));
@@ -867,7 +900,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = lane; i < kOddUnits; i += 32) some |= s_marks[i];
         if (__any_sync(0xffffffffu, some != 0) && *gave_up == 0) {
             if (kShared) kv_wait_last();
-            sum_again<T, D, kPlain, kShared>(p, s_place, stretch_end, sq, s_flags, s_marks);
+            sum_again<T, D, kPlain, kShared>(p, s_place, stretch_end, sq, s_flags, s_marks, s_seen);
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAux));
@@ -1210,9 +1243,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ---- the units of the stretch; the first one is there.  This warp watches over the others' waits ----
             if (lane == 0) bar_arrive(smem_addr(&bars.unit[0]));
             Cursor<kShared> c;
-            c.enter(p, s_place, stretch_end);
+            c.enter(p, s_place, stretch_end, s_seen);
             for (int i = 1; !c.done; ++i) {
-                c.next(p);
+                c.next(p, s_seen);
                 const int k = i % kUnitRing;
                 if (!bar_watch(smem_addr(&bars.unit_read[k]), ((i / kUnitRing) & 1) ^ 1, waits)) break;
                 if (lane == 0) {

@@ -1102,3 +1102,88 @@ def test_shared_masked_nan(gpu_ctx, d, out_dtype, kw):
     assert nan and rows
     oracle.check_attend(got, lse, want, rows)
     assert bool(torch.isnan(got[nan].float()).all()) and not bool(torch.isfinite(got[ends].float()).any())
+
+
+def test_attend_padding_is_not_reported(gpu_ctx):
+    """Empty sequences, whatever their lengths and tables say, a batch of none and a call of no rows: no status, nothing written."""
+    torch = torch_()
+    q_lens, kv_lens = [0, 90, 0, 0, 1, 0, 3, 0], [0, 90, 0, 0, 50, 0, 64, 0]
+    for shared_len in (0, 40):
+        s = Setup(gpu_ctx, "bf16", 2, 4, 128, 16, q_lens, kv_lens, seed=71, spare_rows=9, shared_len=shared_len)
+        empty = [i for i, n in enumerate(q_lens) if n == 0]
+        s.lens[empty] = torch.tensor([0, -5, 10 ** 9, 7, 1], dtype=torch.int32, device="cuda")
+        s.table[empty] = -1
+        s.check()
+        st = torch.cuda.current_stream()
+        none = kv.Batch(torch.zeros(1, dtype=torch.int32, device="cuda"), s.lens[:0], s.table[:0])
+        out, ws = torch.full_like(s.q, 7.0), s.workspace()
+        for batch, q, o in ((none, s.q, out), (s.batch, s.q[:0], out[:0])):
+            if shared_len:
+                s.cache.attend_shared(batch, s.shared_table, shared_len, q, o, workspace=ws, status=s.status, stream=st)
+            else:
+                s.cache.attend(batch, q, o, workspace=ws, status=s.status, stream=st)
+        torch.cuda.synchronize()
+        assert bool((out == 7).all()) and int(s.status) == 0
+
+
+@pytest.mark.parametrize("part,out,n,rows,heads,d", [("bf16", "bf16", 2, 4099, 11, 128), ("fp32", "fp16", 3, 2999, 29, 64),
+                                                     ("fp16", "fp32", 5, 5003, 8, 128)])
+def test_merge_more_rows_than_threads(gpu_ctx, part, out, n, rows, heads, d):
+    """So many rows and heads that a thread takes several."""
+    torch = torch_()
+    assert rows * heads > 16 * torch.cuda.get_device_properties(0).multi_processor_count * 256 // (d // 8)
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    parts = torch.randn(n, rows, heads, d, generator=gen, device="cuda").to(types()[part])
+    lse = torch.randn(n, rows, heads, generator=gen, device="cuda") * 10
+    lse[1:, ::7] = float("-inf")
+    lse[:, ::11] = float("-inf")
+    o = torch.full((rows, heads, d), 7.0, device="cuda", dtype=types()[out])
+    l = torch.full((rows, heads), 7.0, device="cuda")
+    kv.merge(gpu_ctx, parts, lse, o, lse=l, stream=torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    want, wl_, tol, ltol = oracle.merge(parts, lse, types()[out])
+    oracle.check_rounded(o, want, tol)
+    none = torch.isinf(wl_)
+    assert torch.equal(l.double()[none], wl_[none]) and bool((o[none] == 0).all())
+    assert bool(((l.double() - wl_)[~none].abs() <= ltol[~none]).all())
+
+
+@pytest.mark.parametrize("window", [1, 5, 60])
+@pytest.mark.parametrize("d,q_lens,kv_lens", [(64, [1, 2, 1], [70, 90, 65]), (128, [1, 2, 1], [70, 90, 65]), (64, [70, 1], [140, 61]),
+                                              (128, [300, 3], [400, 64])])
+def test_shared_prefix_hidden_by_the_window(gpu_ctx, d, q_lens, kv_lens, window):
+    """A window that ends before the shared prefix: its blocks are not looked at, not even their ids."""
+    torch = torch_()
+    s = Setup(gpu_ctx, "fp16", 2, 4, d, 16, q_lens, kv_lens, seed=72, spare_rows=1, shared_len=200)
+    s.check(window=window)
+    s.check(window=window, softcap=20.0, alibi=s.slopes())
+    want = s.want(window=window)
+    s.shared_table[:] = -1
+    got, lse = s.attend(window=window)
+    torch.cuda.synchronize()
+    oracle.check_attend(got, lse, want, slice(0, s.row_start[-1]))
+    assert int(s.status) == 0
+
+
+@pytest.mark.parametrize("shared_len", [100, 1000])
+def test_shared_blocks_that_no_row_sees_may_be_gone(gpu_ctx, shared_len):
+    """Ids between what a prefix mask and what a window lets the batch see are not looked at; those that some row sees are."""
+    torch = torch_()
+    q_lens, kv_lens, window = [1, 2, 0, 90], [30, 40, 5, 95], 50
+    s = Setup(gpu_ctx, "bf16", 2, 4, 64, 16, q_lens, kv_lens, seed=73, shared_len=shared_len)
+    pre = s.ints([20, 3, 10 ** 6, -7])
+    want = s.want(window=window, prefix_len=pre)
+    first = min(shared_len + n - m - window + 1 for n, m in zip(kv_lens, q_lens) if m)
+    kept = s.shared_table.clone()
+    s.shared_table[2:first // 16] = -1
+    got, lse = s.attend(window=window, prefix_len=pre)
+    torch.cuda.synchronize()
+    assert int(s.status) == 0
+    oracle.check_attend(got, lse, want)
+    s.shared_table.copy_(kept)
+    s.shared_table[first // 16] = 2 ** 31 - 1
+    want = s.want(window=window, prefix_len=pre)
+    got, lse = s.attend(window=window, prefix_len=pre)
+    torch.cuda.synchronize()
+    assert int(s.status) == kv.BAD_PAGE
+    oracle.check_attend(got, lse, want)
