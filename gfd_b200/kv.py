@@ -173,11 +173,17 @@ class PagedCache:
         dense = self.block_tokens * self.heads * self.head_dim
         if st[2] != self.head_dim and self.heads > 1 or st[1] != self.heads * self.head_dim:
             raise ValueError("fetch and offload need the tokens of a block contiguous")
-        host_ids, block_ids = np.asarray(host_ids, np.uint64), np.asarray(block_ids, np.uint64)
+        host_ids, block_ids = (np.asarray(x) for x in (host_ids, block_ids))
         if host_ids.shape != block_ids.shape or host_ids.ndim != 1:
             raise ValueError("host_ids and block_ids must be vectors of one length")
-        if block_ids.size and int(block_ids.max()) >= self.blocks:
-            raise ValueError("a block id is outside the cache")
+        if host_ids.size:
+            if host_ids.dtype.kind not in "iu" or block_ids.dtype.kind not in "iu":
+                raise ValueError("host_ids and block_ids must be whole numbers")
+            if int(host_ids.min()) < 0 or int(host_ptr) + (int(host_ids.max()) + 1) * 2 * dense * item >= 1 << 64:
+                raise ValueError("a host block is outside the address space")
+            if int(block_ids.min()) < 0 or int(block_ids.max()) >= self.blocks:
+                raise ValueError("a block id is outside the cache")
+        host_ids, block_ids = host_ids.astype(np.uint64), block_ids.astype(np.uint64)
         nbytes = np.uint64(dense * item)
         host = np.uint64(host_ptr) + host_ids * np.uint64(2) * nbytes
         parts = []
@@ -189,12 +195,12 @@ class PagedCache:
 
     def fetch(self, host_ptr: int, host_ids, block_ids, stream=0):
         """Gathers host blocks (block h: K then V of all its tokens, at host_ptr + h * block bytes
-        in pinned memory) into the cache's blocks, asynchronously on `stream`."""
+        in pinned memory) into the cache's blocks, asynchronously on `stream`.  No block of the cache is named twice."""
         e = self._block_entries(host_ptr, host_ids, block_ids, False)
         self.ctx._check(self.ctx.gather(e, _stream(stream)))
 
     def offload(self, host_ptr: int, host_ids, block_ids, stream=0):
-        """The reverse of fetch: cache blocks to host blocks."""
+        """The reverse of fetch: cache blocks to host blocks, none of which is named twice."""
         e = self._block_entries(host_ptr, host_ids, block_ids, True)
         self.ctx._check(self.ctx.scatter(e, _stream(stream)))
 
@@ -230,6 +236,8 @@ class PagedCache:
         out_dtype = _dtype(out, "out")
         room, room_bytes = 0, 0
         if workspace is not None:
+            if not workspace.is_contiguous():
+                raise ValueError("workspace: must be contiguous")
             room, room_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         return batch._c(rows), _pack_attend(
             *_rows(q, "q", rows, heads, dim, self.dtype), *_rows(out, "out", rows, heads, dim, out_dtype),

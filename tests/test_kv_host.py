@@ -383,3 +383,31 @@ def test_workspace_of_shapes_out_of_range_is_refused(lib):
     for kw in (dict(rows=-1), dict(rows=1 << 30), dict(rows=1 << 62), dict(seqs=-1), dict(seqs=4097), dict(q_heads=0), dict(q_heads=12),
                dict(q_heads=8200), dict(q_heads=1 << 30), dict(max_q=-1), dict(shared=-1), dict(shared=(1 << 30) + 1)):
         assert check(**kw) is not None, kw
+
+
+def test_fetch_refuses_ids_that_are_no_blocks():
+    import torch
+    pool = torch.zeros(6, 2, 16, 2, 64, dtype=torch.float16)
+    c = kv.PagedCache(None, pool[:, 0], pool[:, 1])
+    for host, block in (([-1], [0]), ([0], [-1]), (np.array([-1]), [0]), ([0], np.array([-1])), ([0.5], [0]), ([0], [1.0]), ([0], [6]),
+                        ([1 << 60], [0]), ([(1 << 64) - 1], [0]), ([[0]], [[0]]), ([True], [0])):
+        for f in (c.fetch, c.offload):
+            with pytest.raises(ValueError):
+                f(1 << 30, host, block)
+    half = 16 * 2 * 64 * 2
+    for host, block in ((np.array([2], np.int32), [5]), ([2], np.array([5], np.uint64)), (torch.tensor([2]), torch.tensor([5]))):
+        e = c._block_entries(1 << 30, host, block, False)
+        assert e["src"].tolist() == [(1 << 30) + 4 * half, (1 << 30) + 5 * half]
+        assert e["dst"].tolist() == [pool.data_ptr() + 10 * half, pool.data_ptr() + 11 * half]
+    assert len(c._block_entries(1 << 30, [], [], False)) == 0
+
+
+def test_workspace_must_be_contiguous():
+    import torch
+    pool = torch.zeros(4, 2, 16, 2, 64, dtype=torch.bfloat16)
+    c = kv.PagedCache(None, pool[:, 0], pool[:, 1])
+    i = torch.int32
+    b = kv.Batch(torch.zeros(3, dtype=i), torch.zeros(2, dtype=i), torch.zeros(2, 4, dtype=i))
+    q, out = torch.zeros(5, 4, 64, dtype=torch.bfloat16), torch.zeros(5, 4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        c.attend(b, q, out, workspace=torch.zeros(64, 1024, dtype=torch.uint8)[:, :512])
