@@ -13,8 +13,8 @@ namespace {
 // holds the 8 pairs that rotate together (two 16-byte pieces rot_dim / 2 apart, or 16
 // neighbours when interleaved), the items above copy.  A thread keeps its item for all heads, so the
 // sines and cosines of its 8 angles stay in registers while it walks the heads of a row, 2 of them
-// in flight at a time.  Memory bounds the kernel: 8.5 thousand rows of 32 + 8 + 8 heads of 128 take 51 us,
-// 5.1 TB/s (4 heads in flight and 8 rows a CTA: 76 us; 3 or 5 CTAs an SM: 60, 89).  A CTA takes
+// in flight at a time.  Memory bounds the kernel: 8.5 thousand rows of 32 + 8 + 8 heads of 128 take 53 us,
+// 4.9 TB/s (4 heads in flight and 8 rows a CTA: 76 us; 3 or 5 CTAs an SM: 60, 89).  A CTA takes
 // kMaxRows rows (one where there are few) and forms their places and angles once.  Angles: p * inv_freq is
 // exact in 64 bits up to p = 2^29, and a turn is taken off in 64 bits before the 32-bit sine, so a
 // position of a million is as accurate as a small one.
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const KvAp
 // ---------------------------------------------------------------------------
 // Merge: one group of D / 8 threads per (row, head), 8 elements a thread, 4 parts in flight at a time.
 // out = sum w_i out_i / sum w_i, w_i = e^(lse_i - m), m the greatest lse.  Memory bounds it: 4 fp32 parts of 8191
-// rows of 32 heads of 128 take 93 us, 6.5 TB/s (2 parts in flight: 113).
+// rows of 32 heads of 128 take 93 us, 6.5 TB/s (2 parts in flight: 113); 4 bf16 parts 126 us, 2.7 TB/s.
 // ---------------------------------------------------------------------------
 constexpr int kMergeThreads = 256;
 

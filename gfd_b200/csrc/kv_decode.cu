@@ -13,10 +13,10 @@
 // sum, scores and sums by mma.m16n8k16 from ldmatrix fragments (KvRows16), and writes its rows from
 // registers.  After the stretches are found there is no barrier.
 //
-// Measured: 64 sequences of up to 8192 tokens, 8 heads of 128, in 170 us with their join, 6.0 TB/s; two of
-// 131 thousand, 24 query heads of 64 behind a cap, in 102 us, 5.0 TB/s (there 12 rows' scores and the cap's
-// polynomial fill half of the issue slots).  128 elements a head take 217-221 registers, two CTAs an SM; 64
-// take 156-161, and the third is worth 123 -> 102 us.
+// Measured: 64 sequences of up to 8192 tokens, 8 heads of 128, in 171 us with their join, 6.0 TB/s; two of
+// 131 thousand, 24 query heads of 64 behind a cap, in 100 us, 5.1 TB/s (there 12 rows' scores and the cap's
+// polynomial fill half of the issue slots).  128 elements a head take 213-217 registers, two CTAs an SM; 64
+// take 158-160, and the third CTA is worth 123 -> 102 us.
 
 #include <type_traits>
 

@@ -12,11 +12,13 @@
 // the weights are at most 2^8 and the sums stay in tensor memory untouched, so the rescaling
 // of O is rare.  Sums and maxima are 32-bit; the weights' rounding to the 16-bit type for the
 // second product is the only one before the result's.
-// With 128 elements a head the softmax between the two products bounds a tile (the tensor pipe is
-// active 58 % of the time, both halves' 256 exponentials a key take as long as their products): 881 us for
-// 8192 rows on 8192 keys and 32 heads, 1248 TFLOP/s, 484 us causal.  With 64 the special function unit
-// alone does: 715 us, 770 TFLOP/s.  Short units wait for O to be written before the next one's sums begin:
-// 16 prompts of 512 rows take 96 us, 716 TFLOP/s.
+// No pipe is full: with 128 elements a head the tensor pipe is active 58 % of the time and the special function
+// unit, which takes the exponentials, 59 %; with 64 it is 35 and 65 %, the issue slots 37 and 43 %.  What bounds a tile
+// is the chain of scores, maximum, exponentials and sums of a half, with two softmax warps a scheduler to hide
+// it.  8192 rows on 8192 keys and 32 heads take 866 us, 1270 TFLOP/s, 467 us causal; with 64 elements 721 us,
+// 762 TFLOP/s, 392 us causal; 752 and 687 us causal behind a cap (calls with pauses between them; back to back the
+// power cap takes a sixth).  Short units wait for O to be written before the next one's sums begin: 16 prompts of
+// 512 rows take 93 us, 737 TFLOP/s.
 //
 // Roles: warps 0-3 softmax of half A, 4-7 of half B; 8-11 write finished rows while the softmax
 // is in the next unit; 12 issues the products, 13 loads K and V (TMA boxes of 16 tokens x 64
@@ -412,9 +414,9 @@ __device__ __forceinline__ uint64_t poly_exp2(uint64_t x) {
                  __uint_as_float(__float_as_uint(b) + (__float_as_uint(nb) << 23)));
 }
 
-// Pairs out of 16 that take poly_exp2.  With 64 elements a head the special function unit bounds
-// a tile and one pair is worth 5 % (non-causal, 8192 rows on 8192 keys, 32 heads: 762 us with
-// none, 723 with 1, 739 with 2); with 128 the products do, and each pair costs (912 us, 927 with 1).
+// Pairs out of 16 that take poly_exp2.  With 64 elements a head the special function unit is the busiest pipe
+// and one pair is worth 2 % (non-causal, 8192 rows on 8192 keys, 32 heads: 763 us with none, 747 with 1, 744 with 2);
+// with 128 it is no busier than the tensor pipe and a pair costs 2 % (causal: 489 us, 500 with 1).
 template <int D>
 struct ByPoly {
     static constexpr int value = D == 64 ? 1 : 0;

@@ -238,7 +238,7 @@ enum { GFD_BF16 = 0, GFD_FP16 = 1, GFD_FP32 = 2 };
                                 table, or more rows than max_q_len: sequence s is skipped, its
                                 output rows stay as they were.  row_start not rising from
                                 >= 0 to <= rows: the whole call is skipped                 */
-#define GFD_KV_GAVE_UP 4u    /* a bounded wait inside a kernel ran out: outputs undefined  */
+#define GFD_KV_GAVE_UP 4u    /* a kernel got nowhere for 10 s and gave up: outputs undefined */
 
 #define GFD_KV_MAX_SEQS 4096
 
